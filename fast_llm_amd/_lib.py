@@ -13,7 +13,7 @@ import torch
 
 LIBRARY_PATH = pathlib.Path(__file__).resolve().parent / "csrc" / "libfastmoe_hip.so"
 
-FM_VERSION = 12
+FM_VERSION = 13
 
 _c_i64, _c_int, _c_ptr, _c_size = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
 
@@ -90,6 +90,16 @@ SIGNATURES: dict[str, tuple] = {
     "fm_moe_layer_backward": (_c_int, [_c_ptr, _c_ptr]),
     "fm_few_tokens_workspace_size": (_c_size, [_c_i64] * 5 + [_c_int] * 2),
     "fm_few_tokens_forward": (_c_int, [_c_ptr] * 6 + [_c_i64] * 5 + [_c_int] * 3 + [_c_ptr, _c_size, _c_ptr]),
+    "fm_mx_quantize": (_c_int, [_c_ptr] * 3 + [_c_i64] * 3 + [_c_int] * 2 + [_c_ptr]),
+    "fm_mx_dequantize": (_c_int, [_c_ptr] * 3 + [_c_i64] * 4 + [_c_int] * 2 + [_c_ptr]),
+    "fm_mx_copy_dense_to_sparse": (_c_int, [_c_ptr] * 5 + [_c_i64] * 6 + [_c_int] * 2 + [_c_ptr]),
+    "fm_mx_sparse_matmul": (_c_int, [_c_ptr] * 7 + [_c_i64] * 9 + [_c_int] * 3 + [_c_ptr]),
+    "fm_mx_sparse_matmul_activation": (_c_int, [_c_ptr] * 8 + [_c_i64] * 8 + [_c_int] * 4 + [_c_ptr]),
+    "fm_mx_few_tokens_workspace_size": (_c_size, [_c_i64] * 5 + [_c_int]),
+    "fm_mx_few_tokens_forward": (_c_int, [_c_ptr] * 9 + [_c_i64] * 11 + [_c_int] * 4 + [_c_ptr, _c_size, _c_ptr]),
+    "fm_rms_norm_forward": (_c_int, [_c_ptr] * 7 + [_c_i64] * 2 + [ctypes.c_double] + [_c_int] * 3 + [_c_ptr]),
+    "fm_rms_norm_backward_workspace_size": (_c_size, [_c_i64] * 2),
+    "fm_rms_norm_backward": (_c_int, [_c_ptr] * 6 + [_c_i64] * 2 + [ctypes.c_double] + [_c_int] * 2 + [_c_ptr, _c_size, _c_ptr]),
 }
 
 FM_ERR_INVALID_ARGUMENT, FM_ERR_UNSUPPORTED, FM_ERR_LAUNCH = -1, -2, -3
@@ -97,6 +107,7 @@ FM_NOTE_GENERIC_KERNEL = 1
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 INDEX_DTYPES = {torch.int16: 0, torch.int32: 1, torch.int64: 2}
+MX_FORMATS = {"e4m3": 0, "e2m1": 1}
 ACTIVATIONS = {"gelu": 0, "silu": 1, "relu": 2, "squared_relu": 3, "identity": 4}
 
 

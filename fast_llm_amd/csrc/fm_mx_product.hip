@@ -1,0 +1,164 @@
+// Entry points of the products with e2m1 expert weights: their checks, and which kernel they run on.
+#include "fm_mx_product.h"
+
+using namespace fm;
+
+namespace {
+
+constexpr int64_t kMost32 = (int64_t(1) << 32) - 4096;
+
+// What all of them ask of a microscaled tensor.
+int check_tensor(const char *name, const char *what, const void *values, const void *scales, int64_t rows, int64_t columns, int64_t value_stride,
+                 int64_t scale_stride, int format) {
+    FM_REQUIRE(values && scales, "%s: null %s", name, what);
+    FM_REQUIRE(value_stride >= mx::value_bytes(format, columns) && scale_stride >= mx::scale_bytes(columns), "%s: rows of %s overlap", name, what);
+    FM_REQUIRE(aligned16(values) && value_stride % 16 == 0, "%s: rows of %s are 16-byte aligned", name, what);
+    FM_REQUIRE(reinterpret_cast<uintptr_t>(scales) % 4 == 0 && scale_stride % 4 == 0, "%s: rows of scales of %s are 4-byte aligned", name, what);
+    // 32 rows are addressed in 32 bits from the first.
+    if (value_stride > kMost32 / 64 || scale_stride > kMost32 / 64) return fail(FM_ERR_UNSUPPORTED, "%s: rows of %s are too long", name, what);
+    (void)rows;
+    return FM_OK;
+}
+
+int check_sizes(const char *name, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int format) {
+    FM_REQUIRE(mx::valid_format(format), "%s: bad format %d", name, format);
+    FM_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && columns > 0 && columns <= (int64_t(1) << 28) && inner > 0 && inner <= (int64_t(1) << 24), "%s: bad sizes", name);
+    FM_REQUIRE(num_experts > 0 && num_experts <= 1024, "%s: num_experts = %lld is not in 1 .. 1024", name, static_cast<long long>(num_experts));
+    return FM_OK;
+}
+
+}  // namespace
+
+extern "C" int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
+                                   const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts,
+                                   int64_t lhs_stride, int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride,
+                                   int format, int out_dtype, int index_dtype, void *stream) {
+    const char *name = "fm_mx_sparse_matmul";
+    if (int status = check_sizes(name, rows, columns, inner, num_experts, format)) return status;
+    FM_REQUIRE(valid_dtype(out_dtype), "%s: bad dtype %d", name, out_dtype);
+    FM_REQUIRE(valid_index_dtype(index_dtype), "%s: bad index dtype %d", name, index_dtype);
+    if (rows == 0) return FM_OK;
+    const int64_t padded = mx::padded_columns(inner);
+    if (int status = check_tensor(name, "lhs", lhs, lhs_scales, rows, padded, lhs_stride, lhs_scale_stride, format)) return status;
+    if (int status = check_tensor(name, "rhs", rhs, rhs_scales, num_experts * columns, padded, rhs_stride, rhs_scale_stride, FM_MX_E2M1)) return status;
+    FM_REQUIRE(out && expert_ends && expert_pad_begins, "%s: null tensor", name);
+    FM_REQUIRE(out_stride >= columns, "%s: rows of the result overlap", name);
+    const int size = dtype_size(out_dtype);
+    FM_REQUIRE(reinterpret_cast<uintptr_t>(out) % size == 0, "%s: misaligned result", name);
+    mx::ProductArgs args{};
+    args.x = static_cast<const uint8_t *>(lhs), args.x_scales = static_cast<const uint8_t *>(lhs_scales);
+    args.weight = static_cast<const uint8_t *>(rhs), args.weight_scales = static_cast<const uint8_t *>(rhs_scales), args.out = out;
+    args.x_rows = args.rows = rows, args.x_stride = lhs_stride, args.x_scale_stride = lhs_scale_stride;
+    args.weight_stride = rhs_stride, args.weight_scale_stride = rhs_scale_stride, args.out_stride = out_stride;
+    args.columns = args.out_columns = columns, args.inner = padded, args.experts = num_experts, args.format = format;
+    args.out_vectors = reinterpret_cast<uintptr_t>(out) % (4 * size) == 0 && out_stride % 4 == 0;
+    args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
+    if (int status = mx::stream_product(args, out_dtype, static_cast<hipStream_t>(stream))) return status;
+    return check_launch(name);
+}
+
+extern "C" int fm_mx_sparse_matmul_activation(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out_values,
+                                              void *out_scales, const void *expert_ends, const void *expert_pad_begins, int64_t rows, int64_t columns,
+                                              int64_t inner, int64_t num_experts, int64_t lhs_stride, int64_t lhs_scale_stride, int64_t rhs_stride,
+                                              int64_t rhs_scale_stride, int gated, int activation, int format, int index_dtype, void *stream) {
+    const char *name = "fm_mx_sparse_matmul_activation";
+    if (int status = check_sizes(name, rows, columns, inner, num_experts, format)) return status;
+    FM_REQUIRE(activation >= FM_ACT_GELU && activation <= FM_ACT_IDENTITY, "%s: bad activation %d", name, activation);
+    FM_REQUIRE(valid_index_dtype(index_dtype), "%s: bad index dtype %d", name, index_dtype);
+    if (rows == 0) return FM_OK;
+    const int64_t padded = mx::padded_columns(inner);
+    if (int status = check_tensor(name, "lhs", lhs, lhs_scales, rows, padded, lhs_stride, lhs_scale_stride, format)) return status;
+    if (int status = check_tensor(name, "rhs", rhs, rhs_scales, num_experts * columns * (gated ? 2 : 1), padded, rhs_stride, rhs_scale_stride, FM_MX_E2M1)) return status;
+    FM_REQUIRE(out_values && out_scales && expert_ends && expert_pad_begins, "%s: null tensor", name);
+    FM_REQUIRE(aligned16(out_values) && aligned16(out_scales), "%s: results are 16-byte aligned", name);
+    mx::ProductArgs args{};
+    args.x = static_cast<const uint8_t *>(lhs), args.x_scales = static_cast<const uint8_t *>(lhs_scales);
+    args.weight = static_cast<const uint8_t *>(rhs), args.weight_scales = static_cast<const uint8_t *>(rhs_scales);
+    args.out = out_values, args.out_scales = static_cast<uint8_t *>(out_scales);
+    args.x_rows = args.rows = rows, args.x_stride = lhs_stride, args.x_scale_stride = lhs_scale_stride;
+    args.weight_stride = rhs_stride, args.weight_scale_stride = rhs_scale_stride;
+    args.columns = columns, args.out_columns = mx::padded_columns(columns), args.inner = padded, args.experts = num_experts, args.format = format;
+    args.out_stride = mx::value_bytes(format, args.out_columns), args.out_scale_stride = mx::scale_bytes(args.out_columns);
+    args.gated = gated != 0, args.activation = activation;
+    args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
+    if (int status = mx::stream_product(args, 0, static_cast<hipStream_t>(stream))) return status;
+    return check_launch(name);
+}
+
+namespace {
+
+// Where the scratch of the few-token MLP lies: the activations' values and scales, then the second layer's fp32 sums.
+struct FewTokensLayout {
+    int64_t entries, ffn, hidden_stride;
+    size_t scales_at, sums_at, size;
+};
+
+bool few_tokens_layout(FewTokensLayout &layout, int64_t tokens, int64_t slots, int64_t hidden, int64_t ffn, int64_t experts, int format) {
+    if (tokens <= 0 || slots <= 0 || hidden <= 0 || ffn <= 0 || experts <= 0 || experts > 1024 || !mx::valid_format(format)) return false;
+    if (tokens > mx::kMaxEntries || slots > mx::kMaxEntries || tokens * slots > mx::kMaxEntries) return false;
+    if (hidden > (1 << 20) || ffn > (1 << 20) || tokens > 65535) return false;
+    layout.entries = tokens * slots;
+    layout.ffn = mx::padded_columns(ffn), layout.hidden_stride = (hidden + 3) / 4 * 4;
+    // Rows are addressed in 32 bits.
+    if (layout.entries * max(layout.ffn, mx::padded_columns(hidden)) >= kMost32) return false;
+    const auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    layout.scales_at = rounded(layout.entries * mx::value_bytes(format, layout.ffn));
+    layout.sums_at = layout.scales_at + rounded(layout.entries * mx::scale_bytes(layout.ffn));
+    layout.size = layout.sums_at + layout.entries * layout.hidden_stride * sizeof(float);
+    return true;
+}
+
+}  // namespace
+
+extern "C" size_t fm_mx_few_tokens_workspace_size(int64_t num_tokens, int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int format) {
+    FewTokensLayout layout;
+    return few_tokens_layout(layout, num_tokens, slots_per_token, hidden, ffn, num_experts, format) ? layout.size : 0;
+}
+
+extern "C" int fm_mx_few_tokens_forward(const void *input, const void *input_scales, const void *top_experts, const void *scores, const void *weight_1,
+                                        const void *weight_1_scales, const void *weight_2, const void *weight_2_scales, void *output, int64_t num_tokens,
+                                        int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int64_t input_stride,
+                                        int64_t input_scale_stride, int64_t weight_1_stride, int64_t weight_1_scale_stride, int64_t weight_2_stride,
+                                        int64_t weight_2_scale_stride, int gated, int activation, int format, int out_dtype, void *workspace,
+                                        size_t workspace_size, void *stream) {
+    const char *name = "fm_mx_few_tokens_forward";
+    FM_REQUIRE(activation >= FM_ACT_GELU && activation <= FM_ACT_IDENTITY, "%s: bad activation %d", name, activation);
+    FM_REQUIRE(mx::valid_format(format), "%s: bad format %d", name, format);
+    FM_REQUIRE(valid_dtype(out_dtype), "%s: bad dtype %d", name, out_dtype);
+    FewTokensLayout layout;
+    if (!few_tokens_layout(layout, num_tokens, slots_per_token, hidden, ffn, num_experts, format))
+        return fail(FM_ERR_UNSUPPORTED, "%s: at most %d (token, slot) pairs and 1024 experts", name, mx::kMaxEntries);
+    FM_REQUIRE(top_experts && scores && output, "%s: null tensor", name);
+    FM_REQUIRE(reinterpret_cast<uintptr_t>(output) % dtype_size(out_dtype) == 0, "%s: misaligned output", name);
+    const int64_t padded = mx::padded_columns(hidden), layer_1_rows = num_experts * ffn * (gated ? 2 : 1);
+    if (int status = check_tensor(name, "the input", input, input_scales, num_tokens, padded, input_stride, input_scale_stride, format)) return status;
+    if (int status = check_tensor(name, "layer 1", weight_1, weight_1_scales, layer_1_rows, padded, weight_1_stride, weight_1_scale_stride, FM_MX_E2M1)) return status;
+    if (int status = check_tensor(name, "layer 2", weight_2, weight_2_scales, num_experts * hidden, layout.ffn, weight_2_stride, weight_2_scale_stride, FM_MX_E2M1))
+        return status;
+    if (num_tokens * input_stride >= kMost32) return fail(FM_ERR_UNSUPPORTED, "%s: rows of the input are too far apart", name);
+    FM_REQUIRE(workspace && aligned16(workspace) && workspace_size >= layout.size, "%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", name,
+               layout.size, workspace_size);
+    mx::ProductArgs layer_1{};
+    layer_1.experts = num_experts, layer_1.format = format, layer_1.gated = gated != 0, layer_1.activation = activation;
+    layer_1.top_experts = static_cast<const int64_t *>(top_experts);
+    layer_1.entries = static_cast<int>(layout.entries), layer_1.by_entry = layout.entries < num_experts;
+    mx::ProductArgs layer_2 = layer_1;
+    uint8_t *scratch = static_cast<uint8_t *>(workspace);
+    layer_1.entries_per_row = static_cast<int>(slots_per_token);
+    layer_1.x = static_cast<const uint8_t *>(input), layer_1.x_scales = static_cast<const uint8_t *>(input_scales);
+    layer_1.x_rows = num_tokens, layer_1.x_stride = input_stride, layer_1.x_scale_stride = input_scale_stride;
+    layer_1.weight = static_cast<const uint8_t *>(weight_1), layer_1.weight_scales = static_cast<const uint8_t *>(weight_1_scales);
+    layer_1.weight_stride = weight_1_stride, layer_1.weight_scale_stride = weight_1_scale_stride;
+    layer_1.out = scratch, layer_1.out_scales = scratch + layout.scales_at;
+    layer_1.out_stride = mx::value_bytes(format, layout.ffn), layer_1.out_scale_stride = mx::scale_bytes(layout.ffn);
+    layer_1.columns = ffn, layer_1.out_columns = layout.ffn, layer_1.inner = padded;
+    layer_2.gated = 0, layer_2.entries_per_row = 1;
+    layer_2.x = scratch, layer_2.x_scales = layer_1.out_scales;
+    layer_2.x_rows = layout.entries, layer_2.x_stride = layer_1.out_stride, layer_2.x_scale_stride = layer_1.out_scale_stride;
+    layer_2.weight = static_cast<const uint8_t *>(weight_2), layer_2.weight_scales = static_cast<const uint8_t *>(weight_2_scales);
+    layer_2.weight_stride = weight_2_stride, layer_2.weight_scale_stride = weight_2_scale_stride;
+    layer_2.out = scratch + layout.sums_at, layer_2.out_stride = layout.hidden_stride, layer_2.out_vectors = 1;
+    layer_2.columns = layer_2.out_columns = hidden, layer_2.inner = layout.ffn;
+    if (int status = mx::few_tokens(layer_1, layer_2, static_cast<const float *>(scores), output, out_dtype, static_cast<hipStream_t>(stream))) return status;
+    return check_launch(name);
+}

@@ -1,0 +1,443 @@
+// Root-mean-square norm with the residual's addition, forward (with its result in microscaled values beside it, for a product with
+// quantised weights) and backward.
+//
+//   s = round(x + r) (the stream that goes on; s = x without a residual),  n = round(s * v * w),  v = 1 / sqrt(mean(s^2) + eps)
+//   backward, of the gradients g of n and h of s:  ds = v (g w - s v^2 mean(g w s)) + h  (of x and of r alike),  dw = sum over rows of g s v
+//
+// What is normalised is the rounded stream, so that the backward needs nothing but it: v is computed again from the row that is in
+// registers anyway. All of a row is in the registers of one wavefront (up to 2048 columns), of four or of sixteen (8192, 32768), so each tensor
+// passes once: memory is the bound. Sums are in fp32: a lane's own values, then lanes, then wavefronts, in a fixed order.
+// Rows that are longer, or whose length is no multiple of 8, or that are not aligned to 16 bytes: a value per lane and load, the stream
+// read a second time.
+#include "fm_mx.h"
+
+namespace fm {
+
+namespace norm {
+
+struct Args {
+    const void *input, *residual, *weight;
+    void *stream, *normalized;
+    uint8_t *values, *scales;  // null: no microscaled result
+    const void *grad_normalized, *grad_stream;
+    void *grad_input;
+    float *partials;  // [parts][columns] of the weight's gradient, or null
+    int64_t rows;
+    int columns, padded, format, weight_f32;
+    float eps, inverse_columns;
+};
+
+template <typename T>
+struct Eight {
+    Vec16<T> part[8 / Vec16<T>::N];
+    __device__ __forceinline__ float operator[](int i) const { return to_float(part[i / Vec16<T>::N].v[i % Vec16<T>::N]); }
+    __device__ __forceinline__ void set(int i, float value) { part[i / Vec16<T>::N].v[i % Vec16<T>::N] = from_float<T>(value); }
+};
+
+template <typename T>
+__device__ __forceinline__ Eight<T> zeros() {
+    Eight<T> eight;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) eight.set(i, 0.f);
+    return eight;
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const void *base, int64_t offset) {
+    Eight<T> eight;
+#pragma unroll
+    for (int part = 0; part < 8 / Vec16<T>::N; ++part) eight.part[part] = load16(static_cast<const T *>(base) + offset + part * Vec16<T>::N);
+    return eight;
+}
+template <typename T>
+__device__ __forceinline__ void store_eight(void *base, int64_t offset, const Eight<T> &eight) {
+#pragma unroll
+    for (int part = 0; part < 8 / Vec16<T>::N; ++part) store16(static_cast<T *>(base) + offset + part * Vec16<T>::N, eight.part[part]);
+}
+
+// The weight of eight columns. It has the input's type or fp32.
+template <typename T>
+__device__ __forceinline__ void load_weight(const Args &args, int column, float (&weight)[8]) {
+    if (args.weight_f32) {
+        const Eight<float> eight = load_eight<float>(args.weight, column);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight[i] = eight[i];
+    } else {
+        const Eight<T> eight = load_eight<T>(args.weight, column);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight[i] = eight[i];
+    }
+}
+
+// Sums of kCount values over the kLanes threads of a row, in all of them.
+template <int kLanes, int kCount>
+__device__ __forceinline__ void row_sum(float (&values)[kCount]) {
+#pragma unroll
+    for (int c = 0; c < kCount; ++c) values[c] = wave_sum(values[c]);
+    if constexpr (kLanes > 64) {
+        __shared__ float sums[kCount][kLanes / 64];
+        __syncthreads();  // the sums of the row before have been read
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int c = 0; c < kCount; ++c) sums[c][threadIdx.x >> 6] = values[c];
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kCount; ++c) {
+            values[c] = sums[c][0];
+#pragma unroll
+            for (int w = 1; w < kLanes / 64; ++w) values[c] += sums[c][w];
+        }
+    }
+}
+
+__device__ __forceinline__ float inverse_root(const Args &args, float sum_of_squares) {
+    return 1.f / sqrtf(sum_of_squares * args.inverse_columns + args.eps);
+}
+
+template <int kLanes>
+constexpr int kThreads = kLanes < 256 ? 256 : kLanes;
+
+// kLanes threads a row, kVectors times eight columns each: vector v of lane l is the columns 8 (v kLanes + l) .. + 7.
+template <typename T, int kLanes, int kVectors>
+__global__ __launch_bounds__(kThreads<kLanes>) void forward_kernel(Args args) {
+    const int lane = threadIdx.x % kLanes;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads<kLanes> / kLanes) + threadIdx.x / kLanes;
+    if (row >= args.rows) return;  // whole wavefronts
+    const int64_t start = row * args.columns;
+    Eight<T> stream[kVectors];
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+        const int column = (v * kLanes + lane) * 8;
+        stream[v] = column < args.columns ? load_eight<T>(args.input, start + column) : zeros<T>();
+    }
+    if (args.residual != nullptr) {
+        Eight<T> residual[kVectors];
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+            residual[v] = column < args.columns ? load_eight<T>(args.residual, start + column) : zeros<T>();
+        }
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) stream[v].set(i, stream[v][i] + residual[v][i]);
+            if (column < args.columns) store_eight(args.stream, start + column, stream[v]);
+        }
+    }
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[0] += stream[v][i] * stream[v][i];
+    row_sum<kLanes>(sum);
+    const float inverse = inverse_root(args, sum[0]);
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+        const int column = (v * kLanes + lane) * 8;
+        const bool exists = column < args.columns;
+        Eight<T> result = zeros<T>();
+        if (exists) {
+            float weight[8];
+            load_weight<T>(args, column, weight);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) result.set(i, stream[v][i] * inverse * weight[i]);
+            store_eight(args.normalized, start + column, result);
+        }
+        if (args.values != nullptr) {
+            // Of the rounded result, as its quantisation by itself would be.
+            float values[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) values[i] = result[i];
+            mx::store_eight(args.format, values, args.values + row * mx::value_bytes(args.format, args.padded),
+                            args.scales + row * mx::scale_bytes(args.padded), column, column < args.padded);
+        }
+    }
+}
+
+// Any length and alignment: a workgroup a row, a value a thread.
+constexpr int kAnyThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kAnyThreads) void forward_any_kernel(Args args) {
+    const int64_t row = blockIdx.x, start = row * args.columns;
+    const T *input = static_cast<const T *>(args.input) + start, *residual = static_cast<const T *>(args.residual) + start;
+    T *stream = static_cast<T *>(args.stream) + start;
+    float sum[1] = {0.f};
+    for (int column = threadIdx.x; column < args.columns; column += kAnyThreads) {
+        float value = to_float(input[column]);
+        if (args.residual != nullptr) {
+            const T rounded = from_float<T>(value + to_float(residual[column]));
+            stream[column] = rounded;
+            value = to_float(rounded);
+        }
+        sum[0] += value * value;
+    }
+    row_sum<kAnyThreads>(sum);
+    const float inverse = inverse_root(args, sum[0]);
+    const int end = args.values != nullptr ? (args.padded + kAnyThreads - 1) / kAnyThreads * kAnyThreads : args.columns;
+    for (int column = threadIdx.x; column < end; column += kAnyThreads) {
+        T result = from_float<T>(0.f);
+        if (column < args.columns) {
+            // Each thread reads what it has written itself.
+            const float value = to_float(args.residual != nullptr ? stream[column] : input[column]);
+            const float weight = args.weight_f32 ? static_cast<const float *>(args.weight)[column] : to_float(static_cast<const T *>(args.weight)[column]);
+            result = from_float<T>(value * inverse * weight);
+            static_cast<T *>(args.normalized)[start + column] = result;
+        }
+        if (args.values != nullptr)
+            mx::store_one(args.format, to_float(result), args.values + row * mx::value_bytes(args.format, args.padded),
+                          args.scales + row * mx::scale_bytes(args.padded), column, column < args.padded);
+    }
+}
+
+// A group of kLanes threads walks over rows and keeps its share of the weight's gradient in registers; the groups of a workgroup add
+// theirs up in LDS, the workgroups theirs in `weight_gradient_kernel`.
+template <typename T, int kLanes, int kVectors>
+__global__ __launch_bounds__(kThreads<kLanes>) void backward_kernel(Args args) {
+    constexpr int kGroups = kThreads<kLanes> / kLanes;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    float weight_grad[kVectors][8];
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight_grad[v][i] = 0.f;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group; row < args.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
+        const int64_t start = row * args.columns;
+        Eight<T> stream[kVectors], grad[kVectors], grad_stream[kVectors];
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+            const bool exists = column < args.columns;
+            stream[v] = exists ? load_eight<T>(args.stream, start + column) : zeros<T>();
+            grad[v] = exists ? load_eight<T>(args.grad_normalized, start + column) : zeros<T>();
+            grad_stream[v] = exists && args.grad_stream != nullptr ? load_eight<T>(args.grad_stream, start + column) : zeros<T>();
+        }
+        float sums[2] = {0.f, 0.f};  // of s^2 and of g w s
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+            if (column >= args.columns) continue;
+            float weight[8];
+            load_weight<T>(args, column, weight);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sums[0] += stream[v][i] * stream[v][i];
+                sums[1] += grad[v][i] * weight[i] * stream[v][i];
+            }
+        }
+        row_sum<kLanes>(sums);
+        const float inverse = inverse_root(args, sums[0]), factor = inverse * inverse * sums[1] * args.inverse_columns;
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+            if (column >= args.columns) continue;
+            float weight[8];
+            load_weight<T>(args, column, weight);
+            Eight<T> result;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                result.set(i, inverse * (grad[v][i] * weight[i] - stream[v][i] * factor) + grad_stream[v][i]);
+                weight_grad[v][i] += grad[v][i] * (stream[v][i] * inverse);
+            }
+            store_eight(args.grad_input, start + column, result);
+        }
+    }
+    if (args.partials == nullptr) return;
+    float *target = args.partials + static_cast<int64_t>(blockIdx.x) * args.columns;
+    if constexpr (kGroups == 1) {
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+            if (column >= args.columns) continue;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) target[column + i] = weight_grad[v][i];
+        }
+    } else {
+        __shared__ float shared[kGroups][kLanes * 8];
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) shared[group][i * kLanes + lane] = weight_grad[v][i];
+            __syncthreads();
+            for (int at = threadIdx.x; at < kLanes * 8; at += kThreads<kLanes>) {
+                const int column = v * kLanes * 8 + at, from = at % 8 * kLanes + at / 8;
+                float sum = shared[0][from];
+#pragma unroll
+                for (int g = 1; g < kGroups; ++g) sum += shared[g][from];
+                if (column < args.columns) target[column] = sum;
+            }
+        }
+    }
+}
+
+// Any length and alignment. The weight's gradient: a workgroup's share is in its row of `partials` from the first row on, each value
+// written and read by one thread.
+template <typename T>
+__global__ __launch_bounds__(kAnyThreads) void backward_any_kernel(Args args) {
+    float *target = args.partials + static_cast<int64_t>(blockIdx.x) * args.columns;
+    bool first = true;
+    for (int64_t row = blockIdx.x; row < args.rows; row += gridDim.x) {
+        const int64_t start = row * args.columns;
+        const T *stream = static_cast<const T *>(args.stream) + start, *grad = static_cast<const T *>(args.grad_normalized) + start;
+        const T *grad_stream = static_cast<const T *>(args.grad_stream) + start;
+        const auto weight_at = [&](int column) {
+            return args.weight_f32 ? static_cast<const float *>(args.weight)[column] : to_float(static_cast<const T *>(args.weight)[column]);
+        };
+        float sums[2] = {0.f, 0.f};
+        for (int column = threadIdx.x; column < args.columns; column += kAnyThreads) {
+            const float s = to_float(stream[column]);
+            sums[0] += s * s;
+            sums[1] += to_float(grad[column]) * weight_at(column) * s;
+        }
+        row_sum<kAnyThreads>(sums);
+        const float inverse = inverse_root(args, sums[0]), factor = inverse * inverse * sums[1] * args.inverse_columns;
+        for (int column = threadIdx.x; column < args.columns; column += kAnyThreads) {
+            const float s = to_float(stream[column]), g = to_float(grad[column]);
+            const float more = args.grad_stream != nullptr ? to_float(grad_stream[column]) : 0.f;
+            static_cast<T *>(args.grad_input)[start + column] = from_float<T>(inverse * (g * weight_at(column) - s * factor) + more);
+            if (args.partials != nullptr) target[column] = (first ? 0.f : target[column]) + g * (s * inverse);
+        }
+        first = false;
+    }
+}
+
+// 16 columns a workgroup, 64 threads each that take every 64th part.
+constexpr int kReduceColumns = 16, kReduceThreads = 1024;
+
+template <typename T>
+__global__ __launch_bounds__(kReduceThreads) void weight_gradient_kernel(const float *partials, T *out, int columns, int parts) {
+    __shared__ float sums[kReduceThreads / kReduceColumns][kReduceColumns + 1];
+    const int within = threadIdx.x % kReduceColumns, part = threadIdx.x / kReduceColumns, column = blockIdx.x * kReduceColumns + within;
+    float sum = 0.f;
+    if (column < columns)
+        for (int p = part; p < parts; p += kReduceThreads / kReduceColumns) sum += partials[static_cast<int64_t>(p) * columns + column];
+    sums[part][within] = sum;
+#pragma unroll
+    for (int width = kReduceThreads / kReduceColumns / 2; width > 0; width /= 2) {
+        __syncthreads();
+        if (part < width) sums[part][within] += sums[part + width][within];
+    }
+    if (part == 0 && column < columns) out[column] = from_float<T>(sums[0][within]);
+}
+
+constexpr int64_t kMaxColumns = int64_t(1) << 28;
+constexpr int kMaxParts = 512;
+
+// Threads of a row, 0: `..._any_kernel`.
+static int lanes_of(int64_t columns, bool aligned) {
+    if (!aligned || columns % 8 != 0 || columns > 32768) return 0;
+    return columns <= 2048 ? 64 : columns <= 8192 ? 256 : 1024;
+}
+
+// Workgroups of a backward: what two per CU hold, walking over the rows.
+static int64_t parts_of(int64_t rows, int64_t columns) {
+    const int64_t at_once = columns <= 2048 ? 4 : 1;
+    return min((rows + at_once - 1) / at_once, static_cast<int64_t>(kMaxParts));
+}
+
+template <typename T, typename Launch>
+static void for_shape(int columns, int lanes, Launch launch) {
+    if (lanes == 64 && columns <= 512) launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (lanes == 64 && columns <= 1024) launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (lanes == 64) launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    else if (lanes == 256 && columns <= 4096) launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if (lanes == 256) launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+}
+
+}  // namespace norm
+
+}  // namespace fm
+
+using namespace fm;
+
+static int check_norm(const char *name, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype) {
+    FM_REQUIRE(valid_dtype(dtype), "%s: bad dtype %d", name, dtype);
+    FM_REQUIRE(weight_dtype == dtype || weight_dtype == FM_DTYPE_F32, "%s: bad weight dtype %d: the input's or fp32", name, weight_dtype);
+    FM_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && columns > 0 && columns <= norm::kMaxColumns, "%s: bad sizes %lld x %lld", name,
+               static_cast<long long>(rows), static_cast<long long>(columns));
+    FM_REQUIRE(eps >= 0., "%s: negative eps", name);
+    return FM_OK;
+}
+
+extern "C" int fm_rms_norm_forward(const void *input, const void *residual, const void *weight, void *stream_out, void *normalized, void *values,
+                                   void *scales, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype, int format, void *stream) {
+    const char *name = "fm_rms_norm_forward";
+    if (int status = check_norm(name, rows, columns, eps, dtype, weight_dtype)) return status;
+    FM_REQUIRE((values == nullptr) == (scales == nullptr), "%s: microscaled values and scales come together", name);
+    FM_REQUIRE(values == nullptr || mx::valid_format(format), "%s: bad format %d", name, format);
+    if (rows == 0) return FM_OK;
+    FM_REQUIRE(input && weight && normalized, "%s: null tensor", name);
+    FM_REQUIRE((residual == nullptr) == (stream_out == nullptr), "%s: the residual and the stream that goes on come together", name);
+    FM_REQUIRE(values == nullptr || (aligned16(values) && aligned16(scales)), "%s: microscaled results are 16-byte aligned", name);
+    const bool aligned = aligned16(input) && aligned16(residual) && aligned16(weight) && aligned16(stream_out) && aligned16(normalized);
+    const int lanes = norm::lanes_of(columns, aligned);
+    norm::Args args{};
+    args.input = input, args.residual = residual, args.weight = weight, args.stream = stream_out, args.normalized = normalized;
+    args.values = static_cast<uint8_t *>(values), args.scales = static_cast<uint8_t *>(scales);
+    args.rows = rows, args.columns = static_cast<int>(columns), args.padded = static_cast<int>(mx::padded_columns(columns)), args.format = format;
+    args.weight_f32 = weight_dtype == FM_DTYPE_F32 && dtype != FM_DTYPE_F32;
+    args.eps = static_cast<float>(eps), args.inverse_columns = static_cast<float>(1. / static_cast<double>(columns));
+    FM_DISPATCH_DTYPE(dtype, T, {
+        if (lanes == 0) {
+            norm::forward_any_kernel<T><<<static_cast<uint32_t>(rows), norm::kAnyThreads, 0, static_cast<hipStream_t>(stream)>>>(args);
+        } else {
+            norm::for_shape<T>(static_cast<int>(columns), lanes, [&](auto lanes_constant, auto vectors) {
+                constexpr int kLanes = decltype(lanes_constant)::value, kRows = norm::kThreads<kLanes> / kLanes;
+                norm::forward_kernel<T, kLanes, decltype(vectors)::value>
+                    <<<static_cast<uint32_t>((rows + kRows - 1) / kRows), norm::kThreads<kLanes>, 0, static_cast<hipStream_t>(stream)>>>(args);
+            });
+        }
+    });
+    return check_launch(name);
+}
+
+extern "C" size_t fm_rms_norm_backward_workspace_size(int64_t rows, int64_t columns) {
+    if (rows <= 0 || columns <= 0 || columns > norm::kMaxColumns) return 0;
+    return static_cast<size_t>(norm::parts_of(rows, columns)) * columns * sizeof(float);
+}
+
+extern "C" int fm_rms_norm_backward(const void *grad_normalized, const void *grad_stream, const void *stream_in, const void *weight, void *grad_input,
+                                    void *grad_weight, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype, void *workspace,
+                                    size_t workspace_size, void *stream) {
+    const char *name = "fm_rms_norm_backward";
+    if (int status = check_norm(name, rows, columns, eps, dtype, weight_dtype)) return status;
+    const size_t needed = fm_rms_norm_backward_workspace_size(rows, columns);
+    if (rows > 0) {
+        FM_REQUIRE(grad_normalized && stream_in && weight && grad_input, "%s: null tensor", name);
+        FM_REQUIRE(grad_weight == nullptr || (workspace && aligned16(workspace) && workspace_size >= needed),
+                   "%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", name, needed, workspace_size);
+    }
+    norm::Args args{};
+    args.stream = const_cast<void *>(stream_in), args.weight = weight, args.grad_normalized = grad_normalized, args.grad_stream = grad_stream;
+    args.grad_input = grad_input, args.partials = grad_weight != nullptr ? static_cast<float *>(workspace) : nullptr;
+    args.rows = rows, args.columns = static_cast<int>(columns);
+    args.weight_f32 = weight_dtype == FM_DTYPE_F32 && dtype != FM_DTYPE_F32;
+    args.eps = static_cast<float>(eps), args.inverse_columns = static_cast<float>(1. / static_cast<double>(columns));
+    const bool aligned = aligned16(grad_normalized) && aligned16(grad_stream) && aligned16(stream_in) && aligned16(weight) && aligned16(grad_input);
+    const int lanes = norm::lanes_of(columns, aligned);
+    // Without rows the weight's gradient is the sum of nothing.
+    const uint32_t parts = rows > 0 ? static_cast<uint32_t>(norm::parts_of(rows, columns)) : 0;
+    if (rows > 0) {
+        FM_DISPATCH_DTYPE(dtype, T, {
+            if (lanes == 0) {
+                norm::backward_any_kernel<T><<<parts, norm::kAnyThreads, 0, static_cast<hipStream_t>(stream)>>>(args);
+            } else {
+                norm::for_shape<T>(static_cast<int>(columns), lanes, [&](auto lanes_constant, auto vectors) {
+                    constexpr int kLanes = decltype(lanes_constant)::value;
+                    norm::backward_kernel<T, kLanes, decltype(vectors)::value>
+                        <<<parts, norm::kThreads<kLanes>, 0, static_cast<hipStream_t>(stream)>>>(args);
+                });
+            }
+        });
+    }
+    if (grad_weight != nullptr) {
+        const uint32_t workgroups = static_cast<uint32_t>((columns + norm::kReduceColumns - 1) / norm::kReduceColumns);
+        FM_DISPATCH_DTYPE(weight_dtype, W, {
+            norm::weight_gradient_kernel<W><<<workgroups, norm::kReduceThreads, 0, static_cast<hipStream_t>(stream)>>>(
+                args.partials, static_cast<W *>(grad_weight), static_cast<int>(columns), static_cast<int>(parts));
+        });
+    }
+    return check_launch(name);
+}

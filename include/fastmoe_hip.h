@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FM_VERSION 12
+#define FM_VERSION 13
 
 /* Element type of activations, weights and outputs. */
 enum fm_dtype { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1, FM_DTYPE_F16 = 2 };
@@ -443,6 +443,72 @@ int fm_moe_layer_sizes(fm_moe_layer *layer);
 int fm_moe_layer_route(const fm_moe_layer *layer, void *stream);
 int fm_moe_layer_forward(const fm_moe_layer *layer, void *stream);
 int fm_moe_layer_backward(const fm_moe_layer *layer, void *stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Microscaled (MX) values (OCP Microscaling Formats 1.0): 32 neighbours along a row share the scale 2^(byte - 127) and are kept in e4m3 (a
+ * byte each) or e2m1 (two to a byte, the even column in the low half). A tensor of [rows, columns] is two arrays of bytes, both row-major:
+ * values, columns (e4m3) or columns / 2 (e2m1) bytes a row, and scales, columns / 32 bytes a row, where `columns` is rounded up to a multiple of
+ * 128; what is behind the last column is zeros, with scale byte 0. Strides between rows are in bytes: multiples of 16 for values, which are 16-byte
+ * aligned, of 4 for scales, which are 4-byte aligned.
+ *   scale   = 2^max(floor(log2(largest magnitude)) - 8 (e4m3) or 2 (e2m1), -127);   element = value / scale, rounded to nearest
+ *   even, saturated at 448 or 6.   A block with an infinity or NaN: scale byte 255 (all of it is NaN), elements 0.
+ * --------------------------------------------------------------------------------------------------------- */
+enum fm_mx_format { FM_MX_E4M3 = 0, FM_MX_E2M1 = 1 };
+
+/* Rows of `input` (of `dtype`, contiguous along the row, `input_row_stride` elements apart) -> contiguous 16-byte aligned values and scales. */
+int fm_mx_quantize(const void *input, void *values, void *scales, int64_t rows, int64_t columns, int64_t input_row_stride, int dtype,
+                   int format, void *stream);
+/* Back, into contiguous rows of `dtype`: element * scale, rounded once. */
+int fm_mx_dequantize(const void *values, const void *scales, void *output, int64_t rows, int64_t columns, int64_t value_row_stride,
+                     int64_t scale_row_stride, int dtype, int format, void *stream);
+/* fm_copy_dense_to_sparse for microscaled rows; the results are contiguous. */
+int fm_mx_copy_dense_to_sparse(const void *values, const void *scales, const void *sparse_rows, void *out_values, void *out_scales,
+                               int64_t num_rows_dense, int64_t columns, int64_t num_experts_per_token, int64_t num_rows_sparse,
+                               int64_t value_row_stride, int64_t scale_row_stride, int format, int index_dtype, void *stream);
+
+/* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs, in e2m1, has `columns` rows of `inner` per expert, lhs is in
+ * `format`. Both layers of an expert MLP are such products. Sums in fp32, one rounding. Of each expert the rows [expert_ends[e - 1],
+ * expert_pad_begins[e]) are computed; all others of `out` (padding, rows behind the last expert) are left as they are, and those of lhs are not
+ * looked at. Expert boundaries need not be multiples of anything. `out_stride` in elements. At most 1024 experts. */
+int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
+                        const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
+                        int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int format, int out_dtype,
+                        int index_dtype, void *stream);
+/* The same product followed by the activation, its result microscaled in `format` (contiguous, padded with zeros; from the fp32 sums, with no
+ * rounding in between): out[i, j] = act(product[i, j]), or gated, with 2 `columns` rows of rhs per expert, act(product[i, j]) * product[i, columns + j]. */
+int fm_mx_sparse_matmul_activation(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out_values,
+                                   void *out_scales, const void *expert_ends, const void *expert_pad_begins, int64_t rows, int64_t columns,
+                                   int64_t inner, int64_t num_experts, int64_t lhs_stride, int64_t lhs_scale_stride, int64_t rhs_stride,
+                                   int64_t rhs_scale_stride, int gated, int activation, int format, int index_dtype, void *stream);
+
+/* The expert MLP of few tokens without a sparse map (fm_few_tokens_forward for microscaled operands):
+ *   output[t] = sum_j scores[t, j] * layer_2[e] act(layer_1[e] input[t]),  e = top_experts[t, j],
+ * the activation's result microscaled in `format` as above; entries outside [0, num_experts) add nothing. weight_1: [num_experts * ffn (* 2), hidden],
+ * per expert the gates and then the ups; weight_2: [num_experts * hidden, ffn], both in e2m1. top_experts int64, scores fp32. At most 4096 (token, slot) pairs
+ * and 1024 experts (FM_ERR_UNSUPPORTED, size 0). `workspace`: 16-byte aligned. */
+size_t fm_mx_few_tokens_workspace_size(int64_t num_tokens, int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int format);
+int fm_mx_few_tokens_forward(const void *input, const void *input_scales, const void *top_experts, const void *scores, const void *weight_1,
+                             const void *weight_1_scales, const void *weight_2, const void *weight_2_scales, void *output, int64_t num_tokens,
+                             int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int64_t input_stride,
+                             int64_t input_scale_stride, int64_t weight_1_stride, int64_t weight_1_scale_stride, int64_t weight_2_stride,
+                             int64_t weight_2_scale_stride, int gated, int activation, int format, int out_dtype, void *workspace,
+                             size_t workspace_size, void *stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Root-mean-square norm with the residual's addition. Contiguous rows of `dtype`; `weight` of `dtype` or fp32.
+ *   stream_out = round(input + residual) (without a residual, null both, the input itself),
+ *   normalized = round(s * v * weight),  s = the (rounded) stream, v = 1 / sqrt(mean(s^2) + eps).
+ * With `values` and `scales` (both or neither) also `normalized`, as rounded, microscaled in `format`, bit for bit as fm_mx_quantize gives it.
+ * Backward, of the gradients of normalized and (may be null) of the stream: grad_input = v (g w - s v^2 mean(g w s)) + grad_stream, of input and
+ * residual alike, one rounding; grad_weight (of weight_dtype; may be null: not computed) = sum over rows of g s v in fp32, in a fixed order, in
+ * a `workspace` of fm_rms_norm_backward_workspace_size bytes (16-byte aligned).
+ * --------------------------------------------------------------------------------------------------------- */
+int fm_rms_norm_forward(const void *input, const void *residual, const void *weight, void *stream_out, void *normalized, void *values,
+                        void *scales, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype, int format, void *stream);
+size_t fm_rms_norm_backward_workspace_size(int64_t rows, int64_t columns);
+int fm_rms_norm_backward(const void *grad_normalized, const void *grad_stream, const void *stream_in, const void *weight, void *grad_input,
+                         void *grad_weight, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype, void *workspace,
+                         size_t workspace_size, void *stream);
 
 #ifdef __cplusplus
 }
