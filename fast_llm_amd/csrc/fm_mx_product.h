@@ -33,6 +33,9 @@ struct ProductArgs {
 
 constexpr int kMaxEntries = 4096;  // the list in LDS, and the scan of every workgroup
 
+// Many rows per expert (fm_mx_tiles.hip).
+bool tile_product_takes(const ProductArgs &args);
+int tile_product(const ProductArgs &args, int out_dtype, hipStream_t stream);
 // Few rows per expert (fm_mx_stream.hip). `out_dtype` where the result is not microscaled.
 int stream_product(const ProductArgs &args, int out_dtype, hipStream_t stream);
 // Both layers and the combine without a sparse map; layer_2.out is fp32 scratch.

@@ -27,6 +27,13 @@ int check_sizes(const char *name, int64_t rows, int64_t columns, int64_t inner, 
     return FM_OK;
 }
 
+int run(const mx::ProductArgs &args, int out_dtype, void *stream) {
+    // The host knows rows with up to 128 of padding per expert.
+    const bool many = args.rows > 192 * args.experts;
+    return many && mx::tile_product_takes(args) ? mx::tile_product(args, out_dtype, static_cast<hipStream_t>(stream))
+                                                : mx::stream_product(args, out_dtype, static_cast<hipStream_t>(stream));
+}
+
 }  // namespace
 
 extern "C" int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
@@ -53,7 +60,7 @@ extern "C" int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, cons
     args.columns = args.out_columns = columns, args.inner = padded, args.experts = num_experts, args.format = format;
     args.out_vectors = reinterpret_cast<uintptr_t>(out) % (4 * size) == 0 && out_stride % 4 == 0;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
-    if (int status = mx::stream_product(args, out_dtype, static_cast<hipStream_t>(stream))) return status;
+    if (int status = run(args, out_dtype, stream)) return status;
     return check_launch(name);
 }
 
@@ -81,7 +88,7 @@ extern "C" int fm_mx_sparse_matmul_activation(const void *lhs, const void *lhs_s
     args.out_stride = mx::value_bytes(format, args.out_columns), args.out_scale_stride = mx::scale_bytes(args.out_columns);
     args.gated = gated != 0, args.activation = activation;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
-    if (int status = mx::stream_product(args, 0, static_cast<hipStream_t>(stream))) return status;
+    if (int status = run(args, 0, stream)) return status;
     return check_launch(name);
 }
 
