@@ -34,6 +34,23 @@ struct Eight {
     __device__ __forceinline__ void set(int i, float value) { part[i / Vec16<T>::N].v[i % Vec16<T>::N] = from_float<T>(value); }
 };
 
+// The same values, but the compiler cannot tell: it computes them once, as they are stored. (Otherwise it may round a product of fp32 straight to fp16
+// for the store and by way of fp32 for what goes on with it.)
+template <typename T>
+__device__ __forceinline__ void settle(Eight<T> &eight) {
+#pragma unroll
+    for (int part = 0; part < 8 / Vec16<T>::N; ++part) {
+        RawVec16 raw = __builtin_bit_cast(RawVec16, eight.part[part]);
+        asm volatile("" : "+v"(raw));
+        eight.part[part] = __builtin_bit_cast(Vec16<T>, raw);
+    }
+}
+template <typename T>
+__device__ __forceinline__ T settled(T value) {
+    asm volatile("" : "+v"(value));
+    return value;
+}
+
 template <typename T>
 __device__ __forceinline__ Eight<T> zeros() {
     Eight<T> eight;
@@ -121,6 +138,7 @@ __global__ __launch_bounds__(kThreads<kLanes>) void forward_kernel(Args args) {
             const int column = (v * kLanes + lane) * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) stream[v].set(i, stream[v][i] + residual[v][i]);
+            settle(stream[v]);
             if (column < args.columns) store_eight(args.stream, start + column, stream[v]);
         }
     }
@@ -141,6 +159,7 @@ __global__ __launch_bounds__(kThreads<kLanes>) void forward_kernel(Args args) {
             load_weight<T>(args, column, weight);
 #pragma unroll
             for (int i = 0; i < 8; ++i) result.set(i, stream[v][i] * inverse * weight[i]);
+            settle(result);
             store_eight(args.normalized, start + column, result);
         }
         if (args.values != nullptr) {
@@ -166,7 +185,7 @@ __global__ __launch_bounds__(kAnyThreads) void forward_any_kernel(Args args) {
     for (int column = threadIdx.x; column < args.columns; column += kAnyThreads) {
         float value = to_float(input[column]);
         if (args.residual != nullptr) {
-            const T rounded = from_float<T>(value + to_float(residual[column]));
+            const T rounded = settled(from_float<T>(value + to_float(residual[column])));
             stream[column] = rounded;
             value = to_float(rounded);
         }
@@ -181,7 +200,7 @@ __global__ __launch_bounds__(kAnyThreads) void forward_any_kernel(Args args) {
             // Each thread reads what it has written itself.
             const float value = to_float(args.residual != nullptr ? stream[column] : input[column]);
             const float weight = args.weight_f32 ? static_cast<const float *>(args.weight)[column] : to_float(static_cast<const T *>(args.weight)[column]);
-            result = from_float<T>(value * inverse * weight);
+            result = settled(from_float<T>(value * inverse * weight));
             static_cast<T *>(args.normalized)[start + column] = result;
         }
         if (args.values != nullptr)
@@ -195,6 +214,8 @@ __global__ __launch_bounds__(kAnyThreads) void forward_any_kernel(Args args) {
 template <typename T, int kLanes, int kVectors>
 __global__ __launch_bounds__(kThreads<kLanes>) void backward_kernel(Args args) {
     constexpr int kGroups = kThreads<kLanes> / kLanes;
+    // The stream's gradient is asked for with the rest of the row, but where 16 wavefronts share a CU's registers.
+    constexpr bool kEarly = kLanes < 1024;
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
     float weight_grad[kVectors][8];
 #pragma unroll
@@ -203,14 +224,14 @@ __global__ __launch_bounds__(kThreads<kLanes>) void backward_kernel(Args args) {
         for (int i = 0; i < 8; ++i) weight_grad[v][i] = 0.f;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group; row < args.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
         const int64_t start = row * args.columns;
-        Eight<T> stream[kVectors], grad[kVectors], grad_stream[kVectors];
+        Eight<T> stream[kVectors], grad[kVectors], grad_stream[kEarly ? kVectors : 1];
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int column = (v * kLanes + lane) * 8;
             const bool exists = column < args.columns;
             stream[v] = exists ? load_eight<T>(args.stream, start + column) : zeros<T>();
             grad[v] = exists ? load_eight<T>(args.grad_normalized, start + column) : zeros<T>();
-            grad_stream[v] = exists && args.grad_stream != nullptr ? load_eight<T>(args.grad_stream, start + column) : zeros<T>();
+            if constexpr (kEarly) grad_stream[v] = exists && args.grad_stream != nullptr ? load_eight<T>(args.grad_stream, start + column) : zeros<T>();
         }
         float sums[2] = {0.f, 0.f};  // of s^2 and of g w s
 #pragma unroll
@@ -233,10 +254,11 @@ __global__ __launch_bounds__(kThreads<kLanes>) void backward_kernel(Args args) {
             if (column >= args.columns) continue;
             float weight[8];
             load_weight<T>(args, column, weight);
+            if constexpr (!kEarly) grad_stream[0] = args.grad_stream != nullptr ? load_eight<T>(args.grad_stream, start + column) : zeros<T>();
             Eight<T> result;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                result.set(i, inverse * (grad[v][i] * weight[i] - stream[v][i] * factor) + grad_stream[v][i]);
+                result.set(i, inverse * (grad[v][i] * weight[i] - stream[v][i] * factor) + grad_stream[kEarly ? v : 0][i]);
                 weight_grad[v][i] += grad[v][i] * (stream[v][i] * inverse);
             }
             store_eight(args.grad_input, start + column, result);

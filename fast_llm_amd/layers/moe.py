@@ -8,12 +8,23 @@ Weight layout as in the reference: `layer_1.weight` [experts * 2 * ffn, hidden] 
 [gate; up] (layers/decoder/mlp/mlp.py:81-87), `layer_2.weight` [experts * ffn, hidden] (stored transposed, :70-79).
 """
 
+import copy
+
 import torch
 
 from fast_llm_amd.functional.config import ActivationType, MLPRecomputeLevel
+from fast_llm_amd.functional.microscaling import (
+    MicroscaledTensor,
+    MicroscalingFormat,
+    mx_mlp,
+    mx_quantize,
+    mx_quantize_expert_weights,
+)
 from fast_llm_amd.functional.mlp import few_tokens_expected, few_tokens_forward, few_tokens_workspace_size, mlp_autograd
 from fast_llm_amd.functional.moe_layer import MoELayerOptions, moe_layer, moe_layer_supported
+from fast_llm_amd.functional.normalization import rms_norm_quantize
 from fast_llm_amd.functional.sparse_copy import get_sparse_map
+from fast_llm_amd.layers.normalization import RMSNorm
 
 
 def attach_grad_buffer(weight: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -261,6 +272,10 @@ class DroplessMoEMLP(torch.nn.Module):
                 losses.setdefault(ROUTER_Z_LOSS, []).append(loss_values[1])
         return output
 
+    def _copy_without_experts(self) -> "DroplessMoEMLP":
+        """A copy in inference mode that routes like this layer and has no experts to run."""
+        return copy.deepcopy(self, {id(self.layer_1): None, id(self.layer_2): None}).eval()
+
     # ---- Hugging Face Mixtral layout ----------------------------------------------------------------------
     # The reference's Mixtral converter (fast_llm/models/gpt/conversion/mixtral.py:65-82) maps, per block,
     #   router.weight  <- block_sparse_moe.gate.weight                                   [experts, hidden]
@@ -299,3 +314,81 @@ class DroplessMoEMLP(torch.nn.Module):
             out[f"{prefix}experts.{i}.w3.weight"] = up.clone()
             out[f"{prefix}experts.{i}.w2.weight"] = down.t().contiguous()
         return out
+
+
+class MicroscaledMoEMLP(torch.nn.Module):
+    """
+    `DroplessMoEMLP` for inference with its expert weights in microscaled 4 bits (0.53 bytes per weight instead of 2) and its
+    activations in `format`. Routing, router and scores are the layer's own, on the unquantised input. With a `normalization` it
+    takes the norm in front of the layer with it: `forward(input_, residual)` adds the residual, normalises, routes, quantises
+    and runs the experts, and returns (output, stream), the stream being what the output is added to.
+    """
+
+    def __init__(
+        self,
+        layer: DroplessMoEMLP,
+        normalization: RMSNorm | None = None,
+        *,
+        format: MicroscalingFormat | str = MicroscalingFormat.e4m3,
+    ):
+        super().__init__()
+        self.format = MicroscalingFormat(format)
+        self.experts, self.experts_per_token, self.shared_experts = layer.experts, layer.experts_per_token, layer.shared_experts
+        self.hidden_size, self.intermediate_size = layer.layer_2.size(1), layer.layer_2.size(0) // layer.experts
+        self.gated, self.activation = layer.gated, layer.activation
+        self.normalization = normalization
+        self.router = layer._copy_without_experts()
+        for name, weight in zip(
+            ("layer_1", "layer_2"), mx_quantize_expert_weights(layer.layer_1, layer.layer_2, layer.experts)
+        ):
+            self.register_buffer(f"{name}_values", weight.values)
+            self.register_buffer(f"{name}_scales", weight.scales)
+        self.eval()
+
+    def train(self, mode: bool = True) -> "MicroscaledMoEMLP":
+        if mode:
+            raise RuntimeError("quantised expert weights are for inference: they have no gradient")
+        return super().train(mode)
+
+    @property
+    def layer_1(self) -> MicroscaledTensor:
+        return MicroscaledTensor(self.layer_1_values, self.layer_1_scales, self.hidden_size, MicroscalingFormat.e2m1)
+
+    @property
+    def layer_2(self) -> MicroscaledTensor:
+        return MicroscaledTensor(self.layer_2_values, self.layer_2_scales, self.intermediate_size, MicroscalingFormat.e2m1)
+
+    @torch.no_grad()
+    def forward(
+        self,
+        input_: torch.Tensor,
+        residual: torch.Tensor | None = None,
+        scores: torch.Tensor | None = None,
+        top_experts: torch.Tensor | None = None,
+    ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+        """`scores`/`top_experts` may be passed to bypass the router."""
+        hidden_states, stream, router_counts = input_.flatten(0, -2), None, None
+        if self.normalization is not None:
+            norm = self.normalization
+            if residual is not None:
+                residual = residual.flatten(0, -2)
+            hidden_states, stream, rows = rms_norm_quantize(hidden_states, norm.weight, residual, norm.eps, self.format)
+        elif residual is not None:
+            raise ValueError("the residual is added in front of the norm, which this layer does not have")
+        else:
+            rows = mx_quantize(hidden_states, self.format)
+        if top_experts is None:
+            scores, top_experts, router_counts = self.router.route_with_counts(hidden_states)
+        output = mx_mlp(
+            rows,
+            scores,
+            top_experts,
+            self.layer_1,
+            self.layer_2,
+            self.experts,
+            gated=self.gated,
+            activation_type=self.activation,
+            dtype=input_.dtype,
+            router_counts=router_counts,
+        ).view_as(input_)
+        return output if stream is None else (output, stream.view_as(input_))
