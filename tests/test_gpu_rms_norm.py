@@ -136,7 +136,7 @@ def test_gradients_that_are_not_asked_for_or_do_not_come(device):
     assert torch.equal(twice, parts[0] + parts[1])
     with pytest.raises(RuntimeError, match="once_differentiable"):
         leaf, grad = x.detach().requires_grad_(True), grads[0].detach().requires_grad_(True)
-        torch.autograd.grad(torch.autograd.grad(rms_norm(leaf, weight), leaf, grad, create_graph=True)[0].sum(), grad)
+        torch.autograd.grad(rms_norm(leaf, weight), leaf, grad, create_graph=True)[0].sum().backward()
 
 
 def test_shapes_strides_and_rows_that_are_special(device):
