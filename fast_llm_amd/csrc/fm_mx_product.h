@@ -21,7 +21,7 @@ struct ProductArgs {
     int64_t experts;
     int format;  // of x, and of a microscaled result
     int gated, activation;
-    int out_vectors;  // groups of four columns of `out` are aligned to their size
+    int out_vectors;  // rows of `out` are aligned to 16 bytes
     // Rows by a sparse map ...
     const void *expert_ends, *expert_pad_begins;
     int index_dtype;

@@ -58,7 +58,7 @@ extern "C" int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, cons
     args.x_rows = args.rows = rows, args.x_stride = lhs_stride, args.x_scale_stride = lhs_scale_stride;
     args.weight_stride = rhs_stride, args.weight_scale_stride = rhs_scale_stride, args.out_stride = out_stride;
     args.columns = args.out_columns = columns, args.inner = padded, args.experts = num_experts, args.format = format;
-    args.out_vectors = reinterpret_cast<uintptr_t>(out) % (4 * size) == 0 && out_stride % 4 == 0;
+    args.out_vectors = aligned16(out) && out_stride * size % 16 == 0;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
     if (int status = run(args, out_dtype, stream)) return status;
     return check_launch(name);

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kWaves * 64) void stream_kernel(ProductArgs args) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = 8 * i + (lane >> 3);
-                    *(FM_LDS(u32x4_t) *)(chunk_lds + s * kSetBytes + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) = chunk.weight[s][i];
+                    *(FM_LDS(u32x4_t) *)(chunk_lds + s * kSetBytes + row * 128 + (((lane & 7) ^ ((row >> 1) & 7)) << 4)) = chunk.weight[s][i];
                 }
             const bool second = c * kChunk + 128 < inner;
 #pragma unroll
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kWaves * 64) void stream_kernel(ProductArgs args) {
 #pragma unroll
                 for (int s = 0; s < kSets; ++s) {
                     const int row = lane & 31;
-                    const u32x4_t fragment = *(FM_LDS(u32x4_t) *)(chunk_lds + s * kSetBytes + row * 128 + (((2 * i + half) ^ (row & 7)) << 4));
+                    const u32x4_t fragment = *(FM_LDS(u32x4_t) *)(chunk_lds + s * kSetBytes + row * 128 + (((2 * i + half) ^ ((row >> 1) & 7)) << 4));
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g)
                         sums[s][g] = multiply<kFormat, i % 2 * 2, i % 2 * 2>(fragment, chunk.x[g][i], chunk.weight_scales[s][i / 2], chunk.x_scales[g][i / 2], sums[s][g]);

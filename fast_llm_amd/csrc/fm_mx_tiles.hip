@@ -1,12 +1,14 @@
 // Products of many microscaled rows per expert with e2m1 expert weights, on tiles of 256 rows x 256 weight rows.
 //
-// Eight wavefronts, two per SIMD, multiply 64 rows x 128 weight rows each (2 x 4 blocks of v_mfma_scale_f32_32x32x64_f8f6f4; D's rows are weight rows, so
-// that a lane has four neighbouring columns of one row). K passes in slices of 128 through three LDS slots: a slice's bytes go straight
-// from memory into LDS, two slices ahead of the multiplications; one barrier a slice. Scales, 16 bytes of a row at a time, take the
-// same way every fourth slice.
+// One workgroup per CU walks over its tiles. Its four wavefronts, one per SIMD, multiply 128 rows x 128 weight rows each (4 x 4 blocks of
+// v_mfma_scale_f32_32x32x64_f8f6f4; D's rows are weight rows, so that a lane has neighbouring columns of one row). K passes in slices of 128
+// through three LDS slots. A slice's bytes go straight from memory into LDS, up to three slices ahead of the multiplications and on into the
+// next tile; the fragments of a step of 64 are read while the step before is multiplied. What a slice needs of memory instructions is spread over its
+// MFMAs in a fixed order. Scales, 16 bytes of a row for four slices, take the same way.
 //
-// A row's slice is 128 bytes (e4m3) or 64 (e2m1), in LDS XOR-swizzled in units of 16 bytes so that eight lanes that read the same unit of
-// neighbouring rows hit all banks.
+// A row's slice is 128 bytes (e4m3) or 64 (e2m1), in LDS XOR-swizzled in units of 16 bytes so that 16 lanes that read the same unit of
+// neighbouring rows hit all 64 banks. Of every 32 weight rows, LDS row 8 a + 4 h + b holds row 16 h + 4 a + b: a lane (h: its half of the
+// wavefront) then has 16 neighbouring columns of its row, and results leave without a way through LDS, which is full of the next tile's slices.
 #include "fm_activation_math.h"
 #include "fm_mx_product.h"
 
@@ -16,8 +18,8 @@ namespace mx {
 
 namespace tiles {
 
-constexpr int kTile = 256, kSlice = 128, kSlots = 3, kThreads = 512, kWaves = 8;
-constexpr int kBlocksN = 4, kBlocksM = 2;
+constexpr int kTile = 256, kSlice = 128, kSlots = 3, kThreads = 256, kWaves = 4;
+constexpr int kBlocks = 4;  // of 32, per wavefront and axis
 constexpr int kWeightBytes = kTile * kSlice / 2, kScaleBytes = 2 * kTile * 16;
 template <int kFormat>
 constexpr int kRowBytes = kFormat == FM_MX_E4M3 ? kSlice : kSlice / 2;
@@ -30,14 +32,34 @@ static_assert(kLdsBytes<FM_MX_E4M3> <= 160 * 1024, "LDS of a CU");
 constexpr uint32_t kOutOfRange = 0x80000000u, kRange = 0x7fffffffu;
 constexpr int kResident = 256;  // workgroups: one per CU
 
-// 16 bytes of each lane -> LDS at `target` + 16 * lane; zeros for offsets out of range.
-__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t offset, int target) {
-    const __amdgpu_buffer_rsrc_t resource = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char *>(uniform_pointer(reinterpret_cast<const char *>(base))), 0, static_cast<int>(kRange), kBufferResourceFlags);
-    // M0 is not handed out by the register allocator and nothing else in this file uses it.
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+template <int kFirst, int kLast, typename F>
+__device__ __forceinline__ void for_each(const F &f) {
+    if constexpr (kFirst < kLast) {
+        f(std::integral_constant<int, kFirst>{});
+        for_each<kFirst + 1, kLast>(f);
+    }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(uniform_pointer(reinterpret_cast<const char *>(base))), 0, static_cast<int>(kRange),
+                                             kBufferResourceFlags);
+}
+
+// 16 bytes of each lane -> LDS at `target` + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and nothing
+// else in this file uses it.)
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
-                 : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource)
+                 : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position))
+                 : "memory");
+}
+
+// The same where `lanes` is ~0, and nothing where it is 0: without a branch, past which the compiler would move what is around it.
+__device__ __forceinline__ void load_to_lds_if(uint32_t lanes, __amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b64 exec, -1"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position)),
+                   "s"(__builtin_amdgcn_readfirstlane(lanes))
                  : "memory");
 }
 
@@ -47,143 +69,301 @@ __device__ __forceinline__ void wait_for_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kNewest) : "memory");
 }
 
-// Where unit `u` of 16 bytes of row `row` is in a slot's rows of kUnits units.
-template <int kUnits>
-__device__ __forceinline__ int unit_address(int row, int u) {
-    return kUnits == 8 ? row * 128 + ((u ^ (row & 7)) << 4) : row * 64 + ((u ^ ((row >> 1) & 3)) << 4);
-}
+__device__ __forceinline__ u32x4_t read_lds(int address, int offset) { return *(FM_LDS(u32x4_t) *)static_cast<uintptr_t>(address + offset); }
 
-__device__ __forceinline__ u32x4_t read_lds(int address) { return *(FM_LDS(u32x4_t) *)static_cast<uintptr_t>(address); }
+// Which tile: as `locate_tile`, with the experts' rows in registers, two experts per lane.
+constexpr int kMaxInRegisters = 128;
+struct Experts {
+    int begin[2], count[2], last[2];  // first row, row tiles, row tiles up to and with this expert's
+    int end[2];
+    int before[3];  // row tiles in front of each 64 experts, and of all
+
+    __device__ __forceinline__ void load(const GemmArgs &args, int lane) {
+        before[0] = 0;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const int e = part * 64 + lane;
+            int64_t first = 0, past = 0;
+            if (e < args.num_experts) rows_of_expert(args, e, first, past);
+            count[part] = first >= 0 && past > first ? static_cast<int>((past - first + kTile - 1) / kTile) : 0;
+            begin[part] = static_cast<int>(first), end[part] = static_cast<int>(past);
+            int sum = count[part];
+#pragma unroll
+            for (int offset = 1; offset < 64; offset <<= 1) {
+                const int other = __shfl_up(sum, offset, 64);
+                if (lane >= offset) sum += other;
+            }
+            last[part] = sum + before[part];
+            before[part + 1] = __builtin_amdgcn_readlane(last[part], 63);
+        }
+    }
+    __device__ __forceinline__ bool locate(const GemmArgs &args, int logical, RowTile &tile) const {
+        if (args.num_experts > kMaxInRegisters) {
+            // The same in all lanes, which the compiler cannot know.
+            RowTile found{};
+            const bool exists = locate_tile<kTile>(args, logical, found);
+            tile.expert = __builtin_amdgcn_readfirstlane(found.expert), tile.tile_n = __builtin_amdgcn_readfirstlane(found.tile_n);
+            tile.rows_valid = __builtin_amdgcn_readfirstlane(found.rows_valid);
+            tile.row0 = __builtin_amdgcn_readfirstlane(static_cast<int>(found.row0));  // rows are counted in 31 bits
+            return __builtin_amdgcn_readfirstlane(static_cast<int>(exists)) != 0;
+        }
+        if (logical >= before[2] * args.tiles_n) return false;
+        const int part = logical >= before[1] * args.tiles_n;
+        const int lasts = part ? last[1] : last[0], counts = part ? count[1] : count[0];
+        const uint64_t owners = __ballot(lasts * args.tiles_n > logical);
+        const int owner = __ffsll(static_cast<unsigned long long>(owners)) - 1;
+        const int owner_count = __builtin_amdgcn_readlane(counts, owner), owner_last = __builtin_amdgcn_readlane(lasts, owner);
+        const int first = __builtin_amdgcn_readlane(part ? begin[1] : begin[0], owner), past = __builtin_amdgcn_readlane(part ? end[1] : end[0], owner);
+        int row_tile;
+        place_in_expert(logical - (owner_last - owner_count) * args.tiles_n, owner_count, args.tiles_n, row_tile, tile.tile_n);
+        tile.expert = part * 64 + owner;
+        tile.row0 = first + row_tile * kTile;
+        tile.rows_valid = min(kTile, past - static_cast<int>(tile.row0));
+        return true;
+    }
+};
 
 template <int kFormat, bool kGated, typename Result>
 __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, GemmArgs placement) {
     constexpr bool kQuantized = std::is_same<Result, uint8_t>::value;
     constexpr int kUnits = kRowBytes<kFormat> / 16, kXBytes = kTile * kRowBytes<kFormat>;
     constexpr int kXLoads = kXBytes / 1024 / kWaves, kWeightLoads = kWeightBytes / 1024 / kWaves, kLoads = kXLoads + kWeightLoads;
+    constexpr int kScaleLoads = kScaleBytes / 1024 / kWaves;
     constexpr int kParts = kFormat == FM_MX_E4M3 ? 2 : 1;
+    constexpr int kColumns = kGated ? kTile / 2 : kTile;  // of the result
     extern __shared__ __attribute__((aligned(1024))) char lds_generic[];
     const int lds = static_cast<int>(reinterpret_cast<uintptr_t>((FM_LDS(char) *)lds_generic));
     const int scales_at = lds + kSlots * kSlotBytes<kFormat>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int wave_n = wave & 1, wave_m = wave >> 1;
     const int slices = static_cast<int>(args.inner) / kSlice, columns = static_cast<int>(args.columns);
-    constexpr int kColumns = kGated ? kTile / 2 : kTile;  // of the result
 
     // The 32 workgroups of an XCD take consecutive tiles.
     int logical = (blockIdx.x % 8) * (kResident / 8) + blockIdx.x / 8;
-    RowTile tile;
-    for (; locate_tile<kTile>(placement, logical, tile); logical += kResident) {
-        const int expert = __builtin_amdgcn_readfirstlane(tile.expert), rows_valid = __builtin_amdgcn_readfirstlane(tile.rows_valid);
-        const int col0 = __builtin_amdgcn_readfirstlane(tile.tile_n) * kColumns;
-        const int64_t row0 = tile.row0;
-        const uint8_t *x = args.x + row0 * args.x_stride;
-        const int64_t weight_row = static_cast<int64_t>(expert) * columns * (kGated ? 2 : 1) + col0;
-        const uint8_t *weight = args.weight + weight_row * args.weight_stride;
+    Experts experts;
+    experts.load(placement, lane);
+    RowTile tile, upcoming;
+    if (!experts.locate(placement, logical, upcoming)) return;
 
-        uint32_t x_offset[kXLoads], weight_offset[kWeightLoads], scale_offset;
-        // Row `t` of the tile's weight rows, from the tile's first; -1: there is none. (Gated: 64 gates and their ups by turns.)
+    // ---- loading: the slices of the workgroup's tiles one after the other, the last tile's followed by zeros -----------
+    __amdgpu_buffer_rsrc_t x_buffer, weight_buffer, scale_buffer;
+    uint32_t x_offset[kXLoads], weight_offset[kWeightLoads], scale_offset[kScaleLoads];
+    int load_slice = 0, load_slot = lds, load_group = 0, load_scales = scales_at;
+    int x_position = 0, weight_position = 0, target = 0, scale_position = 0, scale_target = 0;
+    uint32_t scale_lanes = 0;
+    const uint8_t *scale_base;
+    bool more = true;
+    // `upcoming` is the tile that is loaded from here on.
+    const auto set_up = [&]() {
+        const int rows_valid = more ? upcoming.rows_valid : 0, col0 = upcoming.tile_n * kColumns, columns_valid = more ? columns - col0 : 0;
+        const int64_t weight_row = static_cast<int64_t>(upcoming.expert) * columns * (kGated ? 2 : 1) + col0;
+        x_buffer = buffer_of(args.x + upcoming.row0 * args.x_stride);
+        weight_buffer = buffer_of(args.weight + weight_row * args.weight_stride);
+        // Row of LDS row `t` from the tile's first weight row; -1: there is none. Gated: a wavefront's 64 gates, then their ups.
         const auto weight_row_of = [&](int t) {
-            const int column = kGated ? t / 128 * 64 + t % 64 : t;
-            return col0 + column >= columns ? -1 : kGated && t % 128 >= 64 ? column + columns : column;
+            const int in_block = (t >> 2 & 1) * 16 + (t >> 3 & 3) * 4 + (t & 3), block = t / 32;
+            const int column = (kGated ? block / 4 * 64 + block % 2 * 32 : block * 32) + in_block;
+            return column >= columns_valid ? -1 : kGated && block % 4 >= 2 ? column + columns : column;
         };
 #pragma unroll
         for (int j = 0; j < kXLoads; ++j) {
-            const int slot = (wave * kXLoads + j) * 64 + lane, row = slot / kUnits, at = slot % kUnits;
-            const int unit = kUnits == 8 ? at ^ (row & 7) : at ^ ((row >> 1) & 3);
-            x_offset[j] = row < rows_valid ? static_cast<uint32_t>(row * args.x_stride + unit * 16) : kOutOfRange;
+            const int at = (wave * kXLoads + j) * 64 + lane, row = at / kUnits;
+            const int unit = kUnits == 8 ? at % 8 ^ ((row >> 1) & 7) : at % 4 ^ ((row >> 2) & 3);
+            x_offset[j] = row < rows_valid ? static_cast<uint32_t>(row * static_cast<int>(args.x_stride) + unit * 16) : kOutOfRange;
         }
 #pragma unroll
         for (int j = 0; j < kWeightLoads; ++j) {
-            const int slot = (wave * kWeightLoads + j) * 64 + lane, t = slot / 4, unit = slot % 4 ^ ((t >> 1) & 3), row = weight_row_of(t);
-            weight_offset[j] = row >= 0 ? static_cast<uint32_t>(row * args.weight_stride + unit * 16) : kOutOfRange;
+            const int at = (wave * kWeightLoads + j) * 64 + lane, t = at / 4, unit = at % 4 ^ ((t >> 2) & 3), row = weight_row_of(t);
+            weight_offset[j] = row >= 0 ? static_cast<uint32_t>(row * static_cast<int>(args.weight_stride) + unit * 16) : kOutOfRange;
         }
-        // The lower wavefronts load the scales of 64 rows each, the upper ones those of the weight rows.
-        const uint8_t *scales = wave < 4 ? args.x_scales + row0 * args.x_scale_stride : args.weight_scales + weight_row * args.weight_scale_stride;
-        if (wave < 4) {
-            const int row = wave * 64 + lane;
-            scale_offset = row < rows_valid ? static_cast<uint32_t>(row * args.x_scale_stride) : kOutOfRange;
+        // The lower wavefronts load the scales of the rows, the upper ones those of the weight rows.
+        const bool of_rows = wave < kWaves / 2;
+        scale_base = (of_rows ? args.x_scales + upcoming.row0 * args.x_scale_stride : args.weight_scales + weight_row * args.weight_scale_stride);
+#pragma unroll
+        for (int j = 0; j < kScaleLoads; ++j) {
+            const int t = (wave * kScaleLoads + j) * 64 + lane, row = of_rows ? t < rows_valid ? t : -1 : weight_row_of(t - kTile);
+            scale_offset[j] = row >= 0 ? static_cast<uint32_t>(row * static_cast<int>(of_rows ? args.x_scale_stride : args.weight_scale_stride)) : kOutOfRange;
+        }
+    };
+    // The scales of four slices come together; the last slices of a tile are in groups of two at least, so that a group is not overwritten
+    // before it has been read. A group's 16 bytes end with the row.
+    const auto next_group = [&](int first) { return first + 4 - (slices - first - 4 == 1); };
+    const auto first_scales = [&](int first) { return min(first, slices - 4); };
+    const auto begin_slice = [&]() {
+        if (load_slice == slices) {
+            logical += kResident;
+            more = more && experts.locate(placement, logical, upcoming);
+            set_up();
+            load_slice = load_group = 0;
+        }
+        const bool begins_group = load_slice == load_group;
+        scale_lanes = begins_group ? ~0u : 0;
+        scale_buffer = buffer_of(scale_base);
+        scale_position = first_scales(load_group) * 4;
+        scale_target = load_scales + wave * kScaleLoads * 1024;
+        if (begins_group) load_group = next_group(load_group), load_scales = load_scales == scales_at ? scales_at + kScaleBytes : scales_at;
+        x_position = load_slice * kRowBytes<kFormat>, weight_position = load_slice * (kSlice / 2);
+        target = load_slot;
+        load_slot = load_slot == lds + (kSlots - 1) * kSlotBytes<kFormat> ? lds : load_slot + kSlotBytes<kFormat>;
+        ++load_slice;
+    };
+    // The loads of a slice by number: those of scales, of rows, of weights. The last kLate of them are issued a step after the others, when
+    // the state above may be that of the slice after it, and the next tile's.
+    constexpr int kAllLoads = kScaleLoads + kLoads, kLate = kLoads / 2, kEarly = kAllLoads - kLate;
+    static_assert(kLate >= kWeightLoads && kLate - kWeightLoads <= kXLoads, "late are all of the weights and some rows");
+    constexpr int kLateRows = kLate - kWeightLoads;
+    __amdgpu_buffer_rsrc_t late_x_buffer, late_weight_buffer;
+    uint32_t late_offset[kLate];
+    int late_x_position = 0, late_weight_position = 0, late_target = 0;
+    const auto keep_late = [&]() {
+        late_x_buffer = x_buffer, late_weight_buffer = weight_buffer;
+        late_x_position = x_position, late_weight_position = weight_position, late_target = target;
+#pragma unroll
+        for (int j = 0; j < kLate; ++j) late_offset[j] = j < kLateRows ? x_offset[kXLoads - kLateRows + j] : weight_offset[j - kLateRows];
+    };
+    const auto load_early = [&](auto constant) {
+        constexpr int j = decltype(constant)::value, at = j - kScaleLoads;
+        if constexpr (j < kScaleLoads) load_to_lds_if(scale_lanes, scale_buffer, scale_offset[j], scale_position, scale_target + j * 1024);
+        else load_to_lds(x_buffer, x_offset[at], x_position, target + (wave * kXLoads + at) * 1024);
+    };
+    const auto load_late = [&](auto constant) {
+        constexpr int j = decltype(constant)::value;
+        if constexpr (j < kLateRows) load_to_lds(late_x_buffer, late_offset[j], late_x_position, late_target + (wave * kXLoads + kXLoads - kLateRows + j) * 1024);
+        else load_to_lds(late_weight_buffer, late_offset[j], late_weight_position, late_target + kXBytes + (wave * kWeightLoads + j - kLateRows) * 1024);
+    };
+
+    // ---- multiplying ---------------------------------------------------------------------------------------------------
+    u32x4_t weight_part[2][kBlocks], x_part[2][kBlocks][kParts];
+    uint32_t weight_scales[kBlocks], x_scales[kBlocks], next_weight_scales[kBlocks], next_x_scales[kBlocks];
+    // Lane addresses in a slot, one per unit of a slice; blocks, slots and the wavefront's rows are added.
+    int x_address[2][kParts], weight_address[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = lane & 31;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+            const int unit = kParts == 2 ? 4 * i + 2 * p + half : 2 * i + half;
+            x_address[i][p] = row * kRowBytes<kFormat> + (kUnits == 8 ? unit ^ ((row >> 1) & 7) : unit ^ ((row >> 2) & 3)) * 16;
+        }
+        weight_address[i] = kXBytes + wave_n * 128 * (kSlice / 2) + row * (kSlice / 2) + ((2 * i + half) ^ ((row >> 2) & 3)) * 16;
+    }
+    // Rows of a wavefront: as many blocks of 32 for both halves of the workgroup as the tile's rows need.
+    const auto blocks_of = [&](const RowTile &of) { return of.rows_valid <= kTile / 2 ? kBlocks / 2 : kBlocks; };
+    int slot = lds, group = 0, group_scales = scales_at;  // of the slice that is read
+    int first_row = wave_m * blocks_of(upcoming) * 32;    // of the wavefront, in the tile that is read
+    // Reads by number: of a step's fragments, and after those, with the first step of a slice, of its scales.
+    const auto read = [&](auto constant, auto step_constant, int scale_word) {
+        constexpr int item = decltype(constant)::value, i = decltype(step_constant)::value;
+        if constexpr (item < kBlocks) {
+            weight_part[i][item] = read_lds(weight_address[i] + slot, item * 32 * (kSlice / 2));
+        } else if constexpr (item < kBlocks * (1 + kParts)) {
+            constexpr int m = (item - kBlocks) / kParts, p = (item - kBlocks) % kParts;
+            x_part[i][m][p] = read_lds(x_address[i][p] + slot + first_row * kRowBytes<kFormat>, m * 32 * kRowBytes<kFormat>);
+        } else if constexpr (item < kBlocks * (2 + kParts)) {
+            constexpr int n = item - kBlocks * (1 + kParts);
+            next_weight_scales[n] = *(FM_LDS(uint32_t) *)static_cast<uintptr_t>(scale_word + (kTile + wave_n * 128 + (lane & 31)) * 16 + n * 512);
         } else {
-            const int row = weight_row_of((wave - 4) * 64 + lane);
-            scale_offset = row >= 0 ? static_cast<uint32_t>(row * args.weight_scale_stride) : kOutOfRange;
+            constexpr int m = item - kBlocks * (2 + kParts);
+            next_x_scales[m] = *(FM_LDS(uint32_t) *)static_cast<uintptr_t>(scale_word + (first_row + (lane & 31)) * 16 + m * 512);
         }
-        // The first of the four slices whose scales are loaded together with those of slice 4 group: the row's last ones end with it.
-        const auto first_of_group = [&](int group) { return min(group * 4, slices - 4); };
-        const auto fetch_scales = [&](int group) {
-            const bool exists = group * 4 < slices;
-            load_to_lds(scales + first_of_group(group) * 4, exists ? scale_offset : kOutOfRange, scales_at + (group & 1) * kScaleBytes + wave * 1024);
-        };
-        const auto fetch = [&](int s, int slot) {
-            const bool exists = s < slices;
-            const int target = lds + slot * kSlotBytes<kFormat>;
+    };
+    constexpr int kReads = kBlocks * (1 + kParts), kScaleReads = 2 * kBlocks;
+    const auto take_scales = [&]() {  // byte 2 i of the word is then that of the lane's block in step i
 #pragma unroll
-            for (int j = 0; j < kXLoads; ++j)
-                load_to_lds(x + static_cast<int64_t>(s) * kRowBytes<kFormat>, exists ? x_offset[j] : kOutOfRange, target + (wave * kXLoads + j) * 1024);
-#pragma unroll
-            for (int j = 0; j < kWeightLoads; ++j)
-                load_to_lds(weight + static_cast<int64_t>(s) * (kSlice / 2), exists ? weight_offset[j] : kOutOfRange,
-                            target + kXBytes + (wave * kWeightLoads + j) * 1024);
-        };
+        for (int n = 0; n < kBlocks; ++n) weight_scales[n] = next_weight_scales[n] >> (8 * half), x_scales[n] = next_x_scales[n] >> (8 * half);
+    };
 
-        f32x16_t acc[kBlocksN][kBlocksM];
-#pragma unroll
-        for (int n = 0; n < kBlocksN; ++n)
-#pragma unroll
-            for (int m = 0; m < kBlocksM; ++m) acc[n][m] = f32x16_t{};
-        fetch_scales(0);
-        fetch(0, 0);
-        fetch(1, 1);
-        const bool multiplies = wave_m * 64 < rows_valid;
-        int slot = 0;
+    set_up();
 #pragma unroll 1
-        for (int s = 0; s < slices; ++s) {
-            // Slice s is there, and slice s - 1 has been read: its slot takes slice s + 2.
-            wait_for_loads<kLoads>();
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (s % 4 == 0) fetch_scales(s / 4 + 1);
-            fetch(s + 2, slot == 0 ? 2 : slot - 1);
-            if (multiplies) {
-                const int x_at = lds + slot * kSlotBytes<kFormat>, weight_at = x_at + kXBytes;
-                const int scale_word = scales_at + (s / 4 & 1) * kScaleBytes + (s - first_of_group(s / 4)) * 4;
-                uint32_t x_scales[kBlocksM], weight_scales[kBlocksN];
-#pragma unroll
-                for (int m = 0; m < kBlocksM; ++m)
-                    x_scales[m] = *(FM_LDS(uint32_t) *)static_cast<uintptr_t>(scale_word + (wave_m * 64 + m * 32 + (lane & 31)) * 16) >> (8 * half);
-#pragma unroll
-                for (int n = 0; n < kBlocksN; ++n)
-                    weight_scales[n] = *(FM_LDS(uint32_t) *)static_cast<uintptr_t>(scale_word + (kTile + wave_n * 128 + n * 32 + (lane & 31)) * 16) >> (8 * half);
-                const auto step = [&](auto constant) {
-                    constexpr int i = decltype(constant)::value;
-                    u32x4_t a[kBlocksN], b[kBlocksM][kParts];
-#pragma unroll
-                    for (int m = 0; m < kBlocksM; ++m)
-#pragma unroll
-                        for (int p = 0; p < kParts; ++p)
-                            b[m][p] = read_lds(x_at + unit_address<kUnits>(wave_m * 64 + m * 32 + (lane & 31), (kFormat == FM_MX_E4M3 ? 4 * i + 2 * p : 2 * i) + half));
-#pragma unroll
-                    for (int n = 0; n < kBlocksN; ++n) a[n] = read_lds(weight_at + unit_address<4>(wave_n * 128 + n * 32 + (lane & 31), 2 * i + half));
-#pragma unroll
-                    for (int n = 0; n < kBlocksN; ++n)
-#pragma unroll
-                        for (int m = 0; m < kBlocksM; ++m)
-                            acc[n][m] = multiply<kFormat, 2 * i, 2 * i>(a[n], b[m], weight_scales[n], x_scales[m], acc[n][m]);
-                };
-                step(std::integral_constant<int, 0>{});
-                step(std::integral_constant<int, 1>{});
-            }
-            slot = slot == 2 ? 0 : slot + 1;
-        }
-        wait_for_loads<0>();  // zeros of slices past the end
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+    for (int s = 0; s < kSlots; ++s) {
+        if (s > 0) for_each<0, kLate>(load_late);
+        begin_slice();
+        for_each<0, kEarly>(load_early);
+        keep_late();
+    }
+    wait_for_loads<kLoads + kEarly - kScaleLoads>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    for_each<0, kReads + kScaleReads>([&](auto item) { read(item, std::integral_constant<int, 0>{}, scales_at); });
+    take_scales();
 
+    f32x16_t acc[kBlocks][kBlocks];
+    while (true) {
+        tile = upcoming;
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
+        const auto multiply_tile = [&](auto blocks_constant) {
+            constexpr int kRows = decltype(blocks_constant)::value, kProducts = kBlocks * kRows;
+            const auto product = [&](auto constant, auto step_constant) {
+                // Neighbouring MFMAs share an operand.
+                constexpr int j = decltype(constant)::value, i = decltype(step_constant)::value, n = j / kRows, m = n % 2 ? kRows - 1 - j % kRows : j % kRows;
+                acc[n][m] = multiply<kFormat, 2 * i, 2 * i>(weight_part[i][n], x_part[i][m], weight_scales[n], x_scales[m], acc[n][m]);
+            };
+            constexpr std::integral_constant<int, 0> kFirst{};
+            constexpr std::integral_constant<int, 1> kSecond{};
+            group = 0;
+#pragma unroll 1
+            for (int s = 0; s < slices; ++s) {
+                // The slice that is loaded next, and the one that is read next.
+                keep_late();
+                begin_slice();
+                const int next = s + 1 == slices ? 0 : s + 1;
+                const int next_slot = slot == lds + (kSlots - 1) * kSlotBytes<kFormat> ? lds : slot + kSlotBytes<kFormat>;
+                const bool begins_group = next == 0 || next == next_group(group);
+                group = begins_group ? next : group;
+                group_scales = begins_group ? scales_at + scales_at + kScaleBytes - group_scales : group_scales;
+                const int scale_word = group_scales + (next - first_scales(group)) * 4;
+                __builtin_amdgcn_sched_barrier(0);
+                // First step; beside it the reads of the second, and the rest of the loads of slice s + 2.
+                for_each<0, kProducts>([&](auto j) {
+                    product(j, kFirst);
+                    constexpr int kBusy = kProducts - 2;
+                    if constexpr (j < kBusy) {
+                        for_each<j * kReads / kBusy, (j + 1) * kReads / kBusy>([&](auto item) { read(item, kSecond, 0); });
+                        for_each<j * kLate / kBusy, (j + 1) * kLate / kBusy>(load_late);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                // Second step. Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + 3 takes its slot.
+                product(kFirst, kSecond);
+                __builtin_amdgcn_sched_barrier(0);
+                wait_for_loads<kLoads>();  // all but those of slice s + 2, whose scales were asked for first
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                slot = next_slot;
+                first_row = next == 0 ? wave_m * blocks_of(upcoming) * 32 : first_row;
+                __builtin_amdgcn_sched_barrier(0);
+                for_each<1, kProducts>([&](auto j) {
+                    product(j, kSecond);
+                    constexpr int kItems = kReads + kScaleReads, kBusy = kProducts - 2;
+                    if constexpr (j <= kBusy) {
+                        for_each<(j - 1) * kItems / kBusy, j * kItems / kBusy>([&](auto item) { read(item, kFirst, scale_word); });
+                        for_each<(j - 1) * kEarly / kBusy, j * kEarly / kBusy>(load_early);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                take_scales();
+            }
+        };
+        const int blocks = blocks_of(tile);
+        if (blocks == kBlocks) multiply_tile(std::integral_constant<int, kBlocks>{});
+        else multiply_tile(std::integral_constant<int, kBlocks / 2>{});
+        const bool last_tile = !more;
+
+        // ---- the tile's results: of block (n, m) a lane has columns 16 half .. + 15 of one row ---------------------------
+        const int row_start = wave_m * blocks * 32, col0 = tile.tile_n * kColumns, out_lane = opaque(lane);
         if constexpr (kQuantized) {
             const auto store = [&](auto activate) {
 #pragma unroll
                 for (int n = 0; n < (kGated ? 2 : 4); ++n)
 #pragma unroll
-                    for (int m = 0; m < kBlocksM; ++m) {
-                        // The block of 32 columns of a row is in lanes l and l + 32: quad q of its lane's sums are columns 8 q + 4 half ..
+                    for (int m = 0; m < kBlocks; ++m) {
+                        __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: registers
+                        if (m >= blocks) continue;
                         float values[16];
                         uint32_t largest = 0;
 #pragma unroll
@@ -195,48 +375,49 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                         largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), 32, 64)));
                         const uint32_t byte = scale_byte(kFormat, largest);
                         const float inverse = inverse_scale(byte);
-                        const int row = wave_m * 64 + m * 32 + (lane & 31), column = col0 + wave_n * (kGated ? 64 : 128) + n * 32;
-                        if (row >= rows_valid || column >= args.out_columns) continue;
-                        const int64_t out_row = row0 + row;
-                        uint8_t *target = static_cast<uint8_t *>(args.out) + out_row * args.out_stride;
+                        const int row = row_start + m * 32 + (out_lane & 31), column = col0 + wave_n * (kGated ? 64 : 128) + n * 32;
+                        if (row >= tile.rows_valid || column >= args.out_columns) continue;
+                        const int64_t out_row = tile.row0 + row;
+                        uint8_t *out = static_cast<uint8_t *>(args.out) + out_row * args.out_stride;
+                        uint32_t packed[4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const uint32_t packed = pack_four(kFormat, values[4 * q], values[4 * q + 1], values[4 * q + 2], values[4 * q + 3], inverse);
-                            const int at = column + 8 * q + 4 * half;
-                            if (kFormat == FM_MX_E4M3) *reinterpret_cast<uint32_t *>(target + at) = packed;
-                            else *reinterpret_cast<uint16_t *>(target + at / 2) = static_cast<uint16_t>(packed);
-                        }
-                        if (half == 0) args.out_scales[out_row * args.out_scale_stride + column / 32] = static_cast<uint8_t>(byte);
+                        for (int q = 0; q < 4; ++q) packed[q] = pack_four(kFormat, values[4 * q], values[4 * q + 1], values[4 * q + 2], values[4 * q + 3], inverse);
+                        if (kFormat == FM_MX_E4M3) *reinterpret_cast<u32x4_t *>(out + column + 16 * (out_lane >> 5)) = u32x4_t{packed[0], packed[1], packed[2], packed[3]};
+                        else *reinterpret_cast<u32x2_t *>(out + (column + 16 * (out_lane >> 5)) / 2) = u32x2_t{packed[0] | packed[1] << 16, packed[2] | packed[3] << 16};
+                        if (out_lane < 32) args.out_scales[out_row * args.out_scale_stride + column / 32] = static_cast<uint8_t>(byte);
                     }
             };
             FM_DISPATCH_ACTIVATION(args.activation, kActivation, store([](float value) { return activation_forward<kActivation>(value); }));
         } else {
 #pragma unroll
-            for (int n = 0; n < kBlocksN; ++n)
+            for (int m = 0; m < kBlocks; ++m) {
+                const int row = row_start + m * 32 + (out_lane & 31);
+                if (m >= blocks || row >= tile.rows_valid) continue;
 #pragma unroll
-                for (int m = 0; m < kBlocksM; ++m) {
-                    const int row = wave_m * 64 + m * 32 + (lane & 31);
-                    if (row >= rows_valid) continue;
+                for (int n = 0; n < kBlocks; ++n) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int column = col0 + wave_n * 128 + n * 32 + 16 * (out_lane >> 5);
+                    Result *out = static_cast<Result *>(args.out) + (tile.row0 + row) * args.out_stride + column;
+                    constexpr int N = Vec16<Result>::N;
+                    if (args.out_vectors && column + 15 < columns) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int column = col0 + wave_n * 128 + n * 32 + 8 * q + 4 * half;
-                        Result *target = static_cast<Result *>(args.out) + (row0 + row) * args.out_stride + column;
-                        if (args.out_vectors && column + 3 < columns) {
-                            struct alignas(4 * sizeof(Result)) Four {
-                                Result v[4];
-                            } four;
+                        for (int part = 0; part < 16 / N; ++part) {
+                            Vec16<Result> vector;
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) four.v[c] = from_float<Result>(acc[n][m][4 * q + c]);
-                            *reinterpret_cast<Four *>(target) = four;
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (column + c < columns) target[c] = from_float<Result>(acc[n][m][4 * q + c]);
+                            for (int c = 0; c < N; ++c) vector.v[c] = from_float<Result>(acc[n][m][part * N + c]);
+                            store16(out + part * N, vector);
                         }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (column + c < columns) out[c] = from_float<Result>(acc[n][m][c]);
                     }
                 }
+            }
         }
+        if (last_tile) break;
     }
+    wait_for_loads<0>();  // zeros behind the last tile
 }
 
 template <int kFormat, bool kGated, typename Result>
@@ -262,7 +443,7 @@ static int launch(const ProductArgs &args, hipStream_t stream) {
 
 bool tile_product_takes(const ProductArgs &args) {
     using namespace tiles;
-    // Scales of four slices are loaded at once; offsets from a tile's first row are counted in 31 bits.
+    // Scales of four slices are loaded at once; offsets from a tile's first row are counted in 31 bits, rows and tiles too.
     const int64_t weight_rows = args.gated ? args.columns + kTile : kTile;
     return args.inner >= 4 * kSlice && args.x_stride * kTile < (int64_t(1) << 31) && args.weight_stride * weight_rows < (int64_t(1) << 31) &&
            (args.rows / kTile + args.experts + 1) * ((args.out_columns + 127) / 128) < (int64_t(1) << 30);
