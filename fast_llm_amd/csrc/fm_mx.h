@@ -55,16 +55,16 @@ __device__ __forceinline__ float inverse_scale(uint32_t byte) {
 }
 
 // Four scaled elements of a block, as they are kept: 32 bits of e4m3 or 16 of e2m1. (The conversions round to nearest even; the one to
-// e4m3 makes a NaN of what is over 464, the one to e2m1 saturates.)
+// e4m3 makes a NaN of what is over 464, the one to e2m1 saturates.) Of a block that is not finite, `inverse` 0: zeros.
 __device__ __forceinline__ uint32_t pack_four(int format, float a, float b, float c, float d, float inverse) {
-    const auto scaled = [&](float value) { return inverse == 0.f ? 0.f : value * inverse; };
+    const uint32_t finite = inverse == 0.f ? 0u : ~0u;
     if (format == FM_MX_E4M3) {
-        const auto saturated = [&](float value) { return __builtin_amdgcn_fmed3f(scaled(value), -448.f, 448.f); };
+        const auto saturated = [&](float value) { return __builtin_amdgcn_fmed3f(value * inverse, -448.f, 448.f); };
         const int low = __builtin_amdgcn_cvt_pk_fp8_f32(saturated(a), saturated(b), 0, false);
-        return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(saturated(c), saturated(d), low, true));
+        return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(saturated(c), saturated(d), low, true)) & finite;
     }
-    const uint32_t low = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, scaled(a), scaled(b), 1.f, 0);
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(low, scaled(c), scaled(d), 1.f, 1) & 0xffffu;
+    const uint32_t low = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a * inverse, b * inverse, 1.f, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(low, c * inverse, d * inverse, 1.f, 1) & 0xffffu & finite;
 }
 
 // Eight neighbours per lane, four neighbouring lanes a block: writes the elements (8 or 4 bytes) and, from the block's first lane, the scale.

@@ -2,7 +2,7 @@
 //
 // One workgroup per CU walks over its tiles. Its four wavefronts, one per SIMD, multiply 128 rows x 128 weight rows each (4 x 4 blocks of
 // v_mfma_scale_f32_32x32x64_f8f6f4; D's rows are weight rows, so that a lane has neighbouring columns of one row). K passes in slices of 128
-// through three LDS slots. A slice's bytes go straight from memory into LDS, up to three slices ahead of the multiplications and on into the
+// through three or four LDS slots. A slice's bytes go straight from memory into LDS, as many slices ahead of the multiplications and on into the
 // next tile; the fragments of a step of 64 are read while the step before is multiplied. What a slice needs of memory instructions is spread over its
 // MFMAs in a fixed order. Scales, 16 bytes of a row for four slices, take the same way.
 //
@@ -18,16 +18,21 @@ namespace mx {
 
 namespace tiles {
 
-constexpr int kTile = 256, kSlice = 128, kSlots = 3, kThreads = 256, kWaves = 4;
+constexpr int kTile = 256, kSlice = 128, kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 4;  // of 32, per wavefront and axis
 constexpr int kWeightBytes = kTile * kSlice / 2, kScaleBytes = 2 * kTile * 16;
 template <int kFormat>
 constexpr int kRowBytes = kFormat == FM_MX_E4M3 ? kSlice : kSlice / 2;
 template <int kFormat>
 constexpr int kSlotBytes = kTile * kRowBytes<kFormat> + kWeightBytes;
+// Rows in e2m1 are multiplied in half the time, and a slice is less: one more.
 template <int kFormat>
-constexpr int kLdsBytes = kSlots * kSlotBytes<kFormat> + 2 * kScaleBytes;
-static_assert(kLdsBytes<FM_MX_E4M3> <= 160 * 1024, "LDS of a CU");
+constexpr int kSlots = kFormat == FM_MX_E4M3 ? 3 : 4;
+template <int kFormat>
+constexpr int kScaleSlots = kSlots<kFormat> - 1;
+template <int kFormat>
+constexpr int kLdsBytes = kSlots<kFormat> * kSlotBytes<kFormat> + kScaleSlots<kFormat> * kScaleBytes;
+static_assert(kLdsBytes<FM_MX_E4M3> <= 160 * 1024 && kLdsBytes<FM_MX_E2M1> <= 160 * 1024, "LDS of a CU");
 
 constexpr uint32_t kOutOfRange = 0x80000000u, kRange = 0x7fffffffu;
 constexpr int kResident = 256;  // workgroups: one per CU
@@ -45,22 +50,36 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base)
                                              kBufferResourceFlags);
 }
 
-// 16 bytes of each lane -> LDS at `target` + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and nothing
-// else in this file uses it.)
+// 16 bytes of each lane -> LDS at `target` + kMore + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and
+// nothing else in this file uses it.)
+template <int kMore>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_add_i32 m0, %0, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
-                 : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position))
-                 : "memory");
+                 : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position)), "n"(kMore)
+                 : "memory", "scc");
 }
 
 // The same where `lanes` is ~0, and nothing where it is 0: without a branch, past which the compiler would move what is around it.
+template <int kMore>
 __device__ __forceinline__ void load_to_lds_if(uint32_t lanes, __amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b64 exec, -1"
+    asm volatile("s_add_i32 m0, %0, %5\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b64 exec, -1"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position)),
-                   "s"(__builtin_amdgcn_readfirstlane(lanes))
-                 : "memory");
+                   "s"(__builtin_amdgcn_readfirstlane(lanes)), "n"(kMore)
+                 : "memory", "scc");
+}
+
+// A block of sums, in accumulation registers up to here.
+__device__ __forceinline__ f32x16_t settled(f32x16_t sums) {
+    asm volatile("" : "+a"(sums));
+    return sums;
+}
+
+// The same value, computed no earlier than where this stands.
+__device__ __forceinline__ int here(int value) {
+    asm volatile("" : "+s"(value));
+    return value;
 }
 
 // Returns once at most `kNewest` of the loads this wavefront has issued are on their way, and all that it has asked LDS for is there.
@@ -69,7 +88,10 @@ __device__ __forceinline__ void wait_for_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kNewest) : "memory");
 }
 
-__device__ __forceinline__ u32x4_t read_lds(int address, int offset) { return *(FM_LDS(u32x4_t) *)static_cast<uintptr_t>(address + offset); }
+template <typename T>
+__device__ __forceinline__ T read_lds(int address, int offset) {
+    return *(FM_LDS(T) *)((FM_LDS(char) *)static_cast<uintptr_t>(address) + offset);
+}
 
 // Which tile: as `locate_tile`, with the experts' rows in registers, two experts per lane.
 constexpr int kMaxInRegisters = 128;
@@ -133,6 +155,7 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     constexpr int kColumns = kGated ? kTile / 2 : kTile;  // of the result
     extern __shared__ __attribute__((aligned(1024))) char lds_generic[];
     const int lds = static_cast<int>(reinterpret_cast<uintptr_t>((FM_LDS(char) *)lds_generic));
+    constexpr int kSlots = tiles::kSlots<kFormat>;
     const int scales_at = lds + kSlots * kSlotBytes<kFormat>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int wave_n = wave & 1, wave_m = wave >> 1;
@@ -146,90 +169,100 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     if (!experts.locate(placement, logical, upcoming)) return;
 
     // ---- loading: the slices of the workgroup's tiles one after the other, the last tile's followed by zeros -----------
-    __amdgpu_buffer_rsrc_t x_buffer, weight_buffer, scale_buffer;
-    uint32_t x_offset[kXLoads], weight_offset[kWeightLoads], scale_offset[kScaleLoads];
+    // The loads of a slice are in two parts: those of its scales and most of its rows in the second step after which its slot is free, the others
+    // in the step after that one. Each part has its own registers, so that the next tile's are there when the first part needs them.
+    constexpr int kLate = kLoads / 2, kLateRows = kLate - kWeightLoads, kEarlyRows = kXLoads - kLateRows, kEarly = kScaleLoads + kEarlyRows;
+    static_assert(kLateRows >= 0, "all loads of weights are in the second part");
+    __amdgpu_buffer_rsrc_t x_buffer, scale_buffer, late_x_buffer, late_weight_buffer;
+    uint32_t x_offset[kEarlyRows], scale_offset[kScaleLoads], late_offset[kLate];
     int load_slice = 0, load_slot = lds, load_group = 0, load_scales = scales_at;
-    int x_position = 0, weight_position = 0, target = 0, scale_position = 0, scale_target = 0;
+    int x_position = 0, target = 0, scale_position = 0, scale_target = 0, late_x_position = 0, late_weight_position = 0, late_target = 0;
     uint32_t scale_lanes = 0;
-    const uint8_t *scale_base;
     bool more = true;
     // `upcoming` is the tile that is loaded from here on.
-    const auto set_up = [&]() {
-        const int rows_valid = more ? upcoming.rows_valid : 0, col0 = upcoming.tile_n * kColumns, columns_valid = more ? columns - col0 : 0;
-        const int64_t weight_row = static_cast<int64_t>(upcoming.expert) * columns * (kGated ? 2 : 1) + col0;
+    const auto columns_valid = [&]() { return more ? columns - upcoming.tile_n * kColumns : 0; };
+    const auto first_weight_row = [&]() { return static_cast<int64_t>(upcoming.expert) * columns * (kGated ? 2 : 1) + upcoming.tile_n * kColumns; };
+    // Row of LDS row `t` from the tile's first weight row; -1: there is none. Gated: a wavefront's 64 gates, then their ups.
+    const auto weight_row_of = [&](int t) {
+        const int in_block = (t >> 2 & 1) * 16 + (t >> 3 & 3) * 4 + (t & 3), block = t / 32;
+        const int column = (kGated ? block / 4 * 64 + block % 2 * 32 : block * 32) + in_block;
+        return column >= columns_valid() ? -1 : kGated && block % 4 >= 2 ? column + columns : column;
+    };
+    const auto row_offset = [&](int j) {
+        const int at = (wave * kXLoads + j) * 64 + lane, row = at / kUnits;
+        const int unit = kUnits == 8 ? at % 8 ^ ((row >> 1) & 7) : at % 4 ^ ((row >> 2) & 3);
+        return more && row < upcoming.rows_valid ? static_cast<uint32_t>(row * static_cast<int>(args.x_stride) + unit * 16) : kOutOfRange;
+    };
+    const auto set_up_early = [&]() {
         x_buffer = buffer_of(args.x + upcoming.row0 * args.x_stride);
-        weight_buffer = buffer_of(args.weight + weight_row * args.weight_stride);
-        // Row of LDS row `t` from the tile's first weight row; -1: there is none. Gated: a wavefront's 64 gates, then their ups.
-        const auto weight_row_of = [&](int t) {
-            const int in_block = (t >> 2 & 1) * 16 + (t >> 3 & 3) * 4 + (t & 3), block = t / 32;
-            const int column = (kGated ? block / 4 * 64 + block % 2 * 32 : block * 32) + in_block;
-            return column >= columns_valid ? -1 : kGated && block % 4 >= 2 ? column + columns : column;
-        };
 #pragma unroll
-        for (int j = 0; j < kXLoads; ++j) {
-            const int at = (wave * kXLoads + j) * 64 + lane, row = at / kUnits;
-            const int unit = kUnits == 8 ? at % 8 ^ ((row >> 1) & 7) : at % 4 ^ ((row >> 2) & 3);
-            x_offset[j] = row < rows_valid ? static_cast<uint32_t>(row * static_cast<int>(args.x_stride) + unit * 16) : kOutOfRange;
-        }
-#pragma unroll
-        for (int j = 0; j < kWeightLoads; ++j) {
-            const int at = (wave * kWeightLoads + j) * 64 + lane, t = at / 4, unit = at % 4 ^ ((t >> 2) & 3), row = weight_row_of(t);
-            weight_offset[j] = row >= 0 ? static_cast<uint32_t>(row * static_cast<int>(args.weight_stride) + unit * 16) : kOutOfRange;
-        }
+        for (int j = 0; j < kEarlyRows; ++j) x_offset[j] = row_offset(j);
         // The lower wavefronts load the scales of the rows, the upper ones those of the weight rows.
         const bool of_rows = wave < kWaves / 2;
-        scale_base = (of_rows ? args.x_scales + upcoming.row0 * args.x_scale_stride : args.weight_scales + weight_row * args.weight_scale_stride);
+        scale_buffer = buffer_of(of_rows ? args.x_scales + upcoming.row0 * args.x_scale_stride : args.weight_scales + first_weight_row() * args.weight_scale_stride);
 #pragma unroll
         for (int j = 0; j < kScaleLoads; ++j) {
-            const int t = (wave * kScaleLoads + j) * 64 + lane, row = of_rows ? t < rows_valid ? t : -1 : weight_row_of(t - kTile);
+            const int t = (wave * kScaleLoads + j) * 64 + lane;
+            const int row = of_rows ? more && t < upcoming.rows_valid ? t : -1 : weight_row_of(t - kTile);
             scale_offset[j] = row >= 0 ? static_cast<uint32_t>(row * static_cast<int>(of_rows ? args.x_scale_stride : args.weight_scale_stride)) : kOutOfRange;
         }
     };
-    // The scales of four slices come together; the last slices of a tile are in groups of two at least, so that a group is not overwritten
-    // before it has been read. A group's 16 bytes end with the row.
+    const auto set_up_late = [&]() {
+        late_x_buffer = x_buffer;
+        late_weight_buffer = buffer_of(args.weight + first_weight_row() * args.weight_stride);
+#pragma unroll
+        for (int j = 0; j < kLate; ++j) {
+            if (j < kLateRows) {
+                late_offset[j] = row_offset(kEarlyRows + j);
+            } else {
+                const int at = (wave * kWeightLoads + j - kLateRows) * 64 + lane, t = at / 4, unit = at % 4 ^ ((t >> 2) & 3), row = weight_row_of(t);
+                late_offset[j] = row >= 0 ? static_cast<uint32_t>(row * static_cast<int>(args.weight_stride) + unit * 16) : kOutOfRange;
+            }
+        }
+    };
+    // The scales of four slices come together; the last slices of a tile are in groups of two at least: while a group is read, the space of the one
+    // before it takes one that begins kSlots slices further on, and a group of two (two such, where there are more slots) lies in between. A group's 16 bytes end with the row.
     const auto next_group = [&](int first) { return first + 4 - (slices - first - 4 == 1); };
     const auto first_scales = [&](int first) { return min(first, slices - 4); };
-    const auto begin_slice = [&]() {
-        if (load_slice == slices) {
-            logical += kResident;
-            more = more && experts.locate(placement, logical, upcoming);
-            set_up();
-            load_slice = load_group = 0;
+    const auto next_slot_of = [&](int at) { return at == lds + (kSlots - 1) * kSlotBytes<kFormat> ? lds : at + kSlotBytes<kFormat>; };
+    const auto next_scales = [&](int at) { return at == scales_at + (kScaleSlots<kFormat> - 1) * kScaleBytes ? scales_at : at + kScaleBytes; };
+    const auto begin_late = [&]() { late_x_position = x_position, late_weight_position = x_position / kRowBytes<kFormat> * (kSlice / 2), late_target = target; };
+    // In parts, for the shadows of products.
+    bool begins_load_group = false;
+    const auto begin_early = [&](auto part_constant) {
+        constexpr int part = decltype(part_constant)::value;
+        if constexpr (part == 0) {
+            const int first = here(load_group);
+            begins_load_group = load_slice == first;
+            scale_lanes = begins_load_group ? ~0u : 0;
+            scale_position = first_scales(first) * 4;
+        } else if constexpr (part == 1) {
+            const int first = here(load_group);
+            load_group = begins_load_group ? next_group(first) : first;
+        } else if constexpr (part == 2) {
+            const int at = here(load_scales);
+            scale_target = at + wave * (kScaleLoads * 1024);
+            load_scales = begins_load_group ? next_scales(at) : at;
+        } else {
+            const int slice = here(load_slice);
+            x_position = slice * kRowBytes<kFormat>;
+            load_slice = slice + 1;
+            target = load_slot;
+            load_slot = next_slot_of(load_slot);
         }
-        const bool begins_group = load_slice == load_group;
-        scale_lanes = begins_group ? ~0u : 0;
-        scale_buffer = buffer_of(scale_base);
-        scale_position = first_scales(load_group) * 4;
-        scale_target = load_scales + wave * kScaleLoads * 1024;
-        if (begins_group) load_group = next_group(load_group), load_scales = load_scales == scales_at ? scales_at + kScaleBytes : scales_at;
-        x_position = load_slice * kRowBytes<kFormat>, weight_position = load_slice * (kSlice / 2);
-        target = load_slot;
-        load_slot = load_slot == lds + (kSlots - 1) * kSlotBytes<kFormat> ? lds : load_slot + kSlotBytes<kFormat>;
-        ++load_slice;
     };
-    // The loads of a slice by number: those of scales, of rows, of weights. The last kLate of them are issued a step after the others, when
-    // the state above may be that of the slice after it, and the next tile's.
-    constexpr int kAllLoads = kScaleLoads + kLoads, kLate = kLoads / 2, kEarly = kAllLoads - kLate;
-    static_assert(kLate >= kWeightLoads && kLate - kWeightLoads <= kXLoads, "late are all of the weights and some rows");
-    constexpr int kLateRows = kLate - kWeightLoads;
-    __amdgpu_buffer_rsrc_t late_x_buffer, late_weight_buffer;
-    uint32_t late_offset[kLate];
-    int late_x_position = 0, late_weight_position = 0, late_target = 0;
-    const auto keep_late = [&]() {
-        late_x_buffer = x_buffer, late_weight_buffer = weight_buffer;
-        late_x_position = x_position, late_weight_position = weight_position, late_target = target;
-#pragma unroll
-        for (int j = 0; j < kLate; ++j) late_offset[j] = j < kLateRows ? x_offset[kXLoads - kLateRows + j] : weight_offset[j - kLateRows];
-    };
+    constexpr int kEarlyParts = 4;
     const auto load_early = [&](auto constant) {
         constexpr int j = decltype(constant)::value, at = j - kScaleLoads;
-        if constexpr (j < kScaleLoads) load_to_lds_if(scale_lanes, scale_buffer, scale_offset[j], scale_position, scale_target + j * 1024);
-        else load_to_lds(x_buffer, x_offset[at], x_position, target + (wave * kXLoads + at) * 1024);
+        if constexpr (j < kScaleLoads) load_to_lds_if<j * 1024>(scale_lanes, scale_buffer, scale_offset[j], scale_position, scale_target);
+        else load_to_lds<at * 1024>(x_buffer, x_offset[at], x_position, target + wave * (kXLoads * 1024));
     };
     const auto load_late = [&](auto constant) {
         constexpr int j = decltype(constant)::value;
-        if constexpr (j < kLateRows) load_to_lds(late_x_buffer, late_offset[j], late_x_position, late_target + (wave * kXLoads + kXLoads - kLateRows + j) * 1024);
-        else load_to_lds(late_weight_buffer, late_offset[j], late_weight_position, late_target + kXBytes + (wave * kWeightLoads + j - kLateRows) * 1024);
+        if constexpr (j < kLateRows)
+            load_to_lds<(kEarlyRows + j) * 1024>(late_x_buffer, late_offset[j], late_x_position, late_target + wave * (kXLoads * 1024));
+        else
+            load_to_lds<kXBytes + (j - kLateRows) * 1024>(late_weight_buffer, late_offset[j], late_weight_position, late_target + wave * (kWeightLoads * 1024));
     };
 
     // ---- multiplying ---------------------------------------------------------------------------------------------------
@@ -247,45 +280,64 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         }
         weight_address[i] = kXBytes + wave_n * 128 * (kSlice / 2) + row * (kSlice / 2) + ((2 * i + half) ^ ((row >> 2) & 3)) * 16;
     }
+    const int weight_scale_address = (kTile + wave_n * 128 + (lane & 31)) * 16, x_scale_address = (lane & 31) * 16;
     // Rows of a wavefront: as many blocks of 32 for both halves of the workgroup as the tile's rows need.
     const auto blocks_of = [&](const RowTile &of) { return of.rows_valid <= kTile / 2 ? kBlocks / 2 : kBlocks; };
     int slot = lds, group = 0, group_scales = scales_at;  // of the slice that is read
     int first_row = wave_m * blocks_of(upcoming) * 32;    // of the wavefront, in the tile that is read
-    // Reads by number: of a step's fragments, and after those, with the first step of a slice, of its scales.
-    const auto read = [&](auto constant, auto step_constant, int scale_word) {
-        constexpr int item = decltype(constant)::value, i = decltype(step_constant)::value;
-        if constexpr (item < kBlocks) {
-            weight_part[i][item] = read_lds(weight_address[i] + slot, item * 32 * (kSlice / 2));
-        } else if constexpr (item < kBlocks * (1 + kParts)) {
-            constexpr int m = (item - kBlocks) / kParts, p = (item - kBlocks) % kParts;
-            x_part[i][m][p] = read_lds(x_address[i][p] + slot + first_row * kRowBytes<kFormat>, m * 32 * kRowBytes<kFormat>);
-        } else if constexpr (item < kBlocks * (2 + kParts)) {
-            constexpr int n = item - kBlocks * (1 + kParts);
-            next_weight_scales[n] = *(FM_LDS(uint32_t) *)static_cast<uintptr_t>(scale_word + (kTile + wave_n * 128 + (lane & 31)) * 16 + n * 512);
-        } else {
-            constexpr int m = item - kBlocks * (2 + kParts);
-            next_x_scales[m] = *(FM_LDS(uint32_t) *)static_cast<uintptr_t>(scale_word + (first_row + (lane & 31)) * 16 + m * 512);
-        }
+    // Where a step's reads start, and by number the reads: of the scales (with the first step of a slice), then of the fragments.
+    int x_from[kParts], weight_from, x_scales_from, weight_scales_from;
+    const auto begin_reads = [&](auto step_constant) {
+        constexpr int i = decltype(step_constant)::value;
+        const int rows_at = here(slot + first_row * kRowBytes<kFormat>);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) x_from[p] = x_address[i][p] + rows_at;
+        weight_from = weight_address[i] + slot;
     };
     constexpr int kReads = kBlocks * (1 + kParts), kScaleReads = 2 * kBlocks;
-    const auto take_scales = [&]() {  // byte 2 i of the word is then that of the lane's block in step i
-#pragma unroll
-        for (int n = 0; n < kBlocks; ++n) weight_scales[n] = next_weight_scales[n] >> (8 * half), x_scales[n] = next_x_scales[n] >> (8 * half);
+    const auto read = [&](auto constant, auto step_constant) {
+        constexpr int item = decltype(constant)::value, i = decltype(step_constant)::value, at = i == 0 ? item - kScaleReads : item;
+        if constexpr (at < 0) {
+            if constexpr (item < kBlocks) next_weight_scales[item] = read_lds<uint32_t>(weight_scales_from, item * 512);
+            else next_x_scales[item - kBlocks] = read_lds<uint32_t>(x_scales_from, (item - kBlocks) * 512);
+        } else if constexpr (at < kBlocks) {
+            weight_part[i][at] = read_lds<u32x4_t>(weight_from, at * 32 * (kSlice / 2));
+        } else {
+            constexpr int m = (at - kBlocks) / kParts, p = (at - kBlocks) % kParts;
+            x_part[i][m][p] = read_lds<u32x4_t>(x_from[p], m * 32 * kRowBytes<kFormat>);
+        }
     };
+    const auto begin_scale_reads = [&](int first_slice_of_word, int next) {
+        const int word = here(group_scales + (next - first_slice_of_word) * 4);
+        weight_scales_from = weight_scale_address + word, x_scales_from = x_scale_address + word + first_row * 16;
+    };
+    // Byte 2 i of the word is then that of the lane's block in step i.
+    const auto take_weight_scales = [&](int n) { weight_scales[n] = next_weight_scales[n] >> (8 * half); };
+    const auto take_x_scales = [&]() {
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) x_scales[m] = next_x_scales[m] >> (8 * half);
+    };
+    constexpr std::integral_constant<int, 0> kFirst{};
+    constexpr std::integral_constant<int, 1> kSecond{};
 
-    set_up();
+    set_up_early();
+    set_up_late();
 #pragma unroll 1
     for (int s = 0; s < kSlots; ++s) {
         if (s > 0) for_each<0, kLate>(load_late);
-        begin_slice();
+        for_each<0, kEarlyParts>(begin_early);
         for_each<0, kEarly>(load_early);
-        keep_late();
+        begin_late();
     }
-    wait_for_loads<kLoads + kEarly - kScaleLoads>();
+    wait_for_loads<(kSlots - 2) * kLoads + kEarlyRows>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    for_each<0, kReads + kScaleReads>([&](auto item) { read(item, std::integral_constant<int, 0>{}, scales_at); });
-    take_scales();
+    begin_reads(kFirst);
+    begin_scale_reads(0, 0);
+    for_each<0, kReads + kScaleReads>([&](auto item) { read(item, kFirst); });
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) take_weight_scales(n);
+    take_x_scales();
 
     f32x16_t acc[kBlocks][kBlocks];
     while (true) {
@@ -303,50 +355,74 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                 constexpr int j = decltype(constant)::value, i = decltype(step_constant)::value, n = j / kRows, m = n % 2 ? kRows - 1 - j % kRows : j % kRows;
                 acc[n][m] = multiply<kFormat, 2 * i, 2 * i>(weight_part[i][n], x_part[i][m], weight_scales[n], x_scales[m], acc[n][m]);
             };
-            constexpr std::integral_constant<int, 0> kFirst{};
-            constexpr std::integral_constant<int, 1> kSecond{};
             group = 0;
 #pragma unroll 1
             for (int s = 0; s < slices; ++s) {
-                // The slice that is loaded next, and the one that is read next.
-                keep_late();
-                begin_slice();
-                const int next = s + 1 == slices ? 0 : s + 1;
-                const int next_slot = slot == lds + (kSlots - 1) * kSlotBytes<kFormat> ? lds : slot + kSlotBytes<kFormat>;
-                const bool begins_group = next == 0 || next == next_group(group);
-                group = begins_group ? next : group;
-                group_scales = begins_group ? scales_at + scales_at + kScaleBytes - group_scales : group_scales;
-                const int scale_word = group_scales + (next - first_scales(group)) * 4;
+                if (load_slice == slices) {
+                    logical += kResident;
+                    more = more && experts.locate(placement, logical, upcoming);
+                    set_up_early();
+                    load_slice = load_group = 0;
+                }
+                if (load_slice == 1) set_up_late();
+                int next = 0, next_slot = 0;
+                bool begins_group = false;
                 __builtin_amdgcn_sched_barrier(0);
-                // First step; beside it the reads of the second, and the rest of the loads of slice s + 2.
+                // First step; beside it the reads of the second, the rest of the loads of slice s + kSlots - 1, and what the second step needs to know.
                 for_each<0, kProducts>([&](auto j) {
                     product(j, kFirst);
+                    if constexpr (j == 0) begin_reads(kSecond);
                     constexpr int kBusy = kProducts - 2;
                     if constexpr (j < kBusy) {
-                        for_each<j * kReads / kBusy, (j + 1) * kReads / kBusy>([&](auto item) { read(item, kSecond, 0); });
+                        for_each<j * kReads / kBusy, (j + 1) * kReads / kBusy>([&](auto item) { read(item, kSecond); });
                         for_each<j * kLate / kBusy, (j + 1) * kLate / kBusy>(load_late);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
-                });
-                // Second step. Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + 3 takes its slot.
-                product(kFirst, kSecond);
-                __builtin_amdgcn_sched_barrier(0);
-                wait_for_loads<kLoads>();  // all but those of slice s + 2, whose scales were asked for first
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                slot = next_slot;
-                first_row = next == 0 ? wave_m * blocks_of(upcoming) * 32 : first_row;
-                __builtin_amdgcn_sched_barrier(0);
-                for_each<1, kProducts>([&](auto j) {
-                    product(j, kSecond);
-                    constexpr int kItems = kReads + kScaleReads, kBusy = kProducts - 2;
-                    if constexpr (j <= kBusy) {
-                        for_each<(j - 1) * kItems / kBusy, j * kItems / kBusy>([&](auto item) { read(item, kFirst, scale_word); });
-                        for_each<(j - 1) * kEarly / kBusy, j * kEarly / kBusy>(load_early);
+                    // A part of the state of the next load beside every other product, and then that of the slice that is read next.
+                    constexpr int kApart = kProducts == 16 ? 2 : 1, part = (j - 1) / kApart;
+                    if constexpr ((j - 1) % kApart == 0 && j > 0 && part < kEarlyParts) begin_early(std::integral_constant<int, part>{});
+                    if constexpr (j > 0 && (j - 1) % kApart == 0 && part == kEarlyParts) {
+                        const int following = here(s) + 1;
+                        next = following == slices ? 0 : following;
+                        begins_group = (next == 0) | (next == next_group(group));
+                    }
+                    if constexpr (j > 0 && (j - 1) % kApart == 0 && part == kEarlyParts + 1) {
+                        const int first = here(group), at = here(slot);
+                        group = begins_group ? next : first;
+                        group_scales = begins_group ? next_scales(group_scales) : group_scales;
+                        next_slot = next_slot_of(at);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 });
-                take_scales();
+                // Second step. Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + kSlots takes its slot.
+                product(kFirst, kSecond);
+                __builtin_amdgcn_sched_barrier(0);
+                wait_for_loads<(kSlots - 2) * kLoads>();  // all but those of the slices from s + 2 on (their scales are asked for first)
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                slot = next_slot;
+                first_row = next == 0 ? wave_m * blocks_of(upcoming) * 32 : first_row;
+                for_each<1, kProducts>([&](auto j) {
+                    product(j, kSecond);
+                    if constexpr (j == 1) begin_scale_reads(first_scales(group), next), begin_reads(kFirst);
+                    constexpr int kItems = kReads + kScaleReads, kBusy = kProducts - 2;
+                    if constexpr (j <= kBusy) {
+                        for_each<(j - 1) * kItems / kBusy, j * kItems / kBusy>([&](auto item) { read(item, kFirst); });
+                        for_each<(j - 1) * kEarly / kBusy, j * kEarly / kBusy>(load_early);
+                    }
+                    // (The products of weight block n are behind.)
+                    if constexpr (kRows == kBlocks && j % kRows == kRows - 1 && j / kRows + 1 < kBlocks) take_weight_scales(j / kRows);
+                    if constexpr (j == kProducts - 1) begin_late();
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+#pragma unroll
+                for (int n = kRows == kBlocks ? kBlocks - 1 : 0; n < kBlocks; ++n) take_weight_scales(n);
+                take_x_scales();
+                // The compiler would move products past the branches above, away from what they are to overlap.
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+                    for (int m = 0; m < kRows; ++m) asm volatile("" : "+a"(acc[n][m]));
             }
         };
         const int blocks = blocks_of(tile);
@@ -364,12 +440,13 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                     for (int m = 0; m < kBlocks; ++m) {
                         __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: registers
                         if (m >= blocks) continue;
+                        f32x16_t gates = settled(acc[n][m]), ups = settled(acc[kGated ? n + 2 : n][m]);
                         float values[16];
                         uint32_t largest = 0;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            values[i] = activate(acc[n][m][i]);
-                            if constexpr (kGated) values[i] *= acc[n + 2][m][i];
+                            values[i] = activate(gates[i]);
+                            if constexpr (kGated) values[i] *= ups[i];
                             largest = max(largest, magnitude_bits(values[i]));
                         }
                         largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), 32, 64)));
@@ -396,6 +473,7 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
 #pragma unroll
                 for (int n = 0; n < kBlocks; ++n) {
                     __builtin_amdgcn_sched_barrier(0);
+                    const f32x16_t values = settled(acc[n][m]);
                     const int column = col0 + wave_n * 128 + n * 32 + 16 * (out_lane >> 5);
                     Result *out = static_cast<Result *>(args.out) + (tile.row0 + row) * args.out_stride + column;
                     constexpr int N = Vec16<Result>::N;
@@ -404,13 +482,13 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                         for (int part = 0; part < 16 / N; ++part) {
                             Vec16<Result> vector;
 #pragma unroll
-                            for (int c = 0; c < N; ++c) vector.v[c] = from_float<Result>(acc[n][m][part * N + c]);
+                            for (int c = 0; c < N; ++c) vector.v[c] = from_float<Result>(values[part * N + c]);
                             store16(out + part * N, vector);
                         }
                     } else {
 #pragma unroll
                         for (int c = 0; c < 16; ++c)
-                            if (column + c < columns) out[c] = from_float<Result>(acc[n][m][c]);
+                            if (column + c < columns) out[c] = from_float<Result>(values[c]);
                     }
                 }
             }
