@@ -21,6 +21,7 @@ struct ProductArgs {
     int64_t experts;
     int format;  // of x, and of a microscaled result
     int gated, activation;
+    int out_dtype;    // where it is not microscaled
     int out_vectors;  // rows of `out` are aligned to 16 bytes
     // Rows by a sparse map ...
     const void *expert_ends, *expert_pad_begins;
@@ -35,9 +36,9 @@ constexpr int kMaxEntries = 4096;  // the list in LDS, and the scan of every wor
 
 // Many rows per expert (fm_mx_tiles.hip).
 bool tile_product_takes(const ProductArgs &args);
-int tile_product(const ProductArgs &args, int out_dtype, hipStream_t stream);
-// Few rows per expert (fm_mx_stream.hip). `out_dtype` where the result is not microscaled.
-int stream_product(const ProductArgs &args, int out_dtype, hipStream_t stream);
+int tile_product(const ProductArgs &args, hipStream_t stream);
+// Few rows per expert (fm_mx_stream.hip).
+int stream_product(const ProductArgs &args, hipStream_t stream);
 // Both layers and the combine without a sparse map; layer_2.out is fp32 scratch.
 int few_tokens(const ProductArgs &layer_1, const ProductArgs &layer_2, const float *scores, void *out, int out_dtype, hipStream_t stream);
 

@@ -27,11 +27,11 @@ int check_sizes(const char *name, int64_t rows, int64_t columns, int64_t inner, 
     return FM_OK;
 }
 
-int run(const mx::ProductArgs &args, int out_dtype, void *stream) {
+int run(const mx::ProductArgs &args, void *stream) {
     // The host knows rows with up to 128 of padding per expert.
     const bool many = args.rows > 192 * args.experts;
-    return many && mx::tile_product_takes(args) ? mx::tile_product(args, out_dtype, static_cast<hipStream_t>(stream))
-                                                : mx::stream_product(args, out_dtype, static_cast<hipStream_t>(stream));
+    return many && mx::tile_product_takes(args) ? mx::tile_product(args, static_cast<hipStream_t>(stream))
+                                                : mx::stream_product(args, static_cast<hipStream_t>(stream));
 }
 
 }  // namespace
@@ -58,9 +58,10 @@ extern "C" int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, cons
     args.x_rows = args.rows = rows, args.x_stride = lhs_stride, args.x_scale_stride = lhs_scale_stride;
     args.weight_stride = rhs_stride, args.weight_scale_stride = rhs_scale_stride, args.out_stride = out_stride;
     args.columns = args.out_columns = columns, args.inner = padded, args.experts = num_experts, args.format = format;
+    args.out_dtype = out_dtype;
     args.out_vectors = aligned16(out) && out_stride * size % 16 == 0;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
-    if (int status = run(args, out_dtype, stream)) return status;
+    if (int status = run(args, stream)) return status;
     return check_launch(name);
 }
 
@@ -88,7 +89,7 @@ extern "C" int fm_mx_sparse_matmul_activation(const void *lhs, const void *lhs_s
     args.out_stride = mx::value_bytes(format, args.out_columns), args.out_scale_stride = mx::scale_bytes(args.out_columns);
     args.gated = gated != 0, args.activation = activation;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
-    if (int status = run(args, 0, stream)) return status;
+    if (int status = run(args, stream)) return status;
     return check_launch(name);
 }
 
@@ -164,7 +165,7 @@ extern "C" int fm_mx_few_tokens_forward(const void *input, const void *input_sca
     layer_2.x_rows = layout.entries, layer_2.x_stride = layer_1.out_stride, layer_2.x_scale_stride = layer_1.out_scale_stride;
     layer_2.weight = static_cast<const uint8_t *>(weight_2), layer_2.weight_scales = static_cast<const uint8_t *>(weight_2_scales);
     layer_2.weight_stride = weight_2_stride, layer_2.weight_scale_stride = weight_2_scale_stride;
-    layer_2.out = scratch + layout.sums_at, layer_2.out_stride = layout.hidden_stride, layer_2.out_vectors = 1;
+    layer_2.out = scratch + layout.sums_at, layer_2.out_stride = layout.hidden_stride, layer_2.out_vectors = 1, layer_2.out_dtype = FM_DTYPE_F32;
     layer_2.columns = layer_2.out_columns = hidden, layer_2.inner = layout.ffn;
     if (int status = mx::few_tokens(layer_1, layer_2, static_cast<const float *>(scores), output, out_dtype, static_cast<hipStream_t>(stream))) return status;
     return check_launch(name);

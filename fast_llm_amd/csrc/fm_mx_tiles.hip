@@ -527,10 +527,10 @@ bool tile_product_takes(const ProductArgs &args) {
            (args.rows / kTile + args.experts + 1) * ((args.out_columns + 127) / 128) < (int64_t(1) << 30);
 }
 
-int tile_product(const ProductArgs &args, int out_dtype, hipStream_t stream) {
+int tile_product(const ProductArgs &args, hipStream_t stream) {
     using namespace tiles;
     if (args.out_scales != nullptr) return args.gated ? launch<true, uint8_t>(args, stream) : launch<false, uint8_t>(args, stream);
-    switch (out_dtype) {
+    switch (args.out_dtype) {
         case FM_DTYPE_F32: return launch<false, float>(args, stream);
         case FM_DTYPE_BF16: return launch<false, bf16_t>(args, stream);
         default: return launch<false, f16_t>(args, stream);
