@@ -9,6 +9,10 @@
 // passes once: memory is the bound. Sums are in fp32: a lane's own values, then lanes, then wavefronts, in a fixed order.
 // Rows that are longer, or whose length is no multiple of 8, or that are not aligned to 16 bytes: a value per lane and load, the stream
 // read a second time.
+//
+// Measured at 16384 x 2048 bf16 with a residual: forward 268 MB in 45.4 us (5.9 TB/s), backward 268 MB in 45.0 us and 4.2 us for the sum of 512
+// shares of the weight's gradient. (With the loads behind branches, the backward without the next row's: 51 and 89 us.) 5001 x 2048
+// fp16 with e4m3 beside it: 92 MB in 16.9 us.
 #include "fm_mx.h"
 
 namespace fm {
@@ -71,6 +75,24 @@ __device__ __forceinline__ void store_eight(void *base, int64_t offset, const Ei
     for (int part = 0; part < 8 / Vec16<T>::N; ++part) store16(static_cast<T *>(base) + offset + part * Vec16<T>::N, eight.part[part]);
 }
 
+// A row as a buffer: what is read past its end, or of a row (or a tensor) that does not exist, is zero, without a branch. (Behind
+// branches the compiler cannot count which loads are under way and waits for all.)
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_of(const void *base, int64_t row, const Args &args) {
+    const char *start = static_cast<const char *>(base) + row * args.columns * static_cast<int64_t>(sizeof(T));
+    const int bytes = base != nullptr && row < args.rows ? args.columns * static_cast<int>(sizeof(T)) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(uniform_pointer(start)), 0, __builtin_amdgcn_readfirstlane(bytes), kBufferResourceFlags);
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(__amdgpu_buffer_rsrc_t row, int column) {
+    Eight<T> eight;
+#pragma unroll
+    for (int part = 0; part < 8 / Vec16<T>::N; ++part)
+        eight.part[part] = __builtin_bit_cast(
+            Vec16<T>, __builtin_amdgcn_raw_buffer_load_b128(row, (column + part * Vec16<T>::N) * static_cast<int>(sizeof(T)), 0, 0));
+    return eight;
+}
+
 // The weight of eight columns. It has the input's type or fp32.
 template <typename T>
 __device__ __forceinline__ void load_weight(const Args &args, int column, float (&weight)[8]) {
@@ -85,11 +107,29 @@ __device__ __forceinline__ void load_weight(const Args &args, int column, float 
     }
 }
 
+// The sum over a wavefront's lanes in all of them, without LDS: within four, eight, sixteen, then the rows of sixteen and the halves, both
+// of which a swap with itself puts side by side.
+__device__ __forceinline__ float lane_sum(float value) {
+    const auto with = [&](auto control) {
+        value += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, value), decltype(control)::value, 0xf, 0xf, true));
+    };
+    with(std::integral_constant<int, 0xb1>{});   // lanes 1 0 3 2 of every four
+    with(std::integral_constant<int, 0x4e>{});   // 2 3 0 1
+    with(std::integral_constant<int, 0x141>{});  // the eight mirrored
+    with(std::integral_constant<int, 0x140>{});  // the sixteen mirrored
+    const uint32_t bits = __builtin_bit_cast(uint32_t, value);
+    const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+    value = __builtin_bit_cast(float, static_cast<uint32_t>(rows[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(rows[1]));
+    const uint32_t bits_16 = __builtin_bit_cast(uint32_t, value);
+    const auto halves = __builtin_amdgcn_permlane32_swap(bits_16, bits_16, false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(halves[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(halves[1]));
+}
+
 // Sums of kCount values over the kLanes threads of a row, in all of them.
 template <int kLanes, int kCount>
 __device__ __forceinline__ void row_sum(float (&values)[kCount]) {
 #pragma unroll
-    for (int c = 0; c < kCount; ++c) values[c] = wave_sum(values[c]);
+    for (int c = 0; c < kCount; ++c) values[c] = lane_sum(values[c]);
     if constexpr (kLanes > 64) {
         __shared__ float sums[kCount][kLanes / 64];
         __syncthreads();  // the sums of the row before have been read
@@ -117,22 +157,18 @@ constexpr int kThreads = kLanes < 256 ? 256 : kLanes;
 template <typename T, int kLanes, int kVectors>
 __global__ __launch_bounds__(kThreads<kLanes>) void forward_kernel(Args args) {
     const int lane = threadIdx.x % kLanes;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads<kLanes> / kLanes) + threadIdx.x / kLanes;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads<kLanes> / kLanes) + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     if (row >= args.rows) return;  // whole wavefronts
     const int64_t start = row * args.columns;
     Eight<T> stream[kVectors];
+    const __amdgpu_buffer_rsrc_t input = row_of<T>(args.input, row, args);
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int column = (v * kLanes + lane) * 8;
-        stream[v] = column < args.columns ? load_eight<T>(args.input, start + column) : zeros<T>();
-    }
+    for (int v = 0; v < kVectors; ++v) stream[v] = load_eight<T>(input, (v * kLanes + lane) * 8);
     if (args.residual != nullptr) {
         Eight<T> residual[kVectors];
+        const __amdgpu_buffer_rsrc_t residual_row = row_of<T>(args.residual, row, args);
 #pragma unroll
-        for (int v = 0; v < kVectors; ++v) {
-            const int column = (v * kLanes + lane) * 8;
-            residual[v] = column < args.columns ? load_eight<T>(args.residual, start + column) : zeros<T>();
-        }
+        for (int v = 0; v < kVectors; ++v) residual[v] = load_eight<T>(residual_row, (v * kLanes + lane) * 8);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int column = (v * kLanes + lane) * 8;
@@ -209,37 +245,65 @@ __global__ __launch_bounds__(kAnyThreads) void forward_any_kernel(Args args) {
     }
 }
 
+// What a row's backward reads.
+template <typename T, int kLanes, int kVectors, bool kGradStream>
+struct BackwardRow {
+    Eight<T> stream[kVectors], grad[kVectors], grad_stream[kGradStream ? kVectors : 1];
+    __device__ __forceinline__ void load(const Args &args, int64_t row, int lane) {
+        const __amdgpu_buffer_rsrc_t stream_row = row_of<T>(args.stream, row, args), grad_row = row_of<T>(args.grad_normalized, row, args);
+        const __amdgpu_buffer_rsrc_t grad_stream_row = row_of<T>(args.grad_stream, row, args);
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int column = (v * kLanes + lane) * 8;
+            stream[v] = load_eight<T>(stream_row, column);
+            grad[v] = load_eight<T>(grad_row, column);
+            if constexpr (kGradStream) grad_stream[v] = load_eight<T>(grad_stream_row, column);
+        }
+    }
+};
+
 // A group of kLanes threads walks over rows and keeps its share of the weight's gradient in registers; the groups of a workgroup add
 // theirs up in LDS, the workgroups theirs in `weight_gradient_kernel`.
 template <typename T, int kLanes, int kVectors>
-__global__ __launch_bounds__(kThreads<kLanes>) void backward_kernel(Args args) {
+__global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backward_kernel(Args args) {
     constexpr int kGroups = kThreads<kLanes> / kLanes;
-    // The stream's gradient is asked for with the rest of the row, but where 16 wavefronts share a CU's registers.
-    constexpr bool kEarly = kLanes < 1024;
-    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    float weight_grad[kVectors][8];
+    // The next row is asked for before this one is worked on and the weight stays in registers, but where the registers do not hold that (rows of
+    // over 1024 or 4096 columns of fp32; 16 wavefronts on a CU): there the weight and the stream's gradient are read when they are needed.
+    constexpr bool kAhead = kLanes < 1024 && kVectors * sizeof(T) <= 8;
+    using Row = BackwardRow<T, kLanes, kVectors, kAhead>;
+    const int lane = threadIdx.x % kLanes, group = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+    float weight_grad[kVectors][8], weights[kAhead ? kVectors : 1][8];
 #pragma unroll
     for (int v = 0; v < kVectors; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) weight_grad[v][i] = 0.f;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group; row < args.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
-        const int64_t start = row * args.columns;
-        Eight<T> stream[kVectors], grad[kVectors], grad_stream[kEarly ? kVectors : 1];
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+    Row current, next;
+    if constexpr (kAhead) {
+        current.load(args, row, lane);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int column = (v * kLanes + lane) * 8;
-            const bool exists = column < args.columns;
-            stream[v] = exists ? load_eight<T>(args.stream, start + column) : zeros<T>();
-            grad[v] = exists ? load_eight<T>(args.grad_normalized, start + column) : zeros<T>();
-            if constexpr (kEarly) grad_stream[v] = exists && args.grad_stream != nullptr ? load_eight<T>(args.grad_stream, start + column) : zeros<T>();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) weights[v][i] = 0.f;
+            if (column < args.columns) load_weight<T>(args, column, weights[v]);
         }
+    }
+    for (; row < args.rows; row += step) {
+        if constexpr (kAhead) next.load(args, row + step, lane);
+        else current.load(args, row, lane);
+        auto &stream = current.stream;
+        auto &grad = current.grad;
+        const int64_t start = row * args.columns;
         float sums[2] = {0.f, 0.f};  // of s^2 and of g w s
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int column = (v * kLanes + lane) * 8;
-            if (column >= args.columns) continue;
-            float weight[8];
-            load_weight<T>(args, column, weight);
+            if (!kAhead && column >= args.columns) continue;
+            float read[8];
+            if constexpr (!kAhead) load_weight<T>(args, column, read);
+            const float(&weight)[8] = kAhead ? weights[kAhead ? v : 0] : read;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 sums[0] += stream[v][i] * stream[v][i];
@@ -248,21 +312,28 @@ __global__ __launch_bounds__(kThreads<kLanes>) void backward_kernel(Args args) {
         }
         row_sum<kLanes>(sums);
         const float inverse = inverse_root(args, sums[0]), factor = inverse * inverse * sums[1] * args.inverse_columns;
+        // Kept in their own type meanwhile, not widened.
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) settle(stream[v]), settle(grad[v]);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int column = (v * kLanes + lane) * 8;
             if (column >= args.columns) continue;
-            float weight[8];
-            load_weight<T>(args, column, weight);
-            if constexpr (!kEarly) grad_stream[0] = args.grad_stream != nullptr ? load_eight<T>(args.grad_stream, start + column) : zeros<T>();
+            float read[8];
+            if constexpr (!kAhead) {
+                load_weight<T>(args, column, read);
+                current.grad_stream[0] = load_eight<T>(row_of<T>(args.grad_stream, row, args), column);
+            }
+            const float(&weight)[8] = kAhead ? weights[kAhead ? v : 0] : read;
             Eight<T> result;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                result.set(i, inverse * (grad[v][i] * weight[i] - stream[v][i] * factor) + grad_stream[kEarly ? v : 0][i]);
+                result.set(i, inverse * (grad[v][i] * weight[i] - stream[v][i] * factor) + current.grad_stream[kAhead ? v : 0][i]);
                 weight_grad[v][i] += grad[v][i] * (stream[v][i] * inverse);
             }
             store_eight(args.grad_input, start + column, result);
         }
+        if constexpr (kAhead) current = next;
     }
     if (args.partials == nullptr) return;
     float *target = args.partials + static_cast<int64_t>(blockIdx.x) * args.columns;
