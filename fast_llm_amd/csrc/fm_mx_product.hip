@@ -28,8 +28,15 @@ int check_sizes(const char *name, int64_t rows, int64_t columns, int64_t inner, 
 }
 
 int run(const mx::ProductArgs &args, void *stream) {
-    // The host knows rows with up to 128 of padding per expert.
-    const bool many = args.rows > 192 * args.experts;
+    // The tiles read the weights once, at 3.8 TB/s where little is multiplied and there is a tile for every CU; with few rows the weights are read once
+    // per 32 rows of an expert, at 4.8 TB/s. So it depends on how many experts have over 32 rows, and on the tiles. Measured in us, few rows | tiles,
+    // with both layers' weights of 8 experts (4096, 2 x 14336), 64 (2048, 2 x 1408) and 128 (2048, 2 x 768) and tokens at random: 16 rows per
+    // expert 165 | 221, 75 | 82, 74 | 96; 32 rows 273 | 239, 135 | 89, 137 | 95. One expert, 4096 -> 28672 (112 tiles): 32 rows 28 | 34, 48 rows 45 | 36;
+    // 14336 -> 4096 (16 tiles): 128 rows 83 | 102. Of a map the host knows the rows with up to 128 of padding per expert; without one (the
+    // ends are those of the rows) it knows them exactly.
+    const int64_t tiles = (args.out_columns + 255) / 256 * (args.gated ? 2 : 1) * args.experts, times = max(int64_t(1), 80 / tiles);
+    const bool exact = args.expert_ends == args.expert_pad_begins;
+    const bool many = args.rows > (exact ? 32 * times : 128 + 24 * times) * args.experts;
     return many && mx::tile_product_takes(args) ? mx::tile_product(args, static_cast<hipStream_t>(stream))
                                                 : mx::stream_product(args, static_cast<hipStream_t>(stream));
 }
