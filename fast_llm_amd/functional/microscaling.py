@@ -87,13 +87,14 @@ class MicroscaledTensor:
 
     @classmethod
     def empty(cls, rows: int, columns: int, format: MicroscalingFormat | str, device: torch.device) -> "MicroscaledTensor":
-        format, groups = MicroscalingFormat(format), _padded(columns) // MX_COLUMN_MULTIPLE
-        return cls(
-            torch.empty((rows, groups * _BYTES[format]), dtype=torch.uint8, device=device),
-            torch.empty((rows, groups * (MX_COLUMN_MULTIPLE // MX_BLOCK)), dtype=torch.uint8, device=device),
-            columns,
-            format,
-        )
+        assert columns > 0
+        # Right by construction: the checks of `__post_init__` take as long as a small launch.
+        out = cls.__new__(cls)
+        out.columns, out.format = columns, MicroscalingFormat(format)
+        groups = _padded(columns) // MX_COLUMN_MULTIPLE
+        out.values = torch.empty((rows, groups * _BYTES[out.format]), dtype=torch.uint8, device=device)
+        out.scales = torch.empty((rows, groups * (MX_COLUMN_MULTIPLE // MX_BLOCK)), dtype=torch.uint8, device=device)
+        return out
 
 
 def _tag(format: MicroscalingFormat) -> int:

@@ -12,7 +12,7 @@ from fast_llm_amd.functional.utils import Assert, without_backward
 
 
 def _check(input_: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None) -> None:
-    Assert.eq(tuple(weight.shape), (input_.size(-1),))
+    assert weight.dim() == 1 and weight.size(0) == input_.size(-1) > 0, (weight.shape, input_.shape)
     if weight.dtype != input_.dtype and weight.dtype != torch.float32:
         raise ValueError(f"the weight has the input's type ({input_.dtype}) or float32, not {weight.dtype}")
     if residual is not None:
@@ -100,7 +100,6 @@ def rms_norm_quantize(
     """
     _check(input_, weight, residual)
     columns = input_.size(-1)
-    Assert.custom(lambda count: count > 0, columns)
     quantized = MicroscaledTensor.empty(input_.numel() // columns, columns, format, input_.device)
     normalized, stream = _forward(input_, weight, residual, eps, quantized)
     if torch.is_grad_enabled() and (input_.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
