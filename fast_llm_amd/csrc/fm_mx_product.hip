@@ -34,7 +34,7 @@ int run(const mx::ProductArgs &args, void *stream) {
     // expert 165 | 221, 75 | 82, 74 | 96; 32 rows 273 | 239, 135 | 89, 137 | 95. One expert, 4096 -> 28672 (112 tiles): 32 rows 28 | 34, 48 rows 45 | 36;
     // 14336 -> 4096 (16 tiles): 128 rows 83 | 102. Of a map the host knows the rows with up to 128 of padding per expert; without one (the
     // ends are those of the rows) it knows them exactly.
-    const int64_t tiles = (args.out_columns + 255) / 256 * (args.gated ? 2 : 1) * args.experts, times = max(int64_t(1), 80 / tiles);
+    const int64_t tiles = (args.out_columns + 255) / 256 * (args.gated ? 2 : 1) * args.experts, times = min(max(80 / tiles, int64_t(1)), int64_t(4));
     const bool exact = args.expert_ends == args.expert_pad_begins;
     const bool many = args.rows > (exact ? 32 * times : 128 + 24 * times) * args.experts;
     return many && mx::tile_product_takes(args) ? mx::tile_product(args, static_cast<hipStream_t>(stream))
@@ -150,7 +150,7 @@ extern "C" int fm_mx_few_tokens_forward(const void *input, const void *input_sca
     if (int status = check_tensor(name, "layer 1", weight_1, weight_1_scales, layer_1_rows, padded, weight_1_stride, weight_1_scale_stride, FM_MX_E2M1)) return status;
     if (int status = check_tensor(name, "layer 2", weight_2, weight_2_scales, num_experts * hidden, layout.ffn, weight_2_stride, weight_2_scale_stride, FM_MX_E2M1))
         return status;
-    if (num_tokens * input_stride >= kMost32) return fail(FM_ERR_UNSUPPORTED, "%s: rows of the input are too far apart", name);
+    if (num_tokens * max(input_stride, input_scale_stride) >= kMost32) return fail(FM_ERR_UNSUPPORTED, "%s: rows of the input are too far apart", name);
     FM_REQUIRE(workspace && aligned16(workspace) && workspace_size >= layout.size, "%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", name,
                layout.size, workspace_size);
     mx::ProductArgs layer_1{};

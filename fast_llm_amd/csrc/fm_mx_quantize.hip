@@ -279,6 +279,7 @@ extern "C" int fm_mx_copy_dense_to_sparse(const void *values, const void *scales
     FM_REQUIRE(num_rows_dense == 1 || (value_row_stride >= mx::value_bytes(format, padded) && scale_row_stride >= mx::scale_bytes(padded)), "%s: rows overlap", name);
     FM_REQUIRE(aligned16(values) && value_row_stride % 16 == 0 && aligned16(out_values), "%s: rows of values are 16-byte aligned", name);
     FM_REQUIRE(reinterpret_cast<uintptr_t>(scales) % 4 == 0 && scale_row_stride % 4 == 0 && aligned16(out_scales), "%s: rows of scales are 4-byte aligned", name);
+    if (num_rows_dense >= mx::kMaxWorkgroups) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     mx::dispatch_kernel<<<static_cast<uint32_t>(num_rows_dense), mx::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
         static_cast<const uint8_t *>(values), static_cast<const uint8_t *>(scales), static_cast<uint8_t *>(out_values), static_cast<uint8_t *>(out_scales),
         sparse_rows, static_cast<int>(num_experts_per_token), num_rows_sparse, value_row_stride, scale_row_stride,

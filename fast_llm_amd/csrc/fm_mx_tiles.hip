@@ -523,7 +523,8 @@ bool tile_product_takes(const ProductArgs &args) {
     using namespace tiles;
     // Scales of four slices are loaded at once; offsets from a tile's first row are counted in 31 bits, rows and tiles too.
     const int64_t weight_rows = args.gated ? args.columns + kTile : kTile;
-    return args.inner >= 4 * kSlice && args.x_stride * kTile < (int64_t(1) << 31) && args.weight_stride * weight_rows < (int64_t(1) << 31) &&
+    const int64_t x_stride = max(args.x_stride, args.x_scale_stride), weight_stride = max(args.weight_stride, args.weight_scale_stride);
+    return args.inner >= 4 * kSlice && x_stride * kTile < (int64_t(1) << 31) && weight_stride * weight_rows < (int64_t(1) << 31) &&
            (args.rows / kTile + args.experts + 1) * ((args.out_columns + 127) / 128) < (int64_t(1) << 30);
 }
 

@@ -467,22 +467,30 @@ extern "C" int fm_rms_norm_forward(const void *input, const void *residual, cons
     const bool aligned = aligned16(input) && aligned16(residual) && aligned16(weight) && aligned16(stream_out) && aligned16(normalized);
     const int lanes = norm::lanes_of(columns, aligned);
     norm::Args args{};
-    args.input = input, args.residual = residual, args.weight = weight, args.stream = stream_out, args.normalized = normalized;
-    args.values = static_cast<uint8_t *>(values), args.scales = static_cast<uint8_t *>(scales);
-    args.rows = rows, args.columns = static_cast<int>(columns), args.padded = static_cast<int>(mx::padded_columns(columns)), args.format = format;
+    args.weight = weight, args.columns = static_cast<int>(columns), args.padded = static_cast<int>(mx::padded_columns(columns)), args.format = format;
     args.weight_f32 = weight_dtype == FM_DTYPE_F32 && dtype != FM_DTYPE_F32;
     args.eps = static_cast<float>(eps), args.inverse_columns = static_cast<float>(1. / static_cast<double>(columns));
-    FM_DISPATCH_DTYPE(dtype, T, {
-        if (lanes == 0) {
-            norm::forward_any_kernel<T><<<static_cast<uint32_t>(rows), norm::kAnyThreads, 0, static_cast<hipStream_t>(stream)>>>(args);
-        } else {
-            norm::for_shape<T>(static_cast<int>(columns), lanes, [&](auto lanes_constant, auto vectors) {
-                constexpr int kLanes = decltype(lanes_constant)::value, kRows = norm::kThreads<kLanes> / kLanes;
-                norm::forward_kernel<T, kLanes, decltype(vectors)::value>
-                    <<<static_cast<uint32_t>((rows + kRows - 1) / kRows), norm::kThreads<kLanes>, 0, static_cast<hipStream_t>(stream)>>>(args);
-            });
-        }
-    });
+    // A launch counts its threads in 32 bits: up to 1024 per row.
+    constexpr int64_t kRowsAtOnce = (int64_t(1) << 22) - 4;
+    const auto past = [](const void *pointer, int64_t bytes) { return pointer == nullptr ? nullptr : const_cast<char *>(static_cast<const char *>(pointer)) + bytes; };
+    for (int64_t row = 0; row < rows; row += kRowsAtOnce) {
+        const int64_t bytes = row * columns * dtype_size(dtype);
+        args.input = past(input, bytes), args.residual = past(residual, bytes), args.stream = past(stream_out, bytes), args.normalized = past(normalized, bytes);
+        args.values = reinterpret_cast<uint8_t *>(past(values, row * mx::value_bytes(format, args.padded)));
+        args.scales = reinterpret_cast<uint8_t *>(past(scales, row * mx::scale_bytes(args.padded)));
+        args.rows = min(rows - row, kRowsAtOnce);
+        FM_DISPATCH_DTYPE(dtype, T, {
+            if (lanes == 0) {
+                norm::forward_any_kernel<T><<<static_cast<uint32_t>(args.rows), norm::kAnyThreads, 0, static_cast<hipStream_t>(stream)>>>(args);
+            } else {
+                norm::for_shape<T>(static_cast<int>(columns), lanes, [&](auto lanes_constant, auto vectors) {
+                    constexpr int kLanes = decltype(lanes_constant)::value, kRows = norm::kThreads<kLanes> / kLanes;
+                    norm::forward_kernel<T, kLanes, decltype(vectors)::value>
+                        <<<static_cast<uint32_t>((args.rows + kRows - 1) / kRows), norm::kThreads<kLanes>, 0, static_cast<hipStream_t>(stream)>>>(args);
+                });
+            }
+        });
+    }
     return check_launch(name);
 }
 

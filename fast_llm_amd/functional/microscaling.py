@@ -117,11 +117,12 @@ def mx_quantize(input_: torch.Tensor, format: MicroscalingFormat | str = Microsc
     nearest even and saturated. A block with an infinity or NaN is NaN altogether.
     """
     format = MicroscalingFormat(format)
-    input_ = input_.detach().flatten(0, -2)
+    columns = input_.size(-1)
+    input_ = input_.detach().reshape(input_.numel() // max(columns, 1), columns)
     if input_.stride(1) != 1:
         input_ = input_.contiguous()
     device = _lib.require_device(input_)
-    rows, columns = input_.shape
+    rows = input_.size(0)
     out = MicroscaledTensor.empty(rows, columns, format, device)
     _lib.call(
         "fm_mx_quantize", device, input_.data_ptr(), out.values.data_ptr(), out.scales.data_ptr(), rows, columns,

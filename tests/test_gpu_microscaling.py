@@ -371,3 +371,73 @@ def test_mlp_replays_from_a_graph_and_runs_on_any_stream(tokens, device):
             assert torch.equal(output, result)
             assert torch.equal(call(*arguments), result)
             torch.cuda.synchronize()
+
+
+# ---- calls at the ends of what is allowed ----------------------------------------------------------------
+@pytest.mark.parametrize("index_dtype", [torch.int16, torch.int32, torch.int64])
+@pytest.mark.parametrize("format", FORMATS)
+def test_tiles_take_strides_and_index_types(index_dtype, format, device):
+    generator = torch.Generator().manual_seed(5)
+    inner, columns = 640, 132
+    sparse_map = _map([500, 259, 5], device, index_dtype, block=1, phantom=3)  # boundaries of any kind
+    lhs = _whole(generator, (2 * sparse_map.num_rows, inner), device, format)
+    rhs = _whole(generator, (2 * 3 * columns, inner), device, "e2m1")
+    operands = [MicroscaledTensor(t.values[::2], t.scales[::2], inner, t.format) for t in (lhs, rhs)]
+    rows, weight = (_values(t) for t in operands)
+    for offset in (0, 1):  # aligned to groups of four and not
+        wide = torch.full((sparse_map.num_rows, 2 * columns), -7.0, dtype=torch.bfloat16, device=device)
+        mx_sparse_matmul(*operands, sparse_map, wide[:, 8 + offset : 8 + offset + columns])
+        expected = torch.full(wide.shape, -7.0, dtype=torch.bfloat16)
+        for expert, begin, end in _real_rows(sparse_map):
+            product = rows[begin:end] @ weight[expert * columns : (expert + 1) * columns].t()
+            expected[begin:end, 8 + offset : 8 + offset + columns] = product.bfloat16()
+        assert torch.equal(wide.cpu(), expected)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("of_rows", [True, False])
+def test_scales_that_are_far_apart(of_rows, format, device):
+    """The rows of scales of one tile lie over 2 GiB of memory, those of a block of 32 rows within 4 GiB."""
+    generator = torch.Generator().manual_seed(3)
+    lhs, rhs = _whole(generator, (200, 512), device, format), _whole(generator, (200, 512), device, "e2m1")
+    plain = mx_sparse_matmul(lhs, rhs, dtype=torch.float32)
+    tensor = lhs if of_rows else rhs
+    apart = torch.empty(200, 1 << 24, dtype=torch.uint8, device=device)[:, :16]
+    apart.copy_(tensor.scales)
+    tensor.scales = apart
+    assert torch.equal(mx_sparse_matmul(lhs, rhs, dtype=torch.float32), plain)
+
+
+def test_a_row_by_itself_is_quantised(device):
+    row = torch.randn(100, device=device)
+    for ours, theirs in zip(_stored(mx_quantize(row)), _stored(mx_quantize(row[None]))):
+        assert torch.equal(ours, theirs)
+    assert mx_quantize(row.view(2, 1, 50).transpose(0, 2)).shape == (50, 2) and mx_quantize(row.view(2, 50)[:0]).shape == (0, 50)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_two_streams_at_once(tokens, format, device):
+    """Calls on two streams share nothing but their inputs."""
+    generator = torch.Generator().manual_seed(tokens)
+    weight_1, weight_2 = mx_quantize_expert_weights(
+        torch.randn(4 * 512, 256, generator=generator).to(device), torch.randn(4 * 256, 256, generator=generator).to(device), 4
+    )
+    inputs = [torch.randn(tokens, 256, generator=generator).to(device).bfloat16() for _ in range(2)]
+    scores, top_experts = (t.to(device) for t in torch.topk(torch.rand(tokens, 4, generator=generator), 2))
+
+    def call(x):
+        rows = mx_quantize(x, format)
+        return mx_mlp(rows, scores, top_experts, weight_1, weight_2, 4, gated=True, activation_type="silu")
+
+    alone = [call(x) for x in inputs]
+    streams = [torch.cuda.Stream(device) for _ in inputs]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(8):
+        for x, stream in zip(inputs, streams):
+            with torch.cuda.stream(stream):
+                results.append(call(x))
+    torch.cuda.synchronize()
+    for i, result in enumerate(results):
+        assert torch.equal(result, alone[i % 2])

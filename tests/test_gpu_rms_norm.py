@@ -204,3 +204,16 @@ def test_module_and_graph(device):
         eager = step(*(t.clone().requires_grad_(True) for t in new))
         assert all(torch.equal(a, b) for a, b in zip(captured, eager))
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize(("rows", "columns"), [((1 << 26) + 5, 8), ((1 << 24) + 3, 3)])
+def test_more_rows_than_a_launch_counts_threads(rows, columns, device):
+    x = torch.randn(1 << 16, columns, device=device, dtype=torch.float16).repeat(rows // (1 << 16) + 1, 1)[:rows]
+    weight = torch.randn(columns, device=device, dtype=torch.float16)
+    first, _, quantized = rms_norm_quantize(x[: 1 << 16], weight)
+    normalized, _, values = rms_norm_quantize(x, weight)
+    for start in range(0, rows, 1 << 22):
+        end = min(start + (1 << 22), rows)
+        assert torch.equal(normalized[start:end], first.repeat(64, 1)[: end - start])
+        assert torch.equal(values.values[start:end], quantized.values.repeat(64, 1)[: end - start])
+        assert torch.equal(values.scales[start:end], quantized.scales.repeat(64, 1)[: end - start])

@@ -164,3 +164,15 @@ def test_norm_validates_before_launching(library):
 
     for bad in (dict(grad=None), dict(workspace=None), dict(workspace_size=255), dict(workspace=FAKE + 4)):
         assert backward(**bad) == INVALID, bad
+
+
+def test_sizes_past_what_is_counted_in_32_bits_are_refused(library):
+    assert library.fm_mx_quantize(FAKE, FAKE, FAKE, 1 << 31, 64, 64, 1, 0, None) == UNSUPPORTED
+    assert library.fm_mx_quantize(FAKE, FAKE, FAKE, 1 << 30, 1 << 20, 1 << 20, 1, 0, None) == UNSUPPORTED
+    assert library.fm_mx_dequantize(FAKE, FAKE, FAKE, 1 << 30, 1 << 20, 1 << 20, 1 << 15, 1, 0, None) == UNSUPPORTED
+    assert library.fm_mx_copy_dense_to_sparse(FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 24, 64, 2, 1 << 25, 128, 4, 0, 1, None) == UNSUPPORTED
+    # 200 rows, or their scales, over more than 4 GiB
+    few_tokens = library.fm_mx_few_tokens_forward
+    for stride, scale_stride in ((1 << 25, 4), (128, 1 << 25)):
+        status = few_tokens(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 200, 2, 64, 100, 8, stride, scale_stride, 64, 4, 64, 4, 1, 1, 0, 1, FAKE, 1 << 24, None)
+        assert status == UNSUPPORTED, (stride, scale_stride)
