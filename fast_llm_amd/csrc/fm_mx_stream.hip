@@ -97,13 +97,15 @@ __global__ __launch_bounds__(kSplit * kAcross * 64, kGated ? 3 : 4) void stream_
     const int first = (blockIdx.x * kAcross + across) * 32;  // of the result's columns
     const int columns = static_cast<int>(args.columns), inner = static_cast<int>(args.inner), chunks = (inner + kChunk - 1) / kChunk;
     const int64_t weight_stride = args.weight_stride, scale_stride = args.weight_scale_stride;
+    // To the end of the last row and no further: loads of 16 bytes reach behind it.
+    const auto scale_bytes_of = [&](int64_t count, int64_t stride) { return count > 0 ? (count - 1) * stride + inner / kBlock : 0; };
     __amdgpu_buffer_rsrc_t weight[kSets], weight_scale_buffers[kSets];
 #pragma unroll
     for (int s = 0; s < kSets; ++s) {
         const int valid = min(columns - first, 32);  // may be negative: nothing is read
         const int64_t row = static_cast<int64_t>(expert) * columns * kSets + first + s * columns;
         weight[s] = buffer_of(args.weight + row * weight_stride, valid * weight_stride);
-        weight_scale_buffers[s] = buffer_of(args.weight_scales + row * scale_stride, valid * scale_stride);
+        weight_scale_buffers[s] = buffer_of(args.weight_scales + row * scale_stride, scale_bytes_of(valid, scale_stride));
     }
     const uint32_t weight_offset = static_cast<uint32_t>((lane >> 3) * weight_stride + (lane & 7) * 16);
     const uint32_t eight_rows = static_cast<uint32_t>(8 * weight_stride);
@@ -158,10 +160,10 @@ __global__ __launch_bounds__(kSplit * kAcross * 64, kGated ? 3 : 4) void stream_
         __amdgpu_buffer_rsrc_t x, x_scale_buffer;
         if constexpr (kSource == kByEntries) {
             x = buffer_of(args.x, args.x_rows * args.x_stride);
-            x_scale_buffer = buffer_of(args.x_scales, args.x_rows * args.x_scale_stride);
+            x_scale_buffer = buffer_of(args.x_scales, scale_bytes_of(args.x_rows, args.x_scale_stride));
         } else {
             x = buffer_of(args.x + (first_row + base) * args.x_stride, min(rows - base, 32) * args.x_stride);
-            x_scale_buffer = buffer_of(args.x_scales + (first_row + base) * args.x_scale_stride, min(rows - base, 32) * args.x_scale_stride);
+            x_scale_buffer = buffer_of(args.x_scales + (first_row + base) * args.x_scale_stride, scale_bytes_of(min(rows - base, 32), args.x_scale_stride));
         }
         const auto row_of = [&](int token) {  // of x; -1: none
             if (base + token >= rows) return -1;

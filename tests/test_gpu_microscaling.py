@@ -408,6 +408,20 @@ def test_scales_that_are_far_apart(of_rows, format, device):
     assert torch.equal(mx_sparse_matmul(lhs, rhs, dtype=torch.float32), plain)
 
 
+@pytest.mark.parametrize("rows", [8, 300])
+@pytest.mark.parametrize("inner", [128, 640])
+def test_scales_that_end_with_their_memory(rows, inner, device):
+    generator = torch.Generator().manual_seed(rows + inner)
+    lhs, rhs = _whole(generator, (rows, inner), device, "e4m3"), _whole(generator, (64, inner), device, "e2m1")
+    expected = _values(lhs) @ _values(rhs).t()
+    for tensor in (lhs, rhs):
+        memory = torch.empty(tensor.rows, 1 << 16, dtype=torch.uint8, device=device)
+        scales = memory[:, memory.size(1) - tensor.scales.size(1) :]
+        scales.copy_(tensor.scales)
+        tensor.scales = scales
+    assert torch.equal(mx_sparse_matmul(lhs, rhs, dtype=torch.float32).cpu().double(), expected)
+
+
 def test_a_row_by_itself_is_quantised(device):
     row = torch.randn(100, device=device)
     for ours, theirs in zip(_stored(mx_quantize(row)), _stored(mx_quantize(row[None]))):
