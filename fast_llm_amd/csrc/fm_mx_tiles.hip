@@ -129,7 +129,13 @@ struct Experts {
             tile.row0 = __builtin_amdgcn_readfirstlane(static_cast<int>(found.row0));  // rows are counted in 31 bits
             return __builtin_amdgcn_readfirstlane(static_cast<int>(exists)) != 0;
         }
-        if (logical >= before[2] * args.tiles_n) return false;
+        // Where half of the workgroups or fewer have a tile in the last round, they have the halves of one each: 14336 -> 4096, 16384 rows of 8 experts (1104
+        // tiles, 80 in the last round) in e4m3 757 -> 724 us, in e2m1 548 -> 533.
+        const int total = before[2] * args.tiles_n, last_round = total & ~(kResident - 1);
+        const bool halved = total - last_round <= kResident / 2 && logical >= last_round;
+        const bool second = halved && (logical & 1);
+        if (halved) logical = last_round + (logical - last_round) / 2;
+        if (logical >= total) return false;
         const int part = logical >= before[1] * args.tiles_n;
         const int lasts = part ? last[1] : last[0], counts = part ? count[1] : count[0];
         const uint64_t owners = __ballot(lasts * args.tiles_n > logical);
@@ -139,9 +145,9 @@ struct Experts {
         int row_tile;
         place_in_expert(logical - (owner_last - owner_count) * args.tiles_n, owner_count, args.tiles_n, row_tile, tile.tile_n);
         tile.expert = part * 64 + owner;
-        tile.row0 = first + row_tile * kTile;
-        tile.rows_valid = min(kTile, past - static_cast<int>(tile.row0));
-        return true;
+        tile.row0 = first + row_tile * kTile + (second ? kTile / 2 : 0);
+        tile.rows_valid = min(halved ? kTile / 2 : kTile, past - static_cast<int>(tile.row0));
+        return tile.rows_valid > 0;  // (a workgroup whose second half is empty has nothing after it)
     }
 };
 

@@ -395,6 +395,22 @@ def test_tiles_take_strides_and_index_types(index_dtype, format, device):
 
 
 @pytest.mark.parametrize("format", FORMATS)
+# Of tiles of 256 x 256: 156, fewer than CUs; 453, over half a round after a whole one; 297 and 300, under half a round after a whole one, where the
+# second halves of an expert's last tile have 40, 2, 0 and 0 rows.
+@pytest.mark.parametrize("counts", [[9864, 3201], [30000, 8300], [25000, 130], [20096, 5128, 0]], ids=str)
+def test_rounds_of_tiles(counts, format, device):
+    generator = torch.Generator().manual_seed(sum(counts))
+    inner, columns = 512, 516
+    sparse_map = _map(counts, device)
+    lhs = _whole(generator, (sparse_map.num_rows, inner), device, format)
+    rhs = _whole(generator, (len(counts) * columns, inner), device, "e2m1")
+    out = mx_sparse_matmul(lhs, rhs, sparse_map, dtype=torch.float32).cpu()
+    rows, weight = _values(lhs).float(), _values(rhs).float().view(len(counts), columns, inner)
+    for expert, begin, end in _real_rows(sparse_map):
+        assert torch.equal(out[begin:end], rows[begin:end] @ weight[expert].t())
+
+
+@pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("of_rows", [True, False])
 def test_scales_that_are_far_apart(of_rows, format, device):
     """The rows of scales of one tile lie over 2 GiB of memory, those of a block of 32 rows within 4 GiB."""
