@@ -70,10 +70,20 @@ __device__ __forceinline__ void load_to_lds_if(uint32_t lanes, __amdgpu_buffer_r
                  : "memory", "scc");
 }
 
-// A block of sums, in accumulation registers up to here.
-__device__ __forceinline__ f32x16_t settled(f32x16_t sums) {
-    asm volatile("" : "+a"(sums));
-    return sums;
+// The products before this are done when it is over. (The compiler counts a product's 16 passes up to the instructions that it knows to read its sums,
+// and does not look into assembly.)
+__device__ __forceinline__ void wait_for_products() { asm volatile("s_nop 15\n\ts_nop 7"); }
+
+// A block of sums, in accumulation registers up to here. (One by one: the compiler would copy a block that is handed over whole.) After `wait_for_products`.
+__device__ __forceinline__ f32x16_t settled(const f32x16_t &sums) {
+    f32x16_t values;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float value;
+        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(value) : "a"(sums[i]));
+        values[i] = value;
+    }
+    return values;
 }
 
 // The same value, computed no earlier than where this stands.
@@ -435,6 +445,9 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         if (blocks == kBlocks) multiply_tile(std::integral_constant<int, kBlocks>{});
         else multiply_tile(std::integral_constant<int, kBlocks / 2>{});
         const bool last_tile = !more;
+        __builtin_amdgcn_sched_barrier(0);
+        wait_for_products();
+        __builtin_amdgcn_sched_barrier(0);
 
         // ---- the tile's results: of block (n, m) a lane has columns 16 half .. + 15 of one row ---------------------------
         const int row_start = wave_m * blocks * 32, col0 = tile.tile_n * kColumns, out_lane = opaque(lane);
