@@ -9,6 +9,10 @@
 // A row's slice is 128 bytes (e4m3) or 64 (e2m1), in LDS XOR-swizzled in units of 16 bytes so that 16 lanes that read the same unit of
 // neighbouring rows hit all 64 banks. Of every 32 weight rows, LDS row 8 a + 4 h + b holds row 16 h + 4 a + b: a lane (h: its half of the
 // wavefront) then has 16 neighbouring columns of its row, and results leave without a way through LDS, which is full of the next tile's slices.
+//
+// Measured, 16384 rows of 8 experts: 4096 -> 2 x 14336 with the gated activation 1473 us (e4m3, 2.6 PFLOP/s), 14336 -> 4096 720 us (2.7) and in e2m1
+// 530 us (3.6); a loop of the instruction in registers on random data: 4.16 and 6.58. The chip is at its power limit (1.9 to 2.0 GHz; with zeros for
+// data 17 % faster). 30006 rows of 64 experts, 2048 -> 2 x 1408: 170 us, of which the results' way out takes 22 %.
 #include "fm_activation_math.h"
 #include "fm_mx_product.h"
 
