@@ -97,6 +97,11 @@ SIGNATURES: dict[str, tuple] = {
     "fm_mx_sparse_matmul_activation": (_c_int, [_c_ptr] * 8 + [_c_i64] * 8 + [_c_int] * 4 + [_c_ptr]),
     "fm_mx_few_tokens_workspace_size": (_c_size, [_c_i64] * 5 + [_c_int]),
     "fm_mx_few_tokens_forward": (_c_int, [_c_ptr] * 9 + [_c_i64] * 11 + [_c_int] * 4 + [_c_ptr, _c_size, _c_ptr]),
+    "fm_mx_mlp_workspace_size": (_c_size, [_c_i64] * 5 + [_c_int] * 2),
+    "fm_mx_mlp_forward": (
+        _c_int,
+        [_c_ptr] * 9 + [_c_i64] * 11 + [_c_int] * 4 + [_c_ptr, _c_size, _c_i64, _c_ptr, _c_size, _c_ptr],
+    ),
     "fm_rms_norm_forward": (_c_int, [_c_ptr] * 7 + [_c_i64] * 2 + [ctypes.c_double] + [_c_int] * 3 + [_c_ptr]),
     "fm_rms_norm_backward_workspace_size": (_c_size, [_c_i64] * 2),
     "fm_rms_norm_backward": (_c_int, [_c_ptr] * 6 + [_c_i64] * 2 + [ctypes.c_double] + [_c_int] * 2 + [_c_ptr, _c_size, _c_ptr]),

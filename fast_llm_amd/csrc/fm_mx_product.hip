@@ -177,3 +177,94 @@ extern "C" int fm_mx_few_tokens_forward(const void *input, const void *input_sca
     if (int status = mx::few_tokens(layer_1, layer_2, static_cast<const float *>(scores), output, out_dtype, static_cast<hipStream_t>(stream))) return status;
     return check_launch(name);
 }
+
+namespace {
+
+// Where the scratch of the MLP with a sparse map lies: the map, the activations, and the rows in front of layer 1, which the rows behind layer 2 replace.
+struct MlpLayout {
+    int64_t rows;
+    int index_dtype;
+    size_t ends_at, pad_begins_at, map_at, map_size, rows_at, row_scales_at, activations_at, activation_scales_at, size;
+};
+
+bool mlp_layout(MlpLayout &layout, int64_t tokens, int64_t slots, int64_t hidden, int64_t ffn, int64_t experts, int format, int out_dtype) {
+    if (tokens <= 0 || slots <= 0 || hidden <= 0 || ffn <= 0 || experts <= 0 || experts > 1024 || !mx::valid_format(format) || !valid_dtype(out_dtype)) return false;
+    if (tokens >= (int64_t(1) << 24) || slots > 1024 || tokens * slots >= (int64_t(1) << 31) - 128 * 1024 || hidden > (1 << 24) || ffn > (1 << 24)) return false;
+    constexpr int64_t kBlock = 128;
+    layout.rows = (tokens * slots + experts * kBlock) / kBlock * kBlock;
+    layout.index_dtype = layout.rows < 32768 ? FM_INDEX_I16 : FM_INDEX_I32;
+    const size_t index_size = layout.rows < 32768 ? 2 : 4;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t start = at;
+        at += (bytes + 255) / 256 * 256;
+        return start;
+    };
+    const int64_t padded = mx::padded_columns(hidden), ffn_padded = mx::padded_columns(ffn);
+    take(tokens * slots * index_size);  // sparse_rows
+    layout.ends_at = take(experts * index_size), layout.pad_begins_at = take(experts * index_size);
+    layout.map_size = max(fm_sparse_map_workspace_size(tokens, slots, experts), fm_sparse_map_from_router_workspace_size(tokens, experts));
+    layout.map_at = take(layout.map_size);
+    layout.activations_at = take(layout.rows * mx::value_bytes(format, ffn_padded)), layout.activation_scales_at = take(layout.rows * mx::scale_bytes(ffn_padded));
+    layout.rows_at = at, layout.row_scales_at = at + (layout.rows * mx::value_bytes(format, padded) + 255) / 256 * 256;
+    const size_t before = layout.row_scales_at - at + layout.rows * mx::scale_bytes(padded), after = layout.rows * hidden * dtype_size(out_dtype);
+    take(max(before, after));
+    layout.size = at;
+    return true;
+}
+
+}  // namespace
+
+extern "C" size_t fm_mx_mlp_workspace_size(int64_t num_tokens, int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int format,
+                                           int out_dtype) {
+    MlpLayout layout;
+    return mlp_layout(layout, num_tokens, slots_per_token, hidden, ffn, num_experts, format, out_dtype) ? layout.size : 0;
+}
+
+extern "C" int fm_mx_mlp_forward(const void *input, const void *input_scales, const void *top_experts, const void *scores, const void *weight_1,
+                                 const void *weight_1_scales, const void *weight_2, const void *weight_2_scales, void *output, int64_t num_tokens,
+                                 int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int64_t input_stride,
+                                 int64_t input_scale_stride, int64_t weight_1_stride, int64_t weight_1_scale_stride, int64_t weight_2_stride,
+                                 int64_t weight_2_scale_stride, int gated, int activation, int format, int out_dtype, const void *router_workspace,
+                                 size_t router_workspace_size, int64_t shared_experts, void *workspace, size_t workspace_size, void *stream) {
+    const char *name = "fm_mx_mlp_forward";
+    FM_REQUIRE(mx::valid_format(format), "%s: bad format %d", name, format);
+    FM_REQUIRE(valid_dtype(out_dtype), "%s: bad dtype %d", name, out_dtype);
+    FM_REQUIRE(activation >= FM_ACT_GELU && activation <= FM_ACT_IDENTITY, "%s: bad activation %d", name, activation);
+    MlpLayout layout;
+    if (!mlp_layout(layout, num_tokens, slots_per_token, hidden, ffn, num_experts, format, out_dtype)) return fail(FM_ERR_UNSUPPORTED, "%s: bad sizes", name);
+    FM_REQUIRE(top_experts && scores && output, "%s: null tensor", name);
+    FM_REQUIRE(shared_experts >= 0 && (router_workspace == nullptr || shared_experts < slots_per_token), "%s: bad shared_experts", name);
+    // All that the launches below check, before the first of them.
+    const int64_t padded = mx::padded_columns(hidden), layer_1_rows = num_experts * ffn * (gated ? 2 : 1);
+    if (int status = check_tensor(name, "the input", input, input_scales, num_tokens, padded, input_stride, input_scale_stride, format)) return status;
+    if (int status = check_tensor(name, "layer 1", weight_1, weight_1_scales, layer_1_rows, padded, weight_1_stride, weight_1_scale_stride, FM_MX_E2M1)) return status;
+    if (int status = check_tensor(name, "layer 2", weight_2, weight_2_scales, num_experts * hidden, mx::padded_columns(ffn), weight_2_stride, weight_2_scale_stride, FM_MX_E2M1))
+        return status;
+    FM_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_size >= layout.size,
+               "%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", name, layout.size, workspace_size);
+    char *scratch = static_cast<char *>(workspace);
+    void *ends = scratch + layout.ends_at, *pad_begins = scratch + layout.pad_begins_at, *map_scratch = scratch + layout.map_at;
+    void *rows = scratch + layout.rows_at, *row_scales = scratch + layout.row_scales_at;
+    void *activations = scratch + layout.activations_at, *activation_scales = scratch + layout.activation_scales_at;
+    const int64_t *experts = static_cast<const int64_t *>(top_experts);
+    const int index = layout.index_dtype;
+    int status = router_workspace != nullptr
+                     ? fm_sparse_map_from_router(experts, router_workspace, router_workspace_size, num_tokens, num_experts, slots_per_token - shared_experts,
+                                                 shared_experts, 128, index, scratch, ends, pad_begins, map_scratch, layout.map_size, stream)
+                     : fm_sparse_map(experts, num_tokens, slots_per_token, num_experts, 128, index, scratch, ends, pad_begins, map_scratch, layout.map_size, stream);
+    if (status < 0) return status;
+    status = fm_mx_copy_dense_to_sparse(input, input_scales, scratch, rows, row_scales, num_tokens, hidden, slots_per_token, layout.rows, input_stride,
+                                        input_scale_stride, format, index, stream);
+    if (status < 0) return status;
+    status = fm_mx_sparse_matmul_activation(rows, row_scales, weight_1, weight_1_scales, activations, activation_scales, ends, pad_begins, layout.rows, ffn, hidden,
+                                            num_experts, mx::value_bytes(format, padded), mx::scale_bytes(padded), weight_1_stride, weight_1_scale_stride, gated,
+                                            activation, format, index, stream);
+    if (status < 0) return status;
+    const int64_t ffn_padded = mx::padded_columns(ffn);
+    status = fm_mx_sparse_matmul(activations, activation_scales, weight_2, weight_2_scales, rows, ends, pad_begins, layout.rows, hidden, ffn, num_experts,
+                                 mx::value_bytes(format, ffn_padded), mx::scale_bytes(ffn_padded), weight_2_stride, weight_2_scale_stride, hidden, format,
+                                 out_dtype, index, stream);
+    if (status < 0) return status;
+    return fm_copy_sparse_to_dense(rows, scores, scratch, output, num_tokens, hidden, slots_per_token, layout.rows, out_dtype, FM_DTYPE_F32, index, stream);
+}

@@ -17,7 +17,7 @@ import torch
 from fast_llm_amd import _lib
 from fast_llm_amd.functional.config import ActivationType
 from fast_llm_amd.functional.mlp import _activation_tag
-from fast_llm_amd.functional.sparse_copy import SparseMap, copy_sparse_to_dense, get_sparse_map
+from fast_llm_amd.functional.sparse_copy import SparseMap
 from fast_llm_amd.functional.utils import Assert, div, without_backward
 
 MX_BLOCK = 32
@@ -52,14 +52,19 @@ class MicroscaledTensor:
     format: MicroscalingFormat
 
     def __post_init__(self):
-        self.format = MicroscalingFormat(self.format)
-        groups = _padded(self.columns) // MX_COLUMN_MULTIPLE
-        Assert.eq(self.values.dtype, self.scales.dtype, torch.uint8)
-        Assert.eq(self.values.dim(), self.scales.dim(), 2)
-        Assert.eq(self.values.size(0), self.scales.size(0))
-        Assert.eq(self.values.size(1), groups * _BYTES[self.format])
-        Assert.eq(self.scales.size(1), groups * (MX_COLUMN_MULTIPLE // MX_BLOCK))
-        assert self.columns > 0 and self.values.stride(1) == 1 and self.scales.stride(1) == 1
+        if type(self.format) is not MicroscalingFormat:
+            self.format = MicroscalingFormat(self.format)
+        # One expression: it runs with every call that a tensor is made for.
+        groups, values, scales = _padded(self.columns) // MX_COLUMN_MULTIPLE, self.values, self.scales
+        assert (
+            self.columns > 0
+            and values.dtype == scales.dtype == torch.uint8
+            and values.dim() == scales.dim() == 2
+            and values.size(0) == scales.size(0)
+            and values.size(1) == groups * _BYTES[self.format]
+            and scales.size(1) == groups * (MX_COLUMN_MULTIPLE // MX_BLOCK)
+            and values.stride(1) == scales.stride(1) == 1
+        ), (values.dtype, values.shape, scales.dtype, scales.shape, self.columns, self.format)
 
     @property
     def rows(self) -> int:
@@ -288,24 +293,29 @@ def mx_mlp(
     )
     if tokens == 0 or slots == 0:
         return torch.zeros((tokens, hidden), dtype=dtype, device=device)
-    scores = scores.detach().float().contiguous()
-    size = 0
+    assert not top_experts.is_floating_point()
+    library, format_tag, dtype_tag, size = _lib.lib(), _tag(input_.format), _lib.dtype_tag(dtype), 0
     if tokens * slots <= MX_FEW_TOKENS_ROWS * num_experts:
-        size = _lib.lib().fm_mx_few_tokens_workspace_size(tokens, slots, hidden, ffn, num_experts, _tag(input_.format))
-    if size:
-        top_experts = top_experts.to(torch.int64).contiguous()
-        out = torch.empty((tokens, hidden), dtype=dtype, device=device)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        _lib.call(
-            "fm_mx_few_tokens_forward", device, input_.values.data_ptr(), input_.scales.data_ptr(), top_experts.data_ptr(),
-            scores.data_ptr(), weight_1.values.data_ptr(), weight_1.scales.data_ptr(), weight_2.values.data_ptr(),
-            weight_2.scales.data_ptr(), out.data_ptr(), tokens, slots, hidden, ffn, num_experts, *_strides(input_),
-            *_strides(weight_1), *_strides(weight_2), int(gated), activation, _tag(input_.format), _lib.dtype_tag(dtype),
-            workspace.data_ptr(), size,
-        )  # fmt: skip
-    else:
-        sparse_map = get_sparse_map(top_experts, num_experts, router_counts=router_counts)
-        rows = mx_copy_dense_to_sparse(input_, sparse_map)
-        rows = mx_sparse_matmul_activation(rows, weight_1, sparse_map, gated, activation_type)
-        out = copy_sparse_to_dense(mx_sparse_matmul(rows, weight_2, sparse_map, dtype=dtype), scores, sparse_map)
+        size = library.fm_mx_few_tokens_workspace_size(tokens, slots, hidden, ffn, num_experts, format_tag)
+    name, counts = "fm_mx_few_tokens_forward", ()
+    if not size:
+        # With a sparse map, from the router's own counts where they are of these very experts.
+        size = library.fm_mx_mlp_workspace_size(tokens, slots, hidden, ffn, num_experts, format_tag, dtype_tag)
+        name, counts = "fm_mx_mlp_forward", (None, 0, 0)
+        if router_counts is not None and router_counts.describes(top_experts):
+            Assert.eq(router_counts.tokens, tokens)
+            Assert.eq(router_counts.shared_experts + router_counts.experts_per_token, slots)
+            Assert.eq(router_counts.shared_experts + router_counts.routed_experts, num_experts)
+            _lib.require_device(top_experts, router_counts.workspace)
+            counts = router_counts.workspace
+            counts = counts.data_ptr(), counts.numel() * counts.element_size(), router_counts.shared_experts
+    top_experts, scores = top_experts.to(torch.int64).contiguous(), scores.detach().float().contiguous()
+    out = torch.empty((tokens, hidden), dtype=dtype, device=device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _lib.call(
+        name, device, input_.values.data_ptr(), input_.scales.data_ptr(), top_experts.data_ptr(), scores.data_ptr(),
+        weight_1.values.data_ptr(), weight_1.scales.data_ptr(), weight_2.values.data_ptr(), weight_2.scales.data_ptr(),
+        out.data_ptr(), tokens, slots, hidden, ffn, num_experts, *_strides(input_), *_strides(weight_1), *_strides(weight_2),
+        int(gated), activation, format_tag, dtype_tag, *counts, workspace.data_ptr(), size,
+    )  # fmt: skip
     return without_backward(out) if requires_grad else out

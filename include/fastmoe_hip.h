@@ -493,6 +493,17 @@ int fm_mx_few_tokens_forward(const void *input, const void *input_scales, const 
                              int64_t input_scale_stride, int64_t weight_1_stride, int64_t weight_1_scale_stride, int64_t weight_2_stride,
                              int64_t weight_2_scale_stride, int gated, int activation, int format, int out_dtype, void *workspace,
                              size_t workspace_size, void *stream);
+/* The same MLP for any number of tokens, by way of a sparse map padded to multiples of 128: the launches of fm_sparse_map, fm_mx_copy_dense_to_sparse,
+ * fm_mx_sparse_matmul_activation, fm_mx_sparse_matmul (into rows of `out_dtype`) and fm_copy_sparse_to_dense one after the other, with their results, bit for bit.
+ * `router_workspace`: null, or what fm_router_forward left for these top_experts with their `shared_experts` (as for fm_sparse_map_from_router, with its
+ * precondition). `workspace`: 256-byte aligned. */
+size_t fm_mx_mlp_workspace_size(int64_t num_tokens, int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int format, int out_dtype);
+int fm_mx_mlp_forward(const void *input, const void *input_scales, const void *top_experts, const void *scores, const void *weight_1,
+                      const void *weight_1_scales, const void *weight_2, const void *weight_2_scales, void *output, int64_t num_tokens,
+                      int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int64_t input_stride,
+                      int64_t input_scale_stride, int64_t weight_1_stride, int64_t weight_1_scale_stride, int64_t weight_2_stride,
+                      int64_t weight_2_scale_stride, int gated, int activation, int format, int out_dtype, const void *router_workspace,
+                      size_t router_workspace_size, int64_t shared_experts, void *workspace, size_t workspace_size, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Root-mean-square norm with the residual's addition. Contiguous rows of `dtype`; `weight` of `dtype` or fp32.

@@ -8,7 +8,8 @@ from fast_llm_amd.functional.microscaling import (
     MicroscaledTensor, mx_copy_dense_to_sparse, mx_dequantize, mx_mlp, mx_quantize, mx_quantize_expert_weights, mx_sparse_matmul,
     mx_sparse_matmul_activation,
 )  # fmt: skip
-from fast_llm_amd.functional.sparse_copy import SparseMap, get_sparse_map
+from fast_llm_amd.functional.routing import router
+from fast_llm_amd.functional.sparse_copy import SparseMap, copy_sparse_to_dense, get_sparse_map
 from oracle import mx_oracle
 
 pytestmark = pytest.mark.gpu
@@ -471,3 +472,29 @@ def test_two_streams_at_once(tokens, format, device):
     torch.cuda.synchronize()
     for i, result in enumerate(results):
         assert torch.equal(result, alone[i % 2])
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize(("tokens", "experts", "slots"), [(300, 4, 2), (700, 60, 3), (33000, 2, 1)])
+@pytest.mark.parametrize("counted", [False, True])
+def test_mlp_is_its_operators_one_after_the_other(counted, tokens, experts, slots, format, device, monkeypatch):
+    monkeypatch.setattr(microscaling, "MX_FEW_TOKENS_ROWS", 0)
+    generator = torch.Generator().manual_seed(tokens)
+    hidden, ffn = 264, 200
+    weight_1, weight_2 = mx_quantize_expert_weights(
+        torch.randn(experts * 2 * ffn, hidden, generator=generator).to(device), torch.randn(experts * ffn, hidden, generator=generator).to(device), experts
+    )
+    rows = mx_quantize(torch.randn(tokens, hidden, generator=generator).to(device), format)
+    logits = torch.randn(tokens, experts, generator=generator).to(device)
+    scores, top_experts, _, _, counts = router(logits, slots, return_counts=True)
+    if not counted:
+        counts, top_experts = None, top_experts.clone()
+        top_experts[tokens // 2, 0] = -1
+    sparse_map = get_sparse_map(top_experts, experts)
+    between = mx_sparse_matmul_activation(mx_copy_dense_to_sparse(rows, sparse_map), weight_1, sparse_map, True, "silu")
+    for dtype in DTYPES:
+        expected = copy_sparse_to_dense(mx_sparse_matmul(between, weight_2, sparse_map, dtype=dtype), scores.float(), sparse_map)
+        output = mx_mlp(
+            rows, scores, top_experts, weight_1, weight_2, experts, gated=True, activation_type="silu", dtype=dtype, router_counts=counts
+        )
+        assert torch.equal(output, expected)

@@ -176,3 +176,21 @@ def test_sizes_past_what_is_counted_in_32_bits_are_refused(library):
     for stride, scale_stride in ((1 << 25, 4), (128, 1 << 25)):
         status = few_tokens(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 200, 2, 64, 100, 8, stride, scale_stride, 64, 4, 64, 4, 1, 1, 0, 1, FAKE, 1 << 24, None)
         assert status == UNSUPPORTED, (stride, scale_stride)
+
+
+def test_mlp_entry_point_validates_before_launching(library):
+    size = library.fm_mx_mlp_workspace_size
+    # 3 * 2 rows of 8 experts: 1024, int16; ffn 100 and hidden 64 are stored as 128
+    fixed = 3 * 256 + -(-max(library.fm_sparse_map_workspace_size(3, 2, 8), library.fm_sparse_map_from_router_workspace_size(3, 8)) // 256) * 256
+    assert size(3, 2, 64, 100, 8, 0, 1) == fixed + 1024 * 128 + 1024 * 4 + 1024 * 128 + 1024 * 4
+    for bad in ((0, 2, 64, 64, 8, 0, 1), (3, 0, 64, 64, 8, 0, 1), (3, 2, 64, 64, 1025, 0, 1), (3, 2, 64, 64, 8, 2, 1), (3, 2, 64, 64, 8, 0, 3), (1 << 24, 2, 64, 64, 8, 0, 1)):
+        assert size(*bad) == 0, bad
+
+    def forward(tokens=3, workspace=FAKE, workspace_size=1 << 30, activation=1, format=0, dtype=1, scores=FAKE, input_stride=128, weight_stride=64, router=None, shared=0):
+        return library.fm_mx_mlp_forward(FAKE, FAKE, FAKE, scores, FAKE, FAKE, FAKE, FAKE, FAKE, tokens, 2, 64, 100, 8, input_stride, 4, weight_stride, 4, 64, 4,
+                                         1, activation, format, dtype, router, 0, shared, workspace, workspace_size, None)  # fmt: skip
+
+    for bad in (dict(workspace=None), dict(workspace=FAKE + 16), dict(workspace_size=2000), dict(activation=-1), dict(format=3), dict(dtype=3),
+                dict(scores=None), dict(input_stride=120), dict(weight_stride=48), dict(shared=-1), dict(router=FAKE, shared=2)):  # fmt: skip
+        assert forward(**bad) == INVALID, bad
+    assert forward(tokens=1 << 24) == UNSUPPORTED
