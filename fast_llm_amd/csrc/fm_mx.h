@@ -67,6 +67,20 @@ __device__ __forceinline__ uint32_t pack_four(int format, float a, float b, floa
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(low, c * inverse, d * inverse, 1.f, 1) & 0xffffu & finite;
 }
 
+// Where eight columns from `column` on are read in a row of any length from 8: the row's last eight in place of what goes past its end.
+__device__ __forceinline__ int window(int column, int columns) { return min(column, columns - 8); }
+// Of such a window the values from `by` on (below 8) to the front, with zeros behind them.
+__device__ __forceinline__ void shift_down(float (&values)[8], int by) {
+#pragma unroll
+    for (int step = 4; step > 0; step /= 2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float next = i + step < 8 ? values[(i + step) % 8] : 0.f;
+            values[i] = by & step ? next : values[i];
+        }
+}
+constexpr int kNowhere = 0x7fffff00;  // past the end of any row
+
 // Eight neighbours per lane, four neighbouring lanes a block: writes the elements (8 or 4 bytes) and, from the block's first lane, the scale.
 // `column`: of the lane's first value, a multiple of 8. All lanes of the wavefront take part; `store`: whether this one's block exists.
 __device__ __forceinline__ void store_eight(int format, const float (&values)[8], uint8_t *row_values, uint8_t *row_scales, int64_t column, bool store) {

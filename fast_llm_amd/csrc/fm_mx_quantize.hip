@@ -36,19 +36,19 @@ struct Pieces {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_eight(__amdgpu_buffer_rsrc_t row, int column, float (&values)[8]) {
+__device__ __forceinline__ void load_eight(__amdgpu_buffer_rsrc_t row, int offset, float (&values)[8]) {
     constexpr int N = Vec16<T>::N;
 #pragma unroll
     for (int part = 0; part < 8 / N; ++part) {
-        const auto vector = __builtin_bit_cast(
-            Vec16<T>, __builtin_amdgcn_raw_buffer_load_b128(row, (column + part * N) * static_cast<int>(sizeof(T)), 0, kNonTemporal));
+        const auto vector = __builtin_bit_cast(Vec16<T>, __builtin_amdgcn_raw_buffer_load_b128(row, offset + part * 16, 0, kNonTemporal));
 #pragma unroll
         for (int i = 0; i < N; ++i) values[part * N + i] = to_float(vector.v[i]);
     }
 }
 
-// Four neighbouring lanes have a block, sixteen the 128 columns whose four scales make a word.
-template <typename T, int kFormat>
+// Four neighbouring lanes have a block, sixteen the 128 columns whose four scales make a word. kWhole: the rows are whole vectors of eight, aligned to 16
+// bytes; otherwise (from 8 columns on) loads are aligned as the values are, and the last lane of a row reads its last eight columns.
+template <typename T, int kFormat, bool kWhole>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *input, uint8_t *values, uint8_t *scales, int64_t rows, int64_t columns,
                                                             int64_t input_stride, int padded) {
     const int lane = threadIdx.x & 63;
@@ -56,8 +56,9 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *input, uint
     Pieces pieces(padded);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
+        const int column = pieces.part * kPiece + lane * 8, size = static_cast<int>(sizeof(T)), count = static_cast<int>(columns);
         load_eight<T>(row_buffer(input + pieces.row * input_stride, pieces.row < rows ? columns * static_cast<int64_t>(sizeof(T)) : 0),
-                      pieces.part * kPiece + lane * 8, loaded[u]);
+                      kWhole ? column * size : column < count ? window(column, count) * size : kNowhere, loaded[u]);
         pieces.next();
     }
     pieces = Pieces(padded);
@@ -68,6 +69,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *input, uint
         const __amdgpu_buffer_rsrc_t scale_row = row_buffer(scales + pieces.row * scale_bytes(padded), exists ? scale_bytes(padded) : 0);
         const int column = pieces.part * kPiece + lane * 8;
         pieces.next();
+        if constexpr (!kWhole) shift_down(loaded[u], max(column - window(column, static_cast<int>(columns)), 0) & 7);
         uint32_t largest = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) largest = max(largest, magnitude_bits(loaded[u][i]));
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *input, uint
     }
 }
 
-// Rows whose length or alignment does not allow loads of eight values: 256 columns of a row at a time.
+// Rows of less than eight columns: a value per lane.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantize_any_kernel(const T *input, uint8_t *values, uint8_t *scales, int64_t rows, int64_t columns,
                                                                 int64_t input_stride, int padded, int format) {
@@ -148,9 +150,9 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t *val
 #pragma unroll
         for (int i = 0; i < 8; ++i) result[i] *= factor;
         const __amdgpu_buffer_rsrc_t row = row_buffer(output + pieces.row * columns, pieces.row < rows ? columns * static_cast<int64_t>(sizeof(T)) : 0);
-        const int at = (pieces.part * kPiece + lane * 8) * static_cast<int>(sizeof(T));
+        const int column = pieces.part * kPiece + lane * 8, at = column * static_cast<int>(sizeof(T));
         pieces.next();
-        if (vectors) {
+        if (vectors || column + 8 <= columns) {
             constexpr int N = Vec16<T>::N;
 #pragma unroll
             for (int part = 0; part < 8 / N; ++part) {
@@ -162,6 +164,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t *val
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+                if (column + i >= columns) break;
                 if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, result[i]), row, at + 4 * i, 0, 0);
                 else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_float<T>(result[i])), row, at + 2 * i, 0, 0);
             }
@@ -218,18 +221,21 @@ extern "C" int fm_mx_quantize(const void *input, void *values, void *scales, int
     FM_REQUIRE(input && values && scales, "%s: null tensor", name);
     FM_REQUIRE(aligned16(values) && aligned16(scales), "%s: results are 16-byte aligned", name);
     const int64_t padded = mx::padded_columns(columns);
-    const bool vectors = columns % 8 == 0 && aligned16(input) && (rows == 1 || input_row_stride * dtype_size(dtype) % 16 == 0);
+    FM_REQUIRE(reinterpret_cast<uintptr_t>(input) % dtype_size(dtype) == 0, "%s: misaligned input", name);
+    const bool whole = columns % 8 == 0 && aligned16(input) && (rows == 1 || input_row_stride * dtype_size(dtype) % 16 == 0);
     if (rows >= (int64_t(1) << 31) || mx::piece_workgroups(rows, padded) == 0) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     FM_DISPATCH_DTYPE(dtype, T, {
         const T *typed = static_cast<const T *>(input);
         uint8_t *value_pointer = static_cast<uint8_t *>(values), *scale_pointer = static_cast<uint8_t *>(scales);
-        if (vectors) {
+        if (columns >= 8) {
             const auto launch = [&](auto kernel) {
                 kernel<<<static_cast<uint32_t>(mx::piece_workgroups(rows, padded)), mx::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                     typed, value_pointer, scale_pointer, rows, columns, input_row_stride, static_cast<int>(padded));
             };
-            if (format == FM_MX_E4M3) launch(mx::quantize_kernel<T, FM_MX_E4M3>);
-            else launch(mx::quantize_kernel<T, FM_MX_E2M1>);
+            if (whole && format == FM_MX_E4M3) launch(mx::quantize_kernel<T, FM_MX_E4M3, true>);
+            else if (whole) launch(mx::quantize_kernel<T, FM_MX_E2M1, true>);
+            else if (format == FM_MX_E4M3) launch(mx::quantize_kernel<T, FM_MX_E4M3, false>);
+            else launch(mx::quantize_kernel<T, FM_MX_E2M1, false>);
         } else {
             const int64_t workgroups = min(rows * ((padded + mx::kThreads - 1) / mx::kThreads), mx::kMaxWorkgroups - 1);
             mx::quantize_any_kernel<T><<<static_cast<uint32_t>(workgroups), mx::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
