@@ -7,12 +7,12 @@
 // What is normalised is the rounded stream, so that the backward needs nothing but it: v is computed again from the row that is in
 // registers anyway. All of a row is in the registers of one wavefront (up to 2048 columns), of four or of sixteen (8192, 32768), so each tensor
 // passes once: memory is the bound. Sums are in fp32: a lane's own values, then lanes, then wavefronts, in a fixed order.
-// Rows that are longer, or whose length is no multiple of 8, or that are not aligned to 16 bytes: a value per lane and load, the stream
-// read a second time.
+// Rows whose length is no multiple of 8 or that are not aligned to 16 bytes: the same loads, aligned as the values are, with a last lane that takes the
+// row's last eight columns. Rows of less than 8 columns and longer ones: a value per lane and load, the stream read a second time.
 //
-// Measured at 16384 x 2048 bf16 with a residual: forward 268 MB in 45.4 us (5.9 TB/s), backward 268 MB in 45.0 us and 4.2 us for the sum of 512
-// shares of the weight's gradient. (With the loads behind branches, the backward without the next row's: 51 and 89 us.) 5001 x 2048
-// fp16 with e4m3 beside it: 92 MB in 16.9 us.
+// Measured at 16384 x 2048 bf16 with a residual: forward 268 MB in 43.1 us (6.2 TB/s), backward 268 MB in 44.3 us and 4.2 us for the sum of 512
+// shares of the weight's gradient; with 2047 columns the same within 2 us (a value per lane took 80 and 306 us). (With the loads behind branches, the
+// backward without the next row's: 51 and 89 us.) 5001 x 2048 fp16 with e4m3 beside it: 92 MB in 16.3 us.
 #include "fm_mx.h"
 
 namespace fm {
@@ -55,32 +55,12 @@ __device__ __forceinline__ T settled(T value) {
     return value;
 }
 
-template <typename T>
-__device__ __forceinline__ Eight<T> zeros() {
-    Eight<T> eight;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) eight.set(i, 0.f);
-    return eight;
-}
-template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const void *base, int64_t offset) {
-    Eight<T> eight;
-#pragma unroll
-    for (int part = 0; part < 8 / Vec16<T>::N; ++part) eight.part[part] = load16(static_cast<const T *>(base) + offset + part * Vec16<T>::N);
-    return eight;
-}
-template <typename T>
-__device__ __forceinline__ void store_eight(void *base, int64_t offset, const Eight<T> &eight) {
-#pragma unroll
-    for (int part = 0; part < 8 / Vec16<T>::N; ++part) store16(static_cast<T *>(base) + offset + part * Vec16<T>::N, eight.part[part]);
-}
-
 // A row as a buffer: what is read past its end, or of a row (or a tensor) that does not exist, is zero, without a branch. (Behind
 // branches the compiler cannot count which loads are under way and waits for all.)
 template <typename T>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_of(const void *base, int64_t row, const Args &args) {
     const char *start = static_cast<const char *>(base) + row * args.columns * static_cast<int64_t>(sizeof(T));
-    const int bytes = base != nullptr && row < args.rows ? args.columns * static_cast<int>(sizeof(T)) : 0;
+    const int bytes = base != nullptr && row < args.rows ? args.columns * static_cast<int>(sizeof(T)) : 0;  // up to 128 KiB
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(uniform_pointer(start)), 0, __builtin_amdgcn_readfirstlane(bytes), kBufferResourceFlags);
 }
 template <typename T>
@@ -89,19 +69,45 @@ __device__ __forceinline__ Eight<T> load_eight(__amdgpu_buffer_rsrc_t row, int c
 #pragma unroll
     for (int part = 0; part < 8 / Vec16<T>::N; ++part)
         eight.part[part] = __builtin_bit_cast(
-            Vec16<T>, __builtin_amdgcn_raw_buffer_load_b128(row, (column + part * Vec16<T>::N) * static_cast<int>(sizeof(T)), 0, 0));
+            Vec16<T>, __builtin_amdgcn_raw_buffer_load_b128(row, column * static_cast<int>(sizeof(T)) + part * 16, 0, 0));
     return eight;
 }
-
-// The weight of eight columns. It has the input's type or fp32.
 template <typename T>
-__device__ __forceinline__ void load_weight(const Args &args, int column, float (&weight)[8]) {
+__device__ __forceinline__ void store_eight(__amdgpu_buffer_rsrc_t row, int column, const Eight<T> &eight) {
+    typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4_t;
+#pragma unroll
+    for (int part = 0; part < 8 / Vec16<T>::N; ++part)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, eight.part[part]), row, column * static_cast<int>(sizeof(T)) + part * 16, 0, 0);
+}
+
+// Where the eight columns that a lane has from `column` on are read and written, and how many of them are in front of `column`. Rows that are not
+// kWhole, multiples of 8 and aligned to 16 bytes, have a last lane that takes the row's last eight: of what it shares with the lane before it computes and
+// writes the same, and counts it in no sum.
+constexpr int kNowhere = mx::kNowhere / 4;
+template <bool kWhole>
+__device__ __forceinline__ int place(int column, int columns) {
+    return kWhole ? column : column < columns ? mx::window(column, columns) : kNowhere;
+}
+template <bool kWhole>
+__device__ __forceinline__ int shared(int column, int columns) {
+    return kWhole ? 0 : column < columns ? column - mx::window(column, columns) : 0;
+}
+
+// The weight, a row of the input's type or fp32, and eight of its columns.
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t weight_row(const Args &args) {
+    Args one = args;
+    one.rows = 1;
+    return args.weight_f32 ? row_of<float>(args.weight, 0, one) : row_of<T>(args.weight, 0, one);
+}
+template <typename T>
+__device__ __forceinline__ void load_weight(const Args &args, __amdgpu_buffer_rsrc_t row, int column, float (&weight)[8]) {
     if (args.weight_f32) {
-        const Eight<float> eight = load_eight<float>(args.weight, column);
+        const Eight<float> eight = load_eight<float>(row, column);
 #pragma unroll
         for (int i = 0; i < 8; ++i) weight[i] = eight[i];
     } else {
-        const Eight<T> eight = load_eight<T>(args.weight, column);
+        const Eight<T> eight = load_eight<T>(row, column);
 #pragma unroll
         for (int i = 0; i < 8; ++i) weight[i] = eight[i];
     }
@@ -154,62 +160,64 @@ template <int kLanes>
 constexpr int kThreads = kLanes < 256 ? 256 : kLanes;
 
 // kLanes threads a row, kVectors times eight columns each: vector v of lane l is the columns 8 (v kLanes + l) .. + 7.
-template <typename T, int kLanes, int kVectors>
+template <typename T, int kLanes, int kVectors, bool kWhole>
 __global__ __launch_bounds__(kThreads<kLanes>) void forward_kernel(Args args) {
     const int lane = threadIdx.x % kLanes;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads<kLanes> / kLanes) + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     if (row >= args.rows) return;  // whole wavefronts
-    const int64_t start = row * args.columns;
+    const auto column_of = [&](int v) { return (v * kLanes + lane) * 8; };
+    const auto place_of = [&](int v) { return place<kWhole>(column_of(v), args.columns); };
+    const auto shared_of = [&](int v) { return shared<kWhole>(column_of(v), args.columns); };
     Eight<T> stream[kVectors];
     const __amdgpu_buffer_rsrc_t input = row_of<T>(args.input, row, args);
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v) stream[v] = load_eight<T>(input, (v * kLanes + lane) * 8);
+    for (int v = 0; v < kVectors; ++v) stream[v] = load_eight<T>(input, place_of(v));
     if (args.residual != nullptr) {
         Eight<T> residual[kVectors];
-        const __amdgpu_buffer_rsrc_t residual_row = row_of<T>(args.residual, row, args);
+        const __amdgpu_buffer_rsrc_t residual_row = row_of<T>(args.residual, row, args), out = row_of<T>(args.stream, row, args);
 #pragma unroll
-        for (int v = 0; v < kVectors; ++v) residual[v] = load_eight<T>(residual_row, (v * kLanes + lane) * 8);
+        for (int v = 0; v < kVectors; ++v) residual[v] = load_eight<T>(residual_row, place_of(v));
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const int column = (v * kLanes + lane) * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) stream[v].set(i, stream[v][i] + residual[v][i]);
             settle(stream[v]);
-            if (column < args.columns) store_eight(args.stream, start + column, stream[v]);
+            store_eight(out, place_of(v), stream[v]);
         }
     }
     float sum[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[0] += stream[v][i] * stream[v][i];
+        for (int i = 0; i < 8; ++i) {
+            const float value = kWhole || i >= shared_of(v) ? stream[v][i] : 0.f;
+            sum[0] += value * value;
+        }
     row_sum<kLanes>(sum);
     const float inverse = inverse_root(args, sum[0]);
+    const __amdgpu_buffer_rsrc_t weights = weight_row<T>(args), out = row_of<T>(args.normalized, row, args);
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
-        const int column = (v * kLanes + lane) * 8;
-        const bool exists = column < args.columns;
-        Eight<T> result = zeros<T>();
-        if (exists) {
-            float weight[8];
-            load_weight<T>(args, column, weight);
+        float weight[8];
+        load_weight<T>(args, weights, place_of(v), weight);
+        Eight<T> result;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) result.set(i, stream[v][i] * inverse * weight[i]);
-            settle(result);
-            store_eight(args.normalized, start + column, result);
-        }
+        for (int i = 0; i < 8; ++i) result.set(i, stream[v][i] * inverse * weight[i]);
+        settle(result);
+        store_eight(out, place_of(v), result);
         if (args.values != nullptr) {
-            // Of the rounded result, as its quantisation by itself would be.
+            // Of the rounded result, as its quantisation by itself would be; zeros (not what an infinite root makes of them) behind the row.
             float values[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) values[i] = result[i];
+            for (int i = 0; i < 8; ++i) values[i] = column_of(v) < args.columns ? result[i] : 0.f;
+            if constexpr (!kWhole) mx::shift_down(values, shared_of(v));
             mx::store_eight(args.format, values, args.values + row * mx::value_bytes(args.format, args.padded),
-                            args.scales + row * mx::scale_bytes(args.padded), column, column < args.padded);
+                            args.scales + row * mx::scale_bytes(args.padded), column_of(v), column_of(v) < args.padded);
         }
     }
 }
 
-// Any length and alignment: a workgroup a row, a value a thread.
+// Rows of less than eight columns and the longest: a workgroup a row, a value a thread.
 constexpr int kAnyThreads = 256;
 
 template <typename T>
@@ -246,7 +254,7 @@ __global__ __launch_bounds__(kAnyThreads) void forward_any_kernel(Args args) {
 }
 
 // What a row's backward reads.
-template <typename T, int kLanes, int kVectors, bool kGradStream>
+template <typename T, int kLanes, int kVectors, bool kWhole, bool kGradStream>
 struct BackwardRow {
     Eight<T> stream[kVectors], grad[kVectors], grad_stream[kGradStream ? kVectors : 1];
     __device__ __forceinline__ void load(const Args &args, int64_t row, int lane) {
@@ -254,7 +262,7 @@ struct BackwardRow {
         const __amdgpu_buffer_rsrc_t grad_stream_row = row_of<T>(args.grad_stream, row, args);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const int column = (v * kLanes + lane) * 8;
+            const int column = place<kWhole>((v * kLanes + lane) * 8, args.columns);
             stream[v] = load_eight<T>(stream_row, column);
             grad[v] = load_eight<T>(grad_row, column);
             if constexpr (kGradStream) grad_stream[v] = load_eight<T>(grad_stream_row, column);
@@ -264,15 +272,18 @@ struct BackwardRow {
 
 // A group of kLanes threads walks over rows and keeps its share of the weight's gradient in registers; the groups of a workgroup add
 // theirs up in LDS, the workgroups theirs in `weight_gradient_kernel`.
-template <typename T, int kLanes, int kVectors>
+template <typename T, int kLanes, int kVectors, bool kWhole>
 __global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backward_kernel(Args args) {
     constexpr int kGroups = kThreads<kLanes> / kLanes;
     // The next row is asked for before this one is worked on and the weight stays in registers, but where the registers do not hold that (rows of
     // over 1024 or 4096 columns of fp32; 16 wavefronts on a CU): there the weight and the stream's gradient are read when they are needed.
     constexpr bool kAhead = kLanes < 1024 && kVectors * sizeof(T) <= 8;
-    using Row = BackwardRow<T, kLanes, kVectors, kAhead>;
+    using Row = BackwardRow<T, kLanes, kVectors, kWhole, kAhead>;
     const int lane = threadIdx.x % kLanes, group = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+    const auto place_of = [&](int v) { return place<kWhole>((v * kLanes + lane) * 8, args.columns); };
+    const auto shared_of = [&](int v) { return shared<kWhole>((v * kLanes + lane) * 8, args.columns); };
+    const __amdgpu_buffer_rsrc_t weight_buffer = weight_row<T>(args);
     float weight_grad[kVectors][8], weights[kAhead ? kVectors : 1][8];
 #pragma unroll
     for (int v = 0; v < kVectors; ++v)
@@ -284,10 +295,7 @@ __global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backw
         current.load(args, row, lane);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const int column = (v * kLanes + lane) * 8;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) weights[v][i] = 0.f;
-            if (column < args.columns) load_weight<T>(args, column, weights[v]);
+            load_weight<T>(args, weight_buffer, place_of(v), weights[v]);
         }
     }
     for (; row < args.rows; row += step) {
@@ -295,19 +303,18 @@ __global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backw
         else current.load(args, row, lane);
         auto &stream = current.stream;
         auto &grad = current.grad;
-        const int64_t start = row * args.columns;
+        const __amdgpu_buffer_rsrc_t out = row_of<T>(args.grad_input, row, args);
         float sums[2] = {0.f, 0.f};  // of s^2 and of g w s
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const int column = (v * kLanes + lane) * 8;
-            if (!kAhead && column >= args.columns) continue;
             float read[8];
-            if constexpr (!kAhead) load_weight<T>(args, column, read);
+            if constexpr (!kAhead) load_weight<T>(args, weight_buffer, place_of(v), read);
             const float(&weight)[8] = kAhead ? weights[kAhead ? v : 0] : read;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sums[0] += stream[v][i] * stream[v][i];
-                sums[1] += grad[v][i] * weight[i] * stream[v][i];
+                const bool counts = kWhole || i >= shared_of(v);
+                sums[0] += counts ? stream[v][i] * stream[v][i] : 0.f;
+                sums[1] += counts ? grad[v][i] * weight[i] * stream[v][i] : 0.f;
             }
         }
         row_sum<kLanes>(sums);
@@ -317,12 +324,10 @@ __global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backw
         for (int v = 0; v < kVectors; ++v) settle(stream[v]), settle(grad[v]);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const int column = (v * kLanes + lane) * 8;
-            if (column >= args.columns) continue;
             float read[8];
             if constexpr (!kAhead) {
-                load_weight<T>(args, column, read);
-                current.grad_stream[0] = load_eight<T>(row_of<T>(args.grad_stream, row, args), column);
+                load_weight<T>(args, weight_buffer, place_of(v), read);
+                current.grad_stream[0] = load_eight<T>(row_of<T>(args.grad_stream, row, args), place_of(v));
             }
             const float(&weight)[8] = kAhead ? weights[kAhead ? v : 0] : read;
             Eight<T> result;
@@ -331,19 +336,22 @@ __global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backw
                 result.set(i, inverse * (grad[v][i] * weight[i] - stream[v][i] * factor) + current.grad_stream[kAhead ? v : 0][i]);
                 weight_grad[v][i] += grad[v][i] * (stream[v][i] * inverse);
             }
-            store_eight(args.grad_input, start + column, result);
+            store_eight(out, place_of(v), result);
         }
         if constexpr (kAhead) current = next;
     }
     if (args.partials == nullptr) return;
     float *target = args.partials + static_cast<int64_t>(blockIdx.x) * args.columns;
+    if constexpr (!kWhole)
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) mx::shift_down(weight_grad[v], shared_of(v));
     if constexpr (kGroups == 1) {
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int column = (v * kLanes + lane) * 8;
-            if (column >= args.columns) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) target[column + i] = weight_grad[v][i];
+            for (int i = 0; i < 8; ++i)
+                if (kWhole ? column < args.columns : column + i < args.columns) target[column + i] = weight_grad[v][i];
         }
     } else {
         __shared__ float shared[kGroups][kLanes * 8];
@@ -364,7 +372,7 @@ __global__ __launch_bounds__(kThreads<kLanes>, kLanes < 1024 ? 2 : 1) void backw
     }
 }
 
-// Any length and alignment. The weight's gradient: a workgroup's share is in its row of `partials` from the first row on, each value
+// Rows of less than eight columns and the longest. The weight's gradient: a workgroup's share is in its row of `partials` from the first row on, each value
 // written and read by one thread.
 template <typename T>
 __global__ __launch_bounds__(kAnyThreads) void backward_any_kernel(Args args) {
@@ -418,8 +426,8 @@ constexpr int64_t kMaxColumns = int64_t(1) << 28;
 constexpr int kMaxParts = 512;
 
 // Threads of a row, 0: `..._any_kernel`.
-static int lanes_of(int64_t columns, bool aligned) {
-    if (!aligned || columns % 8 != 0 || columns > 32768) return 0;
+static int lanes_of(int64_t columns) {
+    if (columns < 8 || columns > 32768) return 0;
     return columns <= 2048 ? 64 : columns <= 8192 ? 256 : 1024;
 }
 
@@ -429,14 +437,18 @@ static int64_t parts_of(int64_t rows, int64_t columns) {
     return min((rows + at_once - 1) / at_once, static_cast<int64_t>(kMaxParts));
 }
 
-template <typename T, typename Launch>
-static void for_shape(int columns, int lanes, Launch launch) {
-    if (lanes == 64 && columns <= 512) launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-    else if (lanes == 64 && columns <= 1024) launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else if (lanes == 64) launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-    else if (lanes == 256 && columns <= 4096) launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    else if (lanes == 256) launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-    else launch(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+template <typename Launch>
+static void for_shape(int columns, int lanes, bool whole, Launch launch) {
+    const auto with = [&](auto lanes_constant, auto vectors) {
+        if (whole) launch(lanes_constant, vectors, std::true_type{});
+        else launch(lanes_constant, vectors, std::false_type{});
+    };
+    if (lanes == 64 && columns <= 512) with(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (lanes == 64 && columns <= 1024) with(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (lanes == 64) with(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    else if (lanes == 256 && columns <= 4096) with(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if (lanes == 256) with(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    else with(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
 }
 
 }  // namespace norm
@@ -464,8 +476,8 @@ extern "C" int fm_rms_norm_forward(const void *input, const void *residual, cons
     FM_REQUIRE(input && weight && normalized, "%s: null tensor", name);
     FM_REQUIRE((residual == nullptr) == (stream_out == nullptr), "%s: the residual and the stream that goes on come together", name);
     FM_REQUIRE(values == nullptr || (aligned16(values) && aligned16(scales)), "%s: microscaled results are 16-byte aligned", name);
-    const bool aligned = aligned16(input) && aligned16(residual) && aligned16(weight) && aligned16(stream_out) && aligned16(normalized);
-    const int lanes = norm::lanes_of(columns, aligned);
+    const bool whole = columns % 8 == 0 && aligned16(input) && aligned16(residual) && aligned16(weight) && aligned16(stream_out) && aligned16(normalized);
+    const int lanes = norm::lanes_of(columns);
     norm::Args args{};
     args.weight = weight, args.columns = static_cast<int>(columns), args.padded = static_cast<int>(mx::padded_columns(columns)), args.format = format;
     args.weight_f32 = weight_dtype == FM_DTYPE_F32 && dtype != FM_DTYPE_F32;
@@ -483,9 +495,9 @@ extern "C" int fm_rms_norm_forward(const void *input, const void *residual, cons
             if (lanes == 0) {
                 norm::forward_any_kernel<T><<<static_cast<uint32_t>(args.rows), norm::kAnyThreads, 0, static_cast<hipStream_t>(stream)>>>(args);
             } else {
-                norm::for_shape<T>(static_cast<int>(columns), lanes, [&](auto lanes_constant, auto vectors) {
+                norm::for_shape(static_cast<int>(columns), lanes, whole, [&](auto lanes_constant, auto vectors, auto whole_constant) {
                     constexpr int kLanes = decltype(lanes_constant)::value, kRows = norm::kThreads<kLanes> / kLanes;
-                    norm::forward_kernel<T, kLanes, decltype(vectors)::value>
+                    norm::forward_kernel<T, kLanes, decltype(vectors)::value, decltype(whole_constant)::value>
                         <<<static_cast<uint32_t>((args.rows + kRows - 1) / kRows), norm::kThreads<kLanes>, 0, static_cast<hipStream_t>(stream)>>>(args);
                 });
             }
@@ -516,8 +528,8 @@ extern "C" int fm_rms_norm_backward(const void *grad_normalized, const void *gra
     args.rows = rows, args.columns = static_cast<int>(columns);
     args.weight_f32 = weight_dtype == FM_DTYPE_F32 && dtype != FM_DTYPE_F32;
     args.eps = static_cast<float>(eps), args.inverse_columns = static_cast<float>(1. / static_cast<double>(columns));
-    const bool aligned = aligned16(grad_normalized) && aligned16(grad_stream) && aligned16(stream_in) && aligned16(weight) && aligned16(grad_input);
-    const int lanes = norm::lanes_of(columns, aligned);
+    const bool whole = columns % 8 == 0 && aligned16(grad_normalized) && aligned16(grad_stream) && aligned16(stream_in) && aligned16(weight) && aligned16(grad_input);
+    const int lanes = norm::lanes_of(columns);
     // Without rows the weight's gradient is the sum of nothing.
     const uint32_t parts = rows > 0 ? static_cast<uint32_t>(norm::parts_of(rows, columns)) : 0;
     if (rows > 0) {
@@ -525,9 +537,9 @@ extern "C" int fm_rms_norm_backward(const void *grad_normalized, const void *gra
             if (lanes == 0) {
                 norm::backward_any_kernel<T><<<parts, norm::kAnyThreads, 0, static_cast<hipStream_t>(stream)>>>(args);
             } else {
-                norm::for_shape<T>(static_cast<int>(columns), lanes, [&](auto lanes_constant, auto vectors) {
+                norm::for_shape(static_cast<int>(columns), lanes, whole, [&](auto lanes_constant, auto vectors, auto whole_constant) {
                     constexpr int kLanes = decltype(lanes_constant)::value;
-                    norm::backward_kernel<T, kLanes, decltype(vectors)::value>
+                    norm::backward_kernel<T, kLanes, decltype(vectors)::value, decltype(whole_constant)::value>
                         <<<parts, norm::kThreads<kLanes>, 0, static_cast<hipStream_t>(stream)>>>(args);
                 });
             }

@@ -498,3 +498,20 @@ def test_mlp_is_its_operators_one_after_the_other(counted, tokens, experts, slot
             rows, scores, top_experts, weight_1, weight_2, experts, gated=True, activation_type="silu", dtype=dtype, router_counts=counts
         )
         assert torch.equal(output, expected)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("columns", [7, 8, 9, 31, 100, 129, 511, 515, 1029])
+def test_quantize_rows_of_any_length_and_alignment(columns, dtype, format, device):
+    generator = torch.Generator().manual_seed(columns)
+    values = torch.randn(9, columns, generator=generator).to(dtype)
+    elements, scales = mx_oracle.quantize(values, format)
+    for stride, offset in ((columns, 1), (columns + 1, 0), (columns + 5, 3)):
+        storage = torch.full((9 * stride + offset + 16,), 100.0, dtype=dtype, device=device)
+        view = storage[offset : offset + 9 * stride].view(9, stride)[:, :columns]
+        view.copy_(values)
+        quantized = mx_quantize(view, format)
+        for ours, theirs in zip(_stored(quantized), mx_oracle.pack(elements, scales, format)):
+            assert torch.equal(ours, theirs)
+        assert torch.equal(mx_dequantize(quantized, dtype).cpu(), mx_oracle.values_of(elements, scales).to(dtype))

@@ -217,3 +217,38 @@ def test_more_rows_than_a_launch_counts_threads(rows, columns, device):
         assert torch.equal(normalized[start:end], first.repeat(64, 1)[: end - start])
         assert torch.equal(values.values[start:end], quantized.values.repeat(64, 1)[: end - start])
         assert torch.equal(values.scales[start:end], quantized.scales.repeat(64, 1)[: end - start])
+
+
+@pytest.mark.parametrize("columns", [9, 100, 513, 1027, 2044, 2049, 4091, 8190, 8194, 32763])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [0, 1])
+def test_rows_of_any_length_and_alignment(columns, dtype, offset, device):
+    """What a row's last lane shares with the lane before it counts once, and is written once or with the same value; nothing else is written."""
+    rows = 7
+    x, residual, weight, grads = _inputs(rows, columns, dtype, dtype, device)
+
+    def placed(values):
+        storage = torch.full((values.numel() + 16,), 3.0, dtype=dtype, device=device)
+        view = storage[offset : offset + values.numel()].view(values.shape)
+        view.copy_(values)
+        return view
+
+    leaves = [placed(t).requires_grad_(True) for t in (x, residual, weight)]
+    normalized, stream = rms_norm(leaves[0], leaves[2], leaves[1])
+    expected, expected_stream = mx_oracle.rms_norm(x, weight, residual, 1e-5)
+    assert torch.equal(stream.cpu(), expected_stream)
+    tolerance = ((_steps(columns) / 2 + 4) * 2.0**-24 + torch.finfo(dtype).eps / 2) * expected.abs() + torch.finfo(dtype).smallest_normal
+    assert ((normalized.cpu().double() - expected).abs() <= tolerance).all()
+    # Placed or not: the same kernel's bits, or those of the one for whole vectors up to the order of a sum.
+    grad_input, grad_residual, grad_weight = torch.autograd.grad((normalized, stream), leaves, [placed(g) for g in grads])
+    assert torch.equal(grad_input, grad_residual)
+    plain = [t.to(device).requires_grad_(True) for t in (x, residual, weight)]
+    results = torch.autograd.grad(rms_norm(plain[0], plain[2], plain[1]), plain, [g.to(device) for g in grads])
+    wide_grad, wide_weight = mx_oracle.rms_norm_backward(grads[0], grads[1], expected_stream, weight, 1e-5)
+    for ours, theirs, wide in ((grad_input, results[0], wide_grad), (grad_weight, results[2], wide_weight)):
+        # Sums of either order are off by a few steps of fp32 of the largest of their terms, results by half a step each.
+        slack = 2.0**-12 * wide.abs().max() if dtype == torch.float32 else 2 * torch.finfo(dtype).eps * wide.abs().max()
+        assert (ours.double().cpu() - wide).abs().max() <= slack and (ours - theirs).double().abs().max().cpu() <= slack
+    _, _, quantized = rms_norm_quantize(leaves[0].detach(), leaves[2].detach(), leaves[1].detach())
+    reference = mx_quantize(normalized)
+    assert torch.equal(quantized.values, reference.values) and torch.equal(quantized.scales, reference.scales)
