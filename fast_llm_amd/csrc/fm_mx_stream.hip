@@ -44,9 +44,6 @@ template <int kCachePolicy = 0>
 __device__ __forceinline__ u32x4_t load_16(__amdgpu_buffer_rsrc_t buffer, uint32_t offset) {
     return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(buffer, static_cast<int>(offset), 0, kCachePolicy));
 }
-__device__ __forceinline__ u32x2_t load_8(__amdgpu_buffer_rsrc_t buffer, uint32_t offset) {
-    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(buffer, static_cast<int>(offset), 0, 0));
-}
 
 // The scales of a row in a chunk, for the lanes of a group: byte 0 (and 2, where a row has two groups) of a word is that of the group's block.
 __device__ __forceinline__ void align_scales(u32x2_t &scales, bool second, int group) {

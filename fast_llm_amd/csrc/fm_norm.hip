@@ -475,6 +475,8 @@ extern "C" int fm_rms_norm_forward(const void *input, const void *residual, cons
     if (rows == 0) return FM_OK;
     FM_REQUIRE(input && weight && normalized, "%s: null tensor", name);
     FM_REQUIRE((residual == nullptr) == (stream_out == nullptr), "%s: the residual and the stream that goes on come together", name);
+    FM_REQUIRE(normalized != input && normalized != residual && stream_out != input && (stream_out == nullptr || stream_out != residual) && normalized != stream_out,
+               "%s: a result in place of an input", name);
     FM_REQUIRE(values == nullptr || (aligned16(values) && aligned16(scales)), "%s: microscaled results are 16-byte aligned", name);
     const bool whole = columns % 8 == 0 && aligned16(input) && aligned16(residual) && aligned16(weight) && aligned16(stream_out) && aligned16(normalized);
     const int lanes = norm::lanes_of(columns);
@@ -519,6 +521,7 @@ extern "C" int fm_rms_norm_backward(const void *grad_normalized, const void *gra
     const size_t needed = fm_rms_norm_backward_workspace_size(rows, columns);
     if (rows > 0) {
         FM_REQUIRE(grad_normalized && stream_in && weight && grad_input, "%s: null tensor", name);
+        FM_REQUIRE(grad_input != grad_normalized && grad_input != grad_stream && grad_input != stream_in, "%s: a result in place of an input", name);
         FM_REQUIRE(grad_weight == nullptr || (workspace && aligned16(workspace) && workspace_size >= needed),
                    "%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", name, needed, workspace_size);
     }

@@ -512,7 +512,8 @@ int fm_mx_mlp_forward(const void *input, const void *input_scales, const void *t
  * With `values` and `scales` (both or neither) also `normalized`, as rounded, microscaled in `format`, bit for bit as fm_mx_quantize gives it.
  * Backward, of the gradients of normalized and (may be null) of the stream: grad_input = v (g w - s v^2 mean(g w s)) + grad_stream, of input and
  * residual alike, one rounding; grad_weight (of weight_dtype; may be null: not computed) = sum over rows of g s v in fp32, in a fixed order, in
- * a `workspace` of fm_rms_norm_backward_workspace_size bytes (16-byte aligned).
+ * a `workspace` of fm_rms_norm_backward_workspace_size bytes (16-byte aligned). No result may overlap an input: rows are read and written in parts
+ * that can share columns (the same pointer for both is refused).
  * --------------------------------------------------------------------------------------------------------- */
 int fm_rms_norm_forward(const void *input, const void *residual, const void *weight, void *stream_out, void *normalized, void *values,
                         void *scales, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype, int format, void *stream);

@@ -194,3 +194,13 @@ def test_mlp_entry_point_validates_before_launching(library):
                 dict(scores=None), dict(input_stride=120), dict(weight_stride=48), dict(shared=-1), dict(router=FAKE, shared=2)):  # fmt: skip
         assert forward(**bad) == INVALID, bad
     assert forward(tokens=1 << 24) == UNSUPPORTED
+
+
+def test_norm_is_not_computed_in_place(library):
+    a, b, c, d = (FAKE * i for i in range(1, 5))
+    for stream, normalized in ((a, c), (b, c), (c, a), (c, b), (c, c)):
+        assert library.fm_rms_norm_forward(a, b, d, stream, normalized, None, None, 4, 64, 1e-5, 1, 1, 0, None) == INVALID, (stream, normalized)
+        assert b"in place" in library.fm_last_error()
+    for result in (a, b, c):
+        assert library.fm_rms_norm_backward(a, b, c, d, result, None, 4, 64, 1e-5, 1, 1, None, 0, None) == INVALID, result
+        assert b"in place" in library.fm_last_error()
