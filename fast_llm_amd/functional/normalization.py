@@ -24,10 +24,10 @@ def _forward(
     input_: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None, eps: float, quantized: MicroscaledTensor | None
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The normalised rows and the stream (the input itself without a residual)."""
-    input_, weight = input_.detach().contiguous(), weight.detach().contiguous()
+    input_, weight = input_.contiguous(), weight.contiguous()
     normalized, stream = torch.empty_like(input_), None
     if residual is not None:
-        residual, stream = residual.detach().contiguous(), torch.empty_like(input_)
+        residual, stream = residual.contiguous(), torch.empty_like(input_)
     device = _lib.require_device(input_, weight, residual)
     columns = input_.size(-1)
     _lib.call(
@@ -49,30 +49,37 @@ class _RMSNorm(torch.autograd.Function):
         return normalized if residual is None else (normalized, stream)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_normalized: torch.Tensor | None, grad_stream: torch.Tensor | None = None):
-        stream, weight = ctx.saved_tensors
-        if grad_normalized is None:
-            # Nothing depends on the norm.
-            grad_weight = torch.zeros_like(weight) if ctx.needs_input_grad[1] else None
-            return grad_stream, grad_weight, grad_stream if ctx.needs_input_grad[2] else None, None
-        grad_normalized, weight = grad_normalized.contiguous(), weight.contiguous()
-        if grad_stream is not None:
-            grad_stream = grad_stream.contiguous()
-        grad_input, grad_weight, workspace, size = torch.empty_like(stream), None, None, 0
-        columns = stream.size(-1)
-        rows = stream.numel() // columns
-        device = _lib.require_device(grad_normalized, grad_stream, stream, weight)
-        if ctx.needs_input_grad[1]:
-            grad_weight = torch.empty_like(weight)
-            size = _lib.lib().fm_rms_norm_backward_workspace_size(rows, columns)
-            workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        _lib.call(
-            "fm_rms_norm_backward", device, grad_normalized.data_ptr(), _lib.ptr(grad_stream), stream.data_ptr(),
-            weight.data_ptr(), grad_input.data_ptr(), _lib.ptr(grad_weight), rows, columns, ctx.eps,
-            _lib.dtype_tag(stream.dtype), _lib.dtype_tag(weight.dtype), _lib.ptr(workspace), size,
-        )  # fmt: skip
-        return grad_input, grad_weight, grad_input if ctx.needs_input_grad[2] else None, None
+    def backward(ctx, *grads: torch.Tensor | None):
+        # Without the guard where no graph of the gradients is made: in small steps its host time counts.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, *grads)
+
+
+def _backward(ctx, grad_normalized: torch.Tensor | None, grad_stream: torch.Tensor | None = None):
+    stream, weight = ctx.saved_tensors
+    _, needs_weight, needs_residual, _ = ctx.needs_input_grad
+    if grad_normalized is None:
+        # Nothing depends on the norm.
+        return grad_stream, torch.zeros_like(weight) if needs_weight else None, grad_stream if needs_residual else None, None
+    grad_normalized, weight = grad_normalized.contiguous(), weight.contiguous()
+    if grad_stream is not None:
+        grad_stream = grad_stream.contiguous()
+    grad_input, grad_weight, workspace, size = torch.empty_like(stream), None, None, 0
+    columns = weight.size(0)
+    rows = stream.numel() // columns
+    device = _lib.require_device(grad_normalized, grad_stream, stream, weight)
+    if needs_weight:
+        grad_weight = torch.empty_like(weight)
+        size = _lib.lib().fm_rms_norm_backward_workspace_size(rows, columns)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _lib.call(
+        "fm_rms_norm_backward", device, grad_normalized.data_ptr(), _lib.ptr(grad_stream), stream.data_ptr(),
+        weight.data_ptr(), grad_input.data_ptr(), _lib.ptr(grad_weight), rows, columns, ctx.eps,
+        _lib.dtype_tag(stream.dtype), _lib.dtype_tag(weight.dtype), _lib.ptr(workspace), size,
+    )  # fmt: skip
+    return grad_input, grad_weight, grad_input if needs_residual else None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def rms_norm(
