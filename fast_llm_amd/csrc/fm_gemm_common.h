@@ -54,6 +54,10 @@ struct GemmArgs {
 
 #define FM_LDS(T) __attribute__((address_space(3))) T
 
+// Goes between a scalar write of M0 and the load into LDS that reads it: one wait state, which the hardware does not keep by itself and the compiler does
+// not add inside of assembly.
+#define FM_M0_WAIT "\n\ts_nop 0\n\t"
+
 constexpr int kBufferResourceFlags = 0x00020000;  // raw buffer, 32-bit data format, no swizzle
 
 // The same value, but the compiler cannot tell: what is computed from it is computed where it is written, not hoisted

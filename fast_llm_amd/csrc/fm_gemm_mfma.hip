@@ -238,13 +238,13 @@ struct TileLoader {
         const int wave_address = __builtin_amdgcn_readfirstlane(slot_address + block_of(wave_index, 0) * 1024);
         // M0 is not handed out by the register allocator and nothing else in this file uses it.
         if constexpr (kRotates) {
-            asm volatile("s_add_i32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds"
+            asm volatile("s_add_i32 m0, %0, %3" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, %4 offen lds"
                          :
                          : "s"(wave_address), "v"(lane_offset), "s"(resource), "n"((block_of(0, j) - block_of(0, 0)) * 1024), "s"(slice_offset)
                          : "memory", "scc");
             return;
         }
-        asm volatile("s_add_i32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+        asm volatile("s_add_i32 m0, %0, %3" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(wave_address), "v"(lane_offset), "s"(resource), "n"((block_of(0, j) - block_of(0, 0)) * 1024)
                      : "memory", "scc");
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(kMfmaThreads, kWaves / 4) void grouped_gemm_mfma_ke
             static_cast<int>(sizeof(TileRecord)), kBufferResourceFlags);
         const uint32_t lane_offset = (opaque(static_cast<int>(threadIdx.x)) & 15) * 4;
         const int spot = __builtin_amdgcn_readfirstlane(kRecordSpot);
-        asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+        asm volatile("s_mov_b32 m0, %0" FM_M0_WAIT "buffer_load_dword %1, %2, 0 offen lds"
                      :
                      : "s"(spot), "v"(lane_offset), "s"(resource)
                      : "memory");

@@ -87,7 +87,7 @@ struct Operand {
             const uint32_t lane_offset =
                 row + j * kRowsPerLoad < rows_left ? offset[j % kOffsets] + j / kOffsets * 4 * stride : kOutOfRange;
             const int at = __builtin_amdgcn_readfirstlane(slot + target + j * 1024);
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+            asm volatile("s_mov_b32 m0, %0" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(at), "v"(lane_offset), "s"(resource)
                          : "memory");

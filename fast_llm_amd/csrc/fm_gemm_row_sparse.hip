@@ -76,7 +76,7 @@ struct Operand {
         for (int j = 0; j < kLoads; ++j) {
             const uint32_t lane_offset = row[j] < rows_left ? offset[j] : kOutOfRange;
             const int target = __builtin_amdgcn_readfirstlane(slot + (wave * kLoads + j) * 1024);
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+            asm volatile("s_mov_b32 m0, %0" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(target), "v"(lane_offset), "s"(resource)
                          : "memory");

@@ -80,7 +80,7 @@ struct Operand {
             const uint32_t lane_offset = k[j] < k_left ? offset[j] : kOutOfRange;
             const int target = __builtin_amdgcn_readfirstlane(slot + (wave * kLoads + j) * 1024);
             // M0 is not handed out by the register allocator and nothing else in this file uses it.
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+            asm volatile("s_mov_b32 m0, %0" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(target), "v"(lane_offset), "s"(resource)
                          : "memory");

@@ -58,7 +58,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base)
 // nothing else in this file uses it.)
 template <int kMore>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
-    asm volatile("s_add_i32 m0, %0, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_add_i32 m0, %0, %4" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position)), "n"(kMore)
                  : "memory", "scc");
