@@ -55,10 +55,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base)
 }
 
 // 16 bytes of each lane -> LDS at `target` + kMore + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and
-// nothing else in this file uses it.)
+// nothing else in this file uses it. Where the compiler has spilled the resource or the position, it brings them back by vector instructions, maybe right in
+// front of this: five wait states up to the load that reads them, which are more than M0's.)
 template <int kMore>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
-    asm volatile("s_add_i32 m0, %0, %4" FM_M0_WAIT "buffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_add_i32 m0, %0, %4\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position)), "n"(kMore)
                  : "memory", "scc");
@@ -67,7 +68,7 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uin
 // The same where `lanes` is ~0, and nothing where it is 0: without a branch, past which the compiler would move what is around it.
 template <int kMore>
 __device__ __forceinline__ void load_to_lds_if(uint32_t lanes, __amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
-    asm volatile("s_add_i32 m0, %0, %5\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b64 exec, -1"
+    asm volatile("s_add_i32 m0, %0, %5\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\ts_nop 1\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b64 exec, -1"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "s"(__builtin_amdgcn_readfirstlane(position)),
                    "s"(__builtin_amdgcn_readfirstlane(lanes)), "n"(kMore)
