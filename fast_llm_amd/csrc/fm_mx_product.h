@@ -34,6 +34,11 @@ struct ProductArgs {
 
 constexpr int kMaxEntries = 4096;  // the list in LDS, and the scan of every workgroup
 
+// Which kernel a product by a map runs on (fm_mx_product.hip).
+bool runs_on_tiles(const ProductArgs &args);
+// How many wavefronts share a reduction in the kernel for few rows (fm_mx_stream.hip): 1, 4 or 8.
+int stream_split(const ProductArgs &args);
+
 // Many rows per expert (fm_mx_tiles.hip).
 bool tile_product_takes(const ProductArgs &args);
 int tile_product(const ProductArgs &args, hipStream_t stream);

@@ -28,6 +28,12 @@ int check_sizes(const char *name, int64_t rows, int64_t columns, int64_t inner, 
 }
 
 int run(const mx::ProductArgs &args, void *stream) {
+    return mx::runs_on_tiles(args) ? mx::tile_product(args, static_cast<hipStream_t>(stream)) : mx::stream_product(args, static_cast<hipStream_t>(stream));
+}
+
+}  // namespace
+
+bool mx::runs_on_tiles(const ProductArgs &args) {
     // The tiles read the weights once, at 3.8 TB/s where little is multiplied and there is a tile for every CU; with few rows the weights are read once
     // per 32 rows of an expert, at 4.8 TB/s. So it depends on how many experts have over 32 rows, and on the tiles. Measured in us, few rows | tiles,
     // with both layers' weights of 8 experts (4096, 2 x 14336), 64 (2048, 2 x 1408) and 128 (2048, 2 x 768) and tokens at random: 16 rows per
@@ -37,11 +43,8 @@ int run(const mx::ProductArgs &args, void *stream) {
     const int64_t tiles = (args.out_columns + 255) / 256 * (args.gated ? 2 : 1) * args.experts, times = min(max(80 / tiles, int64_t(1)), int64_t(4));
     const bool exact = args.expert_ends == args.expert_pad_begins;
     const bool many = args.rows > (exact ? 32 * times : 128 + 24 * times) * args.experts;
-    return many && mx::tile_product_takes(args) ? mx::tile_product(args, static_cast<hipStream_t>(stream))
-                                                : mx::stream_product(args, static_cast<hipStream_t>(stream));
+    return many && tile_product_takes(args);
 }
-
-}  // namespace
 
 extern "C" int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                                    const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts,

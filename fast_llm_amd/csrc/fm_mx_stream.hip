@@ -303,35 +303,43 @@ static int launch_stream(const ProductArgs &args, int workgroup_rows, hipStream_
     return FM_OK;
 }
 
+// Rows of workgroups where the rows are found by their entries: one per entry where there are fewer of them than experts.
+static int entry_workgroup_rows(const ProductArgs &args) { return args.by_entry ? args.entries : static_cast<int>(args.experts); }
+
 // As few wavefronts share a reduction as give the device six wavefronts per CU.
-template <int kFormat, bool kGated, bool kQuantized, Source kSource>
-static int launch_split(const ProductArgs &args, int workgroup_rows, hipStream_t stream) {
+int stream_split(const ProductArgs &args) {
     // A map's rows have 128 of padding per expert; of its last ones it is not known whether there is anything in them.
-    const int64_t busy = kSource == kByMap ? min(max(args.rows - 128 * args.experts, int64_t(2)), args.experts) : workgroup_rows;
+    const int64_t busy = args.top_experts == nullptr ? min(max(args.rows - 128 * args.experts, int64_t(2)), args.experts) : entry_workgroup_rows(args);
     const int64_t sets = (args.out_columns + 31) / 32 * busy, chunks = (args.inner + kChunk - 1) / kChunk;
     constexpr int kWanted = 12 * 256;
-    if (sets >= kWanted || chunks < 4) return launch_stream<kFormat, kGated, kQuantized, kSource, 1, 4>(args, workgroup_rows, stream);
-    if (sets * 4 >= kWanted || chunks < 8) return launch_stream<kFormat, kGated, kQuantized, kSource, 4, 1>(args, workgroup_rows, stream);
-    return launch_stream<kFormat, kGated, kQuantized, kSource, 8, 1>(args, workgroup_rows, stream);
+    if (sets >= kWanted || chunks < 4) return 1;
+    return sets * 4 >= kWanted || chunks < 8 ? 4 : 8;
+}
+
+template <int kFormat, bool kGated, bool kQuantized, Source kSource>
+static int launch_split(const ProductArgs &args, hipStream_t stream) {
+    const int workgroup_rows = kSource == kByMap ? static_cast<int>(args.experts) : entry_workgroup_rows(args);
+    switch (stream_split(args)) {
+        case 1: return launch_stream<kFormat, kGated, kQuantized, kSource, 1, 4>(args, workgroup_rows, stream);
+        case 4: return launch_stream<kFormat, kGated, kQuantized, kSource, 4, 1>(args, workgroup_rows, stream);
+        default: return launch_stream<kFormat, kGated, kQuantized, kSource, 8, 1>(args, workgroup_rows, stream);
+    }
 }
 
 template <bool kGated, bool kQuantized, Source kSource>
-static int launch_format(const ProductArgs &args, int workgroup_rows, hipStream_t stream) {
-    return args.format == FM_MX_E4M3 ? launch_split<FM_MX_E4M3, kGated, kQuantized, kSource>(args, workgroup_rows, stream)
-                                     : launch_split<FM_MX_E2M1, kGated, kQuantized, kSource>(args, workgroup_rows, stream);
+static int launch_format(const ProductArgs &args, hipStream_t stream) {
+    return args.format == FM_MX_E4M3 ? launch_split<FM_MX_E4M3, kGated, kQuantized, kSource>(args, stream)
+                                     : launch_split<FM_MX_E2M1, kGated, kQuantized, kSource>(args, stream);
 }
 
 int stream_product(const ProductArgs &args, hipStream_t stream) {
-    const int experts = static_cast<int>(args.experts);
-    if (args.out_scales == nullptr) return launch_format<false, false, kByMap>(args, experts, stream);
-    return args.gated ? launch_format<true, true, kByMap>(args, experts, stream) : launch_format<false, true, kByMap>(args, experts, stream);
+    if (args.out_scales == nullptr) return launch_format<false, false, kByMap>(args, stream);
+    return args.gated ? launch_format<true, true, kByMap>(args, stream) : launch_format<false, true, kByMap>(args, stream);
 }
 
 int few_tokens(const ProductArgs &layer_1, const ProductArgs &layer_2, const float *scores, void *out, int out_dtype, hipStream_t stream) {
-    const int workgroup_rows = layer_1.by_entry ? layer_1.entries : static_cast<int>(layer_1.experts);
-    int status = layer_1.gated ? launch_format<true, true, kByEntries>(layer_1, workgroup_rows, stream)
-                               : launch_format<false, true, kByEntries>(layer_1, workgroup_rows, stream);
-    if (status == FM_OK) status = launch_format<false, false, kByEntries>(layer_2, workgroup_rows, stream);
+    int status = layer_1.gated ? launch_format<true, true, kByEntries>(layer_1, stream) : launch_format<false, true, kByEntries>(layer_1, stream);
+    if (status == FM_OK) status = launch_format<false, false, kByEntries>(layer_2, stream);
     if (status != FM_OK) return status;
     const int slots = layer_1.entries_per_row, tokens = layer_1.entries / slots, hidden = static_cast<int>(layer_2.columns);
     FM_DISPATCH_DTYPE(out_dtype, T, {
