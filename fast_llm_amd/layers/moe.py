@@ -358,7 +358,6 @@ class MicroscaledMoEMLP(torch.nn.Module):
     def layer_2(self) -> MicroscaledTensor:
         return MicroscaledTensor(self.layer_2_values, self.layer_2_scales, self.intermediate_size, MicroscalingFormat.e2m1)
 
-    @torch.no_grad()
     def forward(
         self,
         input_: torch.Tensor,
@@ -366,7 +365,16 @@ class MicroscaledMoEMLP(torch.nn.Module):
         scores: torch.Tensor | None = None,
         top_experts: torch.Tensor | None = None,
     ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
-        """`scores`/`top_experts` may be passed to bypass the router."""
+        """`scores`/`top_experts` may be passed to bypass the router. What is computed of a tensor that requires a gradient raises in a backward."""
+        output, stream = self._forward(input_, residual, scores, top_experts)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input_, residual, scores)):
+            output, stream = without_backward(output), None if stream is None else without_backward(stream)
+        return output if stream is None else (output, stream)
+
+    @torch.no_grad()
+    def _forward(
+        self, input_: torch.Tensor, residual: torch.Tensor | None, scores: torch.Tensor | None, top_experts: torch.Tensor | None
+    ) -> tuple[torch.Tensor, torch.Tensor | None]:
         hidden_states, stream, router_counts = input_.flatten(0, -2), None, None
         if self.normalization is not None:
             norm = self.normalization
@@ -391,4 +399,4 @@ class MicroscaledMoEMLP(torch.nn.Module):
             dtype=input_.dtype,
             router_counts=router_counts,
         ).view_as(input_)
-        return output if stream is None else (output, stream.view_as(input_))
+        return output, None if stream is None else stream.view_as(input_)
