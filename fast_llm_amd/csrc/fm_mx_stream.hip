@@ -306,7 +306,7 @@ static int launch_stream(const ProductArgs &args, int workgroup_rows, hipStream_
 // Rows of workgroups where the rows are found by their entries: one per entry where there are fewer of them than experts.
 static int entry_workgroup_rows(const ProductArgs &args) { return args.by_entry ? args.entries : static_cast<int>(args.experts); }
 
-// As few wavefronts share a reduction as give the device six wavefronts per CU.
+// As few wavefronts share a reduction as give the device twelve wavefronts per CU.
 int stream_split(const ProductArgs &args) {
     // A map's rows have 128 of padding per expert; of its last ones it is not known whether there is anything in them.
     const int64_t busy = args.top_experts == nullptr ? min(max(args.rows - 128 * args.experts, int64_t(2)), args.experts) : entry_workgroup_rows(args);

@@ -10,9 +10,11 @@
 // neighbouring rows hit all 64 banks. Of every 32 weight rows, LDS row 8 a + 4 h + b holds row 16 h + 4 a + b: a lane (h: its half of the
 // wavefront) then has 16 neighbouring columns of its row, and results leave without a way through LDS, which is full of the next tile's slices.
 //
-// Measured, 16384 rows of 8 experts: 4096 -> 2 x 14336 with the gated activation 1473 us (e4m3, 2.6 PFLOP/s), 14336 -> 4096 720 us (2.7) and in e2m1
-// 530 us (3.6); a loop of the instruction in registers on random data: 4.16 and 6.58. The chip is at its power limit (1.9 to 2.0 GHz; with zeros for
-// data 17 % faster). 30006 rows of 64 experts, 2048 -> 2 x 1408: 170 us, of which the results' way out takes 22 %.
+// Measured on two cards, 16384 rows of 8 experts: 4096 -> 2 x 14336 with the gated activation 1534 and 1604 us (e4m3, 2.5 and 2.4 PFLOP/s), 14336 -> 4096
+// 742 and 774 us (2.6 and 2.5) and in e2m1 545 and 565 us (3.5 and 3.4); a loop of the instruction in registers on random data reaches 3.94 and 6.14 on the
+// second. Two bounds: the clock under the power of random data (1.7 to 1.8 GHz of 2.4; in e2m1 1.9; with zeros for data the products take 76 to 84 % of the
+// time), and the one wavefront of a SIMD, which issues loads and reads beside its products (matrix units busy 65 % of the cycles, in e2m1 44 %; without
+// the loads 3.1 and 4.5 PFLOP/s, without reads too 3.2 and 5.0). 30006 rows of 64 experts, 2048 -> 2 x 1408: 172 us, busy 48 %, the results' way out 22 %.
 #include "fm_activation_math.h"
 #include "fm_mx_product.h"
 
@@ -56,7 +58,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base)
 
 // 16 bytes of each lane -> LDS at `target` + kMore + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and
 // nothing else in this file uses it. Where the compiler has spilled the resource or the position, it brings them back by vector instructions, maybe right in
-// front of this: five wait states up to the load that reads them, which are more than M0's.)
+// front of this: five wait states up to the load that reads them, which are more than M0's. With M0's only, 0.5 to 2 % faster, three loads of the kernels for
+// e4m3 rows would come too early.)
 template <int kMore>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int position, int target) {
     asm volatile("s_add_i32 m0, %0, %4\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
@@ -136,7 +139,7 @@ struct Experts {
     }
     __device__ __forceinline__ bool locate(const GemmArgs &args, int logical, RowTile &tile) const {
         if (args.num_experts > kMaxInRegisters) {
-            // The same in all lanes, which the compiler cannot know.
+            // (Without halves in the last round.) The same in all lanes, which the compiler cannot know.
             RowTile found{};
             const bool exists = locate_tile<kTile>(args, logical, found);
             tile.expert = __builtin_amdgcn_readfirstlane(found.expert), tile.tile_n = __builtin_amdgcn_readfirstlane(found.tile_n);

@@ -6,7 +6,8 @@
 //
 // What is normalised is the rounded stream, so that the backward needs nothing but it: v is computed again from the row that is in
 // registers anyway. All of a row is in the registers of one wavefront (up to 2048 columns), of four or of sixteen (8192, 32768), so each tensor
-// passes once: memory is the bound. Sums are in fp32: a lane's own values, then lanes, then wavefronts, in a fixed order.
+// passes once: memory is the bound. Sums are in fp32: a lane's own values, then lanes, then wavefronts, in a fixed order. (No row is scaled first, so a sum of
+// squares over 3.4e38 gives v = 0: values from 1.8e19 / sqrt(columns) on.)
 // Rows whose length is no multiple of 8 or that are not aligned to 16 bytes: the same loads, aligned as the values are, with a last lane that takes the
 // row's last eight columns. Rows of less than 8 columns and longer ones: a value per lane and load, the stream read a second time.
 //

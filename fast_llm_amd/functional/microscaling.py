@@ -268,8 +268,10 @@ def mx_mlp(
     """
     The dropless expert MLP in inference on e2m1 weights (`mx_quantize_expert_weights`):
     output[t] = sum_j scores[t, j] * W2[e] act(W1[e] input[t]), e = top_experts[t, j], the activations microscaled between the
-    layers in the input's format. Entries of `top_experts` outside [0, num_experts) add nothing. `input_` [tokens, hidden] may be a
-    plain tensor: it is then quantised to e4m3. `dtype` of the output: the plain input's type, or bfloat16.
+    layers in the input's format. Sums are in fp32, with one rounding of the output; with over `MX_FEW_TOKENS_ROWS` rows per expert layer 2's rows are
+    also rounded to `dtype` (float32: not at all), as they are in `mlp_autograd`. Entries of `top_experts` outside [0, num_experts) add
+    nothing. `input_` [tokens, hidden] may be a plain tensor: it is then quantised to e4m3. `dtype` of the output: the plain input's type,
+    or bfloat16.
     `router_counts` as in `get_sparse_map`.
     """
     if isinstance(input_, torch.Tensor):

@@ -89,6 +89,7 @@ def rms_norm(
     stream = input_ + residual (rounded to their type; `input_` itself without one),
     normalized = stream / sqrt(mean(stream^2) + eps) * weight, over the last axis. Returns `normalized`, with a residual
     (`normalized`, `stream`). Differentiable (once) in `input_`, `weight` and `residual`; `weight` has the input's type or float32.
+    Squares are summed in fp32: rows with values from 1.8e19 / sqrt(columns) on, whose sum overflows, become zeros.
     Rows of any length and alignment; can be captured into a graph, its backward while no eager graph of the same leaves is alive.
     """
     _check(input_, weight, residual)

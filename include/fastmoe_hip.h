@@ -467,7 +467,9 @@ int fm_mx_copy_dense_to_sparse(const void *values, const void *scales, const voi
                                int64_t value_row_stride, int64_t scale_row_stride, int format, int index_dtype, void *stream);
 
 /* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs, in e2m1, has `columns` rows of `inner` per expert, lhs is in
- * `format`. Both layers of an expert MLP are such products. Sums in fp32, one rounding. Of each expert the rows [expert_ends[e - 1],
+ * `format`. Both layers of an expert MLP are such products. Sums in fp32, one rounding. (The matrix instruction adds 64 products and the sum so far at a
+ * time, aligned to the largest of them: with lhs in e4m3 it drops what lies under 2^-17 of that, so a sum is off by up to `inner` times as much, 4.6e-6 of the
+ * result's size in the mean; with both in e2m1 a sum is as exact as fp32.) Of each expert the rows [expert_ends[e - 1],
  * expert_pad_begins[e]) are computed; all others of `out` (padding, rows behind the last expert) are left as they are, and those of lhs are not
  * looked at. Expert boundaries need not be multiples of anything. `out_stride` in elements. At most 1024 experts. */
 int fm_mx_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
@@ -494,7 +496,8 @@ int fm_mx_few_tokens_forward(const void *input, const void *input_scales, const 
                              int64_t weight_2_scale_stride, int gated, int activation, int format, int out_dtype, void *workspace,
                              size_t workspace_size, void *stream);
 /* The same MLP for any number of tokens, by way of a sparse map padded to multiples of 128: the launches of fm_sparse_map, fm_mx_copy_dense_to_sparse,
- * fm_mx_sparse_matmul_activation, fm_mx_sparse_matmul (into rows of `out_dtype`) and fm_copy_sparse_to_dense one after the other, with their results, bit for bit.
+ * fm_mx_sparse_matmul_activation, fm_mx_sparse_matmul (into rows of `out_dtype`: a rounding per slot that fm_mx_few_tokens_forward does not have) and
+ * fm_copy_sparse_to_dense one after the other, with their results, bit for bit.
  * `router_workspace`: null, or what fm_router_forward left for these top_experts with their `shared_experts` (as for fm_sparse_map_from_router, with its
  * precondition). `workspace`: 256-byte aligned. */
 size_t fm_mx_mlp_workspace_size(int64_t num_tokens, int64_t slots_per_token, int64_t hidden, int64_t ffn, int64_t num_experts, int format, int out_dtype);
@@ -509,6 +512,8 @@ int fm_mx_mlp_forward(const void *input, const void *input_scales, const void *t
  * Root-mean-square norm with the residual's addition. Contiguous rows of `dtype`; `weight` of `dtype` or fp32.
  *   stream_out = round(input + residual) (without a residual, null both, the input itself),
  *   normalized = round(s * v * weight),  s = the (rounded) stream, v = 1 / sqrt(mean(s^2) + eps).
+ * Squares are summed in fp32: of a row whose sum of squares is over 3.4e38 (values from 1.8e19 / sqrt(columns) on) v is 0 and so are the finite results; with an
+ * eps that is 0 or next to it, squares of values under 1e-19 lose bits and then vanish. fp16 rows have neither.
  * With `values` and `scales` (both or neither) also `normalized`, as rounded, microscaled in `format`, bit for bit as fm_mx_quantize gives it.
  * Backward, of the gradients of normalized and (may be null) of the stream: grad_input = v (g w - s v^2 mean(g w s)) + grad_stream, of input and
  * residual alike, one rounding; grad_weight (of weight_dtype; may be null: not computed) = sum over rows of g s v in fp32, in a fixed order, in
