@@ -6,7 +6,7 @@ are those of the OCP Microscaling Formats specification 1.0, as include/fastmoe_
 the axis that the product sums over: layer 1 as the layer stores it, [experts * ffn (* 2, gates then ups), hidden]; layer 2 transposed expert by
 expert, [experts * hidden, ffn] (`mx_quantize_expert_weights`).
 
-The reference has no counterpart. Nothing here has a backward.
+The reference has no counterpart. Nothing here has a backward or a forward-mode derivative, and `torch.jit`'s tracer is refused.
 """
 
 import dataclasses
@@ -18,7 +18,7 @@ from fast_llm_amd import _lib
 from fast_llm_amd.functional.config import ActivationType
 from fast_llm_amd.functional.mlp import _activation_tag
 from fast_llm_amd.functional.sparse_copy import SparseMap
-from fast_llm_amd.functional.utils import Assert, div, without_backward
+from fast_llm_amd.functional.utils import Assert, div, refuse_traced, without_backward
 
 MX_BLOCK = 32
 # Rows are stored padded with zeros to a multiple of this many columns.
@@ -121,6 +121,7 @@ def mx_quantize(input_: torch.Tensor, format: MicroscalingFormat | str = Microsc
     scale = 2^max(floor(log2(largest magnitude)) - emax, -127) with emax = 8 (e4m3) or 2 (e2m1), element = value / scale rounded to
     nearest even and saturated. A block with an infinity or NaN is NaN altogether.
     """
+    refuse_traced(input_)
     format = MicroscalingFormat(format)
     columns = input_.size(-1)
     input_ = input_.detach().reshape(input_.numel() // max(columns, 1), columns)
@@ -138,6 +139,7 @@ def mx_quantize(input_: torch.Tensor, format: MicroscalingFormat | str = Microsc
 
 def mx_dequantize(input_: MicroscaledTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that `input_` stands for, each rounded once to `dtype`."""
+    refuse_traced()
     device = _lib.require_device(input_.values, input_.scales)
     out = torch.empty(input_.shape, dtype=dtype, device=device)
     _lib.call(
@@ -162,6 +164,7 @@ def mx_quantize_expert_weights(
 
 def mx_copy_dense_to_sparse(input_: MicroscaledTensor, sparse_map: SparseMap) -> MicroscaledTensor:
     """`copy_dense_to_sparse` of microscaled rows. Padding rows of the result stay uninitialised."""
+    refuse_traced()
     device = _lib.require_device(input_.values, input_.scales, sparse_map.sparse_rows)
     Assert.eq(input_.rows, sparse_map.num_rows_dense)
     Assert.eq(tuple(sparse_map.sparse_rows.shape), (sparse_map.num_rows_dense, sparse_map.num_experts_per_token))
@@ -178,6 +181,7 @@ def mx_copy_dense_to_sparse(input_: MicroscaledTensor, sparse_map: SparseMap) ->
 
 def _product_operands(lhs: MicroscaledTensor, rhs: MicroscaledTensor, sparse_map: SparseMap | None) -> tuple:
     """Experts, their ends and the ends of their rows, rows of `rhs` per expert."""
+    refuse_traced()
     if rhs.format != MicroscalingFormat.e2m1:
         raise NotImplementedError(f"expert weights are in e2m1, not {rhs.format}")
     Assert.eq(lhs.columns, rhs.columns)
@@ -274,6 +278,7 @@ def mx_mlp(
     or bfloat16.
     `router_counts` as in `get_sparse_map`.
     """
+    refuse_traced(scores)
     if isinstance(input_, torch.Tensor):
         requires_grad = input_.requires_grad or scores.requires_grad
         dtype = dtype or input_.dtype

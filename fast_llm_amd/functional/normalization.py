@@ -8,7 +8,7 @@ from torch.autograd.function import once_differentiable
 
 from fast_llm_amd import _lib
 from fast_llm_amd.functional.microscaling import MicroscaledTensor, MicroscalingFormat, _tag
-from fast_llm_amd.functional.utils import Assert, without_backward
+from fast_llm_amd.functional.utils import Assert, refuse_traced, without_backward
 
 
 def _check(input_: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None) -> None:
@@ -105,8 +105,9 @@ def rms_norm_quantize(
 ) -> tuple[torch.Tensor, torch.Tensor, MicroscaledTensor]:
     """
     `rms_norm` for inference: (`normalized`, `stream`, `mx_quantize(normalized, format)`) in one pass, bit for bit what the single
-    calls give. Without a residual the stream is `input_`. No backward.
+    calls give. Without a residual the stream is `input_`. No backward, no forward-mode derivative, not for `torch.jit`'s tracer.
     """
+    refuse_traced(input_, weight, residual)
     _check(input_, weight, residual)
     columns = input_.size(-1)
     quantized = MicroscaledTensor.empty(input_.numel() // columns, columns, format, input_.device)

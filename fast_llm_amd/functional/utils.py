@@ -53,6 +53,17 @@ def is_traced() -> bool:
     return forward_ad._current_level >= 0 or torch.jit.is_tracing()
 
 
+def refuse_traced(*tensors: torch.Tensor | None) -> None:
+    """For what runs outside the autograd functions and has none to step aside to: raise under `torch.jit`'s tracer, which would record its results as
+    uninitialised memory, and where one of `tensors` carries a tangent."""
+    if not is_traced():
+        return
+    if torch.jit.is_tracing():
+        raise NotImplementedError("torch.jit's tracer does not see what this operator computes")
+    if any(tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None for tensor in tensors):
+        raise NotImplementedError("this operator has no forward-mode derivative")
+
+
 class _ForwardBackwardPair(torch.autograd.Function):
     """One autograd node for every wrapped pair: the pair itself travels as the first argument. The last argument is
     an empty tensor that requires a gradient, so that autograd visits the node even when none of the caller's tensors
