@@ -1,0 +1,644 @@
+"""
+What is measured: the mixture-of-experts MLP in 8 bits with a scale for each block of 128, in training and in serving.
+
+Five operators that a training step calls one after the other: the quantisation of activations, gradients and weights (along their rows, and
+along their columns with the result transposed), the grouped product of 8-bit rows with 8-bit expert weights (forward, input gradient, one
+token), the weights' gradient from 8-bit rows, the activation that keeps its input in 8 bits for its backward, and the whole MLP's forward and
+backward made of them. Sizes are the benchmark's (`fast_llm_amd.workloads.WORKLOADS`) and generic ones.
+
+Definition of the format: 128 neighbours along a row share the scale 2^e, e the smallest integer with (largest magnitude) <= 448 * 2^e, at least
+-127, stored as the byte e + 127; elements are value / 2^e in e4m3, rounded to nearest even. Rows are stored padded with zeros to whole
+blocks. With a sparse map the rows that no token has count as zeros.
+"""
+
+import torch
+
+own = False
+
+_DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+# hidden, ffn, experts, experts per token
+_MIXTRAL, _FINE_GRAINED, _WIDE, _RAGGED = (4096, 14336, 8, 2), (2048, 1408, 64, 6), (2048, 768, 128, 8), (1288, 3456, 16, 2)
+_BLOCK = 128  # of the format, and of a sparse map's padding
+
+
+# ---- the cases -------------------------------------------------------------------------------------------
+def _quantize(form: str, rows: int, columns: int, dtype: str, groups: int = 1, experts: int = 0, slots: int = 1) -> dict:
+    """`rows`: of each group, or tokens where there is a map."""
+    return {"kind": "quantize", "form": form, "rows": rows, "columns": columns, "dtype": dtype, "groups": groups, "experts": experts, "slots": slots}
+
+
+def _product(tokens: int, inner: int, columns: int, experts: int, slots: int, dtype: str = "bf16", zipf: float = 0.0) -> dict:
+    return {
+        "kind": "product", "tokens": tokens, "inner": inner, "columns": columns, "experts": experts, "slots": slots, "dtype": dtype, "zipf": zipf,
+    }  # fmt: skip
+
+
+def _gradient(tokens: int, rows: int, columns: int, experts: int, slots: int, dtype: str = "bf16", accumulate: bool = False, zipf: float = 0.0) -> dict:
+    return {
+        "kind": "gradient", "tokens": tokens, "rows": rows, "columns": columns, "experts": experts, "slots": slots, "dtype": dtype,
+        "accumulate": accumulate, "zipf": zipf,
+    }  # fmt: skip
+
+
+def _activation(tokens: int, ffn: int, experts: int, slots: int, dtype: str = "bf16", gated: bool = True, activation: str = "silu") -> dict:
+    return {
+        "kind": "activation", "tokens": tokens, "ffn": ffn, "experts": experts, "slots": slots, "dtype": dtype, "gated": gated,
+        "activation": activation, "zipf": 0.0,
+    }  # fmt: skip
+
+
+def _mlp(tokens: int, shape: tuple, dtype: str = "bf16", gated: bool = True, activation: str = "silu", zipf: float = 0.0) -> dict:
+    return {
+        "kind": "mlp", "tokens": tokens, "hidden": shape[0], "ffn": shape[1], "experts": shape[2], "slots": shape[3], "dtype": dtype,
+        "gated": gated, "activation": activation, "zipf": zipf,
+    }  # fmt: skip
+
+
+def listed() -> list[dict]:
+    cases = {
+        # The gradient of the second layer's output in a training step: for the input gradient and for the weights'.
+        "quantize_gradient": _quantize("both", 8192, 4096, "bf16", experts=8, slots=2),
+        # The first layer's weights of eight experts after an optimizer step: for the forward pass and for the backward.
+        "quantize_experts": _quantize("both", 2 * 14336, 4096, "bf16", groups=8),
+        # The first layer's product for one generated token: two experts' weights are read.
+        "product_token": _product(1, 4096, 2 * 14336, 8, 2),
+        # The first layer's product in batched generation with many small experts.
+        "product_batch": _product(96, 2048, 2 * 768, 128, 8),
+        # The first layer's product for several prompts, many small experts.
+        "product_prompt": _product(5001, 2048, 2 * 1408, 64, 6, "fp16"),
+        # The second layer's product of a training step.
+        "product_step": _product(8192, 14336, 4096, 8, 2),
+        # The first layer's weight gradient of many small experts, added to a full-precision gradient buffer.
+        "gradient_wide": _gradient(16384, 2 * 768, 2048, 128, 8, "fp32", accumulate=True),
+        # The second layer's weight gradient where the routing prefers some experts.
+        "gradient_skewed": _gradient(8192, 14336, 4096, 8, 2, zipf=1.2),
+        # The smallest benchmark configuration's activation, forward and backward: tests and debugging runs.
+        "activation_tiny": _activation(512, 512, 8, 2, "fp32", activation="gelu"),
+        # The activation of a training step with many small experts, forward and backward.
+        "activation_step": _activation(16384, 1408, 64, 6),
+        # A training step's MLP, forward and backward, with many small experts.
+        "mlp_step_fine": _mlp(4096, _FINE_GRAINED),
+        # The benchmark's headline shape as a training step.
+        "mlp_step": _mlp(8192, _MIXTRAL),
+    }
+    return [{"name": name, **case} for name, case in cases.items()]
+
+
+def _log_uniform(rng, low: int, high: int, multiple: int = 1) -> int:
+    value = low * (high / low) ** rng.random()
+    return max(low, min(high, round(value / multiple) * multiple))
+
+
+# No case does more than the listed ones of its kind.
+_MOST = {"quantize": 8 * 28672 * 4096, "product": 2 * 16384 * 14336 * 4096, "gradient": 2 * 16384 * 14336 * 4096, "activation": 98304 * 1408, "mlp": 18 * 16384 * 14336 * 4096}
+_MOST_WEIGHTS = 8 * 3 * 4096 * 14336
+
+
+def draw(rng) -> dict:
+    while True:
+        kind = rng.choice(("quantize", "quantize", "product", "product", "product", "gradient", "gradient", "activation", "mlp", "mlp"))
+        multiple = rng.choice((1, 8, 32, 128))
+        dtype = rng.choice(("bf16", "bf16", "fp16"))
+        if kind == "quantize":
+            form = rng.choice(("rows", "both", "both"))
+            groups = rng.choice((1, 4, 16)) if form == "both" else 1
+            experts, slots = (rng.choice((8, 64, 128)), rng.choice((1, 2, 6))) if form == "both" and groups == 1 else (0, 1)
+            rows, columns = _log_uniform(rng, 1, 16384), _log_uniform(rng, 64, 8192, multiple)
+            case = _quantize(form, rows, columns, rng.choice((dtype, "fp32")), groups, experts, slots)
+            if rows * groups * slots * columns <= _MOST["quantize"]:
+                return case
+            continue
+        shape = rng.choice((_MIXTRAL, _FINE_GRAINED, _WIDE, _RAGGED, None, None))
+        gated = rng.random() < 0.85
+        if shape is None:
+            experts = rng.choice((8, 16, 32, 60, 64, 128))
+            ffn = _log_uniform(rng, 512, 8192, 128 if gated else multiple)
+            shape = (_log_uniform(rng, 512, 4096, max(multiple, 8)), ffn, experts, rng.choice((1, 2, 4, 6, 8)))
+        hidden, ffn, experts, slots = shape
+        tokens = _log_uniform(rng, 1, 256) if rng.random() < 0.4 else _log_uniform(rng, 256, 16384)
+        zipf = rng.choice((0.0, 0.6, 1.2)) if experts <= 16 else 0.0
+        activation = rng.choice(("silu", "silu", "gelu", "squared_relu"))
+        weights = experts * hidden * ffn * (3 if gated else 2)
+        if kind == "product":
+            inner, columns = rng.choice(((hidden, 2 * ffn), (ffn, hidden), (2 * ffn, hidden), (hidden, ffn)))
+            case, weights, cost = _product(tokens, inner, columns, experts, slots, dtype, zipf), experts * inner * columns, 2 * tokens * slots * inner * columns
+        elif kind == "gradient":
+            rows = rng.choice((ffn, 2 * ffn))
+            case, cost = _gradient(tokens, rows, hidden, experts, slots, rng.choice((dtype, "fp32")), rng.random() < 0.5, zipf), 2 * tokens * slots * rows * hidden
+        elif kind == "activation":
+            case, cost = _activation(tokens, ffn, experts, slots, rng.choice((dtype, dtype, "fp32")), gated, activation), tokens * slots * ffn
+        else:
+            case, cost = _mlp(tokens, shape, dtype, gated, activation, zipf), (18 if gated else 12) * tokens * slots * hidden * ffn
+        # The plain form pads experts to the fullest one.
+        fullest = tokens if zipf else min(tokens, 2 * tokens * slots // experts + 64)
+        if cost <= _MOST[kind] and weights <= _MOST_WEIGHTS and fullest * experts * max(hidden, 2 * ffn) <= 1 << 31:
+            return case
+
+
+# ---- inputs ----------------------------------------------------------------------------------------------
+def _normal(generator: torch.Generator, shape: tuple, dtype: torch.dtype, std: float = 1.0) -> torch.Tensor:
+    return (torch.randn(shape, generator=generator, device="cuda") * std).to(dtype)
+
+
+def _hidden_states(generator: torch.Generator, rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
+    """Features of unlike size, as the residual stream has them."""
+    sizes = torch.exp(0.5 * torch.randn(columns, generator=generator, device="cuda"))
+    return (torch.randn(rows, columns, generator=generator, device="cuda") * sizes).to(dtype)
+
+
+def _gradients(generator: torch.Generator, rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
+    """Tokens of unlike weight in the loss."""
+    sizes = torch.exp(0.5 * torch.randn(rows, 1, generator=generator, device="cuda"))
+    return (torch.randn(rows, columns, generator=generator, device="cuda") * sizes).to(dtype)
+
+
+def _padded(size: int) -> int:
+    return -(-size // _BLOCK) * _BLOCK
+
+
+def _stored(values: torch.Tensor) -> dict:
+    """fp32 rows as they are kept: the bytes of the elements, padded, and of the scales."""
+    elements, exponents = _parts(values)
+    return {
+        "values": elements.flatten(1).to(torch.float8_e4m3fn).view(torch.uint8),
+        "scales": (exponents + 127).to(torch.uint8),
+        "columns": values.size(1),
+    }
+
+
+def _stored_weights(generator: torch.Generator, experts: int, rows: int, columns: int, transposed: bool) -> list[dict]:
+    """Normal weights [experts * rows, columns], and where asked for also [experts * columns, rows]."""
+    out = [
+        {
+            "values": torch.empty(experts * r, _padded(c), dtype=torch.uint8, device="cuda"),
+            "scales": torch.empty(experts * r, _padded(c) // _BLOCK, dtype=torch.uint8, device="cuda"),
+            "columns": c,
+        }
+        for r, c in ((rows, columns), (columns, rows))[: 1 + transposed]
+    ]
+    for expert in range(experts):
+        weight = _normal(generator, (rows, columns), torch.bfloat16, 0.02).float()
+        for to, form in zip(out, (weight, weight.t())):
+            part, size = _stored(form.contiguous()), form.size(0)
+            to["values"][expert * size : (expert + 1) * size] = part["values"]
+            to["scales"][expert * size : (expert + 1) * size] = part["scales"]
+    return out
+
+
+def _routing(generator: torch.Generator, tokens: int, experts: int, slots: int, zipf: float) -> tuple[torch.Tensor, torch.Tensor]:
+    logits = torch.randn(tokens, experts, generator=generator, device="cuda")
+    if zipf:
+        logits -= zipf * torch.arange(1, experts + 1, device="cuda").log()
+    top_logits, top_experts = torch.topk(logits, slots, dim=-1)
+    return torch.softmax(top_logits, dim=-1), top_experts
+
+
+def _sparse_layout(state: dict, generator: torch.Generator, tokens: int, experts: int, slots: int, zipf: float) -> None:
+    """Where the experts' rows lie, in a layout with room for the worst routing."""
+    _, top_experts = _routing(generator, tokens, experts, slots, zipf)
+    counts = torch.bincount(top_experts.flatten(), minlength=experts)
+    ends = (((counts + _BLOCK - 1) // _BLOCK) * _BLOCK).cumsum(0)
+    begins = torch.cat((ends.new_zeros(1), ends[:-1]))
+    most = (tokens * slots + experts * _BLOCK) // _BLOCK * _BLOCK
+    index_dtype = torch.int16 if most < 32768 else torch.int32
+    state["expert_ends"], state["expert_pad_begins"] = ends.to(index_dtype), (begins + counts).to(index_dtype)
+    state["sparse_rows"], state["fullest"] = most, int(counts.max())
+
+
+def prepare(case: dict, seed: int) -> dict:
+    generator = torch.Generator("cuda").manual_seed(seed)
+    dtype = _DTYPES[case["dtype"]]
+    state = dict(case)
+    if case["kind"] == "quantize":
+        rows = case["rows"] * case["groups"]
+        if case["experts"]:
+            _sparse_layout(state, generator, case["rows"], case["experts"], case["slots"], 0.0)
+            rows = state["sparse_rows"]
+        if case["groups"] > 1:
+            state["input"] = _normal(generator, (rows, case["columns"]), dtype, 0.02)
+        else:
+            state["input"] = _gradients(generator, rows, case["columns"], dtype)
+    elif case["kind"] == "product":
+        (state["weight"],) = _stored_weights(generator, case["experts"], case["columns"], case["inner"], False)
+        _sparse_layout(state, generator, case["tokens"], case["experts"], case["slots"], case["zipf"])
+        state["rows"] = _stored(_hidden_states(generator, state["sparse_rows"], case["inner"], torch.float32))
+        # Padding rows are left as they are.
+        state["out"] = torch.zeros(state["sparse_rows"], case["columns"], dtype=dtype, device="cuda")
+    elif case["kind"] == "gradient":
+        _sparse_layout(state, generator, case["tokens"], case["experts"], case["slots"], case["zipf"])
+        real = _rows_of_tokens(state)[0][:, None]
+        for name, columns in (("lhs", case["rows"]), ("rhs", case["columns"])):
+            make = _gradients if name == "lhs" else _hidden_states
+            values = torch.where(real, make(generator, state["sparse_rows"], columns, torch.float32), 0.0)
+            state[name] = _stored(values.t().contiguous())
+            del values
+        # The gradient buffer with what the batches before left in it; every pass is one batch more where it accumulates.
+        state["gradient"] = _normal(generator, (case["experts"] * case["rows"], case["columns"]), dtype, 10.0)
+    elif case["kind"] == "activation":
+        _sparse_layout(state, generator, case["tokens"], case["experts"], case["slots"], 0.0)
+        state["input"] = _hidden_states(generator, state["sparse_rows"], case["ffn"] * (2 if case["gated"] else 1), dtype)
+        state["grad_output"] = _gradients(generator, state["sparse_rows"], case["ffn"], dtype)
+    else:
+        hidden, ffn, experts = case["hidden"], case["ffn"], case["experts"]
+        layer_1_rows = ffn * (2 if case["gated"] else 1)
+        # Quantised after the last optimizer step: there are several batches to one.
+        state["layer_1"], state["layer_1_transposed"] = _stored_weights(generator, experts, layer_1_rows, hidden, True)
+        state["layer_2"], state["layer_2_transposed"] = _stored_weights(generator, experts, ffn, hidden, True)
+        # What the gradients are of, with the buffers that they are written to.
+        state["weights"] = [torch.zeros(experts * rows, hidden, dtype=dtype, device="cuda") for rows in (layer_1_rows, ffn)]
+        for weight in state["weights"]:
+            weight.requires_grad_(True)
+            weight.grad_buffer = torch.zeros_like(weight, requires_grad=False)
+        state["input"] = _hidden_states(generator, case["tokens"], hidden, dtype).requires_grad_(True)
+        state["scores"], state["top_experts"] = _routing(generator, case["tokens"], experts, case["slots"], case["zipf"])
+        state["scores"].requires_grad_(True)
+        state["grad_output"] = _gradients(generator, case["tokens"], hidden, dtype)
+        state["fullest"] = int(torch.bincount(state["top_experts"].flatten(), minlength=experts).max())
+    return state
+
+
+# ---- plain forms -----------------------------------------------------------------------------------------
+def _parts(values: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Elements [rows, blocks, 128] (as floats) and exponents [rows, blocks] of fp32 rows."""
+    rows, columns = values.shape
+    blocks = torch.nn.functional.pad(values, (0, -columns % _BLOCK)).view(rows, -1, _BLOCK)
+    # frexp: largest = m 2^e with m in [1/2, 1), and 448 = 7/8 2^9
+    mantissa, exponents = torch.frexp(blocks.abs().amax(-1))
+    exponents = torch.where(mantissa > 0, exponents - 9 + (mantissa > 0.875), -127).clamp_min(-127)
+    return torch.ldexp(blocks, -exponents[..., None]).to(torch.float8_e4m3fn).float(), exponents
+
+
+def _quantized(values: torch.Tensor) -> torch.Tensor:
+    """The values that remain of fp32 rows."""
+    elements, exponents = _parts(values)
+    return torch.ldexp(elements, exponents[..., None]).flatten(1)[:, : values.size(1)]
+
+
+def _values(stored: dict) -> torch.Tensor:
+    """The fp32 values that stored rows stand for."""
+    scales = torch.ldexp(torch.ones((), device="cuda"), stored["scales"].int() - 127)
+    return (stored["values"].view(torch.float8_e4m3fn).float() * scales.repeat_interleave(_BLOCK, dim=1))[:, : stored["columns"]]
+
+
+def _said(values: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Elements and scales of quantised fp32 rows, in their types."""
+    elements, exponents = _parts(values)
+    elements = elements.flatten(1)[:, : values.size(1)].to(torch.float8_e4m3fn)
+    return elements, (exponents + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def _named(**quantized) -> dict:
+    outputs = {}
+    for name, (elements, scales) in quantized.items():
+        outputs[f"{name}_elements"], outputs[f"{name}_scales"] = elements, scales
+    return outputs
+
+
+def _rows_of_tokens(state: dict) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which rows of the sparse layout tokens have, and of those the places in a layout [experts, fullest]."""
+    ends, pad_begins = state["expert_ends"].long(), state["expert_pad_begins"].long()
+    row = torch.arange(state["sparse_rows"], device="cuda")
+    expert = torch.searchsorted(ends, row, right=True).clamp_max(state["experts"] - 1)
+    begins = torch.cat((ends.new_zeros(1), ends[:-1]))
+    real = row < pad_begins[expert]
+    return real, (expert * state["fullest"] + row - begins[expert])[real]
+
+
+def _by_expert(rows: torch.Tensor, places: torch.Tensor, state: dict) -> torch.Tensor:
+    padded = torch.zeros(state["experts"] * state["fullest"], rows.size(1), device="cuda")
+    padded[places] = rows
+    return padded.view(state["experts"], state["fullest"], -1)
+
+
+def _activate(values: torch.Tensor, gated: bool, activation: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """act(x) and act'(x)."""
+    x = values.chunk(2, dim=-1)[0] if gated else values
+    if activation == "silu":
+        sigma = 1 / (1 + torch.exp(-x))
+        return x * sigma, sigma * (1 + x * (1 - sigma))
+    if activation == "gelu":
+        tanh = torch.tanh(0.7978845608028654 * (x + 0.044715 * x * x * x))
+        return 0.5 * x * (1 + tanh), 0.5 * (1 + tanh) + 0.5 * x * (1 - tanh * tanh) * 0.7978845608028654 * (1 + 0.134145 * x * x)
+    positive = x.clamp_min(0)
+    return positive * positive, 2 * positive
+
+
+def _activation_forward(values: torch.Tensor, gated: bool, activation: str) -> torch.Tensor:
+    out = _activate(values, gated, activation)[0]
+    return out * values.chunk(2, dim=-1)[1] if gated else out
+
+
+def _activation_backward(grad: torch.Tensor, values: torch.Tensor, gated: bool, activation: str) -> torch.Tensor:
+    out, slope = _activate(values, gated, activation)
+    return torch.cat((grad * values.chunk(2, dim=-1)[1] * slope, grad * out), dim=-1) if gated else grad * slope
+
+
+def _plain_quantize(state: dict) -> dict:
+    values = state["input"].float()
+    if state["experts"]:
+        values = torch.where(_rows_of_tokens(state)[0][:, None], values, 0.0)
+    if state["form"] == "rows":
+        return _named(rows=_said(values))
+    transposed = values.view(state["groups"], -1, state["columns"]).transpose(1, 2).reshape(state["groups"] * state["columns"], -1)
+    return _named(rows=_said(values), transposed=_said(transposed))
+
+
+def _plain_product(state: dict) -> torch.Tensor:
+    real, places = _rows_of_tokens(state)
+    weight = _values(state["weight"]).view(state["experts"], state["columns"], -1)
+    sums = torch.bmm(_by_expert(_values(state["rows"])[real], places, state), weight.transpose(1, 2).contiguous())
+    out = torch.zeros_like(state["out"])
+    out[real] = sums.view(-1, state["columns"])[places].to(out.dtype)
+    return out
+
+
+def _plain_gradient(state: dict) -> torch.Tensor:
+    real, places = _rows_of_tokens(state)
+    lhs, rhs = (_by_expert(_values(state[name]).t()[real], places, state) for name in ("lhs", "rhs"))
+    sums = torch.bmm(lhs.transpose(1, 2).contiguous(), rhs).view(state["gradient"].shape)
+    if state["accumulate"]:
+        sums = sums + state["gradient"].float()
+    return state["gradient"].copy_(sums)
+
+
+def _plain_activation(state: dict) -> dict:
+    gated, activation = state["gated"], state["activation"]
+    real = _rows_of_tokens(state)[0][:, None]
+    input_, grad_output = (torch.where(real, state[name].float(), 0.0) for name in ("input", "grad_output"))
+    kept = torch.cat([_quantized(part) for part in input_.chunk(2, dim=-1)], dim=-1) if gated else _quantized(input_)
+    grad = _activation_backward(grad_output, kept, gated, activation)
+    return _named(
+        output=_said(_activation_forward(input_, gated, activation)),
+        checkpoint=_said(input_),
+        grad=_said(grad),
+        grad_transposed=_said(grad.t().contiguous()),
+        output_transposed=_said(_activation_forward(kept, gated, activation).t().contiguous()),
+    )
+
+
+def _plain_mlp(state: dict) -> dict:
+    experts, fullest, dtype = state["experts"], state["fullest"], _DTYPES[state["dtype"]]
+    hidden, slots, tokens, gated, activation = state["hidden"], state["slots"], state["tokens"], state["gated"], state["activation"]
+    flat = state["top_experts"].flatten()
+    chosen = torch.nn.functional.one_hot(flat, experts)
+    places = flat * fullest + (chosen.cumsum(0) - chosen).gather(1, flat[:, None])[:, 0]
+    token = torch.arange(tokens, device="cuda").repeat_interleave(slots)
+    scores, grad_output = state["scores"].detach(), state["grad_output"].float()
+
+    def product(rows: torch.Tensor, weight: dict) -> torch.Tensor:
+        """Rows of the entries times the transposed weights of their experts, in the MLP's type."""
+        weight = _values(weight).view(experts, -1, weight["columns"]).transpose(1, 2).contiguous()
+        return torch.bmm(_by_expert(rows, places, state), weight).flatten(0, 1)[places].to(dtype).float()
+
+    def columns(rows: torch.Tensor) -> torch.Tensor:
+        """[experts, columns, rows padded to whole blocks] of the entries' rows, quantised along the rows."""
+        padded = _by_expert(rows, places, state)
+        return _quantized(padded.transpose(1, 2).reshape(-1, fullest)).view(experts, -1, fullest)
+
+    rows = _quantized(state["input"].detach().float())[token]
+    layer_1 = product(rows, state["layer_1"])
+    kept = _quantized(layer_1)
+    layer_2 = product(_quantized(_activation_forward(layer_1, gated, activation)), state["layer_2_transposed"])
+    del layer_1
+    output = (layer_2.view(tokens, slots, hidden) * scores[..., None]).sum(1).to(dtype)
+    grad_scores = (layer_2.view(tokens, slots, hidden) * grad_output[:, None]).sum(2).to(dtype)
+    del layer_2
+    grad_2 = (grad_output[:, None] * scores[..., None]).to(dtype).float().view(-1, hidden)
+    grad_activation = product(_quantized(grad_2), state["layer_2"])
+    grad_weight_2 = torch.bmm(columns(_activation_forward(kept, gated, activation)), columns(grad_2).transpose(1, 2).contiguous())
+    del grad_2
+    grad_1 = _activation_backward(grad_activation, kept, gated, activation)
+    del grad_activation, kept
+    grad_input = product(_quantized(grad_1), state["layer_1_transposed"]).view(tokens, slots, hidden).sum(1).to(dtype)
+    grad_weight_1 = torch.bmm(columns(grad_1), columns(rows).transpose(1, 2).contiguous())
+    return {
+        "output": output, "grad_input": grad_input, "grad_scores": grad_scores, "grad_weight_1": grad_weight_1.flatten(0, 1).to(dtype),
+        "grad_weight_2": grad_weight_2.flatten(0, 1).to(dtype),
+    }  # fmt: skip
+
+
+# ---- one pass --------------------------------------------------------------------------------------------
+def run(state: dict):
+    if own:
+        return _run_own(state)
+    plain = {"quantize": _plain_quantize, "product": _plain_product, "gradient": _plain_gradient, "activation": _plain_activation, "mlp": _plain_mlp}
+    return plain[state["kind"]](state)
+
+
+def _run_own(state: dict):
+    from fast_llm_amd.functional import block_scaling
+    from fast_llm_amd.functional.sparse_copy import SparseMap, get_sparse_map
+
+    def said(quantized) -> tuple[torch.Tensor, torch.Tensor]:
+        return quantized.elements, quantized.block_scales
+
+    if state["kind"] == "mlp":
+        sparse_map = get_sparse_map(state["top_experts"], state["experts"])
+        weights = block_scaling.BlockScaledWeights(
+            *(block_scaling.BlockScaledTensor(**state[name]) for name in ("layer_1", "layer_1_transposed", "layer_2", "layer_2_transposed"))
+        )
+        for weight in state["weights"]:
+            weight.param_grad_is_zero = True
+        output = block_scaling.block_mlp(
+            state["input"], state["scores"], *state["weights"], weights, gated=state["gated"], activation_type=state["activation"], sparse_map=sparse_map
+        )
+        grad_input, grad_scores = torch.autograd.grad(output, (state["input"], state["scores"]), state["grad_output"])
+        # The scores' gradient has values of the MLP's type, whatever the scores' own.
+        return {
+            "output": output.detach(), "grad_input": grad_input, "grad_scores": grad_scores.to(state["input"].dtype),
+            "grad_weight_1": state["weights"][0].grad_buffer, "grad_weight_2": state["weights"][1].grad_buffer,
+        }  # fmt: skip
+    sparse_map = None
+    if state["experts"]:
+        tokens = state["rows"] if state["kind"] == "quantize" else state["tokens"]
+        sparse_map = SparseMap(
+            None, state["expert_ends"], state["expert_pad_begins"], tokens, state["sparse_rows"], tokens * state["slots"], state["experts"], state["slots"]
+        )
+    if state["kind"] == "quantize":
+        if state["form"] == "rows":
+            return _named(rows=said(block_scaling.block_quantize(state["input"])))
+        rows, transposed = block_scaling.block_quantize_both(state["input"], groups=state["groups"], sparse_map=sparse_map)
+        return _named(rows=said(rows), transposed=said(transposed))
+    if state["kind"] == "product":
+        rows, weight = (block_scaling.BlockScaledTensor(**state[name]) for name in ("rows", "weight"))
+        return block_scaling.block_sparse_matmul(rows, weight, sparse_map, out=state["out"])
+    if state["kind"] == "gradient":
+        lhs, rhs = (block_scaling.BlockScaledTensor(**state[name]) for name in ("lhs", "rhs"))
+        return block_scaling.block_input_row_sparse_matmul(lhs, rhs, sparse_map, out=state["gradient"], accumulate=state["accumulate"])
+    output, checkpoint = block_scaling.block_activation_forward(state["input"], state["gated"], state["activation"], sparse_map)
+    grad, grad_transposed, output_transposed = block_scaling.block_activation_backward(
+        state["grad_output"], checkpoint, state["gated"], state["activation"], sparse_map
+    )
+    return _named(
+        output=said(output), checkpoint=said(checkpoint), grad=said(grad), grad_transposed=said(grad_transposed), output_transposed=said(output_transposed)
+    )
+
+
+# ---- the definitions in 64 bits --------------------------------------------------------------------------
+def _exact_quantized(values: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Elements and scales, [rows, columns] and [rows, blocks], by the definition: the grid's spacing at a value's size is
+    2^(its exponent - 3), and no finer than at the smallest normal value, 2^-6."""
+    values = values.double()
+    columns = values.size(1)
+    largest = torch.nn.functional.pad(values.abs(), (0, -columns % _BLOCK)).unflatten(1, (-1, _BLOCK)).amax(-1)
+    scales = torch.exp2(torch.ceil(torch.log2(largest / 448)).clamp(-127, 127))
+    scaled = values / scales.repeat_interleave(_BLOCK, dim=1)[:, :columns]
+    spacing = torch.exp2(torch.floor(torch.log2(scaled.abs().clamp_min(2.0**-200))).clamp_min(-6) - 3)
+    return torch.round(scaled / spacing) * spacing, scales
+
+
+def _exact_kept(values: torch.Tensor) -> torch.Tensor:
+    elements, scales = _exact_quantized(values)
+    return elements * scales.repeat_interleave(_BLOCK, dim=1)[:, : values.size(1)]
+
+
+def _exact_values(stored: dict, rows: slice = slice(None), columns: slice = slice(None)) -> torch.Tensor:
+    """What the bytes stand for; `columns`: from a block's first."""
+    bytes_ = stored["values"][rows, : stored["columns"]][:, columns]
+    scales = torch.exp2(stored["scales"][rows].double() - 127)[:, (columns.start or 0) // _BLOCK :]
+    sign, exponent, fraction = bytes_ >> 7, (bytes_ >> 3 & 15).double(), (bytes_ & 7).double() / 8
+    size = torch.where(exponent > 0, (1 + fraction) * torch.exp2(exponent - 7), fraction * 2.0**-6)
+    return (1 - 2 * sign.double()) * size * scales.repeat_interleave(_BLOCK, dim=1)[:, : bytes_.size(1)]
+
+
+def _exact_activation(values: torch.Tensor, case: dict) -> torch.Tensor:
+    gate = values[:, : case["ffn"]]
+    if case["activation"] == "silu":
+        out = gate * torch.sigmoid(gate)
+    elif case["activation"] == "gelu":
+        out = torch.nn.functional.gelu(gate, approximate="tanh")
+    else:
+        out = torch.relu(gate) ** 2
+    return out * values[:, case["ffn"] :] if case["gated"] else out
+
+
+def _exact_activation_gradient(grad: torch.Tensor, values: torch.Tensor, case: dict) -> torch.Tensor:
+    values = values.detach().requires_grad_(True)
+    with torch.enable_grad():
+        return torch.autograd.grad(_exact_activation(values, case), values, grad)[0]
+
+
+def _experts_rows(state: dict):
+    """(expert, its first row, the end of its tokens' rows, the end of its rows)"""
+    ends, pad_begins = state["expert_ends"].tolist(), state["expert_pad_begins"].tolist()
+    return zip(range(state["experts"]), [0] + ends[:-1], pad_begins, ends)
+
+
+def _exact_step(case: dict, state: dict) -> dict:
+    dtype, hidden, ffn, tokens = _DTYPES[case["dtype"]], case["hidden"], case["ffn"], case["tokens"]
+    layer_1_rows = ffn * (2 if case["gated"] else 1)
+    rows, scores, grad_output = _exact_kept(state["input"].detach()), state["scores"].detach().double(), state["grad_output"].double()
+    outputs = {
+        "output": torch.zeros(tokens, hidden, dtype=torch.float64, device="cuda"),
+        "grad_input": torch.zeros(tokens, hidden, dtype=torch.float64, device="cuda"),
+        "grad_scores": torch.zeros(tokens, case["slots"], dtype=torch.float64, device="cuda"),
+        "grad_weight_1": torch.zeros(case["experts"] * layer_1_rows, hidden, dtype=torch.float64, device="cuda"),
+        "grad_weight_2": torch.zeros(case["experts"] * ffn, hidden, dtype=torch.float64, device="cuda"),
+    }
+
+    def along_rows(values: torch.Tensor) -> torch.Tensor:
+        return _exact_kept(values.t().contiguous())
+
+    for expert in range(case["experts"]):
+        token, slot = torch.where(state["top_experts"] == expert)
+        if not token.numel():
+            continue
+        of_1, of_2, of_hidden = (slice(expert * size, (expert + 1) * size) for size in (layer_1_rows, ffn, hidden))
+        x, score, grad = rows[token], scores[token, slot, None], grad_output[token]
+        layer_1 = (x @ _exact_values(state["layer_1"], of_1).t()).to(dtype).double()
+        kept = torch.cat([_exact_kept(part) for part in layer_1.split(ffn, dim=1)], dim=1)
+        layer_2 = (_exact_kept(_exact_activation(layer_1, case)) @ _exact_values(state["layer_2_transposed"], of_hidden).t()).to(dtype).double()
+        outputs["output"].index_add_(0, token, layer_2 * score)
+        outputs["grad_scores"][token, slot] = (layer_2 * grad).sum(1)
+        grad_2 = (grad * score).to(dtype).double()
+        grad_activation = (_exact_kept(grad_2) @ _exact_values(state["layer_2"], of_2).t()).to(dtype).double()
+        outputs["grad_weight_2"][of_2] = along_rows(_exact_activation(kept, case)) @ along_rows(grad_2).t()
+        grad_1 = _exact_activation_gradient(grad_activation, kept, case)
+        kept_1 = torch.cat([_exact_kept(part) for part in grad_1.split(ffn, dim=1)], dim=1)
+        grad_rows = (kept_1 @ _exact_values(state["layer_1_transposed"], of_hidden).t()).to(dtype).double()
+        outputs["grad_input"].index_add_(0, token, grad_rows)
+        outputs["grad_weight_1"][of_1] = along_rows(grad_1) @ along_rows(x).t()
+    return outputs
+
+
+def exact(case: dict, seed: int):
+    state = prepare(case, seed)
+    if case["kind"] == "mlp":
+        return _exact_step(case, state)
+    if case["kind"] == "quantize":
+        values = state["input"].double()
+        if case["experts"]:
+            kept = torch.zeros_like(values)
+            for _, begin, end, _ in _experts_rows(state):
+                kept[begin:end] = values[begin:end]
+            values = kept
+        outputs = {"rows": [_exact_quantized(part) for part in values.chunk(case["groups"])]}
+        if case["form"] == "both":
+            outputs["transposed"] = [_exact_quantized(part.t().contiguous()) for part in values.chunk(case["groups"])]
+        return _named(**{name: tuple(torch.cat(part) for part in zip(*parts)) for name, parts in outputs.items()})
+    if case["kind"] == "product":
+        out = torch.zeros(state["sparse_rows"], case["columns"], dtype=torch.float64, device="cuda")
+        for expert, begin, end, _ in _experts_rows(state):
+            weight = _exact_values(state["weight"], slice(expert * case["columns"], (expert + 1) * case["columns"]))
+            out[begin:end] = _exact_values(state["rows"], slice(begin, end)) @ weight.t()
+        return out
+    if case["kind"] == "gradient":
+        out = state["gradient"].double() if case["accumulate"] else torch.zeros(state["gradient"].shape, dtype=torch.float64, device="cuda")
+        for expert, begin, _, end in _experts_rows(state):
+            # The padding holds zeros.
+            lhs, rhs = (_exact_values(state[name], columns=slice(begin, end)) for name in ("lhs", "rhs"))
+            out[expert * case["rows"] : (expert + 1) * case["rows"]] += lhs @ rhs.t()
+        return out
+    rows = torch.zeros(state["sparse_rows"], 1, dtype=torch.float64, device="cuda")
+    for _, begin, end, _ in _experts_rows(state):
+        rows[begin:end] = 1
+    input_, grad_output = state["input"].double() * rows, state["grad_output"].double() * rows
+    kept = torch.cat([_exact_kept(part) for part in input_.split(case["ffn"], dim=1)], dim=1)
+    grad = _exact_activation_gradient(grad_output, kept, case)
+    return _named(
+        output=_exact_quantized(_exact_activation(input_, case)),
+        checkpoint=_exact_quantized(input_),
+        grad=_exact_quantized(grad),
+        grad_transposed=_exact_quantized(grad.t().contiguous()),
+        output_transposed=_exact_quantized(_exact_activation(kept, case).t().contiguous()),
+    )
+
+
+# ---- what a pass cannot do without -----------------------------------------------------------------------
+_QUANTIZED = 1 + 1 / _BLOCK  # bytes of a value
+
+
+def _selected(case: dict) -> float:
+    """Experts that some token is expected to select."""
+    return (1 - (1 - case["slots"] / case["experts"]) ** case["tokens"]) * case["experts"]
+
+
+def work(case: dict) -> dict:
+    size = 4 if case["dtype"] == "fp32" else 2
+    if case["kind"] == "quantize":
+        values = case["rows"] * case["groups"] * case["slots"] * case["columns"]
+        forms = 2 if case["form"] == "both" else 1
+        return {"bytes": values * (size + forms * _QUANTIZED), "flops": 4 * forms * values}
+    entries = case["tokens"] * case["slots"]
+    if case["kind"] == "product":
+        inner, columns = case["inner"], case["columns"]
+        return {
+            "bytes": (_selected(case) * inner * columns + entries * inner) * _QUANTIZED + entries * columns * size,
+            "flops": 2 * entries * inner * columns,
+        }
+    if case["kind"] == "gradient":
+        weights = case["experts"] * case["rows"] * case["columns"]
+        return {
+            "bytes": entries * (case["rows"] + case["columns"]) * _QUANTIZED + weights * size * (2 if case["accumulate"] else 1),
+            "flops": 2 * entries * case["rows"] * case["columns"],
+        }
+    if case["kind"] == "activation":
+        values, parts = entries * case["ffn"], 2 if case["gated"] else 1
+        # Forward: input in, result and checkpoint out; backward: checkpoint and gradient in, both forms of the gradient and the result out.
+        return {"bytes": values * ((parts + 1) * size + (parts + 1 + 3 * parts + 1) * _QUANTIZED), "flops": 60 * values}
+    products = case["hidden"] * case["ffn"] * (3 if case["gated"] else 2)
+    return {
+        # Weights in both forms, their gradients, the tokens and their gradients there and back.
+        "bytes": _selected(case) * products * 2 * _QUANTIZED + case["experts"] * products * size + 4 * case["tokens"] * case["hidden"] * size,
+        "flops": 6 * entries * products,
+    }
