@@ -8,7 +8,8 @@ backward made of them. Sizes are the benchmark's (`fast_llm_amd.workloads.WORKLO
 
 Definition of the format: 128 neighbours along a row share the scale 2^e, e the smallest integer with (largest magnitude) <= 448 * 2^e, at least
 -127, stored as the byte e + 127; elements are value / 2^e in e4m3, rounded to nearest even. Rows are stored padded with zeros to whole
-blocks. With a sparse map the rows that no token has count as zeros.
+blocks; the scales of the rows' first blocks come first, then those of their second blocks. With a sparse map the rows that no token has count
+as zeros.
 """
 
 import torch
@@ -156,32 +157,35 @@ def _padded(size: int) -> int:
     return -(-size // _BLOCK) * _BLOCK
 
 
-def _stored(values: torch.Tensor) -> dict:
-    """fp32 rows as they are kept: the bytes of the elements, padded, and of the scales."""
-    elements, exponents = _parts(values)
+def _room(rows: int, columns: int) -> dict:
+    """Where rows are kept: the bytes of the elements [rows, padded], and of the scales [blocks, rows (a multiple of 16)]."""
     return {
-        "values": elements.flatten(1).to(torch.float8_e4m3fn).view(torch.uint8),
-        "scales": (exponents + 127).to(torch.uint8),
-        "columns": values.size(1),
+        "values": torch.empty(rows, _padded(columns), dtype=torch.uint8, device="cuda"),
+        "scales": torch.zeros(_padded(columns) // _BLOCK, -(-rows // 16) * 16, dtype=torch.uint8, device="cuda"),
+        "columns": columns,
     }
+
+
+def _store(values: torch.Tensor, to: dict, first: int = 0) -> dict:
+    """fp32 rows in their place from row `first` on."""
+    elements, exponents = _parts(values)
+    rows = slice(first, first + values.size(0))
+    to["values"][rows] = elements.flatten(1).to(torch.float8_e4m3fn).view(torch.uint8)
+    to["scales"][:, rows] = (exponents + 127).to(torch.uint8).t()
+    return to
+
+
+def _stored(values: torch.Tensor) -> dict:
+    return _store(values, _room(*values.shape))
 
 
 def _stored_weights(generator: torch.Generator, experts: int, rows: int, columns: int, transposed: bool) -> list[dict]:
     """Normal weights [experts * rows, columns], and where asked for also [experts * columns, rows]."""
-    out = [
-        {
-            "values": torch.empty(experts * r, _padded(c), dtype=torch.uint8, device="cuda"),
-            "scales": torch.empty(experts * r, _padded(c) // _BLOCK, dtype=torch.uint8, device="cuda"),
-            "columns": c,
-        }
-        for r, c in ((rows, columns), (columns, rows))[: 1 + transposed]
-    ]
+    out = [_room(experts * r, c) for r, c in ((rows, columns), (columns, rows))[: 1 + transposed]]
     for expert in range(experts):
         weight = _normal(generator, (rows, columns), torch.bfloat16, 0.02).float()
         for to, form in zip(out, (weight, weight.t())):
-            part, size = _stored(form.contiguous()), form.size(0)
-            to["values"][expert * size : (expert + 1) * size] = part["values"]
-            to["scales"][expert * size : (expert + 1) * size] = part["scales"]
+            _store(form.contiguous(), to, expert * form.size(0))
     return out
 
 
@@ -276,7 +280,7 @@ def _quantized(values: torch.Tensor) -> torch.Tensor:
 
 def _values(stored: dict) -> torch.Tensor:
     """The fp32 values that stored rows stand for."""
-    scales = torch.ldexp(torch.ones((), device="cuda"), stored["scales"].int() - 127)
+    scales = torch.ldexp(torch.ones((), device="cuda"), stored["scales"][:, : stored["values"].size(0)].t().int() - 127)
     return (stored["values"].view(torch.float8_e4m3fn).float() * scales.repeat_interleave(_BLOCK, dim=1))[:, : stored["columns"]]
 
 
@@ -495,7 +499,7 @@ def _exact_kept(values: torch.Tensor) -> torch.Tensor:
 def _exact_values(stored: dict, rows: slice = slice(None), columns: slice = slice(None)) -> torch.Tensor:
     """What the bytes stand for; `columns`: from a block's first."""
     bytes_ = stored["values"][rows, : stored["columns"]][:, columns]
-    scales = torch.exp2(stored["scales"][rows].double() - 127)[:, (columns.start or 0) // _BLOCK :]
+    scales = torch.exp2(stored["scales"][:, : stored["values"].size(0)].t()[rows].double() - 127)[:, (columns.start or 0) // _BLOCK :]
     sign, exponent, fraction = bytes_ >> 7, (bytes_ >> 3 & 15).double(), (bytes_ & 7).double() / 8
     size = torch.where(exponent > 0, (1 + fraction) * torch.exp2(exponent - 7), fraction * 2.0**-6)
     return (1 - 2 * sign.double()) * size * scales.repeat_interleave(_BLOCK, dim=1)[:, : bytes_.size(1)]
