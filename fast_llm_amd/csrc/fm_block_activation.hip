@@ -1,0 +1,189 @@
+// The MLP's activation between products of 8 bits: forward into the second layer's rows and a checkpoint of the input, both of 8 bits; backward from that
+// checkpoint into what the remaining products read: the input's gradient along its rows and its columns, and the forward's result along its columns.
+//
+// Both are one pass over their operands and no 16-bit copy leaves them. The forward is bound by memory. Of the backward every element has four conversions and
+// the slope of the activation, so that memory and arithmetic weigh about the same; a lane keeps its three results (gate's and up's gradient, output)
+// in registers between the two directions of quantisation, eight rows x four columns of each.
+#include "fm_activation_math.h"
+#include "fm_block_rows.h"
+
+namespace fm {
+
+namespace block {
+
+struct ActivationArgs {
+    const void *input;                    // forward
+    const void *grad_output;              // backward
+    uint8_t *checkpoint, *checkpoint_scales;
+    uint8_t *output, *output_scales;      // backward: transposed
+    uint8_t *grad, *grad_scales, *grad_transposed, *grad_transposed_scales;
+    int64_t rows, columns;                // of the result
+    int64_t input_stride, grad_output_stride, checkpoint_stride, checkpoint_scale_stride, output_stride, output_scale_stride, grad_stride, grad_scale_stride,
+        transposed_stride, transposed_scale_stride;
+    uint32_t column_blocks;
+    RowMap map;
+};
+
+template <typename T, int kActivation, bool kGated>
+__global__ __launch_bounds__(kRowThreads) void activation_forward_kernel(ActivationArgs args) {
+    const uint32_t column_block = blockIdx.x % args.column_blocks;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x / args.column_blocks) * kBlock, column = static_cast<int64_t>(column_block) * kBlock + threadIdx.x % 8 * 16;
+    const int count = rows_in_block(args.map, row0, args.rows);
+#pragma unroll 2
+    for (int step = 0; step < kRowSteps; ++step) {
+        const int in_block = step * (kRowThreads / 8) + static_cast<int>(threadIdx.x) / 8;
+        const int64_t row = row0 + in_block, left = in_block < count ? args.columns - column : 0;
+        const T *input = static_cast<const T *>(args.input) + row * args.input_stride + column;
+        float gate[16], up[16], result[16];
+        load_values(input, left, gate);
+        if constexpr (kGated) load_values(input + args.columns, left, up);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            result[i] = activation_forward<kActivation>(gate[i]);
+            if constexpr (kGated) result[i] *= up[i];
+        }
+        const bool exists = row < args.rows;
+        uint8_t *checkpoint = args.checkpoint + row * args.checkpoint_stride + column, *scales = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row;
+        store_row(gate, checkpoint, scales, exists);
+        // (Gated: whole blocks of columns.)
+        if constexpr (kGated) store_row(up, checkpoint + args.columns, scales + args.column_blocks * args.checkpoint_scale_stride, exists);
+        store_row(result, args.output + row * args.output_stride + column, args.output_scales + column_block * args.output_scale_stride + row, exists);
+    }
+}
+
+template <typename T, int kActivation, bool kGated>
+__global__ __launch_bounds__(kSquareThreads) void activation_backward_kernel(ActivationArgs args) {
+    __shared__ __attribute__((aligned(16))) Square shared;
+    const uint32_t column_block = blockIdx.x % args.column_blocks;
+    const int64_t row_block = blockIdx.x / args.column_blocks, row0 = row_block * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
+    const int cg = threadIdx.x & 31, row_group = threadIdx.x >> 5;
+    const int exist = static_cast<int>(min(args.rows - row0, static_cast<int64_t>(kBlock))), count = rows_in_block(args.map, row0, args.rows);
+    const int64_t column = column0 + cg * kLaneColumns;
+    constexpr int kParts = kGated ? 2 : 1;
+    float grads[kParts][kLaneRows][kLaneColumns], output[kLaneRows][kLaneColumns];
+#pragma unroll
+    for (int r = 0; r < kLaneRows; ++r) {
+        const int in_block = row_group * kLaneRows + r;
+        const int64_t row = row0 + in_block, left = in_block < count ? args.columns - column : 0;
+        float gate[kLaneColumns] = {}, up[kLaneColumns] = {}, grad[kLaneColumns];
+        load_values(static_cast<const T *>(args.grad_output) + row * args.grad_output_stride + column, left, grad);
+        if (left > 0) {
+            const uint8_t *checkpoint = args.checkpoint + row * args.checkpoint_stride + column, *scales = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row;
+            unpack_four(*reinterpret_cast<const uint32_t *>(checkpoint), scale_value(*scales), gate);
+            if constexpr (kGated)
+                unpack_four(*reinterpret_cast<const uint32_t *>(checkpoint + args.columns), scale_value(scales[args.column_blocks * args.checkpoint_scale_stride]), up);
+        }
+#pragma unroll
+        for (int c = 0; c < kLaneColumns; ++c) {
+            float out;
+            const float slope = activation_backward<kActivation>(gate[c], out);
+            if constexpr (kGated) {
+                grads[0][r][c] = slope * up[c] * grad[c];
+                grads[1][r][c] = out * grad[c];
+                out *= up[c];
+            } else {
+                grads[0][r][c] = slope * grad[c];
+            }
+            output[r][c] = out;
+        }
+    }
+    const int columns = static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock)));
+    const int64_t scales_of_rows = row_block * args.transposed_scale_stride;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+        const int64_t first_column = column0 + part * args.columns;
+        column_maxima(grads[part], shared);
+        store_rows(grads[part], shared, args.grad + row0 * args.grad_stride + first_column, args.grad_stride, exist);
+        __syncthreads();
+        stage_columns(grads[part], shared);
+        __syncthreads();
+        store_row_scales(shared, args.grad_scales + (column_block + part * args.column_blocks) * args.grad_scale_stride + row0, exist);
+        store_columns(shared, args.grad_transposed + first_column * args.transposed_stride + row0, args.transposed_stride,
+                      args.grad_transposed_scales + scales_of_rows + first_column, columns);
+        __syncthreads();
+    }
+    column_maxima(output, shared);
+    __syncthreads();
+    stage_columns(output, shared);
+    __syncthreads();
+    store_columns(shared, args.output + column0 * args.output_stride + row0, args.output_stride, args.output_scales + row_block * args.output_scale_stride + column0, columns);
+}
+
+template <typename T, bool kGated>
+static void launch_activation(bool forward, int activation, const ActivationArgs &args, uint32_t grid, hipStream_t stream) {
+    FM_DISPATCH_ACTIVATION(activation, kActivation, {
+        if (forward) activation_forward_kernel<T, kActivation, kGated><<<grid, kRowThreads, 0, stream>>>(args);
+        else activation_backward_kernel<T, kActivation, kGated><<<grid, kSquareThreads, 0, stream>>>(args);
+    });
+}
+
+// Checks and launch of both directions; `args` without what is computed here.
+static int run_activation(const char *name, bool forward, ActivationArgs args, const void *expert_ends, const void *expert_pad_begins, int64_t num_experts, int gated,
+                          int activation, int dtype, int index_dtype, void *stream) {
+    FM_REQUIRE(valid_dtype(dtype), "%s: bad dtype %d", name, dtype);
+    FM_REQUIRE(activation >= FM_ACT_GELU && activation <= FM_ACT_IDENTITY, "%s: bad activation %d", name, activation);
+    FM_REQUIRE(args.rows >= 0 && args.rows < (int64_t(1) << 31) && args.columns > 0 && args.columns <= kMaxColumns / 2, "%s: bad sizes", name);
+    if (int status = check_map(name, args.map, expert_ends, expert_pad_begins, num_experts, index_dtype)) return status;
+    if (gated && args.columns % kBlock != 0) return fail(FM_ERR_UNSUPPORTED, "%s: a gated activation has whole blocks of %d columns", name, kBlock);
+    if (args.rows == 0) return FM_OK;
+    const int64_t parts = gated ? 2 : 1, input_columns = parts * args.columns, padded = padded_columns(args.columns), padded_input = padded_columns(input_columns);
+    const int64_t row_padding = padded_columns(args.rows);
+    const void *plain = forward ? args.input : args.grad_output;
+    FM_REQUIRE(plain && reinterpret_cast<uintptr_t>(plain) % dtype_size(dtype) == 0, "%s: null or misaligned tensor", name);
+    FM_REQUIRE(args.rows <= 1 || (forward ? args.input_stride >= input_columns : args.grad_output_stride >= args.columns), "%s: rows overlap", name);
+    args.column_blocks = static_cast<uint32_t>(padded / kBlock);
+    if (forward) args.checkpoint_stride = padded_input, args.output_stride = padded;
+    else args.grad_stride = padded_input, args.transposed_stride = args.output_stride = row_padding;
+    if (int status = check_tensor(name, "the checkpoint", args.checkpoint, args.checkpoint_scales, args.rows, padded_input, args.checkpoint_stride,
+                                  args.checkpoint_scale_stride)) return status;
+    if (int status = check_tensor(name, "the output", args.output, args.output_scales, forward ? args.rows : args.columns, args.output_stride, args.output_stride,
+                                  args.output_scale_stride)) return status;
+    if (!forward) {
+        if (int status = check_tensor(name, "the gradient", args.grad, args.grad_scales, args.rows, padded_input, padded_input, args.grad_scale_stride)) return status;
+        if (int status = check_tensor(name, "the transposed gradient", args.grad_transposed, args.grad_transposed_scales, input_columns, row_padding, row_padding,
+                                      args.transposed_scale_stride)) return status;
+    }
+    const int64_t grid = row_padding / kBlock * args.column_blocks;
+    if (grid >= (int64_t(1) << 32) / kSquareThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
+    FM_DISPATCH_DTYPE(dtype, T, {
+        if (gated) launch_activation<T, true>(forward, activation, args, static_cast<uint32_t>(grid), static_cast<hipStream_t>(stream));
+        else launch_activation<T, false>(forward, activation, args, static_cast<uint32_t>(grid), static_cast<hipStream_t>(stream));
+    });
+    return check_launch(name);
+}
+
+}  // namespace block
+
+}  // namespace fm
+
+using namespace fm;
+
+extern "C" int fm_block_activation_forward(const void *input, void *output, void *output_scales, void *checkpoint, void *checkpoint_scales,
+                                           const void *expert_ends, const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t num_experts,
+                                           int64_t input_stride, int64_t output_scale_stride, int64_t checkpoint_scale_stride, int gated, int activation,
+                                           int dtype, int index_dtype, void *stream) {
+    block::ActivationArgs args{};
+    args.input = input, args.output = static_cast<uint8_t *>(output), args.output_scales = static_cast<uint8_t *>(output_scales);
+    args.checkpoint = static_cast<uint8_t *>(checkpoint), args.checkpoint_scales = static_cast<uint8_t *>(checkpoint_scales);
+    args.rows = rows, args.columns = columns, args.input_stride = input_stride;
+    args.output_scale_stride = output_scale_stride, args.checkpoint_scale_stride = checkpoint_scale_stride;
+    return block::run_activation("fm_block_activation_forward", true, args, expert_ends, expert_pad_begins, num_experts, gated, activation, dtype, index_dtype, stream);
+}
+
+extern "C" int fm_block_activation_backward(const void *grad_output, const void *checkpoint, const void *checkpoint_scales, void *grad, void *grad_scales,
+                                            void *grad_transposed, void *grad_transposed_scales, void *output_transposed, void *output_transposed_scales,
+                                            const void *expert_ends, const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t num_experts,
+                                            int64_t grad_output_stride, int64_t checkpoint_stride, int64_t checkpoint_scale_stride, int64_t grad_scale_stride,
+                                            int64_t grad_transposed_scale_stride, int64_t output_transposed_scale_stride, int gated, int activation, int dtype,
+                                            int index_dtype, void *stream) {
+    block::ActivationArgs args{};
+    args.grad_output = grad_output;
+    args.checkpoint = static_cast<uint8_t *>(const_cast<void *>(checkpoint)), args.checkpoint_scales = static_cast<uint8_t *>(const_cast<void *>(checkpoint_scales));
+    args.grad = static_cast<uint8_t *>(grad), args.grad_scales = static_cast<uint8_t *>(grad_scales);
+    args.grad_transposed = static_cast<uint8_t *>(grad_transposed), args.grad_transposed_scales = static_cast<uint8_t *>(grad_transposed_scales);
+    args.output = static_cast<uint8_t *>(output_transposed), args.output_scales = static_cast<uint8_t *>(output_transposed_scales);
+    args.rows = rows, args.columns = columns, args.grad_output_stride = grad_output_stride;
+    args.checkpoint_stride = checkpoint_stride, args.checkpoint_scale_stride = checkpoint_scale_stride, args.grad_scale_stride = grad_scale_stride;
+    args.transposed_scale_stride = grad_transposed_scale_stride, args.output_scale_stride = output_transposed_scale_stride;
+    return block::run_activation("fm_block_activation_backward", false, args, expert_ends, expert_pad_begins, num_experts, gated, activation, dtype, index_dtype, stream);
+}

@@ -1,0 +1,474 @@
+// Products of operands of 8 bits with a scale per block of 128, on tiles of 256 x 256: rows times expert weights, and weight gradients (the same product with
+// an expert's part of the reduction in place of its part of the rows). Both operands lie along the reduction.
+//
+// One workgroup per CU walks over its tiles. Its four wavefronts, one per SIMD, multiply 128 rows x 128 weight rows each (4 x 4 blocks of
+// v_mfma_scale_f32_32x32x64_f8f6f4, 256 accumulation registers; D's rows are weight rows, so that a lane has neighbouring columns of one row). The reduction
+// passes in slices of 128, a block of the format, through two LDS slots of 64 KB. A slice's bytes go straight from memory into LDS; they are asked for as soon
+// as the slice two before them has been read, half a slice before it has been multiplied, and on into the next tile. The fragments of a step of 64 are
+// read while the step before is multiplied: each product has one or two reads or loads in its shadow. The scales, a byte for each row and slice,
+// come as bytes to the registers of the lanes that hold the rows: 32 neighbours at a time, since the scales of a slice are next to each other.
+//
+// A row's slice is 128 bytes, in LDS XOR-swizzled in units of 16 bytes so that 16 lanes that read the same unit of neighbouring rows hit all 64
+// banks. Of every 32 weight rows, LDS row 8 a + 4 h + b holds row 16 h + 4 a + b: a lane (h: its half of the wavefront) then has 16 neighbouring
+// columns of its row, and results leave without a way through LDS, which is full of the next tile's slices.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "fm_block_product.h"
+
+namespace fm {
+
+namespace block {
+
+namespace tiles {
+
+using mx::i32x8_t;
+
+constexpr int kTile = 256, kSlice = kBlock, kThreads = 256, kWaves = 4;
+constexpr int kBlocks = 4;  // of 32, per wavefront and axis
+constexpr int kOperandBytes = kTile * kSlice, kSlotBytes = 2 * kOperandBytes, kSlots = 2, kLdsBytes = kSlots * kSlotBytes;
+constexpr int kLoads = kOperandBytes / 1024 / kWaves;  // of a wavefront, per operand and slice
+constexpr int kResident = 256;                         // workgroups: one per CU
+// The loads run this many slices ahead; a tile has no fewer, so that they are at most one tile ahead. (What is behind a tile's last slice is zero.)
+constexpr int kMinSlices = kSlots;
+
+template <int kFirst, int kLast, typename F>
+__device__ __forceinline__ void for_each(const F &f) {
+    if constexpr (kFirst < kLast) {
+        f(std::integral_constant<int, kFirst>{});
+        for_each<kFirst + 1, kLast>(f);
+    }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(uniform_pointer(reinterpret_cast<const char *>(base))), 0,
+                                             __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), kBufferResourceFlags);
+}
+
+// 16 bytes of each lane -> LDS at `target` + kMore + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and nothing else
+// in this file uses it. Where the compiler has spilled the resource, it brings it back by vector instructions, maybe right in front of this: five wait
+// states up to the load that reads it, which are more than M0's.)
+template <int kMore>
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int target) {
+    asm volatile("s_add_i32 m0, %0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(target)), "v"(offset), "s"(resource), "n"(kMore)
+                 : "memory", "scc");
+}
+
+// The products before this are done when it is over. (The compiler counts a product's 16 passes up to the instructions that it knows to read its sums,
+// and does not look into assembly.)
+__device__ __forceinline__ void wait_for_products() { asm volatile("s_nop 15\n\ts_nop 7"); }
+
+// A block of sums, in accumulation registers up to here. (One by one: the compiler would copy a block that is handed over whole.) After `wait_for_products`.
+__device__ __forceinline__ f32x16_t settled(const f32x16_t &sums) {
+    f32x16_t values;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float value;
+        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(value) : "a"(sums[i]));
+        values[i] = value;
+    }
+    return values;
+}
+
+// Returns once all loads and stores that this wavefront has issued are done, and all that it has asked LDS for is there.
+__device__ __forceinline__ void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ u32x4_t read_lds(int address, int offset) {
+    return *(FM_LDS(u32x4_t) *)((FM_LDS(char) *)static_cast<uintptr_t>(address) + offset);
+}
+
+// D[m][n] += sum over 64 k of A[m][k] 2^sa B[n][k] 2^sb: lane l holds row l % 32 of both, 16 bytes of each of two blocks of 32 k. Of D it holds column
+// n = l % 32, rows m = 8 (i / 4) + 4 (l / 32) + i % 4.
+__device__ __forceinline__ f32x16_t multiply(const u32x4_t (&a)[2], const u32x4_t (&b)[2], uint32_t scale_a, uint32_t scale_b, f32x16_t c) {
+    const auto wide = [](const u32x4_t (&v)[2]) {
+        return i32x8_t{static_cast<int>(v[0][0]), static_cast<int>(v[0][1]), static_cast<int>(v[0][2]), static_cast<int>(v[0][3]),
+                       static_cast<int>(v[1][0]), static_cast<int>(v[1][1]), static_cast<int>(v[1][2]), static_cast<int>(v[1][3])};
+    };
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 0, 0, 0, static_cast<int>(scale_a), 0, static_cast<int>(scale_b));
+}
+
+// The same value, computed no earlier than where this stands.
+__device__ __forceinline__ uint32_t here(uint32_t value) {
+    asm volatile("" : "+s"(value));
+    return value;
+}
+
+// Where a tile lies. Wave-uniform.
+struct Tile {
+    int expert, tile_n, row0, rows_valid;
+    int first_slice, slices;  // of the reduction
+};
+
+// Which tile: by rows as `locate_tile`, by the reduction expert after expert; with the experts' ranges in registers, two experts per lane.
+constexpr int kMaxInRegisters = 128;
+template <bool kByInner>
+struct Places {
+    int begin[2], end[2];  // rows, or slices of the reduction
+    int count[2], last[2]; // by rows: row tiles, row tiles up to and with this expert's
+    int before[3];         // row tiles in front of each 64 experts, and of all
+
+    // (Without a map all of them.)
+    static __device__ __forceinline__ void range_of_expert(const GemmArgs &args, int expert, int64_t &first, int64_t &past) {
+        first = 0, past = args.rows;
+        if (args.expert_ends != nullptr) rows_of_expert(args, expert, first, past);
+    }
+    // The expert's part of the reduction, in whole slices: it begins at one.
+    static __device__ __forceinline__ void slices_of_expert(const GemmArgs &args, int expert, int &first, int &past) {
+        int64_t from, to;
+        range_of_expert(args, expert, from, to);
+        from = max(from, static_cast<int64_t>(0));
+        first = static_cast<int>(from / kSlice);
+        past = to > from ? static_cast<int>((to + kSlice - 1) / kSlice) : first;
+    }
+    __device__ __forceinline__ void load(const GemmArgs &args, int lane) {
+        before[0] = 0;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const int e = part * 64 + lane;
+            begin[part] = end[part] = count[part] = last[part] = 0;
+            if constexpr (kByInner) {
+                if (e < args.num_experts) slices_of_expert(args, e, begin[part], end[part]);
+            } else {
+                int64_t first = 0, past = 0;
+                if (e < args.num_experts) range_of_expert(args, e, first, past);
+                count[part] = first >= 0 && past > first ? static_cast<int>((past - first + kTile - 1) / kTile) : 0;
+                begin[part] = static_cast<int>(first), end[part] = static_cast<int>(past);
+                int sum = count[part];
+#pragma unroll
+                for (int offset = 1; offset < 64; offset <<= 1) {
+                    const int other = __shfl_up(sum, offset, 64);
+                    if (lane >= offset) sum += other;
+                }
+                last[part] = sum + before[part];
+                before[part + 1] = __builtin_amdgcn_readlane(last[part], 63);
+            }
+        }
+    }
+    __device__ __forceinline__ bool locate(const GemmArgs &args, int logical, int slices, Tile &tile) const {
+        if constexpr (kByInner) {
+            const int per_expert = args.tiles_m * args.tiles_n, expert = logical / per_expert;
+            if (expert >= args.num_experts) return false;
+            int row_tile;
+            place_in_expert(logical - expert * per_expert, args.tiles_m, args.tiles_n, row_tile, tile.tile_n);
+            int first, past;
+            if (args.num_experts > kMaxInRegisters) {
+                slices_of_expert(args, expert, first, past);
+                first = __builtin_amdgcn_readfirstlane(first), past = __builtin_amdgcn_readfirstlane(past);
+            } else {
+                const bool part = expert >= 64;
+                first = __builtin_amdgcn_readlane(part ? begin[1] : begin[0], expert & 63), past = __builtin_amdgcn_readlane(part ? end[1] : end[0], expert & 63);
+            }
+            tile.expert = expert, tile.row0 = row_tile * kTile;
+            tile.rows_valid = min(kTile, static_cast<int>(args.sparse_size) - tile.row0);
+            tile.first_slice = first, tile.slices = past - first;
+            return true;
+        }
+        tile.first_slice = 0, tile.slices = slices;
+        if (args.num_experts > kMaxInRegisters) {
+            // (Without halves in the last round.) The same in all lanes, which the compiler cannot know.
+            RowTile found{};
+            const bool exists = locate_tile<kTile>(args, logical, found);
+            tile.expert = __builtin_amdgcn_readfirstlane(found.expert), tile.tile_n = __builtin_amdgcn_readfirstlane(found.tile_n);
+            tile.rows_valid = __builtin_amdgcn_readfirstlane(found.rows_valid);
+            tile.row0 = __builtin_amdgcn_readfirstlane(static_cast<int>(found.row0));  // rows are counted in 31 bits
+            return __builtin_amdgcn_readfirstlane(static_cast<int>(exists)) != 0;
+        }
+        // Where half of the workgroups or fewer have a tile in the last round, they have the halves of one each.
+        const int total = before[2] * args.tiles_n, last_round = total & ~(kResident - 1);
+        const bool halved = total - last_round <= kResident / 2 && logical >= last_round;
+        const bool second = halved && (logical & 1);
+        if (halved) logical = last_round + (logical - last_round) / 2;
+        if (logical >= total) return false;
+        const int part = logical >= before[1] * args.tiles_n;
+        const int lasts = part ? last[1] : last[0], counts = part ? count[1] : count[0];
+        const uint64_t owners = __ballot(lasts * args.tiles_n > logical);
+        const int owner = __ffsll(static_cast<unsigned long long>(owners)) - 1;
+        const int owner_count = __builtin_amdgcn_readlane(counts, owner), owner_last = __builtin_amdgcn_readlane(lasts, owner);
+        const int first = __builtin_amdgcn_readlane(part ? begin[1] : begin[0], owner), past = __builtin_amdgcn_readlane(part ? end[1] : end[0], owner);
+        int row_tile;
+        place_in_expert(logical - (owner_last - owner_count) * args.tiles_n, owner_count, args.tiles_n, row_tile, tile.tile_n);
+        tile.expert = part * 64 + owner;
+        tile.row0 = first + row_tile * kTile + (second ? kTile / 2 : 0);
+        tile.rows_valid = min(halved ? kTile / 2 : kTile, past - tile.row0);
+        return tile.rows_valid > 0;  // (a workgroup whose second half is empty has nothing after it)
+    }
+};
+
+template <bool kByInner, typename Result>
+__global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, GemmArgs placement) {
+    extern __shared__ __attribute__((aligned(1024))) char lds_generic[];
+    const int lds = static_cast<int>(reinterpret_cast<uintptr_t>((FM_LDS(char) *)lds_generic));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int wave_n = wave & 1, wave_m = wave >> 1;
+    const int inner_slices = static_cast<int>(args.inner / kSlice), columns = static_cast<int>(args.columns);
+
+    // The 32 workgroups of an XCD take consecutive tiles.
+    int logical = (blockIdx.x % 8) * (kResident / 8) + blockIdx.x / 8;
+    Places<kByInner> places;
+    places.load(placement, lane);
+    Tile tile, upcoming;
+    if (!places.locate(placement, logical, inner_slices, upcoming)) return;
+
+    // ---- loading: the slices of the workgroup's tiles one after the other, the last tile's followed by zeros -----------
+    // `upcoming` is the tile that is loaded. Of every 16 rows a wavefront's load j and load j + 2 have the same swizzle.
+    const uint32_t x_stride = static_cast<uint32_t>(args.x_stride), weight_stride = static_cast<uint32_t>(args.weight_stride);
+    uint32_t x_offset[2], weight_offset[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int row = wave * kLoads * 8 + j * 8 + (lane >> 3), unit = (lane & 7) ^ ((row >> 1) & 7);
+        x_offset[j] = static_cast<uint32_t>(row) * x_stride + unit * 16;
+        // LDS row 32 c + 8 a + 4 h + b is row 32 c + 16 h + 4 a + b.
+        const int weight_row = wave * kLoads * 8 + (lane >> 5) * 16 + (lane >> 3 & 3);
+        weight_offset[j] = static_cast<uint32_t>(weight_row) * weight_stride + unit * 16;
+    }
+    const uint8_t *x_from = nullptr, *weight_from = nullptr, *x_scales_from = nullptr, *weight_scales_from = nullptr;
+    uint32_t x_bytes = 0, weight_bytes = 0, x_rows = 0, weight_rows = 0;  // ranges: of a slice, and of its scales; empty behind the tile's last slice
+    int load_slice = 0, load_target = lds;
+    bool more = true;
+    const auto slices_of = [](const Tile &of) { return max(of.slices, kMinSlices); };
+    const auto begin_loads = [&]() {
+        const int64_t column0 = static_cast<int64_t>(upcoming.tile_n) * kTile, weight_row = (kByInner ? 0 : static_cast<int64_t>(upcoming.expert) * columns) + column0;
+        const int64_t first = upcoming.first_slice;
+        x_from = args.x + upcoming.row0 * args.x_stride + first * kSlice;
+        weight_from = args.weight + weight_row * args.weight_stride + first * kSlice;
+        x_scales_from = args.x_scales + first * args.x_scale_stride + upcoming.row0;
+        weight_scales_from = args.weight_scales + first * args.weight_scale_stride + weight_row;
+        const bool any = more && upcoming.slices > 0;
+        x_rows = any ? upcoming.rows_valid : 0;
+        weight_rows = any ? min(kTile, columns - static_cast<int>(column0)) : 0;
+        x_bytes = any ? (x_rows - 1) * x_stride + kSlice : 0;
+        weight_bytes = any ? (weight_rows - 1) * weight_stride + kSlice : 0;
+        load_slice = 0;
+    };
+    const auto advance = [&]() {
+        ++load_slice;
+        const bool any = load_slice < upcoming.slices;
+        x_from += kSlice, weight_from += kSlice, x_scales_from += args.x_scale_stride, weight_scales_from += args.weight_scale_stride;
+        x_bytes = any ? x_bytes : 0, weight_bytes = any ? weight_bytes : 0, x_rows = any ? x_rows : 0, weight_rows = any ? weight_rows : 0;
+        load_target = load_target == lds ? lds + kSlotBytes : lds;
+    };
+    const auto load = [&](auto constant) {
+        constexpr int item = decltype(constant)::value, j = item % kLoads;
+        if constexpr (item < kLoads)
+            load_to_lds<kOperandBytes + j * 1024>(buffer_of(weight_from, weight_bytes), weight_offset[j % 2] + (j / 4 * 32 + j % 4 * 4) * here(weight_stride),
+                                                  load_target + wave * (kLoads * 1024));
+        else
+            load_to_lds<j * 1024>(buffer_of(x_from, x_bytes), x_offset[j % 2] + j / 2 * 16 * here(x_stride), load_target + wave * (kLoads * 1024));
+    };
+    // Scales: of the slice that is multiplied, of the next one, and of the one after, on their way.
+    uint32_t scales[2 * kBlocks], next_scales[2 * kBlocks], coming_scales[2 * kBlocks];
+    const int weight_scale_lane = wave_n * 128 + (lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3);
+    // (Rows of a tile of up to 128 are shared by both halves of the workgroup.)
+    const auto blocks_of = [&](const Tile &of) { return of.rows_valid <= kTile / 2 ? kBlocks / 2 : kBlocks; };
+    const auto load_scale = [&](auto constant) {
+        constexpr int item = decltype(constant)::value, at = item % kBlocks;
+        if constexpr (item < kBlocks)
+            coming_scales[item] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(weight_scales_from, weight_rows), weight_scale_lane + at * 32, 0, 0);
+        else
+            coming_scales[item] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(x_scales_from, x_rows), wave_m * blocks_of(upcoming) * 32 + (lane & 31) + at * 32, 0, 0);
+    };
+    constexpr int kItems = 2 * kLoads, kScales = 2 * kBlocks;
+
+    // ---- multiplying ---------------------------------------------------------------------------------------------------
+    u32x4_t weight_part[2][kBlocks][2], x_part[2][kBlocks][2];
+    int address[2][2];  // of a lane in a row block, by step and part
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) address[i][p] = (lane & 31) * kSlice + ((4 * i + 2 * p + half) ^ ((lane >> 1) & 7)) * 16;
+    int slot = lds, first_row = 0;  // of the slice that is read, and of the wavefront in the tile that it is of
+    constexpr int kReads = 4 * kBlocks;
+    constexpr std::integral_constant<int, 0> kFirst{};
+    constexpr std::integral_constant<int, 1> kSecond{};
+    // Where a step's reads start, and by number the reads: the fragments of the wavefront's weight rows, then of its rows.
+    int weight_from_lds[2], x_from_lds[2];
+    const auto begin_reads = [&](auto step_constant) {
+        constexpr int i = decltype(step_constant)::value;
+        const int weights_at = static_cast<int>(here(slot + wave_n * 128 * kSlice)), rows_at = static_cast<int>(here(slot + first_row * kSlice));
+#pragma unroll
+        for (int p = 0; p < 2; ++p) weight_from_lds[p] = address[i][p] + weights_at, x_from_lds[p] = address[i][p] + rows_at;
+    };
+    const auto read = [&](auto constant, auto step_constant) {
+        constexpr int item = decltype(constant)::value, i = decltype(step_constant)::value, p = item % 2, block = item / 2 % kBlocks;
+        if constexpr (item < 2 * kBlocks) weight_part[i][block][p] = read_lds(weight_from_lds[p], kOperandBytes + block * 32 * kSlice);
+        else x_part[i][block][p] = read_lds(x_from_lds[p], block * 32 * kSlice);
+    };
+
+    begin_loads();
+    for_each<0, kItems>(load);
+    for_each<0, kScales>(load_scale);
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) asm volatile("" : "+v"(coming_scales[i]));
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) scales[i] = coming_scales[i];
+    advance();
+    for_each<0, kItems>(load);
+    for_each<0, kScales>(load_scale);
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) asm volatile("" : "+v"(coming_scales[i]));
+    advance();
+    wait_for_memory();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    first_row = wave_m * blocks_of(upcoming) * 32;
+    begin_reads(kFirst);
+    for_each<0, kReads>([&](auto item) { read(item, kFirst); });
+
+    f32x16_t acc[kBlocks][kBlocks];
+    while (true) {
+        tile = upcoming;
+        const int slices = slices_of(tile), blocks = blocks_of(tile);
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
+        const auto multiply_tile = [&](auto blocks_constant) {
+            constexpr int kRows = decltype(blocks_constant)::value, kProducts = kBlocks * kRows;
+            const auto product = [&](auto constant, auto step_constant) {
+                // Neighbouring products share an operand.
+                constexpr int j = decltype(constant)::value, i = decltype(step_constant)::value, n = j / kRows, m = n % 2 ? kRows - 1 - j % kRows : j % kRows;
+                acc[n][m] = multiply(weight_part[i][n], x_part[i][m], scales[n], scales[kBlocks + m], acc[n][m]);
+            };
+#pragma unroll 1
+            for (int s = 0; s < slices; ++s) {
+                if (load_slice == slices_of(upcoming)) {
+                    logical += kResident;
+                    more = more && places.locate(placement, logical, inner_slices, upcoming);
+                    begin_loads();
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // First step; beside it the reads of the second.
+                for_each<0, kProducts>([&](auto j) {
+                    product(j, kFirst);
+                    if constexpr (j == 0) begin_reads(kSecond);
+                    constexpr int kBusy = kProducts - 2;
+                    if constexpr (j < kBusy) for_each<j * kReads / kBusy, (j + 1) * kReads / kBusy>([&](auto item) { read(item, kSecond); });
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                // Second step. Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + 2 takes its slot.
+                product(kFirst, kSecond);
+                __builtin_amdgcn_sched_barrier(0);
+                wait_for_memory();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < kScales; ++i) asm volatile("" : "+v"(coming_scales[i]));
+#pragma unroll
+                for (int i = 0; i < kScales; ++i) next_scales[i] = coming_scales[i];
+                slot = slot == lds ? lds + kSlotBytes : lds;
+                if (s + 1 == slices) first_row = wave_m * blocks_of(upcoming) * 32;
+                __builtin_amdgcn_sched_barrier(0);
+                for_each<1, kProducts>([&](auto j) {
+                    product(j, kSecond);
+                    if constexpr (j == 1) begin_reads(kFirst);
+                    constexpr int kBusy = kProducts - 2;
+                    if constexpr (j <= kBusy) {
+                        for_each<(j - 1) * kReads / kBusy, j * kReads / kBusy>([&](auto item) { read(item, kFirst); });
+                        for_each<(j - 1) * kItems / kBusy, j * kItems / kBusy>(load);
+                        for_each<(j - 1) * kScales / kBusy, j * kScales / kBusy>(load_scale);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                // The compiler would move products past the branches above, away from what they are to overlap.
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+                    for (int m = 0; m < kRows; ++m) asm volatile("" : "+a"(acc[n][m]));
+                advance();
+#pragma unroll
+                for (int i = 0; i < kScales; ++i) scales[i] = next_scales[i];
+            }
+        };
+        if (blocks == kBlocks) multiply_tile(std::integral_constant<int, kBlocks>{});
+        else multiply_tile(std::integral_constant<int, kBlocks / 2>{});
+        const bool last_tile = !more;
+        __builtin_amdgcn_sched_barrier(0);
+        wait_for_products();
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- the tile's results: of block (n, m) a lane has columns 16 half .. + 15 of one row ---------------------------
+        const int row_start = wave_m * blocks * 32, col0 = tile.tile_n * kTile, out_lane = opaque(lane);
+        const int64_t out_row = (kByInner ? tile.expert * args.rows : 0) + tile.row0;
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) {
+            const int row = row_start + m * 32 + (out_lane & 31);
+            if (m >= blocks || row >= tile.rows_valid) continue;
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) {
+                __builtin_amdgcn_sched_barrier(0);
+                f32x16_t values = settled(acc[n][m]);
+                const int column = col0 + wave_n * 128 + n * 32 + 16 * (out_lane >> 5);
+                Result *out = static_cast<Result *>(args.out) + (out_row + row) * args.out_stride + column;
+                constexpr int N = Vec16<Result>::N;
+                if (args.out_vectors && column + 15 < columns) {
+                    if (kByInner && args.accumulate) {
+#pragma unroll
+                        for (int part = 0; part < 16 / N; ++part) {
+                            const Vec16<Result> vector = load16(out + part * N);
+#pragma unroll
+                            for (int c = 0; c < N; ++c) values[part * N + c] += to_float(vector.v[c]);
+                        }
+                    }
+#pragma unroll
+                    for (int part = 0; part < 16 / N; ++part) {
+                        Vec16<Result> vector;
+#pragma unroll
+                        for (int c = 0; c < N; ++c) vector.v[c] = from_float<Result>(values[part * N + c]);
+                        store16(out + part * N, vector);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        if (column + c < columns) out[c] = from_float<Result>(values[c] + (kByInner && args.accumulate ? to_float(out[c]) : 0.f));
+                }
+            }
+        }
+        if (last_tile) break;
+    }
+    wait_for_memory();  // zeros behind the last tile
+}
+
+template <bool kByInner, typename Result>
+static int launch(const ProductArgs &args, hipStream_t stream) {
+    const auto kernel = tile_kernel<kByInner, Result>;
+    static std::atomic<uint64_t> configured{0};
+    if (int status = allow_lds(reinterpret_cast<const void *>(kernel), kLdsBytes, configured)) return status;
+    GemmArgs placement{};
+    placement.expert_ends = args.expert_ends, placement.expert_pad_begins = args.expert_pad_begins, placement.index_dtype = args.index_dtype;
+    placement.rows = kByInner ? args.inner : args.rows, placement.sparse_size = args.rows, placement.num_experts = static_cast<int>(args.experts);
+    placement.tiles_m = static_cast<int>((args.rows + kTile - 1) / kTile);
+    placement.tiles_n = static_cast<int>((args.columns + kTile - 1) / kTile);
+    kernel<<<kResident, kThreads, kLdsBytes, stream>>>(args, placement);
+    return FM_OK;
+}
+
+template <bool kByInner>
+static int launch(const ProductArgs &args, hipStream_t stream) {
+    switch (args.out_dtype) {
+        case FM_DTYPE_F32: return launch<kByInner, float>(args, stream);
+        case FM_DTYPE_BF16: return launch<kByInner, bf16_t>(args, stream);
+        default: return launch<kByInner, f16_t>(args, stream);
+    }
+}
+
+}  // namespace tiles
+
+bool tile_product_takes(const ProductArgs &args) {
+    // Offsets from a tile's first row are counted in 32 bits; rows and tiles in 31.
+    const int64_t row_tiles = (args.rows / tiles::kTile + 1) * (args.by_inner ? args.experts : 1) + args.experts;
+    return std::max(args.x_stride, args.weight_stride) * tiles::kTile < (int64_t(1) << 31) &&
+           row_tiles * ((args.columns + tiles::kTile - 1) / tiles::kTile) < (int64_t(1) << 30);
+}
+
+int tile_product(const ProductArgs &args, hipStream_t stream) {
+    return args.by_inner ? tiles::launch<true>(args, stream) : tiles::launch<false>(args, stream);
+}
+
+}  // namespace block
+
+}  // namespace fm

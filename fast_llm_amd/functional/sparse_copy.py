@@ -32,6 +32,8 @@ class SparseMap:
     num_rows_unpadded: int
     num_experts: int
     num_experts_per_token: int
+    # Every expert's rows are padded to a multiple of this (not in the reference's class, whose padding it is always).
+    pad_to_multiple: int = MAX_DROPLESS_BLOCK_SIZE_ROW
 
 
 def get_sparse_map(
@@ -94,7 +96,7 @@ def get_sparse_map(
             workspace_size,
         )
         return _finish_sparse_map(
-            sparse_rows, expert_ends, expert_pad_begins, num_experts, dynamic_shape, max_rows
+            sparse_rows, expert_ends, expert_pad_begins, num_experts, dynamic_shape, max_rows, pad_to_multiple
         )
     workspace_size = library.fm_sparse_map_workspace_size(num_rows_dense, num_experts_per_token, num_experts)
     workspace = torch.empty(workspace_size, dtype=torch.uint8, device=device)
@@ -113,7 +115,7 @@ def get_sparse_map(
         _lib.ptr(workspace),
         workspace_size,
     )
-    return _finish_sparse_map(sparse_rows, expert_ends, expert_pad_begins, num_experts, dynamic_shape, max_rows)
+    return _finish_sparse_map(sparse_rows, expert_ends, expert_pad_begins, num_experts, dynamic_shape, max_rows, pad_to_multiple)
 
 
 def _finish_sparse_map(
@@ -123,6 +125,7 @@ def _finish_sparse_map(
     num_experts: int,
     dynamic_shape: bool,
     max_rows: int,
+    pad_to_multiple: int,
 ) -> SparseMap:
     num_rows_dense, num_experts_per_token = sparse_rows.shape
     return SparseMap(
@@ -134,6 +137,7 @@ def _finish_sparse_map(
         num_rows_unpadded=num_rows_dense * num_experts_per_token,
         num_experts=num_experts,
         num_experts_per_token=num_experts_per_token,
+        pad_to_multiple=pad_to_multiple,
     )
 
 

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FM_VERSION 13
+#define FM_VERSION 14
 
 /* Element type of activations, weights and outputs. */
 enum fm_dtype { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1, FM_DTYPE_F16 = 2 };
@@ -526,6 +526,64 @@ size_t fm_rms_norm_backward_workspace_size(int64_t rows, int64_t columns);
 int fm_rms_norm_backward(const void *grad_normalized, const void *grad_stream, const void *stream_in, const void *weight, void *grad_input,
                          void *grad_weight, int64_t rows, int64_t columns, double eps, int dtype, int weight_dtype, void *workspace,
                          size_t workspace_size, void *stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Values of 8 bits with a scale for each block of 128: 128 neighbours along a row share the scale 2^(byte - 127) and are kept in e4m3. A tensor of
+ * [rows, columns] is two arrays of bytes: values, row-major, `columns` bytes a row where `columns` is rounded up to a multiple of 128 (zeros behind the last
+ * column); and scales, the blocks of 128 columns one after the other, of each a byte per row: `scale_stride` bytes from one block's to the next one's, at least
+ * the rows rounded up to a multiple of 16. Strides are in bytes and multiples of 16, values and scales are 16-byte aligned. Results are contiguous.
+ *   scale = the smallest power of two, from 2^-127 on, with (largest magnitude) <= 448 * scale;   element = value / scale, rounded to nearest even.
+ *   A block with an infinity or NaN: scale byte 255 (all of it is NaN), elements 0.
+ * `expert_ends` and `expert_pad_begins` [num_experts] (of `index_dtype`, as in fm_sparse_map; null, both: all rows count) say which rows tokens have;
+ * the experts' rows begin at multiples of 128 here (whatever they hold, nothing out of range is read or written). The rows that no token has are not
+ * looked at and count as zeros: the padding of an expert and what is behind the last one. At most 1024 experts.
+ * --------------------------------------------------------------------------------------------------------- */
+/* `groups` matrices of `rows` x `columns` one after the other, rows `input_row_stride` elements apart, quantised along the rows ([groups * rows, columns]),
+ * along the columns with the result transposed ([groups * columns, rows], padded to a multiple of 128 with zeros), or both: what is null is not computed. With
+ * a map there is one group, and the transposed form. */
+int fm_block_quantize(const void *input, void *values, void *scales, void *transposed_values, void *transposed_scales, const void *expert_ends,
+                      const void *expert_pad_begins, int64_t groups, int64_t rows, int64_t columns, int64_t num_experts, int64_t input_row_stride,
+                      int64_t scale_stride, int64_t transposed_scale_stride, int dtype, int index_dtype, void *stream);
+/* The transposed form of rows that are of 8 bits already: exact but for elements that become subnormal under the scale of their new block. */
+int fm_block_transpose(const void *values, const void *scales, void *transposed_values, void *transposed_scales, const void *expert_ends,
+                       const void *expert_pad_begins, int64_t groups, int64_t rows, int64_t columns, int64_t num_experts, int64_t value_stride,
+                       int64_t scale_stride, int64_t transposed_scale_stride, int index_dtype, void *stream);
+/* Back, into contiguous rows of `dtype`: element * scale, rounded once. */
+int fm_block_dequantize(const void *values, const void *scales, void *output, int64_t rows, int64_t columns, int64_t value_stride, int64_t scale_stride,
+                        int dtype, void *stream);
+/* fm_copy_dense_to_sparse for such rows. */
+int fm_block_copy_dense_to_sparse(const void *values, const void *scales, const void *sparse_rows, void *out_values, void *out_scales,
+                                  int64_t num_rows_dense, int64_t columns, int64_t num_experts_per_token, int64_t num_rows_sparse, int64_t value_stride,
+                                  int64_t scale_stride, int64_t out_scale_stride, int index_dtype, void *stream);
+
+/* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs has `columns` rows of `inner` per expert. Both layers of an expert MLP and
+ * both input gradients are such products. Sums in fp32 (of 64 products at a time, as fm_mx_sparse_matmul says), one rounding. Only the rows that tokens have are
+ * written, those of lhs that none has are not looked at, and experts may begin anywhere. `out_stride` in elements. Without a map there is one expert. */
+int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
+                           const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
+                           int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int out_dtype, int index_dtype,
+                           void *stream);
+/* The weights' gradients: out[e rows + i, j] (=, or += with `accumulate`) sum over the rows k of expert e of lhs[i, k] * rhs[j, k], lhs [rows, inner] and rhs
+ * [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens have zeros. */
+int fm_block_input_row_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
+                                     const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
+                                     int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int accumulate, int out_dtype,
+                                     int index_dtype, void *stream);
+
+/* The MLP's activation of `input` [rows, columns] (gated: [rows, 2 columns], gates and then ups, `columns` a multiple of 128; FM_ERR_UNSUPPORTED
+ * otherwise): `output` [rows, columns] in 8 bits, of the fp32 result, and `checkpoint`, the input in 8 bits. */
+int fm_block_activation_forward(const void *input, void *output, void *output_scales, void *checkpoint, void *checkpoint_scales, const void *expert_ends,
+                                const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t num_experts, int64_t input_stride,
+                                int64_t output_scale_stride, int64_t checkpoint_scale_stride, int gated, int activation, int dtype, int index_dtype,
+                                void *stream);
+/* Its backward from the checkpoint: the input's gradient for `grad_output` [rows, columns] of `dtype` (rows `grad_output_stride` elements apart) along its rows and
+ * transposed, and the transposed form of the activation of what the checkpoint holds. */
+int fm_block_activation_backward(const void *grad_output, const void *checkpoint, const void *checkpoint_scales, void *grad, void *grad_scales,
+                                 void *grad_transposed, void *grad_transposed_scales, void *output_transposed, void *output_transposed_scales,
+                                 const void *expert_ends, const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t num_experts,
+                                 int64_t grad_output_stride, int64_t checkpoint_stride, int64_t checkpoint_scale_stride, int64_t grad_scale_stride,
+                                 int64_t grad_transposed_scale_stride, int64_t output_transposed_scale_stride, int gated, int activation, int dtype,
+                                 int index_dtype, void *stream);
 
 #ifdef __cplusplus
 }
