@@ -10,7 +10,7 @@ namespace {
 int check_sizes(const char *name, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int out_dtype) {
     FM_REQUIRE(valid_dtype(out_dtype), "%s: bad dtype %d", name, out_dtype);
     FM_REQUIRE(num_experts > 0 && num_experts <= 1024, "%s: num_experts = %lld is not in 1 .. 1024", name, static_cast<long long>(num_experts));
-    FM_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && columns > 0 && columns <= (int64_t(1) << 28) && inner >= 0 && inner <= block::kMaxColumns &&
+    FM_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && columns > 0 && columns <= (int64_t(1) << 28) && inner > 0 && inner <= block::kMaxColumns &&
                    num_experts * std::max(rows, columns) < (int64_t(1) << 40), "%s: bad sizes", name);
     return FM_OK;
 }
@@ -30,7 +30,6 @@ extern "C" int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, c
                                       void *stream) {
     const char *name = "fm_block_sparse_matmul";
     if (int status = check_sizes(name, rows, columns, inner, num_experts, out_dtype)) return status;
-    FM_REQUIRE(inner > 0, "%s: nothing to sum over", name);
     block::RowMap map;
     if (int status = block::check_map(name, map, expert_ends, expert_pad_begins, num_experts, index_dtype)) return status;
     FM_REQUIRE(expert_ends != nullptr || num_experts == 1, "%s: several experts and no map", name);
@@ -62,10 +61,8 @@ extern "C" int fm_block_input_row_sparse_matmul(const void *lhs, const void *lhs
     FM_REQUIRE(expert_ends != nullptr || num_experts == 1, "%s: several experts and no map", name);
     if (rows == 0) return FM_OK;
     const int64_t padded = block::padded_columns(inner);
-    if (inner > 0) {
-        if (int status = block::check_tensor(name, "lhs", lhs, lhs_scales, rows, padded, lhs_stride, lhs_scale_stride)) return status;
-        if (int status = block::check_tensor(name, "rhs", rhs, rhs_scales, columns, padded, rhs_stride, rhs_scale_stride)) return status;
-    }
+    if (int status = block::check_tensor(name, "lhs", lhs, lhs_scales, rows, padded, lhs_stride, lhs_scale_stride)) return status;
+    if (int status = block::check_tensor(name, "rhs", rhs, rhs_scales, columns, padded, rhs_stride, rhs_scale_stride)) return status;
     if (int status = check_result(name, out, columns, out_stride, out_dtype)) return status;
     block::ProductArgs args{};
     args.x = static_cast<const uint8_t *>(lhs), args.x_scales = static_cast<const uint8_t *>(lhs_scales);

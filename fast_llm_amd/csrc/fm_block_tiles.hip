@@ -5,8 +5,8 @@
 // v_mfma_scale_f32_32x32x64_f8f6f4, 256 accumulation registers; D's rows are weight rows, so that a lane has neighbouring columns of one row). The reduction
 // passes in slices of 128, a block of the format, through two LDS slots of 64 KB. A slice's bytes go straight from memory into LDS; they are asked for as soon
 // as the slice two before them has been read, half a slice before it has been multiplied, and on into the next tile. The fragments of a step of 64 are
-// read while the step before is multiplied: each product has one or two reads or loads in its shadow. The scales, a byte for each row and slice,
-// come as bytes to the registers of the lanes that hold the rows: 32 neighbours at a time, since the scales of a slice are next to each other.
+// read while the step before is multiplied: each product has one or two reads or loads in its shadow. The scales of a
+// slice, a byte for each row, are next to each other: a wavefront brings those of its rows with one load, which pass LDS to the lanes that hold the rows.
 //
 // A row's slice is 128 bytes, in LDS XOR-swizzled in units of 16 bytes so that 16 lanes that read the same unit of neighbouring rows hit all 64
 // banks. Of every 32 weight rows, LDS row 8 a + 4 h + b holds row 16 h + 4 a + b: a lane (h: its half of the wavefront) then has 16 neighbouring
@@ -27,11 +27,15 @@ using mx::i32x8_t;
 
 constexpr int kTile = 256, kSlice = kBlock, kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 4;  // of 32, per wavefront and axis
-constexpr int kOperandBytes = kTile * kSlice, kSlotBytes = 2 * kOperandBytes, kSlots = 2, kLdsBytes = kSlots * kSlotBytes;
+constexpr int kOperandBytes = kTile * kSlice, kSlotBytes = 2 * kOperandBytes, kSlots = 2;
+// Scales of a slice: a load per wavefront, of the rows of one half of the tile or of its weight rows, from an address of any alignment in pieces of 16.
+constexpr int kScaleBytes = 1024, kScaleSlots = 3, kScaleSlotBytes = kWaves * kScaleBytes, kScalePieces = 128 / 16 + 1;
+constexpr int kLdsBytes = kSlots * kSlotBytes + kScaleSlots * kScaleSlotBytes;
+static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr int kLoads = kOperandBytes / 1024 / kWaves;  // of a wavefront, per operand and slice
 constexpr int kResident = 256;                         // workgroups: one per CU
-// The loads run this many slices ahead; a tile has no fewer, so that they are at most one tile ahead. (What is behind a tile's last slice is zero.)
-constexpr int kMinSlices = kSlots;
+// The loads of scales run this many slices ahead; a tile has no fewer, so that they are at most one tile ahead. (What is behind a tile's last slice is zero.)
+constexpr int kMinSlices = kSlots + 1;
 
 template <int kFirst, int kLast, typename F>
 __device__ __forceinline__ void for_each(const F &f) {
@@ -73,8 +77,11 @@ __device__ __forceinline__ f32x16_t settled(const f32x16_t &sums) {
     return values;
 }
 
-// Returns once all loads and stores that this wavefront has issued are done, and all that it has asked LDS for is there.
-__device__ __forceinline__ void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// Returns once at most `kNewest` of the loads and stores that this wavefront has issued are on their way, and all that it has asked LDS for is there.
+template <int kNewest>
+__device__ __forceinline__ void wait_for_memory() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kNewest) : "memory");
+}
 
 __device__ __forceinline__ u32x4_t read_lds(int address, int offset) {
     return *(FM_LDS(u32x4_t) *)((FM_LDS(char) *)static_cast<uintptr_t>(address) + offset);
@@ -224,31 +231,56 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         const int weight_row = wave * kLoads * 8 + (lane >> 5) * 16 + (lane >> 3 & 3);
         weight_offset[j] = static_cast<uint32_t>(weight_row) * weight_stride + unit * 16;
     }
-    const uint8_t *x_from = nullptr, *weight_from = nullptr, *x_scales_from = nullptr, *weight_scales_from = nullptr;
-    uint32_t x_bytes = 0, weight_bytes = 0, x_rows = 0, weight_rows = 0;  // ranges: of a slice, and of its scales; empty behind the tile's last slice
-    int load_slice = 0, load_target = lds;
-    bool more = true;
     const auto slices_of = [](const Tile &of) { return max(of.slices, kMinSlices); };
+    // Rows of a tile of up to 128 are shared by both halves of the workgroup.
+    const auto blocks_of = [](const Tile &of) { return of.rows_valid <= kTile / 2 ? kBlocks / 2 : kBlocks; };
+    const auto weight_row_of = [&](const Tile &of) { return (kByInner ? 0 : static_cast<int64_t>(of.expert) * columns) + of.tile_n * kTile; };
+    const auto weight_rows_of = [&](const Tile &of) { return min(kTile, columns - of.tile_n * kTile); };
+    bool more = true;
+    const uint8_t *x_from = nullptr, *weight_from = nullptr;
+    uint32_t x_bytes = 0, weight_bytes = 0;  // of a slice; none behind the tile's last one
+    int load_slice = 0, load_slices = 0, real_slices = 0, load_target = lds;
     const auto begin_loads = [&]() {
-        const int64_t column0 = static_cast<int64_t>(upcoming.tile_n) * kTile, weight_row = (kByInner ? 0 : static_cast<int64_t>(upcoming.expert) * columns) + column0;
-        const int64_t first = upcoming.first_slice;
-        x_from = args.x + upcoming.row0 * args.x_stride + first * kSlice;
-        weight_from = args.weight + weight_row * args.weight_stride + first * kSlice;
-        x_scales_from = args.x_scales + first * args.x_scale_stride + upcoming.row0;
-        weight_scales_from = args.weight_scales + first * args.weight_scale_stride + weight_row;
-        const bool any = more && upcoming.slices > 0;
-        x_rows = any ? upcoming.rows_valid : 0;
-        weight_rows = any ? min(kTile, columns - static_cast<int>(column0)) : 0;
-        x_bytes = any ? (x_rows - 1) * x_stride + kSlice : 0;
-        weight_bytes = any ? (weight_rows - 1) * weight_stride + kSlice : 0;
-        load_slice = 0;
+        const int64_t first = static_cast<int64_t>(upcoming.first_slice) * kSlice;
+        x_from = args.x + upcoming.row0 * args.x_stride + first;
+        weight_from = args.weight + weight_row_of(upcoming) * args.weight_stride + first;
+        load_slice = 0, load_slices = slices_of(upcoming), real_slices = more ? upcoming.slices : 0;
+        x_bytes = real_slices > 0 ? (upcoming.rows_valid - 1) * x_stride + kSlice : 0;
+        weight_bytes = real_slices > 0 ? (weight_rows_of(upcoming) - 1) * weight_stride + kSlice : 0;
     };
     const auto advance = [&]() {
         ++load_slice;
-        const bool any = load_slice < upcoming.slices;
-        x_from += kSlice, weight_from += kSlice, x_scales_from += args.x_scale_stride, weight_scales_from += args.weight_scale_stride;
-        x_bytes = any ? x_bytes : 0, weight_bytes = any ? weight_bytes : 0, x_rows = any ? x_rows : 0, weight_rows = any ? weight_rows : 0;
+        x_from += kSlice, weight_from += kSlice;
+        x_bytes = load_slice < real_slices ? x_bytes : 0, weight_bytes = load_slice < real_slices ? weight_bytes : 0;
         load_target = load_target == lds ? lds + kSlotBytes : lds;
+    };
+    // Scales, a slice further ahead: they come from as many places of memory as there are slices, and are the last to arrive. (As far ahead as the slice
+    // itself, 14336 -> 4096 with 16384 rows of 8 experts took 937 us for 800; as bytes for each block of 32 rows, straight to the lanes that hold
+    // them, 998.) The first two wavefronts bring those of the halves of the tile's rows, the others those of the halves of its weight rows.
+    const bool of_weights = wave >= 2;
+    const int64_t scale_stride = of_weights ? args.weight_scale_stride : args.x_scale_stride;
+    const uint32_t scale_offset = lane < kScalePieces ? lane * 16 : 0x80000000u;
+    const uint8_t *scale_from = nullptr;
+    uint32_t scale_bytes = 0;
+    const int scales_at = lds + kSlots * kSlotBytes;
+    int scale_slice = 0, scale_target = scales_at;
+    const auto first_x_row = [&](const Tile &of, int half_of_tile) { return of.row0 + half_of_tile * blocks_of(of) * 32; };
+    const auto begin_scales = [&]() {
+        const int64_t weight_row = weight_row_of(upcoming);
+        const int64_t row = of_weights ? weight_row + (wave - 2) * 128 : first_x_row(upcoming, wave);
+        const int64_t past = of_weights ? weight_row + weight_rows_of(upcoming) : upcoming.row0 + upcoming.rows_valid;
+        const int64_t from = row & ~int64_t(15);
+        scale_from = (of_weights ? args.weight_scales : args.x_scales) + static_cast<int64_t>(upcoming.first_slice) * scale_stride + from;
+        // Whole pieces: rows of scales are padded to them.
+        scale_bytes = more && upcoming.slices > 0 && past > row ? static_cast<uint32_t>((past - from + 15) & ~int64_t(15)) : 0;
+        scale_slice = 0;
+    };
+    const auto load_scales = [&]() {
+        load_to_lds<0>(buffer_of(scale_from, scale_bytes), scale_offset, scale_target + wave * kScaleBytes);
+        ++scale_slice;
+        scale_from += scale_stride;
+        scale_bytes = scale_slice < upcoming.slices ? scale_bytes : 0;
+        scale_target = scale_target == scales_at + (kScaleSlots - 1) * kScaleSlotBytes ? scales_at : scale_target + kScaleSlotBytes;
     };
     const auto load = [&](auto constant) {
         constexpr int item = decltype(constant)::value, j = item % kLoads;
@@ -258,22 +290,23 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         else
             load_to_lds<j * 1024>(buffer_of(x_from, x_bytes), x_offset[j % 2] + j / 2 * 16 * here(x_stride), load_target + wave * (kLoads * 1024));
     };
-    // Scales: of the slice that is multiplied, of the next one, and of the one after, on their way.
-    uint32_t scales[2 * kBlocks], next_scales[2 * kBlocks], coming_scales[2 * kBlocks];
-    const int weight_scale_lane = wave_n * 128 + (lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3);
-    // (Rows of a tile of up to 128 are shared by both halves of the workgroup.)
-    const auto blocks_of = [&](const Tile &of) { return of.rows_valid <= kTile / 2 ? kBlocks / 2 : kBlocks; };
-    const auto load_scale = [&](auto constant) {
-        constexpr int item = decltype(constant)::value, at = item % kBlocks;
-        if constexpr (item < kBlocks)
-            coming_scales[item] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(weight_scales_from, weight_rows), weight_scale_lane + at * 32, 0, 0);
-        else
-            coming_scales[item] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(x_scales_from, x_rows), wave_m * blocks_of(upcoming) * 32 + (lane & 31) + at * 32, 0, 0);
-    };
-    constexpr int kItems = 2 * kLoads, kScales = 2 * kBlocks;
+    constexpr int kItems = 2 * kLoads;
 
     // ---- multiplying ---------------------------------------------------------------------------------------------------
     u32x4_t weight_part[2][kBlocks][2], x_part[2][kBlocks][2];
+    uint32_t scales[2 * kBlocks], next_scales[2 * kBlocks];
+    constexpr int kScales = 2 * kBlocks;
+    int scale_slot = scales_at, x_scales_at = 0, weight_scales_at = 0;  // of the slice whose scales are read, and a lane's places in it
+    const auto begin_scale_reads = [&](const Tile &of) {
+        x_scales_at = wave_m * kScaleBytes + (first_x_row(of, wave_m) & 15) + (lane & 31);
+        // (The weight row of LDS row `lane % 32`.)
+        weight_scales_at = (2 + wave_n) * kScaleBytes + static_cast<int>((weight_row_of(of) + wave_n * 128) & 15) + (lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3);
+    };
+    const auto read_scale = [&](auto constant) {
+        constexpr int item = decltype(constant)::value, block = item % kBlocks;
+        next_scales[item] = *(FM_LDS(uint8_t) *)((FM_LDS(char) *)static_cast<uintptr_t>((item < kBlocks ? weight_scales_at : x_scales_at) + scale_slot) + block * 32);
+    };
+    const auto next_scale_slot = [&]() { scale_slot = scale_slot == scales_at + (kScaleSlots - 1) * kScaleSlotBytes ? scales_at : scale_slot + kScaleSlotBytes; };
     int address[2][2];  // of a lane in a row block, by step and part
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -297,22 +330,23 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         else x_part[i][block][p] = read_lds(x_from_lds[p], block * 32 * kSlice);
     };
 
+    begin_scales();
     begin_loads();
-    for_each<0, kItems>(load);
-    for_each<0, kScales>(load_scale);
-#pragma unroll
-    for (int i = 0; i < kScales; ++i) asm volatile("" : "+v"(coming_scales[i]));
-#pragma unroll
-    for (int i = 0; i < kScales; ++i) scales[i] = coming_scales[i];
-    advance();
-    for_each<0, kItems>(load);
-    for_each<0, kScales>(load_scale);
-#pragma unroll
-    for (int i = 0; i < kScales; ++i) asm volatile("" : "+v"(coming_scales[i]));
-    advance();
-    wait_for_memory();
+#pragma unroll 1
+    for (int s = 0; s < kMinSlices; ++s) {
+        load_scales();
+        if (s < kSlots) {
+            for_each<0, kItems>(load);
+            advance();
+        }
+    }
+    wait_for_memory<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    begin_scale_reads(upcoming);
+    for_each<0, kScales>(read_scale);
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) scales[i] = next_scales[i];
     first_row = wave_m * blocks_of(upcoming) * 32;
     begin_reads(kFirst);
     for_each<0, kReads>([&](auto item) { read(item, kFirst); });
@@ -336,10 +370,11 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
             };
 #pragma unroll 1
             for (int s = 0; s < slices; ++s) {
-                if (load_slice == slices_of(upcoming)) {
+                if (load_slice == load_slices) begin_loads();
+                if (scale_slice == slices_of(upcoming)) {
                     logical += kResident;
                     more = more && places.locate(placement, logical, inner_slices, upcoming);
-                    begin_loads();
+                    begin_scales();
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 // First step; beside it the reads of the second.
@@ -353,15 +388,15 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                 // Second step. Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + 2 takes its slot.
                 product(kFirst, kSecond);
                 __builtin_amdgcn_sched_barrier(0);
-                wait_for_memory();
+                wait_for_memory<1>();  // all but the scales of slice s + 3, which are asked for last
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-#pragma unroll
-                for (int i = 0; i < kScales; ++i) asm volatile("" : "+v"(coming_scales[i]));
-#pragma unroll
-                for (int i = 0; i < kScales; ++i) next_scales[i] = coming_scales[i];
                 slot = slot == lds ? lds + kSlotBytes : lds;
-                if (s + 1 == slices) first_row = wave_m * blocks_of(upcoming) * 32;
+                next_scale_slot();
+                if (s + 1 == slices) {
+                    first_row = wave_m * blocks_of(upcoming) * 32;
+                    begin_scale_reads(upcoming);
+                }
                 __builtin_amdgcn_sched_barrier(0);
                 for_each<1, kProducts>([&](auto j) {
                     product(j, kSecond);
@@ -370,7 +405,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                     if constexpr (j <= kBusy) {
                         for_each<(j - 1) * kReads / kBusy, j * kReads / kBusy>([&](auto item) { read(item, kFirst); });
                         for_each<(j - 1) * kItems / kBusy, j * kItems / kBusy>(load);
-                        for_each<(j - 1) * kScales / kBusy, j * kScales / kBusy>(load_scale);
+                        for_each<(j - 1) * kScales / kBusy, j * kScales / kBusy>(read_scale);
+                        if constexpr (j == kBusy) load_scales();  // the last of the slice's loads
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 });
@@ -430,7 +466,7 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         }
         if (last_tile) break;
     }
-    wait_for_memory();  // zeros behind the last tile
+    wait_for_memory<0>();  // zeros behind the last tile
 }
 
 template <bool kByInner, typename Result>

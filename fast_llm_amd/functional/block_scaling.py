@@ -283,14 +283,18 @@ def block_input_row_sparse_matmul(
     refuse_traced()
     Assert.eq(lhs.columns, rhs.columns)
     device = _lib.require_device(lhs.values, lhs.scales, rhs.values, rhs.scales, out)
-    pointers, experts, index_tag = _map_pointers(sparse_map, lhs.columns, device)
+    # (A tensor has a column: without rows that one counts for nothing.)
+    empty = sparse_map is not None and sparse_map.num_rows == 0 and lhs.columns == 1
+    pointers, experts, index_tag = _map_pointers(sparse_map, 0 if empty else lhs.columns, device)
     shape = (experts * lhs.rows, rhs.rows)
     if out is None:
         assert not accumulate
         out = torch.empty(shape, dtype=dtype, device=device)
     Assert.eq(tuple(out.shape), shape)
     assert out.stride(1) == 1 or shape[1] == 1
-    if rhs.rows == 0:
+    if empty and not accumulate:
+        out.zero_()
+    if rhs.rows == 0 or empty:
         return out
     _lib.call(
         "fm_block_input_row_sparse_matmul", device, *_pointers(lhs), *_pointers(rhs), out.data_ptr(), *pointers, lhs.rows, rhs.rows,
