@@ -39,11 +39,12 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return byte == 255u ? __builtin_nanf("") : byte == 0u ? __builtin_bit_cast(float, 0x00400000u) : __builtin_bit_cast(float, byte << 23);
 }
 
-// Four elements. Of a block that is not finite, `inverse` 0: zeros. (Nothing is over 448.)
-__device__ __forceinline__ uint32_t pack_four(float a, float b, float c, float d, float inverse) {
+// Four elements of a block that is finite (nothing is over 448), or of any: of one that is not, `inverse` 0, zeros.
+__device__ __forceinline__ uint32_t pack_finite(float a, float b, float c, float d, float inverse) {
     const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a * inverse, b * inverse, 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c * inverse, d * inverse, low, true)) & (inverse == 0.f ? 0u : ~0u);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c * inverse, d * inverse, low, true));
 }
+__device__ __forceinline__ uint32_t pack_four(float a, float b, float c, float d, float inverse) { return pack_finite(a, b, c, d, inverse) & (inverse == 0.f ? 0u : ~0u); }
 __device__ __forceinline__ void unpack_four(uint32_t word, float scale, float (&values)[4]) {
     values[0] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 0) * scale, values[1] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 1) * scale;
     values[2] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 2) * scale, values[3] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 3) * scale;
@@ -92,6 +93,20 @@ __device__ __forceinline__ void load_values(const T *pointer, int64_t left, floa
 #pragma unroll
         for (int i = 0; i < kCount; ++i) values[i] = i < left ? to_float(pointer[i]) : 0.f;
     }
+}
+
+// The same four, as they lie in memory.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) RawFour {
+    T v[4];
+};
+template <typename T>
+__device__ __forceinline__ RawFour<T> load_raw(const T *pointer, int64_t left) {
+    if (left >= 4) return *reinterpret_cast<const RawFour<T> *>(pointer);
+    RawFour<T> four;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) four.v[i] = i < left ? pointer[i] : from_float<T>(0.f);
+    return four;
 }
 
 }  // namespace block

@@ -11,6 +11,26 @@ namespace fm {
 
 namespace block {
 
+// act(x), and act'(x) for the backward. Gelu (in its tanh form) and silu are x times a sigmoid, which has no cancellation where it is small: x sigma(z), with the slope
+// sigma + x sigma (1 - sigma) z'.
+template <int kActivation>
+__device__ __forceinline__ float activate(float x, float &slope) {
+    if constexpr (kActivation == FM_ACT_GELU || kActivation == FM_ACT_SILU) {
+        float z = x, z_slope = 1.f;
+        if constexpr (kActivation == FM_ACT_GELU) {
+            const float square = x * x;
+            z = x * (1.5957691216f + 0.071354816272f * square);
+            z_slope = 1.5957691216f + 0.214064448816f * square;
+        }
+        const float sigma = fast_rcp(1.f + fast_exp(-z)), out = x * sigma;
+        slope = sigma + out * (1.f - sigma) * z_slope;
+        return out;
+    }
+    float out;
+    slope = activation_backward<kActivation>(x, out);
+    return out;
+}
+
 struct ActivationArgs {
     const void *input;                    // forward
     const void *grad_output;              // backward
@@ -39,7 +59,8 @@ __global__ __launch_bounds__(kRowThreads) void activation_forward_kernel(Activat
         if constexpr (kGated) load_values(input + args.columns, left, up);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            result[i] = activation_forward<kActivation>(gate[i]);
+            float slope;
+            result[i] = activate<kActivation>(gate[i], slope);
             if constexpr (kGated) result[i] *= up[i];
         }
         const bool exists = row < args.rows;
@@ -51,62 +72,90 @@ __global__ __launch_bounds__(kRowThreads) void activation_forward_kernel(Activat
     }
 }
 
+// The same values, but the compiler cannot tell.
+template <typename T>
+__device__ __forceinline__ void kept_apart(RawFour<T> &four) {
+    typedef __attribute__((__vector_size__(4 * sizeof(T)))) uint32_t Words;
+    Words words = __builtin_bit_cast(Words, four);
+    asm volatile("" : "+v"(words));
+    four = __builtin_bit_cast(RawFour<T>, words);
+}
+
+// At most 128 registers, for two workgroups on a CU: the second and third result are made from what the first leaves.
 template <typename T, int kActivation, bool kGated>
-__global__ __launch_bounds__(kSquareThreads) void activation_backward_kernel(ActivationArgs args) {
+__global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(ActivationArgs args) {
     __shared__ __attribute__((aligned(16))) Square shared;
     const uint32_t column_block = blockIdx.x % args.column_blocks;
     const int64_t row_block = blockIdx.x / args.column_blocks, row0 = row_block * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
     const int cg = threadIdx.x & 31, row_group = threadIdx.x >> 5;
     const int exist = static_cast<int>(min(args.rows - row0, static_cast<int64_t>(kBlock))), count = rows_in_block(args.map, row0, args.rows);
-    const int64_t column = column0 + cg * kLaneColumns;
-    constexpr int kParts = kGated ? 2 : 1;
-    float grads[kParts][kLaneRows][kLaneColumns], output[kLaneRows][kLaneColumns];
+    const int columns = static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock)));
+    const T *grad_output = static_cast<const T *>(args.grad_output) + row0 * args.grad_output_stride + column0;
+    const uint8_t *gate_from = args.checkpoint + row0 * args.checkpoint_stride + column0, *up_from = gate_from + args.columns;
+    const uint8_t *gate_scales_from = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row0;
+    const uint8_t *up_scales_from = gate_scales_from + args.column_blocks * args.checkpoint_scale_stride;
+    const uint32_t grad_stride = static_cast<uint32_t>(args.grad_output_stride), checkpoint_stride = static_cast<uint32_t>(args.checkpoint_stride);
+    RawFour<T> grad[kLaneRows];
+    float values[kLaneRows][kLaneColumns], output[kLaneRows][kLaneColumns];
+    uint32_t gates[kLaneRows], ups[kLaneRows];
+    // A byte for each row: of those that count, and zero where none does.
+    uint64_t gate_scales = 0, up_scales = 0;
+    const int counting = min(count - row_group * kLaneRows, kLaneRows);
+    if (counting > 0) {
+        const uint64_t bytes = ~uint64_t(0) >> (kLaneRows - counting) * 8;
+        gate_scales = *reinterpret_cast<const uint64_t *>(gate_scales_from + row_group * kLaneRows) & bytes;
+        if constexpr (kGated) up_scales = *reinterpret_cast<const uint64_t *>(up_scales_from + row_group * kLaneRows) & bytes;
+    }
+    const auto scale_of = [](uint64_t scales, int r) { return scale_value(static_cast<uint32_t>(scales >> r * 8) & 255u); };
 #pragma unroll
     for (int r = 0; r < kLaneRows; ++r) {
-        const int in_block = row_group * kLaneRows + r;
-        const int64_t row = row0 + in_block, left = in_block < count ? args.columns - column : 0;
-        float gate[kLaneColumns] = {}, up[kLaneColumns] = {}, grad[kLaneColumns];
-        load_values(static_cast<const T *>(args.grad_output) + row * args.grad_output_stride + column, left, grad);
+        const uint32_t row = row_group * kLaneRows + r, column = cg * kLaneColumns;
+        const int left = static_cast<int>(row) < count ? columns - static_cast<int>(column) : 0;
+        grad[r] = load_raw(grad_output + (row * grad_stride + column), left);
+        gates[r] = ups[r] = 0;
         if (left > 0) {
-            const uint8_t *checkpoint = args.checkpoint + row * args.checkpoint_stride + column, *scales = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row;
-            unpack_four(*reinterpret_cast<const uint32_t *>(checkpoint), scale_value(*scales), gate);
-            if constexpr (kGated)
-                unpack_four(*reinterpret_cast<const uint32_t *>(checkpoint + args.columns), scale_value(scales[args.column_blocks * args.checkpoint_scale_stride]), up);
+            gates[r] = *reinterpret_cast<const uint32_t *>(gate_from + (row * checkpoint_stride + column));
+            if constexpr (kGated) ups[r] = *reinterpret_cast<const uint32_t *>(up_from + (row * checkpoint_stride + column));
         }
+    }
+#pragma unroll
+    for (int r = 0; r < kLaneRows; ++r) {
+        __builtin_amdgcn_sched_barrier(0);  // one row's values at a time: registers
+        float gate[kLaneColumns], up[kLaneColumns];
+        unpack_four(gates[r], scale_of(gate_scales, r), gate);
+        if constexpr (kGated) unpack_four(ups[r], scale_of(up_scales, r), up);
 #pragma unroll
         for (int c = 0; c < kLaneColumns; ++c) {
-            float out;
-            const float slope = activation_backward<kActivation>(gate[c], out);
-            if constexpr (kGated) {
-                grads[0][r][c] = slope * up[c] * grad[c];
-                grads[1][r][c] = out * grad[c];
-                out *= up[c];
-            } else {
-                grads[0][r][c] = slope * grad[c];
-            }
-            output[r][c] = out;
+            float slope;
+            output[r][c] = activate<kActivation>(gate[c], slope);
+            values[r][c] = slope * (kGated ? up[c] * to_float(grad[r].v[c]) : to_float(grad[r].v[c]));
         }
     }
-    const int columns = static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock)));
-    const int64_t scales_of_rows = row_block * args.transposed_scale_stride;
-#pragma unroll
-    for (int part = 0; part < kParts; ++part) {
+    __builtin_amdgcn_sched_barrier(0);
+    const int64_t t_scales = row_block * args.transposed_scale_stride;
+    const auto store_gradient = [&](int part) {
         const int64_t first_column = column0 + part * args.columns;
-        column_maxima(grads[part], shared);
-        store_rows(grads[part], shared, args.grad + row0 * args.grad_stride + first_column, args.grad_stride, exist);
-        __syncthreads();
-        stage_columns(grads[part], shared);
-        __syncthreads();
-        store_row_scales(shared, args.grad_scales + (column_block + part * args.column_blocks) * args.grad_scale_stride + row0, exist);
-        store_columns(shared, args.grad_transposed + first_column * args.transposed_stride + row0, args.transposed_stride,
-                      args.grad_transposed_scales + scales_of_rows + first_column, columns);
-        __syncthreads();
+        store_square<true>(values, shared, args.grad + row0 * args.grad_stride + first_column, static_cast<uint32_t>(args.grad_stride),
+                           args.grad_scales + (column_block + part * args.column_blocks) * args.grad_scale_stride + row0, exist,
+                           args.grad_transposed + first_column * args.transposed_stride + row0, args.transposed_stride, args.grad_transposed_scales + t_scales + first_column, columns);
+    };
+    store_gradient(0);
+    if constexpr (kGated) {
+#pragma unroll
+        for (int r = 0; r < kLaneRows; ++r) {
+            __builtin_amdgcn_sched_barrier(0);
+            // (Converted again: what was converted above would be kept in registers.)
+            float up[kLaneColumns];
+            asm volatile("" : "+v"(ups[r]));
+            unpack_four(ups[r], scale_of(up_scales, r), up);
+            kept_apart(grad[r]);
+#pragma unroll
+            for (int c = 0; c < kLaneColumns; ++c) values[r][c] = output[r][c] * to_float(grad[r].v[c]), output[r][c] *= up[c];
+        }
+        store_gradient(1);
     }
-    column_maxima(output, shared);
-    __syncthreads();
-    stage_columns(output, shared);
-    __syncthreads();
-    store_columns(shared, args.output + column0 * args.output_stride + row0, args.output_stride, args.output_scales + row_block * args.output_scale_stride + column0, columns);
+    store_square<false>(output, shared, nullptr, 0, nullptr, 0, args.output + column0 * args.output_stride + row0, args.output_stride,
+                        args.output_scales + row_block * args.output_scale_stride + column0, columns);
 }
 
 template <typename T, bool kGated>
@@ -144,6 +193,8 @@ static int run_activation(const char *name, bool forward, ActivationArgs args, c
                                       args.transposed_scale_stride)) return status;
     }
     const int64_t grid = row_padding / kBlock * args.column_blocks;
+    if (!forward && (padded_input > kMaxSquareStride || (args.rows > 1 && args.grad_output_stride > kMaxSquareStride / dtype_size(dtype)) || args.checkpoint_stride > kMaxSquareStride))
+        return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     if (grid >= (int64_t(1) << 32) / kSquareThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     FM_DISPATCH_DTYPE(dtype, T, {
         if (gated) launch_activation<T, true>(forward, activation, args, static_cast<uint32_t>(grid), static_cast<hipStream_t>(stream));

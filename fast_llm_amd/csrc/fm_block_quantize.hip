@@ -15,20 +15,20 @@ template <typename T>
 struct Source {
     const T *input;
     int64_t stride;
-    __device__ __forceinline__ void load(int64_t row, int64_t column, int64_t left, float (&values)[kLaneColumns]) const {
-        load_values(input + row * stride + column, left, values);
+    __device__ __forceinline__ void load(int64_t first, uint32_t row, int64_t column0, uint32_t column, int left, float (&values)[kLaneColumns]) const {
+        load_values(input + first * stride + column0 + (row * static_cast<uint32_t>(stride) + column), left, values);
     }
 };
 // ... of an input of 8 bits: four columns of a row have one scale, and what is behind the row's columns is zero.
 struct QuantizedSource {
     const uint8_t *input, *scales;
     int64_t stride, scale_stride;
-    __device__ __forceinline__ void load(int64_t row, int64_t column, int64_t left, float (&values)[kLaneColumns]) const {
+    __device__ __forceinline__ void load(int64_t first, uint32_t row, int64_t column0, uint32_t column, int left, float (&values)[kLaneColumns]) const {
 #pragma unroll
         for (int i = 0; i < kLaneColumns; ++i) values[i] = 0.f;
         if (left <= 0) return;
-        const uint32_t byte = scales[column / kBlock * scale_stride + row];
-        unpack_four(*reinterpret_cast<const uint32_t *>(input + row * stride + column), scale_value(byte), values);
+        const uint32_t byte = (scales + column0 / kBlock * scale_stride + first)[row];
+        unpack_four(*reinterpret_cast<const uint32_t *>(input + first * stride + column0 + (row * static_cast<uint32_t>(stride) + column)), scale_value(byte), values);
         // 2^128, to which the largest values of fp32 were rounded, is not one: the largest takes its place and is rounded to it again.
         constexpr float kLargest = 3.40282346638528859812e+38f;
 #pragma unroll
@@ -53,22 +53,18 @@ __global__ __launch_bounds__(kSquareThreads) void square_kernel(Input input, Squ
     const int64_t row0 = row_block * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
     const int cg = threadIdx.x & 31, row_group = threadIdx.x >> 5;
     const int exist = static_cast<int>(min(args.rows - row0, static_cast<int64_t>(kBlock))), count = rows_in_block(args.map, row0, args.rows);
-    const int64_t first = group * args.rows + row0, column = column0 + cg * kLaneColumns;
+    const int64_t first = group * args.rows + row0;
+    const int columns = static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock)));
     float values[kLaneRows][kLaneColumns];
 #pragma unroll
     for (int r = 0; r < kLaneRows; ++r) {
         const int row = row_group * kLaneRows + r;
-        input.load(first + row, column, row < count ? args.columns - column : 0, values[r]);
+        input.load(first, row, column0, cg * kLaneColumns, row < count ? columns - cg * kLaneColumns : 0, values[r]);
     }
-    column_maxima(values, shared);
-    if constexpr (kRows) store_rows(values, shared, args.values + first * args.value_stride + column0, args.value_stride, exist);
-    __syncthreads();
-    stage_columns(values, shared);
-    __syncthreads();
-    if constexpr (kRows) store_row_scales(shared, args.scales + column_block * args.scale_stride + first, exist);
     const int64_t t_row = group * args.columns + column0;
-    store_columns(shared, args.t_values + t_row * args.t_value_stride + row0, args.t_value_stride, args.t_scales + row_block * args.t_scale_stride + t_row,
-                  static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock))));
+    store_square<kRows>(values, shared, args.values + first * args.value_stride + column0, static_cast<uint32_t>(args.value_stride), args.scales + column_block * args.scale_stride + first, exist,
+                        args.t_values + t_row * args.t_value_stride + row0, args.t_value_stride, args.t_scales + row_block * args.t_scale_stride + t_row,
+                        columns);
 }
 
 template <typename T>
@@ -207,6 +203,7 @@ extern "C" int fm_block_quantize(const void *input, void *values, void *scales, 
         return check_launch(name);
     }
     FM_REQUIRE(groups * columns < (int64_t(1) << 31), "%s: bad sizes", name);
+    if (padded > block::kMaxSquareStride || (all_rows > 1 && input_row_stride > block::kMaxSquareStride / dtype_size(dtype))) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     if (int status = block::check_tensor(name, "the transposed result", transposed_values, transposed_scales, groups * columns, padded_rows, padded_rows,
                                          transposed_scale_stride)) return status;
     if (groups * row_blocks * column_blocks >= block::kMaxThreads / block::kSquareThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
@@ -239,7 +236,8 @@ extern "C" int fm_block_transpose(const void *values, const void *scales, void *
     if (int status = block::check_tensor(name, "the result", transposed_values, transposed_scales, groups * columns, padded_rows, padded_rows,
                                          transposed_scale_stride)) return status;
     const int64_t row_blocks = padded_rows / block::kBlock, column_blocks = padded / block::kBlock;
-    if (groups * row_blocks * column_blocks >= block::kMaxThreads / block::kSquareThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
+    if (value_stride > block::kMaxSquareStride || groups * row_blocks * column_blocks >= block::kMaxThreads / block::kSquareThreads)
+        return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     args.t_values = static_cast<uint8_t *>(transposed_values), args.t_scales = static_cast<uint8_t *>(transposed_scales);
     args.rows = rows, args.columns = columns, args.t_value_stride = padded_rows, args.t_scale_stride = transposed_scale_stride;
     args.row_blocks = static_cast<uint32_t>(row_blocks), args.column_blocks = static_cast<uint32_t>(column_blocks);
