@@ -78,35 +78,42 @@ __device__ __forceinline__ int rows_in_block(const RowMap &map, int64_t row0, in
     return __builtin_amdgcn_readfirstlane(static_cast<int>(max(min(end - row0, static_cast<int64_t>(kBlock)), static_cast<int64_t>(0))));
 }
 
-// kCount neighbours of a row from `pointer` on, of which `left` exist (the others are zeros). At any alignment: the hardware takes vectors at
-// any address.
+// kCount neighbours of a row as they lie in memory, at any alignment: the hardware takes vectors at any address.
 template <typename T, int kCount>
-__device__ __forceinline__ void load_values(const T *pointer, int64_t left, float (&values)[kCount]) {
-    if (left >= kCount) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Unaligned {
-            T v[kCount];
-        };
-        const Unaligned loaded = *reinterpret_cast<const Unaligned *>(pointer);
+struct __attribute__((packed, aligned(sizeof(T)))) Raw {
+    T v[kCount];
+};
+// ... from `pointer` on, of which `left` exist; the others are zeros.
+template <typename T, int kCount>
+__device__ __forceinline__ Raw<T, kCount> load_part(const T *pointer, int left) {
+    Raw<T, kCount> raw;
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) values[i] = to_float(loaded.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) values[i] = i < left ? to_float(pointer[i]) : 0.f;
-    }
+    for (int i = 0; i < kCount; ++i) raw.v[i] = i < left ? pointer[i] : from_float<T>(0.f);
+    return raw;
 }
 
-// The same four, as they lie in memory.
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) RawFour {
-    T v[4];
-};
-template <typename T>
-__device__ __forceinline__ RawFour<T> load_raw(const T *pointer, int64_t left) {
-    if (left >= 4) return *reinterpret_cast<const RawFour<T> *>(pointer);
-    RawFour<T> four;
+// Rows `first_row` + kRowStep r, r < kRows, of a block of 128 x 128 that begins at `block`: kCount neighbours of each from `column` on. Those from `count` on are
+// zeros, and so is what is behind the `columns` that there are. `exist`: rows that may be read. Where the columns are whole, no load is behind a
+// branch, so that all are on their way at once.
+template <int kRows, int kRowStep, typename T, int kCount>
+__device__ __forceinline__ void load_block(const T *block, uint32_t stride, int first_row, int column, int exist, int count, int columns, Raw<T, kCount> (&raw)[kRows]) {
+    if (columns == kBlock) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) four.v[i] = i < left ? pointer[i] : from_float<T>(0.f);
-    return four;
+        for (int r = 0; r < kRows; ++r)
+            raw[r] = *reinterpret_cast<const Raw<T, kCount> *>(block + (static_cast<uint32_t>(min(first_row + r * kRowStep, exist - 1)) * stride + column));
+        if (count < kBlock) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                for (int i = 0; i < kCount; ++i) raw[r].v[i] = first_row + r * kRowStep < count ? raw[r].v[i] : from_float<T>(0.f);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const int row = first_row + r * kRowStep;
+            raw[r] = load_part<T, kCount>(block + (static_cast<uint32_t>(row) * stride + column), row < count ? columns - column : 0);
+        }
+    }
 }
 
 }  // namespace block

@@ -47,41 +47,50 @@ struct ActivationArgs {
 template <typename T, int kActivation, bool kGated>
 __global__ __launch_bounds__(kRowThreads) void activation_forward_kernel(ActivationArgs args) {
     const uint32_t column_block = blockIdx.x % args.column_blocks;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x / args.column_blocks) * kBlock, column = static_cast<int64_t>(column_block) * kBlock + threadIdx.x % 8 * 16;
-    const int count = rows_in_block(args.map, row0, args.rows);
-#pragma unroll 2
-    for (int step = 0; step < kRowSteps; ++step) {
-        const int in_block = step * (kRowThreads / 8) + static_cast<int>(threadIdx.x) / 8;
-        const int64_t row = row0 + in_block, left = in_block < count ? args.columns - column : 0;
-        const T *input = static_cast<const T *>(args.input) + row * args.input_stride + column;
-        float gate[16], up[16], result[16];
-        load_values(input, left, gate);
-        if constexpr (kGated) load_values(input + args.columns, left, up);
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x / args.column_blocks) * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
+    const int count = rows_in_block(args.map, row0, args.rows), exist = static_cast<int>(min(args.rows - row0, static_cast<int64_t>(kBlock)));
+    const int columns = static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock))), first_row = threadIdx.x / 8, column = threadIdx.x % 8 * 16;
+    const T *input = static_cast<const T *>(args.input) + row0 * args.input_stride + column0;
+    uint8_t *output = args.output + row0 * args.output_stride + column0, *output_scales = args.output_scales + column_block * args.output_scale_stride + row0;
+    uint8_t *checkpoint = args.checkpoint + row0 * args.checkpoint_stride + column0, *scales = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row0;
+    // Two rows of a lane at a time.
+#pragma unroll 1
+    for (int begin = 0; begin < kBlock; begin += kRowThreads / 4) {
+        Raw<T, 16> gates[2], ups[2];
+        const uint32_t stride = static_cast<uint32_t>(args.input_stride);
+        load_block<2, kRowThreads / 8>(input, stride, begin + first_row, column, exist, count, columns, gates);
+        if constexpr (kGated) load_block<2, kRowThreads / 8>(input + args.columns, stride, begin + first_row, column, exist, count, columns, ups);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float slope;
-            result[i] = activate<kActivation>(gate[i], slope);
-            if constexpr (kGated) result[i] *= up[i];
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t row = begin + first_row + r * (kRowThreads / 8);
+            const bool exists = static_cast<int>(row) < exist;
+            float gate[16], up[16], result[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float slope;
+                gate[i] = to_float(gates[r].v[i]);
+                result[i] = activate<kActivation>(gate[i], slope);
+                if constexpr (kGated) up[i] = to_float(ups[r].v[i]), result[i] *= up[i];
+            }
+            const uint32_t at = row * static_cast<uint32_t>(args.checkpoint_stride) + column;
+            store_row(gate, checkpoint + at, scales + row, exists);
+            // (Gated: whole blocks of columns.)
+            if constexpr (kGated) store_row(up, checkpoint + args.columns + at, scales + args.column_blocks * args.checkpoint_scale_stride + row, exists);
+            store_row(result, output + (row * static_cast<uint32_t>(args.output_stride) + column), output_scales + row, exists);
         }
-        const bool exists = row < args.rows;
-        uint8_t *checkpoint = args.checkpoint + row * args.checkpoint_stride + column, *scales = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row;
-        store_row(gate, checkpoint, scales, exists);
-        // (Gated: whole blocks of columns.)
-        if constexpr (kGated) store_row(up, checkpoint + args.columns, scales + args.column_blocks * args.checkpoint_scale_stride, exists);
-        store_row(result, args.output + row * args.output_stride + column, args.output_scales + column_block * args.output_scale_stride + row, exists);
     }
 }
 
 // The same values, but the compiler cannot tell.
 template <typename T>
-__device__ __forceinline__ void kept_apart(RawFour<T> &four) {
+__device__ __forceinline__ void kept_apart(Raw<T, 4> &four) {
     typedef __attribute__((__vector_size__(4 * sizeof(T)))) uint32_t Words;
     Words words = __builtin_bit_cast(Words, four);
     asm volatile("" : "+v"(words));
-    four = __builtin_bit_cast(RawFour<T>, words);
+    four = __builtin_bit_cast(Raw<T, 4>, words);
 }
 
-// At most 128 registers, for two workgroups on a CU: the second and third result are made from what the first leaves.
+// At most 128 registers, for two workgroups on a CU: gates, ups and gradients stay as they were read, and the results are made one after the other.
 template <typename T, int kActivation, bool kGated>
 __global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(ActivationArgs args) {
     __shared__ __attribute__((aligned(16))) Square shared;
@@ -95,29 +104,33 @@ __global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(
     const uint8_t *gate_scales_from = args.checkpoint_scales + column_block * args.checkpoint_scale_stride + row0;
     const uint8_t *up_scales_from = gate_scales_from + args.column_blocks * args.checkpoint_scale_stride;
     const uint32_t grad_stride = static_cast<uint32_t>(args.grad_output_stride), checkpoint_stride = static_cast<uint32_t>(args.checkpoint_stride);
-    RawFour<T> grad[kLaneRows];
+    const int first_row = row_group * kLaneRows, first_column = cg * kLaneColumns;
+    Raw<T, kLaneColumns> grad[kLaneRows];
+    load_block<kLaneRows, 1>(grad_output, grad_stride, first_row, first_column, exist, count, columns, grad);
     float values[kLaneRows][kLaneColumns], output[kLaneRows][kLaneColumns];
     uint32_t gates[kLaneRows], ups[kLaneRows];
-    // A byte for each row: of those that count, and zero where none does.
-    uint64_t gate_scales = 0, up_scales = 0;
-    const int counting = min(count - row_group * kLaneRows, kLaneRows);
-    if (counting > 0) {
-        const uint64_t bytes = ~uint64_t(0) >> (kLaneRows - counting) * 8;
-        gate_scales = *reinterpret_cast<const uint64_t *>(gate_scales_from + row_group * kLaneRows) & bytes;
-        if constexpr (kGated) up_scales = *reinterpret_cast<const uint64_t *>(up_scales_from + row_group * kLaneRows) & bytes;
-    }
-    const auto scale_of = [](uint64_t scales, int r) { return scale_value(static_cast<uint32_t>(scales >> r * 8) & 255u); };
 #pragma unroll
     for (int r = 0; r < kLaneRows; ++r) {
-        const uint32_t row = row_group * kLaneRows + r, column = cg * kLaneColumns;
-        const int left = static_cast<int>(row) < count ? columns - static_cast<int>(column) : 0;
-        grad[r] = load_raw(grad_output + (row * grad_stride + column), left);
-        gates[r] = ups[r] = 0;
-        if (left > 0) {
-            gates[r] = *reinterpret_cast<const uint32_t *>(gate_from + (row * checkpoint_stride + column));
-            if constexpr (kGated) ups[r] = *reinterpret_cast<const uint32_t *>(up_from + (row * checkpoint_stride + column));
+        const uint32_t at = min(first_row + r, exist - 1) * checkpoint_stride + first_column;
+        gates[r] = *reinterpret_cast<const uint32_t *>(gate_from + at);
+        if constexpr (kGated) ups[r] = *reinterpret_cast<const uint32_t *>(up_from + at);
+    }
+    // A byte for each row. (Scales are padded to whole pieces of sixteen rows.)
+    const int scale_row = min(first_row, (exist - 1) & ~7);
+    uint64_t gate_scales = *reinterpret_cast<const uint64_t *>(gate_scales_from + scale_row), up_scales = 0;
+    if constexpr (kGated) up_scales = *reinterpret_cast<const uint64_t *>(up_scales_from + scale_row);
+    if (count < kBlock) {
+        // Zeros, whatever the checkpoint holds for rows that do not count.
+        const int counting = min(max(count - first_row, 0), kLaneRows);
+        const uint64_t bytes = counting > 0 ? ~uint64_t(0) >> (kLaneRows - counting) * 8 : 0;
+        gate_scales &= bytes, up_scales &= bytes;
+#pragma unroll
+        for (int r = 0; r < kLaneRows; ++r) {
+            gates[r] = r < counting ? gates[r] : 0u;
+            if constexpr (kGated) ups[r] = r < counting ? ups[r] : 0u;
         }
     }
+    const auto scale_of = [](uint64_t scales, int r) { return scale_value(static_cast<uint32_t>(scales >> r * 8) & 255u); };
 #pragma unroll
     for (int r = 0; r < kLaneRows; ++r) {
         __builtin_amdgcn_sched_barrier(0);  // one row's values at a time: registers
@@ -127,30 +140,36 @@ __global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(
 #pragma unroll
         for (int c = 0; c < kLaneColumns; ++c) {
             float slope;
-            output[r][c] = activate<kActivation>(gate[c], slope);
+            const float out = activate<kActivation>(gate[c], slope);
+            if constexpr (!kGated) output[r][c] = out;
             values[r][c] = slope * (kGated ? up[c] * to_float(grad[r].v[c]) : to_float(grad[r].v[c]));
         }
     }
     __builtin_amdgcn_sched_barrier(0);
     const int64_t t_scales = row_block * args.transposed_scale_stride;
     const auto store_gradient = [&](int part) {
-        const int64_t first_column = column0 + part * args.columns;
-        store_square<true>(values, shared, args.grad + row0 * args.grad_stride + first_column, static_cast<uint32_t>(args.grad_stride),
+        const int64_t from_column = column0 + part * args.columns;
+        store_square<true>(values, shared, args.grad + row0 * args.grad_stride + from_column, static_cast<uint32_t>(args.grad_stride),
                            args.grad_scales + (column_block + part * args.column_blocks) * args.grad_scale_stride + row0, exist,
-                           args.grad_transposed + first_column * args.transposed_stride + row0, args.transposed_stride, args.grad_transposed_scales + t_scales + first_column, columns);
+                           args.grad_transposed + from_column * args.transposed_stride + row0, args.transposed_stride, args.grad_transposed_scales + t_scales + from_column, columns);
     };
     store_gradient(0);
     if constexpr (kGated) {
 #pragma unroll
         for (int r = 0; r < kLaneRows; ++r) {
             __builtin_amdgcn_sched_barrier(0);
-            // (Converted again: what was converted above would be kept in registers.)
-            float up[kLaneColumns];
-            asm volatile("" : "+v"(ups[r]));
+            // (Activated again: what there was above would not fit the registers until here.)
+            float gate[kLaneColumns], up[kLaneColumns];
+            asm volatile("" : "+v"(gates[r]), "+v"(ups[r]));
+            unpack_four(gates[r], scale_of(gate_scales, r), gate);
             unpack_four(ups[r], scale_of(up_scales, r), up);
             kept_apart(grad[r]);
 #pragma unroll
-            for (int c = 0; c < kLaneColumns; ++c) values[r][c] = output[r][c] * to_float(grad[r].v[c]), output[r][c] *= up[c];
+            for (int c = 0; c < kLaneColumns; ++c) {
+                float slope;
+                const float out = activate<kActivation>(gate[c], slope);
+                values[r][c] = out * to_float(grad[r].v[c]), output[r][c] = out * up[c];
+            }
         }
         store_gradient(1);
     }
@@ -193,7 +212,8 @@ static int run_activation(const char *name, bool forward, ActivationArgs args, c
                                       args.transposed_scale_stride)) return status;
     }
     const int64_t grid = row_padding / kBlock * args.column_blocks;
-    if (!forward && (padded_input > kMaxSquareStride || (args.rows > 1 && args.grad_output_stride > kMaxSquareStride / dtype_size(dtype)) || args.checkpoint_stride > kMaxSquareStride))
+    if ((forward && args.rows > 1 && args.input_stride > kMaxSquareStride / dtype_size(dtype)) || padded_input > kMaxSquareStride ||
+        (!forward && ((args.rows > 1 && args.grad_output_stride > kMaxSquareStride / dtype_size(dtype)) || args.checkpoint_stride > kMaxSquareStride)))
         return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     if (grid >= (int64_t(1) << 32) / kSquareThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     FM_DISPATCH_DTYPE(dtype, T, {

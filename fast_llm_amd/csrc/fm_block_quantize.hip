@@ -10,29 +10,44 @@ namespace fm {
 
 namespace block {
 
-// Rows [rows, columns] of an input, and where they go. Groups (of the transposed form): every `rows` rows are a matrix of their own.
+// Rows of an input. `load`: eight rows x four columns of a lane in the square that begins at (`row0`, `column0`).
 template <typename T>
 struct Source {
     const T *input;
     int64_t stride;
-    __device__ __forceinline__ void load(int64_t first, uint32_t row, int64_t column0, uint32_t column, int left, float (&values)[kLaneColumns]) const {
-        load_values(input + first * stride + column0 + (row * static_cast<uint32_t>(stride) + column), left, values);
+    __device__ __forceinline__ void load(int64_t row0, int64_t column0, int exist, int count, int columns, float (&values)[kLaneRows][kLaneColumns]) const {
+        Raw<T, kLaneColumns> raw[kLaneRows];
+        load_block<kLaneRows, 1>(input + row0 * stride + column0, static_cast<uint32_t>(stride), threadIdx.x / 32 * kLaneRows, threadIdx.x % 32 * kLaneColumns, exist, count,
+                                 columns, raw);
+#pragma unroll
+        for (int r = 0; r < kLaneRows; ++r)
+#pragma unroll
+            for (int c = 0; c < kLaneColumns; ++c) values[r][c] = to_float(raw[r].v[c]);
     }
 };
-// ... of an input of 8 bits: four columns of a row have one scale, and what is behind the row's columns is zero.
+// ... of 8 bits: with padding, so that columns are whole.
 struct QuantizedSource {
     const uint8_t *input, *scales;
     int64_t stride, scale_stride;
-    __device__ __forceinline__ void load(int64_t first, uint32_t row, int64_t column0, uint32_t column, int left, float (&values)[kLaneColumns]) const {
+    __device__ __forceinline__ void load(int64_t row0, int64_t column0, int exist, int count, int, float (&values)[kLaneRows][kLaneColumns]) const {
+        const uint32_t first_row = threadIdx.x / 32 * kLaneRows, column = threadIdx.x % 32 * kLaneColumns;
+        const uint8_t *block = input + row0 * stride + column0, *block_scales = scales + column0 / kBlock * scale_stride + row0;
+        uint32_t words[kLaneRows], bytes[kLaneRows];
 #pragma unroll
-        for (int i = 0; i < kLaneColumns; ++i) values[i] = 0.f;
-        if (left <= 0) return;
-        const uint32_t byte = (scales + column0 / kBlock * scale_stride + first)[row];
-        unpack_four(*reinterpret_cast<const uint32_t *>(input + first * stride + column0 + (row * static_cast<uint32_t>(stride) + column)), scale_value(byte), values);
-        // 2^128, to which the largest values of fp32 were rounded, is not one: the largest takes its place and is rounded to it again.
-        constexpr float kLargest = 3.40282346638528859812e+38f;
+        for (int r = 0; r < kLaneRows; ++r) {
+            const uint32_t row = min(static_cast<int>(first_row) + r, exist - 1);
+            words[r] = *reinterpret_cast<const uint32_t *>(block + (row * static_cast<uint32_t>(stride) + column)), bytes[r] = block_scales[row];
+        }
 #pragma unroll
-        for (int i = 0; i < kLaneColumns; ++i) values[i] = byte == 255u ? values[i] : __builtin_amdgcn_fmed3f(values[i], -kLargest, kLargest);
+        for (int r = 0; r < kLaneRows; ++r) {
+            const bool counts = static_cast<int>(first_row) + r < count;
+            const uint32_t byte = counts ? bytes[r] : 0u;
+            unpack_four(counts ? words[r] : 0u, scale_value(byte), values[r]);
+            // 2^128, to which the largest values of fp32 were rounded, is not one: the largest takes its place and is rounded to it again.
+            constexpr float kLargest = 3.40282346638528859812e+38f;
+#pragma unroll
+            for (int i = 0; i < kLaneColumns; ++i) values[r][i] = byte == 255u ? values[r][i] : __builtin_amdgcn_fmed3f(values[r][i], -kLargest, kLargest);
+        }
     }
 };
 
@@ -51,16 +66,11 @@ __global__ __launch_bounds__(kSquareThreads) void square_kernel(Input input, Squ
     const uint32_t column_block = blockIdx.x % args.column_blocks, rest = blockIdx.x / args.column_blocks;
     const int64_t group = rest / args.row_blocks, row_block = rest % args.row_blocks;
     const int64_t row0 = row_block * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
-    const int cg = threadIdx.x & 31, row_group = threadIdx.x >> 5;
     const int exist = static_cast<int>(min(args.rows - row0, static_cast<int64_t>(kBlock))), count = rows_in_block(args.map, row0, args.rows);
     const int64_t first = group * args.rows + row0;
     const int columns = static_cast<int>(min(args.columns - column0, static_cast<int64_t>(kBlock)));
     float values[kLaneRows][kLaneColumns];
-#pragma unroll
-    for (int r = 0; r < kLaneRows; ++r) {
-        const int row = row_group * kLaneRows + r;
-        input.load(first, row, column0, cg * kLaneColumns, row < count ? columns - cg * kLaneColumns : 0, values[r]);
-    }
+    input.load(first, column0, exist, count, columns, values);
     const int64_t t_row = group * args.columns + column0;
     store_square<kRows>(values, shared, args.values + first * args.value_stride + column0, static_cast<uint32_t>(args.value_stride), args.scales + column_block * args.scale_stride + first, exist,
                         args.t_values + t_row * args.t_value_stride + row0, args.t_value_stride, args.t_scales + row_block * args.t_scale_stride + t_row,
@@ -71,17 +81,19 @@ template <typename T>
 __global__ __launch_bounds__(kRowThreads) void row_kernel(const T *input, uint8_t *values, uint8_t *scales, int64_t rows, int64_t columns, int64_t input_stride,
                                                           int64_t value_stride, int64_t scale_stride, uint32_t column_blocks) {
     const uint32_t column_block = blockIdx.x % column_blocks;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x / column_blocks) * kBlock, column = static_cast<int64_t>(column_block) * kBlock + threadIdx.x % 8 * 16;
-    float loaded[kRowSteps][16];
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x / column_blocks) * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
+    const int first_row = threadIdx.x / 8, column = threadIdx.x % 8 * 16, exist = static_cast<int>(min(rows - row0, static_cast<int64_t>(kBlock)));
+    Raw<T, 16> raw[kRowSteps];
+    load_block<kRowSteps, kRowThreads / 8>(input + row0 * input_stride + column0, static_cast<uint32_t>(input_stride), first_row, column, exist, exist,
+                                           static_cast<int>(min(columns - column0, static_cast<int64_t>(kBlock))), raw);
 #pragma unroll
     for (int step = 0; step < kRowSteps; ++step) {
-        const int64_t row = row0 + step * (kRowThreads / 8) + threadIdx.x / 8;
-        load_values(input + row * input_stride + column, row < rows ? columns - column : 0, loaded[step]);
-    }
+        float loaded[16];
 #pragma unroll
-    for (int step = 0; step < kRowSteps; ++step) {
-        const int64_t row = row0 + step * (kRowThreads / 8) + threadIdx.x / 8;
-        store_row(loaded[step], values + row * value_stride + column, scales + column_block * scale_stride + row, row < rows);
+        for (int i = 0; i < 16; ++i) loaded[i] = to_float(raw[step].v[i]);
+        const int row = first_row + step * (kRowThreads / 8);
+        store_row(loaded, values + row0 * value_stride + column0 + (static_cast<uint32_t>(row) * static_cast<uint32_t>(value_stride) + column),
+                  scales + column_block * scale_stride + row0 + row, row < exist);
     }
 }
 
@@ -192,6 +204,7 @@ extern "C" int fm_block_quantize(const void *input, void *values, void *scales, 
         if (int status = block::check_tensor(name, "the result", values, scales, all_rows, padded, padded, scale_stride)) return status;
     const int64_t row_blocks = padded_rows / block::kBlock, column_blocks = padded / block::kBlock;
     const auto hip_stream = static_cast<hipStream_t>(stream);
+    if (padded > block::kMaxSquareStride || (all_rows > 1 && input_row_stride > block::kMaxSquareStride / dtype_size(dtype))) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     if (!along_columns) {
         const int64_t workgroups = (all_rows + block::kBlock - 1) / block::kBlock * column_blocks;
         if (workgroups >= block::kMaxThreads / block::kRowThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
@@ -203,7 +216,6 @@ extern "C" int fm_block_quantize(const void *input, void *values, void *scales, 
         return check_launch(name);
     }
     FM_REQUIRE(groups * columns < (int64_t(1) << 31), "%s: bad sizes", name);
-    if (padded > block::kMaxSquareStride || (all_rows > 1 && input_row_stride > block::kMaxSquareStride / dtype_size(dtype))) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
     if (int status = block::check_tensor(name, "the transposed result", transposed_values, transposed_scales, groups * columns, padded_rows, padded_rows,
                                          transposed_scale_stride)) return status;
     if (groups * row_blocks * column_blocks >= block::kMaxThreads / block::kSquareThreads) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
