@@ -30,7 +30,8 @@ constexpr int kBlocks = 4;  // of 32, per wavefront and axis
 constexpr int kOperandBytes = kTile * kSlice, kSlotBytes = 2 * kOperandBytes, kSlots = 2;
 // Scales of a slice: a load per wavefront, of the rows of one half of the tile or of its weight rows, from an address of any alignment in pieces of 16.
 constexpr int kScaleBytes = 1024, kScaleSlots = 3, kScaleSlotBytes = kWaves * kScaleBytes, kScalePieces = 128 / 16 + 1;
-constexpr int kLdsBytes = kSlots * kSlotBytes + kScaleSlots * kScaleSlotBytes;
+constexpr int kPlaceBytes = 3 * 1024 * 4;  // see Places
+constexpr int kLdsBytes = kSlots * kSlotBytes + kScaleSlots * kScaleSlotBytes + kPlaceBytes;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr int kLoads = kOperandBytes / 1024 / kWaves;  // of a wavefront, per operand and slice
 constexpr int kResident = 256;                         // workgroups: one per CU
@@ -123,102 +124,87 @@ struct Tile {
     int first_slice, slices;  // of the reduction
 };
 
-// Which tile: by rows as `locate_tile`, by the reduction expert after expert; with the experts' ranges in registers, two experts per lane.
-constexpr int kMaxInRegisters = 128;
+// Which tile: by rows as `locate_tile`, by the reduction expert after expert. Where the experts lie is looked up once and kept in LDS.
+constexpr int kMaxExperts = 1024;
+static_assert(kPlaceBytes == 3 * kMaxExperts * 4, "room for the tables");
 template <bool kByInner>
 struct Places {
-    int begin[2], end[2];  // rows, or slices of the reduction
-    int count[2], last[2]; // by rows: row tiles, row tiles up to and with this expert's
-    int before[3];         // row tiles in front of each 64 experts, and of all
+    int at;         // in LDS: of every expert where its rows (or slices of the reduction) begin and end, and by rows the row tiles up to and with its own
+    int row_tiles;  // of all experts
 
+    __device__ __forceinline__ FM_LDS(int) * table(int which) const { return (FM_LDS(int) *)static_cast<uintptr_t>(at + which * kMaxExperts * 4); }
     // (Without a map all of them.)
     static __device__ __forceinline__ void range_of_expert(const GemmArgs &args, int expert, int64_t &first, int64_t &past) {
         first = 0, past = args.rows;
         if (args.expert_ends != nullptr) rows_of_expert(args, expert, first, past);
+        first = max(first, static_cast<int64_t>(0)), past = max(past, first);
     }
-    // The expert's part of the reduction, in whole slices: it begins at one.
-    static __device__ __forceinline__ void slices_of_expert(const GemmArgs &args, int expert, int &first, int &past) {
-        int64_t from, to;
-        range_of_expert(args, expert, from, to);
-        from = max(from, static_cast<int64_t>(0));
-        first = static_cast<int>(from / kSlice);
-        past = to > from ? static_cast<int>((to + kSlice - 1) / kSlice) : first;
-    }
-    __device__ __forceinline__ void load(const GemmArgs &args, int lane) {
-        before[0] = 0;
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-            const int e = part * 64 + lane;
-            begin[part] = end[part] = count[part] = last[part] = 0;
-            if constexpr (kByInner) {
-                if (e < args.num_experts) slices_of_expert(args, e, begin[part], end[part]);
-            } else {
+    // All threads of the workgroup take part.
+    __device__ __forceinline__ void load(const GemmArgs &args) {
+        if (threadIdx.x < 64) {
+            const int lane = threadIdx.x;
+            int before = 0;
+            for (int base = 0; base < args.num_experts; base += 64) {
+                const int e = base + lane;
                 int64_t first = 0, past = 0;
                 if (e < args.num_experts) range_of_expert(args, e, first, past);
-                count[part] = first >= 0 && past > first ? static_cast<int>((past - first + kTile - 1) / kTile) : 0;
-                begin[part] = static_cast<int>(first), end[part] = static_cast<int>(past);
-                int sum = count[part];
+                if constexpr (kByInner) {
+                    // In whole slices: an expert's part begins at one.
+                    if (e < args.num_experts) table(0)[e] = static_cast<int>(first / kSlice), table(1)[e] = past > first ? static_cast<int>((past + kSlice - 1) / kSlice) : static_cast<int>(first / kSlice);
+                } else {
+                    int sum = static_cast<int>((past - first + kTile - 1) / kTile);
 #pragma unroll
-                for (int offset = 1; offset < 64; offset <<= 1) {
-                    const int other = __shfl_up(sum, offset, 64);
-                    if (lane >= offset) sum += other;
+                    for (int offset = 1; offset < 64; offset <<= 1) {
+                        const int other = __shfl_up(sum, offset, 64);
+                        if (lane >= offset) sum += other;
+                    }
+                    sum += before;
+                    before = __builtin_amdgcn_readlane(sum, 63);
+                    if (e < args.num_experts) table(0)[e] = static_cast<int>(first), table(1)[e] = static_cast<int>(past), table(2)[e] = sum;
                 }
-                last[part] = sum + before[part];
-                before[part + 1] = __builtin_amdgcn_readlane(last[part], 63);
             }
         }
+        __syncthreads();
+        if constexpr (!kByInner) row_tiles = __builtin_amdgcn_readfirstlane(table(2)[args.num_experts - 1]);
     }
     __device__ __forceinline__ bool locate(const GemmArgs &args, int logical, int slices, Tile &tile) const {
+        int row_tile;
         if constexpr (kByInner) {
             const int per_expert = args.tiles_m * args.tiles_n, expert = logical / per_expert;
             if (expert >= args.num_experts) return false;
-            int row_tile;
             place_in_expert(logical - expert * per_expert, args.tiles_m, args.tiles_n, row_tile, tile.tile_n);
-            int first, past;
-            if (args.num_experts > kMaxInRegisters) {
-                slices_of_expert(args, expert, first, past);
-                first = __builtin_amdgcn_readfirstlane(first), past = __builtin_amdgcn_readfirstlane(past);
-            } else {
-                const bool part = expert >= 64;
-                first = __builtin_amdgcn_readlane(part ? begin[1] : begin[0], expert & 63), past = __builtin_amdgcn_readlane(part ? end[1] : end[0], expert & 63);
-            }
+            const int first = __builtin_amdgcn_readfirstlane(table(0)[expert]), past = __builtin_amdgcn_readfirstlane(table(1)[expert]);
             tile.expert = expert, tile.row0 = row_tile * kTile;
             tile.rows_valid = min(kTile, static_cast<int>(args.sparse_size) - tile.row0);
             tile.first_slice = first, tile.slices = past - first;
             return true;
         }
-        tile.first_slice = 0, tile.slices = slices;
-        if (args.num_experts > kMaxInRegisters) {
-            // (Without halves in the last round.) The same in all lanes, which the compiler cannot know.
-            RowTile found{};
-            const bool exists = locate_tile<kTile>(args, logical, found);
-            tile.expert = __builtin_amdgcn_readfirstlane(found.expert), tile.tile_n = __builtin_amdgcn_readfirstlane(found.tile_n);
-            tile.rows_valid = __builtin_amdgcn_readfirstlane(found.rows_valid);
-            tile.row0 = __builtin_amdgcn_readfirstlane(static_cast<int>(found.row0));  // rows are counted in 31 bits
-            return __builtin_amdgcn_readfirstlane(static_cast<int>(exists)) != 0;
-        }
         // Where half of the workgroups or fewer have a tile in the last round, they have the halves of one each.
-        const int total = before[2] * args.tiles_n, last_round = total & ~(kResident - 1);
+        const int total = row_tiles * args.tiles_n, last_round = total & ~(kResident - 1);
         const bool halved = total - last_round <= kResident / 2 && logical >= last_round;
         const bool second = halved && (logical & 1);
         if (halved) logical = last_round + (logical - last_round) / 2;
         if (logical >= total) return false;
-        const int part = logical >= before[1] * args.tiles_n;
-        const int lasts = part ? last[1] : last[0], counts = part ? count[1] : count[0];
-        const uint64_t owners = __ballot(lasts * args.tiles_n > logical);
-        const int owner = __ffsll(static_cast<unsigned long long>(owners)) - 1;
-        const int owner_count = __builtin_amdgcn_readlane(counts, owner), owner_last = __builtin_amdgcn_readlane(lasts, owner);
-        const int first = __builtin_amdgcn_readlane(part ? begin[1] : begin[0], owner), past = __builtin_amdgcn_readlane(part ? end[1] : end[0], owner);
-        int row_tile;
-        place_in_expert(logical - (owner_last - owner_count) * args.tiles_n, owner_count, args.tiles_n, row_tile, tile.tile_n);
-        tile.expert = part * 64 + owner;
+        int expert = 0;  // of the first one whose tiles reach past this
+        for (int base = 0;; base += 64) {
+            const int e = min(base + static_cast<int>(threadIdx.x & 63), args.num_experts - 1);
+            const uint64_t owners = __ballot(table(2)[e] * args.tiles_n > logical);
+            if (owners == 0) continue;
+            expert = base + __ffsll(static_cast<unsigned long long>(owners)) - 1;
+            break;
+        }
+        const int past_tiles = __builtin_amdgcn_readfirstlane(table(2)[expert]), first_tile = expert > 0 ? __builtin_amdgcn_readfirstlane(table(2)[expert - 1]) : 0;
+        const int first = __builtin_amdgcn_readfirstlane(table(0)[expert]), past = __builtin_amdgcn_readfirstlane(table(1)[expert]);
+        place_in_expert(logical - first_tile * args.tiles_n, past_tiles - first_tile, args.tiles_n, row_tile, tile.tile_n);
+        tile.expert = expert;
         tile.row0 = first + row_tile * kTile + (second ? kTile / 2 : 0);
         tile.rows_valid = min(halved ? kTile / 2 : kTile, past - tile.row0);
+        tile.first_slice = 0, tile.slices = slices;
         return tile.rows_valid > 0;  // (a workgroup whose second half is empty has nothing after it)
     }
 };
 
-template <bool kByInner, typename Result>
+template <bool kByInner, bool kAccumulate, typename Result>
 __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, GemmArgs placement) {
     constexpr bool kWide = std::is_same<Result, float>::value;
     extern __shared__ __attribute__((aligned(1024))) char lds_generic[];
@@ -230,7 +216,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     // The 32 workgroups of an XCD take consecutive tiles.
     int logical = (blockIdx.x % 8) * (kResident / 8) + blockIdx.x / 8;
     Places<kByInner> places;
-    places.load(placement, lane);
+    places.at = lds + kSlots * kSlotBytes + kScaleSlots * kScaleSlotBytes;
+    places.load(placement);
     Tile tile, upcoming;
     if (!places.locate(placement, logical, inner_slices, upcoming)) return;
 
@@ -469,37 +456,72 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         // ---- the tile's results: of block (n, m) a lane has columns 16 half .. + 15 of one row ---------------------------
         const int row_start = wave_m * blocks * 32, col0 = tile.tile_n * kTile, out_lane = opaque(lane);
         const int64_t out_row = (kByInner ? tile.expert * args.rows : 0) + tile.row0;
+        constexpr int N = Vec16<Result>::N, kVectors = 16 / N;
+        bool stored = false;
+        if constexpr (kAccumulate) {
+            stored = args.out_vectors && columns % 16 == 0;
+            if (stored) {
+                // What is added to is asked for kAhead blocks ahead. Rows and columns that do not exist read the tile's first.
+                constexpr int kAhead = 2;
+                Vec16<Result> previous[kAhead][kVectors];
+                const auto place = [&](int m, int n, bool &exists) {
+                    const int row = row_start + m * 32 + (out_lane & 31), column = wave_n * 128 + n * 32 + 16 * (out_lane >> 5);
+                    exists = m < blocks && row < tile.rows_valid && col0 + column < columns;
+                    return static_cast<Result *>(args.out) + out_row * args.out_stride + col0 + (exists ? row * args.out_stride + column : 0);
+                };
+                const auto load_previous = [&](auto constant) {
+                    constexpr int at = decltype(constant)::value;
+                    bool exists;
+                    const Result *out = place(at / kBlocks, at % kBlocks, exists);
 #pragma unroll
-        for (int m = 0; m < kBlocks; ++m) {
-            const int row = row_start + m * 32 + (out_lane & 31);
-            if (m >= blocks || row >= tile.rows_valid) continue;
+                    for (int part = 0; part < kVectors; ++part) previous[at % kAhead][part] = load16(out + part * N);
+                };
+                for_each<0, kAhead>(load_previous);
+                for_each<0, kBlocks * kBlocks>([&](auto constant) {
+                    constexpr int at = decltype(constant)::value, m = at / kBlocks, n = at % kBlocks;
+                    __builtin_amdgcn_sched_barrier(0);
+                    f32x16_t values = settled(acc[n][m]);
+                    Vec16<Result> vectors[kVectors];
 #pragma unroll
-            for (int n = 0; n < kBlocks; ++n) {
-                __builtin_amdgcn_sched_barrier(0);
-                f32x16_t values = settled(acc[n][m]);
-                const int column = col0 + wave_n * 128 + n * 32 + 16 * (out_lane >> 5);
-                Result *out = static_cast<Result *>(args.out) + (out_row + row) * args.out_stride + column;
-                constexpr int N = Vec16<Result>::N;
-                if (args.out_vectors && column + 15 < columns) {
-                    if (kByInner && args.accumulate) {
+                    for (int part = 0; part < kVectors; ++part)
+#pragma unroll
+                        for (int c = 0; c < N; ++c) vectors[part].v[c] = from_float<Result>(values[part * N + c] + to_float(previous[at % kAhead][part].v[c]));
+                    if constexpr (at + kAhead < kBlocks * kBlocks) load_previous(std::integral_constant<int, at + kAhead>{});
+                    bool exists;
+                    Result *out = place(m, n, exists);
+                    if (exists) {
+#pragma unroll
+                        for (int part = 0; part < kVectors; ++part) store16(out + part * N, vectors[part]);
+                    }
+                });
+                // For the compiler, which would otherwise take one of these loads to be on its way in every slice of the next tile, and wait for all.
+                __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+            }
+        }
+        if (!stored) {
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+                const int row = row_start + m * 32 + (out_lane & 31);
+                if (m >= blocks || row >= tile.rows_valid) continue;
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    f32x16_t values = settled(acc[n][m]);
+                    const int column = col0 + wave_n * 128 + n * 32 + 16 * (out_lane >> 5);
+                    Result *out = static_cast<Result *>(args.out) + (out_row + row) * args.out_stride + column;
+                    if (!kAccumulate && args.out_vectors && column + 15 < columns) {
 #pragma unroll
                         for (int part = 0; part < 16 / N; ++part) {
-                            const Vec16<Result> vector = load16(out + part * N);
+                            Vec16<Result> vector;
 #pragma unroll
-                            for (int c = 0; c < N; ++c) values[part * N + c] += to_float(vector.v[c]);
+                            for (int c = 0; c < N; ++c) vector.v[c] = from_float<Result>(values[part * N + c]);
+                            store16(out + part * N, vector);
                         }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (column + c < columns) out[c] = from_float<Result>(values[c] + (kAccumulate ? to_float(out[c]) : 0.f));
                     }
-#pragma unroll
-                    for (int part = 0; part < 16 / N; ++part) {
-                        Vec16<Result> vector;
-#pragma unroll
-                        for (int c = 0; c < N; ++c) vector.v[c] = from_float<Result>(values[part * N + c]);
-                        store16(out + part * N, vector);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 16; ++c)
-                        if (column + c < columns) out[c] = from_float<Result>(values[c] + (kByInner && args.accumulate ? to_float(out[c]) : 0.f));
                 }
             }
         }
@@ -508,9 +530,9 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     wait_for_memory<0>();  // zeros behind the last tile
 }
 
-template <bool kByInner, typename Result>
+template <bool kByInner, bool kAccumulate, typename Result>
 static int launch(const ProductArgs &args, hipStream_t stream) {
-    const auto kernel = tile_kernel<kByInner, Result>;
+    const auto kernel = tile_kernel<kByInner, kAccumulate, Result>;
     static std::atomic<uint64_t> configured{0};
     if (int status = allow_lds(reinterpret_cast<const void *>(kernel), kLdsBytes, configured)) return status;
     GemmArgs placement{};
@@ -522,12 +544,12 @@ static int launch(const ProductArgs &args, hipStream_t stream) {
     return FM_OK;
 }
 
-template <bool kByInner>
+template <bool kByInner, bool kAccumulate>
 static int launch(const ProductArgs &args, hipStream_t stream) {
     switch (args.out_dtype) {
-        case FM_DTYPE_F32: return launch<kByInner, float>(args, stream);
-        case FM_DTYPE_BF16: return launch<kByInner, bf16_t>(args, stream);
-        default: return launch<kByInner, f16_t>(args, stream);
+        case FM_DTYPE_F32: return launch<kByInner, kAccumulate, float>(args, stream);
+        case FM_DTYPE_BF16: return launch<kByInner, kAccumulate, bf16_t>(args, stream);
+        default: return launch<kByInner, kAccumulate, f16_t>(args, stream);
     }
 }
 
@@ -541,7 +563,8 @@ bool tile_product_takes(const ProductArgs &args) {
 }
 
 int tile_product(const ProductArgs &args, hipStream_t stream) {
-    return args.by_inner ? tiles::launch<true>(args, stream) : tiles::launch<false>(args, stream);
+    if (!args.by_inner) return tiles::launch<false, false>(args, stream);
+    return args.accumulate ? tiles::launch<true, true>(args, stream) : tiles::launch<true, false>(args, stream);
 }
 
 }  // namespace block
