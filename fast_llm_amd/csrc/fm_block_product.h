@@ -24,9 +24,48 @@ struct ProductArgs {
     int index_dtype;
 };
 
+using mx::i32x8_t;
+
+// D[m][n] += sum over 64 k of A[m][k] 2^sa B[n][k] 2^sb: lane l holds row l % 32 of both, 16 bytes of each of two blocks of 32 k. Of D it holds column
+// n = l % 32, rows m = 8 (i / 4) + 4 (l / 32) + i % 4.
+__device__ __forceinline__ f32x16_t multiply(const u32x4_t (&a)[2], const u32x4_t (&b)[2], uint32_t scale_a, uint32_t scale_b, f32x16_t c) {
+    const auto wide = [](const u32x4_t (&v)[2]) {
+        return i32x8_t{static_cast<int>(v[0][0]), static_cast<int>(v[0][1]), static_cast<int>(v[0][2]), static_cast<int>(v[0][3]),
+                       static_cast<int>(v[1][0]), static_cast<int>(v[1][1]), static_cast<int>(v[1][2]), static_cast<int>(v[1][3])};
+    };
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 0, 0, 0, static_cast<int>(scale_a), 0, static_cast<int>(scale_b));
+}
+
+// The same value, computed no earlier than where this stands.
+__device__ __forceinline__ uint32_t here(uint32_t value) {
+    asm volatile("" : "+s"(value));
+    return value;
+}
+
+// Results in fp32 are summed as exactly: the matrix instruction of 8 bits aligns the 64 products that it adds to the largest and drops what lies under
+// 2^-17 of it, 1.5e-5 of a sum of normal values, which a result of 16 bits does not show. For them the operands become bf16 on their way to the matrix
+// units, scales included, which loses nothing (but below 2^-126), and the products of those are exact in fp32: half the rate.
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
+__device__ __forceinline__ f32x16_t multiply_wide(u32x4_t a, u32x4_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// Two neighbours of a word of four elements; `scale`: the byte as an exponent, all of a NaN.
+template <int kPair>
+__device__ __forceinline__ uint32_t widened(uint32_t word, uint32_t scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, __builtin_bit_cast(float, scale), kPair != 0));
+}
+__device__ __forceinline__ uint32_t wide_scale(uint32_t byte) { return byte << 23 | (byte == 255u ? 1u << 22 : 0u); }
+
 // Many rows per expert (fm_block_tiles.hip).
 int tile_product(const ProductArgs &args, hipStream_t stream);
 bool tile_product_takes(const ProductArgs &args);
+// Few rows per expert, by rows (fm_block_stream.hip).
+int stream_product(const ProductArgs &args, hipStream_t stream);
+bool stream_product_takes(const ProductArgs &args);
+// How many wavefronts share a reduction there: 1, 4 or 8.
+int stream_split(const ProductArgs &args);
+// Which of them a product by rows runs on (fm_block_product.hip).
+bool runs_on_tiles(const ProductArgs &args);
 
 }  // namespace block
 

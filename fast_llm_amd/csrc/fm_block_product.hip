@@ -24,6 +24,18 @@ int check_result(const char *name, const void *out, int64_t columns, int64_t out
 
 }  // namespace
 
+bool block::runs_on_tiles(const ProductArgs &args) {
+    // The tiles read the weights once, at 4 TB/s where little is multiplied and there is a tile for every CU; with few rows the weights are read once per 32 rows of
+    // an expert, at up to 6. So it depends on how many experts have over 32 rows, and on the tiles. Measured in us, few rows | tiles, with tokens
+    // at random: 8 experts 4096 -> 2 x 14336, 1 token 42 | 60, 8 rows per expert 153 | 234, 24 rows 197 | 238; 14336 -> 4096 22 | 112, 80 | 164, 103 | 165; 64
+    // experts 2048 -> 2 x 1408, 8 rows 65 | 83, 24 rows 84 | 87; 128 experts 2048 -> 2 x 768, 70 | 86 and 100 | 91. One expert, 4096 -> 28672 (112 tiles): 32 rows 31 | 50, 48 rows
+    // 54 | 50; 14336 -> 4096 (16 tiles): 128 rows 98 | 155, 192 rows 145 | 150. Of a map the host knows the rows with up to 128 of padding per expert; without
+    // one it knows them exactly.
+    const int64_t tiles = (args.columns + 255) / 256 * args.experts, times = std::min(std::max(80 / tiles, int64_t(1)), int64_t(5));
+    const bool many = args.rows > (args.expert_ends != nullptr ? 128 + 24 * times : 32 * times) * args.experts;
+    return (many || !stream_product_takes(args)) && tile_product_takes(args);
+}
+
 extern "C" int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                                       const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
                                       int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int out_dtype, int index_dtype,
@@ -45,8 +57,9 @@ extern "C" int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, c
     args.out_stride = out_stride, args.rows = rows, args.columns = columns, args.inner = padded, args.experts = num_experts, args.out_dtype = out_dtype;
     args.out_vectors = aligned16(out) && out_stride * dtype_size(out_dtype) % 16 == 0;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
-    if (!block::tile_product_takes(args)) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
-    if (int status = block::tile_product(args, static_cast<hipStream_t>(stream))) return status;
+    const bool tiles = block::runs_on_tiles(args);
+    if (!(tiles ? block::tile_product_takes(args) : block::stream_product_takes(args))) return fail(FM_ERR_UNSUPPORTED, "%s: too large", name);
+    if (int status = tiles ? block::tile_product(args, static_cast<hipStream_t>(stream)) : block::stream_product(args, static_cast<hipStream_t>(stream))) return status;
     return check_launch(name);
 }
 
