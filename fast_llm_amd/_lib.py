@@ -109,7 +109,7 @@ SIGNATURES: dict[str, tuple] = {
     "fm_block_transpose": (_c_int, [_c_ptr] * 6 + [_c_i64] * 7 + [_c_int] + [_c_ptr]),
     "fm_block_dequantize": (_c_int, [_c_ptr] * 3 + [_c_i64] * 4 + [_c_int] + [_c_ptr]),
     "fm_block_copy_dense_to_sparse": (_c_int, [_c_ptr] * 5 + [_c_i64] * 7 + [_c_int] + [_c_ptr]),
-    "fm_block_sparse_matmul": (_c_int, [_c_ptr] * 7 + [_c_i64] * 9 + [_c_int] * 2 + [_c_ptr]),
+    "fm_block_sparse_matmul": (_c_int, [_c_ptr] * 7 + [_c_i64] * 9 + [_c_int] * 3 + [_c_ptr]),
     "fm_block_input_row_sparse_matmul": (_c_int, [_c_ptr] * 7 + [_c_i64] * 9 + [_c_int] * 3 + [_c_ptr]),
     "fm_block_activation_forward": (_c_int, [_c_ptr] * 7 + [_c_i64] * 6 + [_c_int] * 4 + [_c_ptr]),
     "fm_block_activation_backward": (_c_int, [_c_ptr] * 11 + [_c_i64] * 9 + [_c_int] * 4 + [_c_ptr]),

@@ -38,8 +38,8 @@ bool block::runs_on_tiles(const ProductArgs &args) {
 
 extern "C" int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                                       const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
-                                      int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int out_dtype, int index_dtype,
-                                      void *stream) {
+                                      int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int exact_sums, int out_dtype,
+                                      int index_dtype, void *stream) {
     const char *name = "fm_block_sparse_matmul";
     if (int status = check_sizes(name, rows, columns, inner, num_experts, out_dtype)) return status;
     block::RowMap map;
@@ -55,6 +55,7 @@ extern "C" int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, c
     args.weight = static_cast<const uint8_t *>(rhs), args.weight_scales = static_cast<const uint8_t *>(rhs_scales), args.out = out;
     args.x_stride = lhs_stride, args.x_scale_stride = lhs_scale_stride, args.weight_stride = rhs_stride, args.weight_scale_stride = rhs_scale_stride;
     args.out_stride = out_stride, args.rows = rows, args.columns = columns, args.inner = padded, args.experts = num_experts, args.out_dtype = out_dtype;
+    args.exact = exact_sums != 0;
     args.out_vectors = aligned16(out) && out_stride * dtype_size(out_dtype) % 16 == 0;
     args.expert_ends = expert_ends, args.expert_pad_begins = expert_pad_begins, args.index_dtype = index_dtype;
     const bool tiles = block::runs_on_tiles(args);

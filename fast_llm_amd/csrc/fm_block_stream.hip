@@ -183,7 +183,7 @@ bool stream_product_takes(const ProductArgs &args) {
            (args.columns + 31) / 32 < (int64_t(1) << 22);
 }
 
-int stream_product(const ProductArgs &args, hipStream_t stream) { return args.out_dtype == FM_DTYPE_F32 ? launch<true>(args, stream) : launch<false>(args, stream); }
+int stream_product(const ProductArgs &args, hipStream_t stream) { return args.out_dtype == FM_DTYPE_F32 || args.exact ? launch<true>(args, stream) : launch<false>(args, stream); }
 
 }  // namespace block
 

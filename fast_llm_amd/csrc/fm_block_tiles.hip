@@ -172,9 +172,8 @@ struct Places {
     }
 };
 
-template <bool kByInner, bool kAccumulate, typename Result>
+template <bool kByInner, bool kAccumulate, bool kWide, typename Result>
 __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, GemmArgs placement) {
-    constexpr bool kWide = std::is_same<Result, float>::value;
     extern __shared__ __attribute__((aligned(1024))) char lds_generic[];
     const int lds = static_cast<int>(reinterpret_cast<uintptr_t>((FM_LDS(char) *)lds_generic));
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -498,9 +497,9 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     wait_for_memory<0>();  // zeros behind the last tile
 }
 
-template <bool kByInner, bool kAccumulate, typename Result>
+template <bool kByInner, bool kAccumulate, bool kWide, typename Result>
 static int launch(const ProductArgs &args, hipStream_t stream) {
-    const auto kernel = tile_kernel<kByInner, kAccumulate, Result>;
+    const auto kernel = tile_kernel<kByInner, kAccumulate, kWide, Result>;
     static std::atomic<uint64_t> configured{0};
     if (int status = allow_lds(reinterpret_cast<const void *>(kernel), kLdsBytes, configured)) return status;
     GemmArgs placement{};
@@ -512,13 +511,9 @@ static int launch(const ProductArgs &args, hipStream_t stream) {
     return FM_OK;
 }
 
-template <bool kByInner, bool kAccumulate>
-static int launch(const ProductArgs &args, hipStream_t stream) {
-    switch (args.out_dtype) {
-        case FM_DTYPE_F32: return launch<kByInner, kAccumulate, float>(args, stream);
-        case FM_DTYPE_BF16: return launch<kByInner, kAccumulate, bf16_t>(args, stream);
-        default: return launch<kByInner, kAccumulate, f16_t>(args, stream);
-    }
+template <bool kByInner, bool kAccumulate, bool kWide>
+static int launch_half(const ProductArgs &args, hipStream_t stream) {
+    return args.out_dtype == FM_DTYPE_BF16 ? launch<kByInner, kAccumulate, kWide, bf16_t>(args, stream) : launch<kByInner, kAccumulate, kWide, f16_t>(args, stream);
 }
 
 }  // namespace tiles
@@ -531,8 +526,14 @@ bool tile_product_takes(const ProductArgs &args) {
 }
 
 int tile_product(const ProductArgs &args, hipStream_t stream) {
-    if (!args.by_inner) return tiles::launch<false, false>(args, stream);
-    return args.accumulate ? tiles::launch<true, true>(args, stream) : tiles::launch<true, false>(args, stream);
+    using namespace tiles;
+    const bool wide = args.out_dtype == FM_DTYPE_F32;
+    if (!args.by_inner) {
+        if (wide) return launch<false, false, true, float>(args, stream);
+        return args.exact ? launch_half<false, false, true>(args, stream) : launch_half<false, false, false>(args, stream);
+    }
+    if (args.accumulate) return wide ? launch<true, true, true, float>(args, stream) : launch_half<true, true, false>(args, stream);
+    return wide ? launch<true, false, true, float>(args, stream) : launch_half<true, false, false>(args, stream);
 }
 
 }  // namespace block

@@ -557,12 +557,14 @@ int fm_block_copy_dense_to_sparse(const void *values, const void *scales, const 
                                   int64_t scale_stride, int64_t out_scale_stride, int index_dtype, void *stream);
 
 /* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs has `columns` rows of `inner` per expert. Both layers of an expert MLP and
- * both input gradients are such products. Sums in fp32 (of 64 products at a time, as fm_mx_sparse_matmul says), one rounding. Only the rows that tokens have are
- * written, those of lhs that none has are not looked at, and experts may begin anywhere. `out_stride` in elements. Without a map there is one expert. */
+ * both input gradients are such products. Sums in fp32, one rounding. For results of 16 bits the matrix instruction aligns eight products to the largest of them and
+ * drops what lies 14 bits under it: a sum of normal values is 1.5e-5 of itself off. Results in fp32, and with `exact_sums` those of 16 bits, are summed as exactly
+ * as fp32, at half the rate. Only the rows that tokens have are written, those of lhs that none has are not looked at, and experts may begin anywhere. `out_stride`
+ * in elements. Without a map there is one expert. */
 int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                            const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
-                           int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int out_dtype, int index_dtype,
-                           void *stream);
+                           int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int exact_sums, int out_dtype,
+                           int index_dtype, void *stream);
 /* The weights' gradients: out[e rows + i, j] (=, or += with `accumulate`) sum over the rows k of expert e of lhs[i, k] * rhs[j, k], lhs [rows, inner] and rhs
  * [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens have zeros. */
 int fm_block_input_row_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
