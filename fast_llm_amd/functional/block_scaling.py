@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from fast_llm_amd import _lib
-from fast_llm_amd.functional.config import MAX_DROPLESS_BLOCK_SIZE_ROW, ActivationType
+from fast_llm_amd.functional.config import ActivationType
 from fast_llm_amd.functional.mlp import _activation_tag
 from fast_llm_amd.functional.sparse_copy import (
     SparseMap,
@@ -442,7 +442,7 @@ def block_mlp(
     the activation's gradient and of the input's per slot are rounded to the input's type, sums are in fp32. Differentiable once.
     Gated, ffn is a multiple of 128.
     """
-    refuse_traced(input_, scores)
+    refuse_traced(input_, scores, weight_1, weight_2)
     Assert.eq(input_.dim(), 2)
     hidden, experts = input_.size(1), sparse_map.num_experts
     ffn = div(weight_2.size(0), experts)

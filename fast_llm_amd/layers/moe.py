@@ -12,6 +12,7 @@ import copy
 
 import torch
 
+from fast_llm_amd.functional.block_scaling import BLOCK, BlockScaledWeights, block_mlp, block_quantize_expert_weights
 from fast_llm_amd.functional.config import ActivationType, MLPRecomputeLevel
 from fast_llm_amd.functional.microscaling import (
     MicroscaledTensor,
@@ -314,6 +315,55 @@ class DroplessMoEMLP(torch.nn.Module):
             out[f"{prefix}experts.{i}.w3.weight"] = up.clone()
             out[f"{prefix}experts.{i}.w2.weight"] = down.t().contiguous()
         return out
+
+
+class BlockScaledMoEMLP(DroplessMoEMLP):
+    """
+    `DroplessMoEMLP`, with its options and its parameters by the same names, whose expert products are of 8 bits with a scale for each block of 128 in training and in
+    inference (`block_mlp`). Routing, router and scores are the layer's own, on the unquantised input. It keeps 8 bits per value of each slot's input and
+    of the first layer's output for the backward, whatever there is to recompute. `forward` quantises the weights; where they stay the same over several
+    calls (micro-batches of a step, serving) `weights = layer.quantize_weights()` does so once, for `layer(input_, weights=weights)`.
+    """
+
+    def __init__(self, hidden_size: int, intermediate_size: int, experts: int, experts_per_token: int, *, gated: bool = True,
+                 recompute_level: MLPRecomputeLevel = MLPRecomputeLevel.none, **options):  # fmt: skip
+        if gated and intermediate_size % BLOCK != 0:
+            raise NotImplementedError(f"a gated activation has whole blocks of {BLOCK} columns, not {intermediate_size}")
+        if recompute_level != MLPRecomputeLevel.none:
+            raise NotImplementedError("what the layer keeps for its backward is settled: there is nothing to recompute")
+        super().__init__(hidden_size, intermediate_size, experts, experts_per_token, gated=gated, **options)
+
+    def quantize_weights(self) -> BlockScaledWeights:
+        """The expert weights as they are now."""
+        return block_quantize_expert_weights(self.layer_1, self.layer_2, self.experts)
+
+    def forward(
+        self,
+        input_: torch.Tensor,
+        scores: torch.Tensor | None = None,
+        top_experts: torch.Tensor | None = None,
+        *,
+        grad_scale: float | None = None,
+        losses: dict | None = None,
+        weights: BlockScaledWeights | None = None,
+    ) -> torch.Tensor:
+        hidden_states, router_counts = input_.flatten(0, -2), None
+        if top_experts is None:
+            scores, top_experts, router_counts = self.route_with_counts(hidden_states, grad_scale, losses)
+        sparse_map = get_sparse_map(
+            top_experts, self.experts, dynamic_shape=self.dropless_dynamic_shape, router_counts=router_counts
+        )
+        return block_mlp(
+            hidden_states,
+            scores,
+            self.layer_1,
+            self.layer_2,
+            weights,
+            gated=self.gated,
+            activation_type=self.activation,
+            sparse_map=sparse_map,
+            training=self.training,
+        ).view_as(input_)
 
 
 class MicroscaledMoEMLP(torch.nn.Module):

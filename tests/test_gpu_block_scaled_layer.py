@@ -1,0 +1,325 @@
+"""The layer on values of 8 bits with a scale per block of 128, its operators as they are used, one after the other, and how they are called."""
+
+import pytest
+import torch
+
+from fast_llm_amd.functional.block_scaling import (
+    block_activation_backward, block_activation_forward, block_copy_dense_to_sparse, block_dequantize, block_input_row_sparse_matmul, block_mlp,
+    block_quantize, block_quantize_both, block_quantize_expert_weights, block_quantize_transposed, block_sparse_matmul,
+)  # fmt: skip
+from fast_llm_amd.functional.sparse_copy import copy_dense_to_sparse_backward, copy_sparse_to_dense, copy_sparse_to_dense_backward, get_sparse_map
+from fast_llm_amd.layers.moe import BlockScaledMoEMLP, DroplessMoEMLP, attach_grad_buffer
+from oracle import block_oracle
+from tests.test_gpu_block_scaling import MLP_TOLERANCE, _difference, _map, _mlp_inputs, _values
+
+pytestmark = pytest.mark.gpu
+
+
+def _layer(device, **options):
+    torch.manual_seed(0)
+    return BlockScaledMoEMLP(512, 640, 8, 2, device=device, **options)
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return torch.equal(a.detach(), b.detach())
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 1500])
+@pytest.mark.parametrize(
+    "options", [{}, {"shared_experts": 1, "gated": False, "full_precision_gradients": True}, {"router_per_expert_scale": True, "dropless_dynamic_shape": True}], ids=str
+)
+def test_layer_is_its_operators_one_after_the_other(tokens, options, device):
+    layer = _layer(device, **options)
+    x = torch.randn(tokens, 512, device=device).bfloat16().requires_grad_(True)
+    grad = torch.randn(tokens, 512, device=device).bfloat16()
+    output = layer(x)
+    output.backward(grad)
+    with torch.no_grad():
+        scores, top_experts = layer.route(x)
+        sparse_map = get_sparse_map(top_experts, layer.experts, dynamic_shape=layer.dropless_dynamic_shape)
+        weights, gated, activation = layer.quantize_weights(), layer.gated, layer.activation
+        rows = block_copy_dense_to_sparse(block_quantize(x), sparse_map)
+        layer_1 = block_sparse_matmul(rows, weights.layer_1, sparse_map, exact_sums=True)
+        hidden, checkpoint = block_activation_forward(layer_1, gated, activation, sparse_map)
+        layer_2 = block_sparse_matmul(hidden, weights.layer_2_transposed, sparse_map)
+        assert _same(output, copy_sparse_to_dense(layer_2, scores, sparse_map))
+        grad_2, _ = copy_sparse_to_dense_backward(grad, (sparse_map, layer_2, scores))
+        grad_rows, grad_columns = block_quantize_both(grad_2, sparse_map=sparse_map)
+        grad_hidden = block_sparse_matmul(grad_rows, weights.layer_2, sparse_map, exact_sums=True)
+        grad_1, grad_1_columns, hidden_columns = block_activation_backward(grad_hidden, checkpoint, gated, activation, sparse_map)
+        dtype = layer.layer_2.grad_buffer.dtype
+        assert _same(layer.layer_2.grad_buffer, block_input_row_sparse_matmul(hidden_columns, grad_columns, sparse_map, dtype=dtype))
+        rows_columns = block_quantize_transposed(rows, sparse_map=sparse_map)
+        assert _same(layer.layer_1.grad_buffer, block_input_row_sparse_matmul(grad_1_columns, rows_columns, sparse_map, dtype=dtype))
+        grad_x = copy_dense_to_sparse_backward(block_sparse_matmul(grad_1, weights.layer_1_transposed, sparse_map), (sparse_map, x.shape))
+        # Of the input's gradient the router has a part of its own.
+    pinned = x.detach().clone().requires_grad_(True)
+    again = layer(pinned, scores=scores, top_experts=top_experts, weights=weights)
+    assert _same(again, output)
+    again.backward(grad)
+    assert _same(pinned.grad, grad_x)
+    assert layer.router.grad is not None and layer.router.grad.any()
+    # Against the layer in 16 bits: each rounding to e4m3 is 2^-4 / sqrt(3) = 0.036 of a value or less in the root mean square. The results of layer 1 have two of them behind them
+    # (0.051), a product of two such 0.072, and with its own rounding and layer 2's weights the output has 0.09. The input's gradient has the
+    # same but for one on its way from the other end, and two more: 0.1.
+    plain = DroplessMoEMLP(512, 640, 8, 2, device=device, **options)
+    plain.load_state_dict(layer.state_dict())
+    other = x.detach().clone().requires_grad_(True)
+    full = plain(other, scores=scores, top_experts=top_experts)
+    full.backward(grad)
+    for ours, theirs in ((output, full), (pinned.grad, other.grad)):
+        assert _difference(ours, theirs.detach().cpu().double()) <= 0.15
+
+
+def test_layer_in_inference_and_under_two_batches(device):
+    layer = _layer(device)
+    x = torch.randn(3, 17, 512, device=device).bfloat16()
+    trained = layer(x)
+    weights = layer.quantize_weights()
+    layer.eval()
+    output = layer(x, weights=weights)
+    assert output.shape == x.shape and _same(output, trained)
+    with pytest.raises(RuntimeError, match="inference"):
+        output.sum().backward()
+    with torch.no_grad():
+        assert not layer(x).requires_grad
+        layer.layer_1.zero_()
+    assert not layer(x).any() and _same(layer(x, weights=weights), output)  # the weights as they are, or as they were given
+    layer.train()
+    losses = {}
+    for _ in range(2):
+        layer(x, grad_scale=1.0, losses=losses, weights=weights).sum().backward()
+    assert all(len(values) == 2 for values in losses.values()) and not layer.layer_1.param_grad_is_zero
+    with pytest.raises(ValueError, match="no tokens"):  # as the layer itself
+        layer(x[:0])
+
+
+def _step(device, tokens=150, dtype=torch.bfloat16, grad_dtype=None, gated=True):
+    """Inputs of an MLP and what one step of it gives."""
+    input_, scores, top_experts, weight_1, weight_2, grad = (t.to(device) for t in _mlp_inputs(tokens, 256, 384, 4, 2, gated, dtype, device, seed=5))
+    weights = [attach_grad_buffer(w.requires_grad_(True), grad_dtype) for w in (weight_1, weight_2)]
+    x, s = input_.requires_grad_(True), scores.requires_grad_(True)
+
+    def step(x=x, s=s, grad=grad, weights=weights, quantized=None):
+        x.grad = s.grad = None
+        for weight in weights:
+            weight.param_grad_is_zero = True
+        output = block_mlp(x, s, *weights, quantized, gated=gated, activation_type="silu", sparse_map=get_sparse_map(top_experts, 4))
+        output.backward(grad)
+        return [t.detach().clone() for t in (output, x.grad, s.grad, *(w.grad_buffer for w in weights if w.requires_grad))]
+
+    return step, x, s, grad, weights, top_experts
+
+
+def test_mlp_of_other_layouts_types_and_frozen_weights(device):
+    step, x, s, grad, weights, top_experts = _step(device)
+    expected = step()
+    assert all(_same(a, b) for a, b in zip(step(), expected))  # nothing depends on the order of anything
+    wide = torch.zeros(150, 300, dtype=torch.bfloat16, device=device)
+    wide[:, 3:259] = x.detach()
+    strided = wide[:, 3:259].requires_grad_(True)
+    scores = s.detach().t().contiguous().t().requires_grad_(True)
+    assert all(_same(a, b) for a, b in zip(step(strided, scores, grad.t().contiguous().t()), expected))
+    # A gradient that is one row for all.
+    one = grad[:1].expand(150, 256)
+    assert all(_same(a, b) for a, b in zip(step(grad=one), step(grad=one.contiguous())))
+    # Weights that lie in wider rows, or transposed.
+    others = [attach_grad_buffer(w.detach().t().contiguous().t().requires_grad_(True)) for w in weights]
+    for weight in others:
+        weight.grad_buffer = torch.empty(weight.shape, dtype=weight.dtype, device=device)
+    assert all(_same(a, b) for a, b in zip(step(weights=others), expected))
+    # What needs no gradient has none and changes nothing else.
+    weights[0].requires_grad_(False)
+    weights[0].grad_buffer.fill_(7)
+    ours = step()
+    assert _same(ours[3], expected[4]) and all(_same(a, b) for a, b in zip(ours[:3], expected)) and (weights[0].grad_buffer == 7).all()
+    output = block_mlp(x.detach(), s.detach(), *weights, gated=True, activation_type="silu", sparse_map=get_sparse_map(top_experts, 4))
+    weights[1].param_grad_is_zero = True
+    output.backward(grad)
+    assert x.grad is not None and _same(weights[1].grad_buffer, expected[4])
+    # Once, and not twice through the same graph.
+    y = x.detach().requires_grad_(True)
+    output = block_mlp(y, s, *weights, gated=True, activation_type="silu", sparse_map=get_sparse_map(top_experts, 4))
+    (first,) = torch.autograd.grad(output, y, grad, create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("grad_dtype", [torch.float32, torch.bfloat16])
+def test_gradients_in_buffers_of_their_own_type(dtype, grad_dtype, device):
+    step, x, s, grad, weights, top_experts = _step(device, dtype=dtype, grad_dtype=grad_dtype)
+    ours = step()
+    expected = block_oracle.mlp_step(
+        *(t.detach().cpu() for t in (x, s, top_experts, *weights)), 4, True, "silu", grad.cpu(), dtype
+    )
+    for name, value in zip(("output", "grad_input", "grad_scores", "grad_weight_1", "grad_weight_2"), ours):
+        assert _difference(value, expected[name]) <= MLP_TOLERANCE, name
+    assert ours[3].dtype == grad_dtype
+
+
+def test_on_another_stream(device):
+    step, *_ = _step(device)
+    expected = step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ours = [step() for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(stream)
+    for each in ours:
+        assert all(_same(a, b) for a, b in zip(each, expected))
+
+
+def test_step_replays_from_a_graph(device):
+    """Forward and backward of the MLP, captured once and replayed on other inputs with eager steps in between."""
+    tokens, inputs = 150, [_mlp_inputs(150, 256, 384, 4, 2, True, torch.bfloat16, device, seed=seed) for seed in range(3)]
+    weights = [attach_grad_buffer(w.to(device).requires_grad_(True)) for w in inputs[0][3:5]]
+
+    def run(x, s, top_experts, grad):
+        for weight in weights:
+            weight.param_grad_is_zero = True
+        output = block_mlp(x, s, *weights, gated=True, activation_type="silu", sparse_map=get_sparse_map(top_experts, 4))
+        return output, *torch.autograd.grad(output, (x, s), grad), *(w.grad_buffer for w in weights)
+
+    def arguments(i):
+        x, s, top_experts, *_, grad = (t.to(device) for t in inputs[i])
+        return x.requires_grad_(True), s.requires_grad_(True), top_experts, grad
+
+    eager = [[t.detach().clone() for t in run(*arguments(i))] for i in range(3)]
+    static = arguments(0)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(*static)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(*static)
+    for _ in range(2):
+        for i in (1, 2, 0):
+            with torch.no_grad():
+                for target, source in zip(static, arguments(i)):
+                    target.copy_(source)
+            for weight in weights:
+                weight.grad_buffer.fill_(float("nan"))
+            graph.replay()
+            assert all(_same(a, b) for a, b in zip(captured, eager[i]))
+            torch.cuda.synchronize()
+            assert all(_same(a, b) for a, b in zip(run(*arguments(1)), eager[1]))
+
+
+# ---- the products ----------------------------------------------------------------------------------------
+# Sums that lose nothing but fp32's own roundings: of `inner` products, each exact, 2^-24 sum |lhs rhs| for each of the additions at most (the matrix instruction adds 16
+# products at a time to the sum so far, and those to each other), and the result's own rounding.
+def _exact_tolerance(lhs, rhs, expected, dtype):
+    return 2.0**-24 * lhs.size(1) * (lhs.abs() @ rhs.abs().t()) + torch.finfo(dtype).eps / 2 * expected.abs() + 1e-38
+
+
+@pytest.mark.parametrize("counts", [[40, 3], [300, 257]], ids=str)
+@pytest.mark.parametrize(("inner", "columns"), [(200, 70), (1024, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_exact_sums_keep_small_terms_beside_large_ones(counts, inner, columns, dtype, device):
+    """Pairs of large terms that cancel in between small ones: what the instruction of 8 bits by itself drops."""
+    generator = torch.Generator().manual_seed(inner + columns)
+    sparse_map = _map(counts, device)
+    rows, experts = sparse_map.num_rows, len(counts)
+    lhs, rhs = torch.randn(rows, inner, generator=generator), torch.randn(experts * columns, inner, generator=generator)
+    lhs[:, ::8], lhs[:, 1::8], rhs[:, ::8], rhs[:, 1::8] = 400.0, 400.0, 4.0, -4.0
+    a, b = block_quantize(lhs.to(device)), block_quantize(rhs.to(device))
+    x, w = _values(a), _values(b)
+    out = block_sparse_matmul(a, b, sparse_map, dtype=dtype, exact_sums=True).cpu().double()
+    for expert, (count, weight) in enumerate(zip(counts, w.split(columns))):
+        begin = sum(-(-c // 128) * 128 for c in counts[:expert])
+        part = slice(begin, begin + count)
+        expected = x[part] @ weight.t()
+        assert ((out[part] - expected).abs() <= _exact_tolerance(x[part], weight, expected, dtype)).all()
+
+
+@pytest.mark.parametrize(("experts", "most"), [(130, 300), (1024, 4)])
+def test_many_experts(experts, most, device):
+    generator = torch.Generator().manual_seed(experts)
+    counts = torch.randint(0, most, (experts,), generator=generator).tolist()
+    counts[7], counts[-1] = 300, 2
+    sparse_map = _map(counts, device, phantom=128)
+    lhs = torch.randint(-4, 5, (sparse_map.num_rows, 256), generator=generator).float()
+    rhs = torch.randint(-4, 5, (experts * 48, 256), generator=generator).float()
+    x, w = block_quantize(lhs.to(device)), block_quantize(rhs.to(device))
+    index = torch.repeat_interleave(torch.arange(experts), torch.tensor([-(-c // 128) * 128 for c in counts]))
+    real = torch.cat([torch.arange(-(-c // 128) * 128) < c for c in counts])
+    rows = torch.nonzero(real).squeeze(1)
+    expected = (lhs[rows, None] @ rhs.view(experts, 48, 256)[index[rows]].mT.contiguous()).squeeze(1)
+    for exact in (False, True):
+        out = torch.full((sparse_map.num_rows, 48), -7.0, device=device)
+        block_sparse_matmul(x, w, sparse_map, out=out, exact_sums=exact)
+        assert torch.equal(out.cpu()[rows], expected)
+        out[rows.to(device)] = -7
+        assert (out == -7).all()
+    left, right = (block_quantize_transposed(t[:, :size].contiguous().to(device), sparse_map=sparse_map) for t, size in ((lhs, 40), (lhs, 72)))
+    gradient = block_input_row_sparse_matmul(left, right, sparse_map, dtype=torch.float32).cpu().view(experts, 40, 72)
+    whole = torch.where(torch.nn.functional.pad(real, (0, 128))[:, None], lhs, 0.0)
+    begin = 0
+    for expert, count in enumerate(counts):
+        part = whole[begin : begin + count]
+        assert torch.equal(gradient[expert], part[:, :40].t() @ part[:, :72]), expert
+        begin += -(-count // 128) * 128
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("counts", [[33], [290]], ids=str)
+def test_blocks_of_nan_with_exact_sums(counts, dtype, device):
+    sparse_map = _map(counts, device)
+    x, w = torch.ones(sparse_map.num_rows, 300), torch.ones(70, 300)
+    x[5, 130], w[11, 299] = float("nan"), float("inf")
+    out = block_sparse_matmul(block_quantize(x.to(device)), block_quantize(w.to(device)), sparse_map, dtype=dtype, exact_sums=True).cpu().float()
+    expected = torch.full((counts[0], 70), 300.0)
+    expected[5], expected[:, 11] = float("nan"), float("nan")
+    assert torch.equal(out[: counts[0]].nan_to_num(-1), expected.nan_to_num(-1))
+
+
+def test_operators_replay_from_a_graph(device):
+    generator = torch.Generator().manual_seed(3)
+    sparse_map = _map([200, 0, 30], device)
+    inputs = [torch.randn(sparse_map.num_rows, 512, generator=generator).to(device) for _ in range(3)]
+    weight = block_quantize(torch.randn(3 * 64, 512, generator=generator).to(device))
+    total = torch.zeros(3 * 512, 256, device=device)
+
+    def run(x):
+        rows, columns = block_quantize_both(x, sparse_map=sparse_map)
+        product = block_sparse_matmul(rows, weight, sparse_map, out=torch.zeros(sparse_map.num_rows, 64, device=device))
+        output, checkpoint = block_activation_forward(x, True, "gelu", sparse_map)
+        back = block_activation_backward(x[:, :256], checkpoint, True, "gelu", sparse_map)
+        return block_dequantize(rows), product, block_dequantize(output), block_dequantize(back[0]), block_input_row_sparse_matmul(
+            columns, back[2], sparse_map, out=total.zero_(), accumulate=True
+        )
+
+    eager = [[t.clone() for t in run(x)] for x in inputs]
+    static = inputs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(static)
+    for _ in range(3):
+        for x, expected in zip(inputs, eager):
+            static.copy_(x)
+            graph.replay()
+            assert all(_same(a, b) for a, b in zip(captured, expected))
+            torch.cuda.synchronize()
+
+
+def test_nothing_to_do(device):
+    empty = torch.empty(0, 256, device=device)
+    assert block_quantize(empty).shape == (0, 256)
+    rows, columns = block_quantize_both(empty)
+    assert rows.shape == (0, 256) and columns.shape == (256, 1) and not columns.values.any() and not block_dequantize(columns).any()
+    assert block_sparse_matmul(rows, block_quantize(torch.ones(5, 256, device=device))).shape == (0, 5)
+    output, checkpoint = block_activation_forward(empty, True, "silu")
+    assert output.shape == (0, 128) and [t.shape for t in block_activation_backward(empty[:, :128], checkpoint, True, "silu")] == [(0, 256), (256, 1), (128, 1)]
+    # Experts that no token has chosen at all.
+    sparse_map = _map([0, 0], device)
+    lhs, rhs = (block_quantize_transposed(torch.empty(0, size, device=device), sparse_map=sparse_map) for size in (40, 24))
+    assert not block_input_row_sparse_matmul(lhs, rhs, sparse_map).any()
+    out = torch.ones(80, 24, device=device)
+    assert (block_input_row_sparse_matmul(lhs, rhs, sparse_map, out=out, accumulate=True) == 1).all()
+    # One row that stands for all of them.
+    row = torch.randn(1, 300, device=device)
+    for ours, theirs in zip(block_quantize_both(row.expand(200, 300)), block_quantize_both(row.repeat(200, 1))):
+        assert _same(ours.values, theirs.values) and _same(ours.scales[:, : ours.rows], theirs.scales[:, : ours.rows])
