@@ -80,6 +80,7 @@ __device__ __forceinline__ f32x16_t settled(const f32x16_t &sums) {
 template <int kNewest>
 __device__ __forceinline__ void wait_for_memory() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kNewest) : "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0), for the compiler, which does not look into assembly and would wait for later reads with the earlier ones
 }
 
 __device__ __forceinline__ u32x4_t read_lds(int address, int offset) {
@@ -189,38 +190,40 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     if (!places.locate(placement, logical, inner_slices, upcoming)) return;
 
     // ---- loading: the slices of the workgroup's tiles one after the other, the last tile's followed by zeros -----------
-    // `upcoming` is the tile that is loaded. Of every 16 rows a wavefront's load j and load j + 2 have the same swizzle.
+    // `upcoming` is the tile that is loaded. Wavefronts 2 m and 2 m + 1 take turns with 8 rows of the tile's half m, so that a lane has the same unit in all its rows. In two
+    // groups: first the blocks of weight rows but the last of each half, and the first 64 rows of each half of the rows; then the others. (A tile of up to 128 rows, which
+    // both halves of the workgroup share, has 32 rows in place of each 64.)
     const uint32_t x_stride = static_cast<uint32_t>(args.x_stride), weight_stride = static_cast<uint32_t>(args.weight_stride);
-    uint32_t x_offset[2], weight_offset[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int row = wave * kLoads * 8 + j * 8 + (lane >> 3), unit = (lane & 7) ^ ((row >> 1) & 7);
-        x_offset[j] = static_cast<uint32_t>(row) * x_stride + unit * 16;
-        // LDS row 32 c + 8 a + 4 h + b is row 32 c + 16 h + 4 a + b.
-        const int weight_row = wave * kLoads * 8 + (lane >> 5) * 16 + (lane >> 3 & 3);
-        weight_offset[j] = static_cast<uint32_t>(weight_row) * weight_stride + unit * 16;
-    }
+    const int load_row = (wave & 1) * 8 + (lane >> 3), load_unit = (lane & 7) ^ ((load_row >> 1) & 7);
+    const uint32_t x_offset = static_cast<uint32_t>(load_row) * x_stride + load_unit * 16;
+    // LDS row 32 c + 8 a + 4 h + b is row 32 c + 16 h + 4 a + b.
+    const uint32_t weight_offset = static_cast<uint32_t>((wave >> 1) * 128 + (lane >> 5) * 16 + (wave & 1) * 4 + (lane >> 3 & 3)) * weight_stride + load_unit * 16;
     const auto slices_of = [](const Tile &of) { return max(of.slices, kMinSlices); };
-    // Rows of a tile of up to 128 are shared by both halves of the workgroup.
     const auto blocks_of = [](const Tile &of) { return of.rows_valid <= kTile / 2 ? kBlocks / 2 : kBlocks; };
     const auto weight_row_of = [&](const Tile &of) { return (kByInner ? 0 : static_cast<int64_t>(of.expert) * columns) + of.tile_n * kTile; };
     const auto weight_rows_of = [&](const Tile &of) { return min(kTile, columns - of.tile_n * kTile); };
     bool more = true;
-    const uint8_t *x_from = nullptr, *weight_from = nullptr;
-    uint32_t x_bytes = 0, weight_bytes = 0;  // of a slice; none behind the tile's last one
+    const uint8_t *x_from[2] = {}, *weight_from = nullptr;
+    uint32_t x_bytes[2] = {}, weight_bytes = 0;  // of a slice; none behind the tile's last one
     int load_slice = 0, load_slices = 0, real_slices = 0, load_target = lds;
     const auto begin_loads = [&]() {
         const int64_t first = static_cast<int64_t>(upcoming.first_slice) * kSlice;
-        x_from = args.x + upcoming.row0 * args.x_stride + first;
         weight_from = args.weight + weight_row_of(upcoming) * args.weight_stride + first;
         load_slice = 0, load_slices = slices_of(upcoming), real_slices = more ? upcoming.slices : 0;
-        x_bytes = real_slices > 0 ? (upcoming.rows_valid - 1) * x_stride + kSlice : 0;
+        const bool whole = blocks_of(upcoming) == kBlocks;
+#pragma unroll
+        for (int group = 0; group < 2; ++group) {
+            const int row = (wave >> 1) * (whole ? 128 : 64) + group * (whole ? 64 : 32), rows = min(upcoming.rows_valid - row, whole ? 64 : 32);
+            x_from[group] = args.x + (upcoming.row0 + row) * args.x_stride + first;
+            x_bytes[group] = real_slices > 0 && rows > 0 ? (rows - 1) * x_stride + kSlice : 0;
+        }
         weight_bytes = real_slices > 0 ? (weight_rows_of(upcoming) - 1) * weight_stride + kSlice : 0;
     };
     const auto advance = [&]() {
         ++load_slice;
-        x_from += kSlice, weight_from += kSlice;
-        x_bytes = load_slice < real_slices ? x_bytes : 0, weight_bytes = load_slice < real_slices ? weight_bytes : 0;
+        weight_from += kSlice, weight_bytes = load_slice < real_slices ? weight_bytes : 0;
+#pragma unroll
+        for (int group = 0; group < 2; ++group) x_from[group] += kSlice, x_bytes[group] = load_slice < real_slices ? x_bytes[group] : 0;
         load_target = load_target == lds ? lds + kSlotBytes : lds;
     };
     // Scales, a slice further ahead: they come from as many places of memory as there are slices, and are the last to arrive. (As far ahead as the slice
@@ -251,29 +254,35 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         scale_bytes = scale_slice < upcoming.slices ? scale_bytes : 0;
         scale_target = scale_target == scales_at + (kScaleSlots - 1) * kScaleSlotBytes ? scales_at : scale_target + kScaleSlotBytes;
     };
+    constexpr int kItems = 2 * kLoads, kFirstWeights = kLoads / kBlocks * (kBlocks - 1), kFirstItems = kFirstWeights + kLoads / 2;
     const auto load = [&](auto constant) {
-        constexpr int item = decltype(constant)::value, j = item % kLoads;
-        if constexpr (item < kLoads)
-            load_to_lds<kOperandBytes + j * 1024>(buffer_of(weight_from, weight_bytes), weight_offset[j % 2] + (j / 4 * 32 + j % 4 * 4) * here(weight_stride),
-                                                  load_target + wave * (kLoads * 1024));
-        else
-            load_to_lds<j * 1024>(buffer_of(x_from, x_bytes), x_offset[j % 2] + j / 2 * 16 * here(x_stride), load_target + wave * (kLoads * 1024));
+        constexpr int item = decltype(constant)::value, group = item < kFirstItems ? 0 : 1;
+        constexpr bool weights = item < kFirstWeights || item >= kItems - (kLoads - kFirstWeights);
+        const int target = load_target + (wave >> 1) * (128 * kSlice) + (wave & 1) * (8 * kSlice);
+        if constexpr (weights) {
+            constexpr int j = group == 0 ? item : item - (kItems - kLoads);
+            load_to_lds<kOperandBytes + j * 16 * kSlice>(buffer_of(weight_from, weight_bytes), weight_offset + (j / 2 * 32 + j % 2 * 8) * here(weight_stride), target);
+        } else {
+            constexpr int j = (item - kFirstWeights) % (kLoads / 2);
+            load_to_lds<(group * 64 + j * 16) * kSlice>(buffer_of(x_from[group], x_bytes[group]), x_offset + j * 16 * here(x_stride), target);
+        }
     };
-    constexpr int kItems = 2 * kLoads;
 
     // ---- multiplying ---------------------------------------------------------------------------------------------------
     u32x4_t weight_part[2][kBlocks][2], x_part[2][kBlocks][2];
     uint32_t scales[2 * kBlocks], next_scales[2 * kBlocks];
     constexpr int kScales = 2 * kBlocks;
-    int scale_slot = scales_at, x_scales_at = 0, weight_scales_at = 0;  // of the slice whose scales are read, and a lane's places in it
+    int scale_slot = scales_at, x_scales_at[2] = {}, weight_scales_at = 0;  // of the slice whose scales are read, and a lane's places in it
     const auto begin_scale_reads = [&](const Tile &of) {
-        x_scales_at = wave_m * kScaleBytes + (first_x_row(of, wave_m) & 15) + (lane & 31);
+        x_scales_at[0] = wave_m * kScaleBytes + (first_x_row(of, wave_m) & 15) + (lane & 31);
+        x_scales_at[1] = x_scales_at[0] + blocks_of(of) * 16;
         // (The weight row of LDS row `lane % 32`.)
         weight_scales_at = (2 + wave_n) * kScaleBytes + static_cast<int>((weight_row_of(of) + wave_n * 128) & 15) + (lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3);
     };
     const auto read_scale = [&](auto constant) {
         constexpr int item = decltype(constant)::value, block = item % kBlocks;
-        next_scales[item] = *(FM_LDS(uint8_t) *)((FM_LDS(char) *)static_cast<uintptr_t>((item < kBlocks ? weight_scales_at : x_scales_at) + scale_slot) + block * 32);
+        if constexpr (item < kBlocks) next_scales[item] = *(FM_LDS(uint8_t) *)((FM_LDS(char) *)static_cast<uintptr_t>(weight_scales_at + scale_slot) + block * 32);
+        else next_scales[item] = *(FM_LDS(uint8_t) *)((FM_LDS(char) *)static_cast<uintptr_t>(x_scales_at[block / 2] + scale_slot) + block % 2 * 32);
     };
     const auto next_scale_slot = [&]() { scale_slot = scale_slot == scales_at + (kScaleSlots - 1) * kScaleSlotBytes ? scales_at : scale_slot + kScaleSlotBytes; };
     int address[2][2];  // of a lane in a row block, by step and part
@@ -281,22 +290,27 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int p = 0; p < 2; ++p) address[i][p] = (lane & 31) * kSlice + ((4 * i + 2 * p + half) ^ ((lane >> 1) & 7)) * 16;
-    int slot = lds, first_row = 0;  // of the slice that is read, and of the wavefront in the tile that it is of
+    int slot = lds;  // of the slice that is read
     constexpr int kReads = 4 * kBlocks;
     constexpr std::integral_constant<int, 0> kFirst{};
     constexpr std::integral_constant<int, 1> kSecond{};
-    // Where a step's reads start, and by number the reads: the fragments of the wavefront's weight rows, then of its rows.
-    int weight_from_lds[2], x_from_lds[2];
+    // Where the reads of a step start, and by number the reads: the fragments of the wavefront's weight rows, then of its rows.
+    int weight_from_lds[2][2], x_from_lds[2][2];
     const auto begin_reads = [&](auto step_constant) {
         constexpr int i = decltype(step_constant)::value;
-        const int weights_at = static_cast<int>(here(slot + wave_n * 128 * kSlice)), rows_at = static_cast<int>(here(slot + first_row * kSlice));
+        const int weights_at = static_cast<int>(here(slot + wave_n * 128 * kSlice)), rows_at = static_cast<int>(here(slot + wave_m * 128 * kSlice));
 #pragma unroll
-        for (int p = 0; p < 2; ++p) weight_from_lds[p] = address[i][p] + weights_at, x_from_lds[p] = address[i][p] + rows_at;
+        for (int p = 0; p < 2; ++p) weight_from_lds[i][p] = address[i][p] + weights_at, x_from_lds[i][p] = address[i][p] + rows_at;
     };
     const auto read = [&](auto constant, auto step_constant) {
         constexpr int item = decltype(constant)::value, i = decltype(step_constant)::value, p = item % 2, block = item / 2 % kBlocks;
-        if constexpr (item < 2 * kBlocks) weight_part[i][block][p] = read_lds(weight_from_lds[p], kOperandBytes + block * 32 * kSlice);
-        else x_part[i][block][p] = read_lds(x_from_lds[p], block * 32 * kSlice);
+        if constexpr (item < 2 * kBlocks) weight_part[i][block][p] = read_lds(weight_from_lds[i][p], kOperandBytes + block * 32 * kSlice);
+        else x_part[i][block][p] = read_lds(x_from_lds[i][p], block * 32 * kSlice);
+    };
+    // The same by their use in the narrow loop: four reads are a block of weight rows, or of rows, over the whole slice.
+    const auto read_block = [&](auto constant) {
+        constexpr int item = decltype(constant)::value, block = item / 4, i = item / 2 % 2, p = item % 2;
+        read(std::integral_constant<int, 2 * block + p>{}, std::integral_constant<int, i>{});
     };
 
     begin_scales();
@@ -316,7 +330,6 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     for_each<0, kScales>(read_scale);
 #pragma unroll
     for (int i = 0; i < kScales; ++i) scales[i] = kWide ? wide_scale(next_scales[i]) : next_scales[i];
-    first_row = wave_m * blocks_of(upcoming) * 32;
     // kWide: a step of 64 is four of 16, and while one is multiplied the fragments of the next become bf16: by number four words of each, the weight rows'
     // first.
     constexpr int kParts = kWide ? 4 : 1, kConversions = kWide ? 2 * kBlocks * 4 : 0;
@@ -329,6 +342,10 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     };
     begin_reads(kFirst);
     for_each<0, kReads>([&](auto item) { read(item, kFirst); });
+    if constexpr (!kWide) {
+        begin_reads(kSecond);
+        for_each<0, kReads>([&](auto item) { read(item, kSecond); });
+    }
     for_each<0, kConversions>([&](auto item) { widen(item, kFirst, kFirst, scales); });
 
     f32x16_t acc[kBlocks][kBlocks];
@@ -341,59 +358,64 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
             for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
+        // In front of what comes next. (A product alone may move, within what has no branches to behind all of it.)
+        const auto keep = [](f32x16_t &sums) { asm volatile("" : "+a"(sums)); };
         const auto multiply_tile = [&](auto blocks_constant) {
             constexpr int kRows = decltype(blocks_constant)::value, kProducts = kBlocks * kRows;
-            constexpr int kSteps = kParts * kProducts;  // products of a step of 64
-            // Reads and loads go with all but the step's last two products; where fragments are widened, they are there before its last part.
-            constexpr int kReadsBusy = kWide ? 2 * kProducts : kProducts - 2, kLoadsBusy = kSteps - 2;
-            const auto product = [&](auto constant, auto step_constant) {
-                // Neighbouring products share an operand.
-                constexpr int at = decltype(constant)::value, i = decltype(step_constant)::value, q = at / kProducts, j = at % kProducts;
-                constexpr int n = j / kRows, m = n % 2 ? kRows - 1 - j % kRows : j % kRows;
-                if constexpr (kWide) acc[n][m] = multiply_wide(wide_weight[q % 2][n], wide_x[q % 2][m], acc[n][m]);
-                else acc[n][m] = multiply(weight_part[i][n], x_part[i][m], scales[n], scales[kBlocks + m], acc[n][m]);
-                // What the next part reads, in this step or the next one (of the next slice, with its scales).
-                constexpr int first = j * kConversions / kProducts, past = (j + 1) * kConversions / kProducts;
-                if constexpr (kWide && q + 1 < kParts) for_each<first, past>([&](auto item) { widen(item, step_constant, std::integral_constant<int, q + 1>{}, scales); });
-                else if constexpr (kWide && i == 0) for_each<first, past>([&](auto item) { widen(item, kSecond, kFirst, scales); });
-                else if constexpr (kWide) for_each<first, past>([&](auto item) { widen(item, kFirst, kFirst, next_scales); });
-            };
-#pragma unroll 1
-            for (int s = 0; s < slices; ++s) {
+            const auto begin_slice = [&]() {
                 if (load_slice == load_slices) begin_loads();
                 if (scale_slice == slices_of(upcoming)) {
                     logical += kResident;
                     more = more && places.locate(placement, logical, inner_slices, upcoming);
                     begin_scales();
                 }
+            };
+            const auto next_slot = [&](bool last) {
+                slot = slot == lds ? lds + kSlotBytes : lds;
+                next_scale_slot();
+                if (last) begin_scale_reads(upcoming);
+            };
+            // Block m of the tile's rows is the wavefront's block `place_of(m)` in LDS.
+            const auto place_of = [](int m) { return kRows == kBlocks ? m : 2 * m; };
+            // Wide: steps of 64. Beside the first the reads of the second, beside the second the reads of the next slice and the loads of the one behind it.
+            constexpr int kSteps = kParts * kProducts;  // products of a step of 64
+            // Reads are there before the step's last part, in which they are widened.
+            constexpr int kReadsBusy = 2 * kProducts, kLoadsBusy = kSteps - 2;
+            const auto wide_product = [&](auto constant, auto step_constant) {
+                // Neighbouring products share an operand.
+                constexpr int at = decltype(constant)::value, i = decltype(step_constant)::value, q = at / kProducts, j = at % kProducts;
+                constexpr int n = j / kRows, m = n % 2 ? kRows - 1 - j % kRows : j % kRows;
+                acc[n][m] = multiply_wide(wide_weight[q % 2][n], wide_x[q % 2][place_of(m)], acc[n][m]);
+                // What the next part reads, in this step or the next one (of the next slice, with its scales).
+                constexpr int first = j * kConversions / kProducts, past = (j + 1) * kConversions / kProducts;
+                if constexpr (q + 1 < kParts) for_each<first, past>([&](auto item) { widen(item, step_constant, std::integral_constant<int, q + 1>{}, scales); });
+                else if constexpr (i == 0) for_each<first, past>([&](auto item) { widen(item, kSecond, kFirst, scales); });
+                else for_each<first, past>([&](auto item) { widen(item, kFirst, kFirst, next_scales); });
+            };
+            const auto wide_slice = [&](bool last) {
+                begin_slice();
                 __builtin_amdgcn_sched_barrier(0);
-                // First step; beside it the reads of the second.
                 for_each<0, kSteps>([&](auto j) {
-                    product(j, kFirst);
+                    wide_product(j, kFirst);
                     if constexpr (j == 0) begin_reads(kSecond);
                     if constexpr (j < kReadsBusy) for_each<j * kReads / kReadsBusy, (j + 1) * kReads / kReadsBusy>([&](auto item) { read(item, kSecond); });
                     __builtin_amdgcn_sched_barrier(0);
                 });
-                // Second step. Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + 2 takes its slot.
-                product(kFirst, kSecond);
+                // Slice s + 1 is there when all wavefronts' loads of it are, and slice s has been read: slice s + 2 takes its slot.
+                wide_product(kFirst, kSecond);
                 __builtin_amdgcn_sched_barrier(0);
                 wait_for_memory<1>();  // all but the scales of slice s + 3, which are asked for last
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                slot = slot == lds ? lds + kSlotBytes : lds;
-                next_scale_slot();
-                if (s + 1 == slices) {
-                    first_row = wave_m * blocks_of(upcoming) * 32;
-                    begin_scale_reads(upcoming);
-                }
+                next_slot(last);
                 __builtin_amdgcn_sched_barrier(0);
                 for_each<1, kSteps>([&](auto j) {
                     // Of the next slice: its scales are there before the last part, in which its first fragments are widened.
-                    if constexpr (kWide && j == kSteps - kProducts) {
+                    if constexpr (j == kSteps - kProducts) {
 #pragma unroll
                         for (int i = 0; i < kScales; ++i) next_scales[i] = wide_scale(next_scales[i]);
                     }
-                    product(j, kSecond);
+                    wide_product(j, kSecond);
                     if constexpr (j == 1) begin_reads(kFirst);
                     if constexpr (j <= kReadsBusy) {
                         for_each<(j - 1) * kReads / kReadsBusy, j * kReads / kReadsBusy>([&](auto item) { read(item, kFirst); });
@@ -403,12 +425,71 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                     if constexpr (j == kLoadsBusy) load_scales();  // the last of the slice's loads
                     __builtin_amdgcn_sched_barrier(0);
                 });
+            };
+            // Narrow: the first step multiplies the whole slice of half of the rows, the second one that of the others. A slice's first group of loads has been read before
+            // its first step and the second group before its second one, and what takes their places is asked for at once, two to three steps before it is read.
+            constexpr int kHalf = kProducts, kPerWeight = kHalf / kBlocks;  // products of a step, and of a block of weight rows in it
+            constexpr int kFirstBusy = kHalf - 2, kFirstReads = 12, kAwaited = kItems + 1;
+            const auto narrow_product = [&](auto constant, auto group_constant) {
+                constexpr int at = decltype(constant)::value, group = decltype(group_constant)::value, n = at / kPerWeight;
+                constexpr int i = at % kPerWeight / (kPerWeight / 2), b = at % (kPerWeight / 2), place = 2 * group + b, m = kRows == kBlocks ? place : group;
+                acc[n][m] = multiply(weight_part[i][n], x_part[i][place], scales[n], scales[kBlocks + place], acc[n][m]);
+                keep(acc[n][m]);
+            };
+            const auto narrow_slice = [&](bool last) {
+                narrow_product(kFirst, kFirst);
+                begin_slice();
+                __builtin_amdgcn_sched_barrier(0);
+                narrow_product(kSecond, kFirst);
+                __builtin_amdgcn_sched_barrier(0);
+                // The second group of slice s is there (all that was asked for after it are two groups and scales), and all wavefronts have read the first one.
+                wait_for_memory<kAwaited>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                load_scales();  // of slice s + 3, where those of this one were
+                __builtin_amdgcn_sched_barrier(0);
+                for_each<2, kHalf>([&](auto j) {
+                    narrow_product(j, kFirst);
+                    // The last block of weight rows and the other half of the rows.
+                    for_each<(j - 2) * kFirstReads / kFirstBusy, (j - 1) * kFirstReads / kFirstBusy>([&](auto item) {
+                        read_block(std::integral_constant<int, item < 4 ? 4 * (kBlocks - 1) + item : 4 * (kBlocks + kBlocks / 2) + item - 4>{});
+                    });
+                    for_each<(j - 2) * kFirstItems / kFirstBusy, (j - 1) * kFirstItems / kFirstBusy>(load);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                narrow_product(kFirst, kSecond);
+                next_slot(last);
+                __builtin_amdgcn_sched_barrier(0);
+                narrow_product(kSecond, kSecond);
+                begin_reads(kFirst);
+                begin_reads(kSecond);
+                // The first group of slice s + 1 is there, and the second one of slice s has been read.
+                wait_for_memory<kAwaited>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                for_each<2, kHalf>([&](auto j) {
+                    narrow_product(j, kSecond);
+                    // The first half of the rows, and each block of weight rows once the present one has been multiplied.
+                    constexpr int kRowReads = 8, kLate = kPerWeight + kRows / 2, kWeightReads = 12;
+                    if constexpr (j < kLate) for_each<4 * kBlocks + (j - 2) * kRowReads / (kLate - 2), 4 * kBlocks + (j - 1) * kRowReads / (kLate - 2)>(read_block);
+                    else for_each<(j - kLate) * kWeightReads / (kHalf - kLate), (j - kLate + 1) * kWeightReads / (kHalf - kLate)>(read_block);
+                    for_each<(j - 2) * kScales / (kHalf - 2), (j - 1) * kScales / (kHalf - 2)>(read_scale);
+                    if constexpr (j < kHalf - 1) for_each<kFirstItems + (j - 2) * (kItems - kFirstItems) / (kHalf - 3), kFirstItems + (j - 1) * (kItems - kFirstItems) / (kHalf - 3)>(load);
+                    if constexpr (j == kHalf - 2) advance();
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            };
+#pragma unroll 1
+            for (int s = 0; s < slices; ++s) {
+                if constexpr (kWide) wide_slice(s + 1 == slices);
+                else narrow_slice(s + 1 == slices);
                 // The compiler would move products past the branches above, away from what they are to overlap.
 #pragma unroll
                 for (int n = 0; n < kBlocks; ++n)
 #pragma unroll
                     for (int m = 0; m < kRows; ++m) asm volatile("" : "+a"(acc[n][m]));
-                advance();
+                if constexpr (kWide) advance();
 #pragma unroll
                 for (int i = 0; i < kScales; ++i) scales[i] = next_scales[i];
             }
