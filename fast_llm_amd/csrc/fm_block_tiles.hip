@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
             load_to_lds<kOperandBytes + j * 16 * kSlice>(buffer_of(weight_from, weight_bytes), weight_offset + (j / 2 * 32 + j % 2 * 8) * here(weight_stride), target);
         } else {
             constexpr int j = (item - kFirstWeights) % (kLoads / 2);
-            load_to_lds<(group * 64 + j * 16) * kSlice>(buffer_of(x_from[group], x_bytes[group]), x_offset + j * 16 * here(x_stride), target);
+            load_to_lds<(group * 64 + j * 16) * kSlice>(buffer_of(x_from[group], x_bytes[group]), x_offset + j * 16 * x_stride, target);
         }
     };
 
