@@ -4,6 +4,7 @@
 // Both are one pass over their operands and no 16-bit copy leaves them. The forward is bound by memory. Of the backward every element has four conversions and
 // the slope of the activation, so that memory and arithmetic weigh about the same; a lane keeps its three results (gate's and up's gradient, output)
 // in registers between the two directions of quantisation, eight rows x four columns of each.
+
 #include "fm_activation_math.h"
 #include "fm_block_rows.h"
 
@@ -11,24 +12,34 @@ namespace fm {
 
 namespace block {
 
+// What values of a type are activated in. Of fp32 it is fp64, which takes no longer than memory does here (a step in fp32 is 2^-24 of a value, and it is a border of
+// e4m3 that decides). What was rounded to 16 bits has hardware exponentials and reciprocals of fp32.
+template <typename T>
+struct ActivatedIn { typedef float Real; };
+template <>
+struct ActivatedIn<float> { typedef double Real; };
+
+__device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.f + fast_exp(-x)); }
+__device__ __forceinline__ double sigmoid(double x) { return 1. / (1. + exp(-x)); }
+
 // act(x), and act'(x) for the backward. Gelu (in its tanh form) and silu are x times a sigmoid, which has no cancellation where it is small: x sigma(z), with the slope
 // sigma + x sigma (1 - sigma) z'.
-template <int kActivation>
-__device__ __forceinline__ float activate(float x, float &slope) {
+template <int kActivation, typename Real>
+__device__ __forceinline__ Real activate(Real x, Real &slope) {
     if constexpr (kActivation == FM_ACT_GELU || kActivation == FM_ACT_SILU) {
-        float z = x, z_slope = 1.f;
+        Real z = x, z_slope = 1;
         if constexpr (kActivation == FM_ACT_GELU) {
-            const float square = x * x;
-            z = x * (1.5957691216f + 0.071354816272f * square);
-            z_slope = 1.5957691216f + 0.214064448816f * square;
+            const Real square = x * x, linear = static_cast<Real>(1.5957691216057308), cubic = static_cast<Real>(0.071354816272600254);
+            z = x * (linear + cubic * square);
+            z_slope = linear + 3 * cubic * square;
         }
-        const float sigma = fast_rcp(1.f + fast_exp(-z)), out = x * sigma;
-        slope = sigma + out * (1.f - sigma) * z_slope;
+        const Real sigma = sigmoid(z), out = x * sigma;
+        slope = sigma + out * (1 - sigma) * z_slope;
         return out;
     }
-    float out;
-    slope = activation_backward<kActivation>(x, out);
-    return out;
+    const Real positive = kActivation == FM_ACT_IDENTITY || x > 0 ? x : 0;
+    slope = kActivation == FM_ACT_SQUARED_RELU ? 2 * positive : kActivation == FM_ACT_IDENTITY || x > 0 ? 1 : 0;
+    return kActivation == FM_ACT_SQUARED_RELU ? positive * positive : positive;
 }
 
 struct ActivationArgs {
@@ -46,6 +57,7 @@ struct ActivationArgs {
 
 template <typename T, int kActivation, bool kGated>
 __global__ __launch_bounds__(kRowThreads) void activation_forward_kernel(ActivationArgs args) {
+    typedef typename ActivatedIn<T>::Real Real;
     const uint32_t column_block = blockIdx.x % args.column_blocks;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x / args.column_blocks) * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
     const int count = rows_in_block(args.map, row0, args.rows), exist = static_cast<int>(min(args.rows - row0, static_cast<int64_t>(kBlock)));
@@ -67,10 +79,10 @@ __global__ __launch_bounds__(kRowThreads) void activation_forward_kernel(Activat
             float gate[16], up[16], result[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float slope;
                 gate[i] = to_float(gates[r].v[i]);
-                result[i] = activate<kActivation>(gate[i], slope);
-                if constexpr (kGated) up[i] = to_float(ups[r].v[i]), result[i] *= up[i];
+                Real slope, out = activate<kActivation, Real>(gate[i], slope);
+                if constexpr (kGated) up[i] = to_float(ups[r].v[i]), out *= up[i];
+                result[i] = static_cast<float>(out);
             }
             const uint32_t at = row * static_cast<uint32_t>(args.checkpoint_stride) + column;
             store_row(gate, checkpoint + at, scales + row, exists);
@@ -90,9 +102,10 @@ __device__ __forceinline__ void kept_apart(Raw<T, 4> &four) {
     four = __builtin_bit_cast(Raw<T, 4>, words);
 }
 
-// At most 128 registers, for two workgroups on a CU: gates, ups and gradients stay as they were read, and the results are made one after the other.
+// At most 128 registers (in fp64 256), for two workgroups on a CU: gates, ups and gradients stay as they were read, and the results are made one after the other.
 template <typename T, int kActivation, bool kGated>
-__global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(ActivationArgs args) {
+__global__ __launch_bounds__(kSquareThreads, sizeof(T) == 4 ? 2 : 4) void activation_backward_kernel(ActivationArgs args) {
+    typedef typename ActivatedIn<T>::Real Real;
     __shared__ __attribute__((aligned(16))) Square shared;
     const uint32_t column_block = blockIdx.x % args.column_blocks;
     const int64_t row_block = blockIdx.x / args.column_blocks, row0 = row_block * kBlock, column0 = static_cast<int64_t>(column_block) * kBlock;
@@ -139,10 +152,12 @@ __global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(
         if constexpr (kGated) unpack_four(ups[r], scale_of(up_scales, r), up);
 #pragma unroll
         for (int c = 0; c < kLaneColumns; ++c) {
-            float slope;
-            const float out = activate<kActivation>(gate[c], slope);
-            if constexpr (!kGated) output[r][c] = out;
-            values[r][c] = slope * (kGated ? up[c] * to_float(grad[r].v[c]) : to_float(grad[r].v[c]));
+            Real slope;
+            const Real out = activate<kActivation, Real>(gate[c], slope);
+            if constexpr (!kGated) output[r][c] = static_cast<float>(out);
+            // (The product of an up, of 4 bits, and a gradient of 16 is exact in fp32.)
+            const Real of_result = to_float(grad[r].v[c]);
+            values[r][c] = static_cast<float>(slope * (kGated ? up[c] * of_result : of_result));
         }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -166,9 +181,9 @@ __global__ __launch_bounds__(kSquareThreads, 4) void activation_backward_kernel(
             kept_apart(grad[r]);
 #pragma unroll
             for (int c = 0; c < kLaneColumns; ++c) {
-                float slope;
-                const float out = activate<kActivation>(gate[c], slope);
-                values[r][c] = out * to_float(grad[r].v[c]), output[r][c] = out * up[c];
+                Real slope;
+                const Real out = activate<kActivation, Real>(gate[c], slope);
+                values[r][c] = static_cast<float>(out * to_float(grad[r].v[c])), output[r][c] = static_cast<float>(out * up[c]);
             }
         }
         store_gradient(1);
