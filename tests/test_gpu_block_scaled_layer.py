@@ -305,6 +305,19 @@ def test_operators_replay_from_a_graph(device):
             torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gelu_is_zero_where_one_plus_tanh_is(dtype, device):
+    """A block of such values alone has no larger one beside it that would hide them. (1 + tanh at -4 is 3e-5, at -6 2e-11, of which fp32 keeps nothing beside 1.)"""
+    x = torch.tensor([-4.0, -6.0, -30.0, 6.0], device=device).to(dtype)[:, None].expand(4, 128).contiguous()
+    output, checkpoint = block_activation_forward(x, False, "gelu")
+    assert (output.elements.float() != 0).all(dim=1).tolist() == [True, False, False, True]
+    assert torch.equal(block_dequantize(output)[1:3], torch.zeros(2, 128, device=device))
+    grad, *_ = block_activation_backward(torch.ones_like(x), checkpoint, False, "gelu")
+    assert (block_dequantize(grad) != 0).all(dim=1).tolist() == [True, False, False, True]
+    # -0 has the sign of the gate: what is left of it is the sign.
+    assert torch.equal(output.values[1:3], torch.full_like(output.values[1:3], 0x80))
+
+
 def test_nothing_to_do(device):
     empty = torch.empty(0, 256, device=device)
     assert block_quantize(empty).shape == (0, 256)
