@@ -369,6 +369,12 @@ def _write_weight_gradient(weight: torch.Tensor, lhs: BlockScaledTensor, rhs: Bl
     block_input_row_sparse_matmul(lhs, rhs, sparse_map, out=weight.grad_buffer, accumulate=not first_write)
 
 
+def _has_fine_results(tensor: torch.Tensor) -> bool:
+    """Whether results of the tensor's type show the error of sums that are not exact: it is a sixteenth of half a step of fp16, which moves results that are rounded and added up by up
+    to half again as much as the roundings do, and a 128th of half a step of bf16."""
+    return tensor.dtype == torch.float16
+
+
 class _BlockMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input_, scores, weight_1, weight_2, weights: BlockScaledWeights, gated, activation_type, sparse_map, training, _anchor):
@@ -376,7 +382,9 @@ class _BlockMLP(torch.autograd.Function):
         layer_1 = block_sparse_matmul(rows, weights.layer_1, sparse_map, dtype=input_.dtype, exact_sums=True)
         activation, checkpoint = block_activation_forward(layer_1, gated, activation_type, sparse_map)
         del layer_1
-        layer_2 = block_sparse_matmul(activation, weights.layer_2_transposed, sparse_map, dtype=input_.dtype)
+        layer_2 = block_sparse_matmul(
+            activation, weights.layer_2_transposed, sparse_map, dtype=input_.dtype, exact_sums=_has_fine_results(input_)
+        )
         del activation
         output = copy_sparse_to_dense(layer_2, scores, sparse_map)
         if training:
@@ -409,7 +417,9 @@ class _BlockMLP(torch.autograd.Function):
         del activation_transposed, grad_transposed
         grad_input = None
         if ctx.needs_input_grad[0]:
-            grad_sparse = block_sparse_matmul(grad, layer_1_transposed, sparse_map, dtype=grad_output.dtype)
+            grad_sparse = block_sparse_matmul(
+                grad, layer_1_transposed, sparse_map, dtype=grad_output.dtype, exact_sums=_has_fine_results(grad_output)
+            )
             grad_input = copy_dense_to_sparse_backward(grad_sparse, (sparse_map, grad_output.shape))
         if weight_1.requires_grad:
             _write_weight_gradient(
@@ -439,7 +449,8 @@ def block_mlp(
     `weight_1` [experts * ffn (* 2), hidden] and `weight_2` [experts * ffn, hidden] are what the gradients are of: they are written to their
     `grad_buffer`s (of any float type) as everywhere. `weights`: the same weights quantised (`block_quantize_expert_weights`), where there are several calls to one
     optimizer step; otherwise they are quantised here. Rows and gradients between the steps are of 8 bits; the results of both layers, of
-    the activation's gradient and of the input's per slot are rounded to the input's type, sums are in fp32. Differentiable once.
+    the activation's gradient and of the input's per slot are rounded to the input's type, sums are in fp32 (exact, as `block_sparse_matmul` says, where results are quantised
+    again and in fp16). Differentiable once.
     Gated, ffn is a multiple of 128.
     """
     refuse_traced(input_, scores, weight_1, weight_2)
