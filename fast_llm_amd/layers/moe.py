@@ -348,6 +348,8 @@ class BlockScaledMoEMLP(DroplessMoEMLP):
         weights: BlockScaledWeights | None = None,
     ) -> torch.Tensor:
         hidden_states, router_counts = input_.flatten(0, -2), None
+        if (scores is None) != (top_experts is None):
+            raise ValueError("a routing of the caller's own has scores and experts")
         if top_experts is None:
             scores, top_experts, router_counts = self.route_with_counts(hidden_states, grad_scale, losses)
         sparse_map = get_sparse_map(

@@ -164,6 +164,9 @@ def test_layers_that_are_refused():
         with pytest.raises(NotImplementedError):
             BlockScaledMoEMLP(64, experts=4, experts_per_token=2, device="cpu", **arguments)
     layer = BlockScaledMoEMLP(64, 100, 4, 2, gated=False, shared_experts=1, device="cpu")
+    for half in (dict(scores=torch.ones(3, 2)), dict(top_experts=torch.zeros(3, 2, dtype=torch.int64))):
+        with pytest.raises(ValueError, match="own"):
+            layer(torch.zeros(3, 64, dtype=torch.bfloat16), **half)
     assert {n: p.shape for n, p in layer.named_parameters()} == {
         n: p.shape for n, p in DroplessMoEMLP(64, 100, 4, 2, gated=False, shared_experts=1, device="cpu").named_parameters()
     }
