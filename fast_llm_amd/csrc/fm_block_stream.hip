@@ -6,6 +6,9 @@
 // LDS operations are carried out in order, so no barrier). kDepth chunks are on their way at a time. Activations, which all workgroups of an expert
 // read, come from L2 as fragments, and the scales as bytes, those of 32 neighbouring rows side by side.
 //
+// One token and two of 8 experts, 4096 -> 2 x 14336: 40 us, 5.8 TB/s of weights; 96 tokens with 8 of 128, 2048 -> 2 x 768: 66 us, 6.1 TB/s. As fragments straight from memory, 16 bytes of
+// each of 32 lines at a time, the first took 60 and 14336 -> 4096 112 for 22.
+//
 // Any number of rows per expert is right (they are walked and the weights read again); the caller decides up to where this is the faster way.
 #include <algorithm>
 
