@@ -62,8 +62,10 @@ __device__ __forceinline__ Real activate(Real x, Real &slope) {
     if constexpr (kActivation == FM_ACT_GELU || kActivation == FM_ACT_SILU) {
         Real z = x, z_slope = 1;
         if constexpr (kActivation == FM_ACT_GELU) {
-            const Real square = x * x, linear = static_cast<Real>(1.5957691216057308), cubic = static_cast<Real>(0.071354816272600254);
-            z = x * (linear + cubic * square);
+            // (Beyond 100 it is x or 0, whose powers would overflow.)
+            const Real bounded = x > 100 ? static_cast<Real>(100) : x < -100 ? static_cast<Real>(-100) : x;
+            const Real square = bounded * bounded, linear = static_cast<Real>(1.5957691216057308), cubic = static_cast<Real>(0.071354816272600254);
+            z = bounded * (linear + cubic * square);
             z_slope = linear + 3 * cubic * square;
         }
         Real complement, sigma = sigmoid<kActivation == FM_ACT_GELU>(z, complement);

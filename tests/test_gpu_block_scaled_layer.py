@@ -318,6 +318,18 @@ def test_gelu_is_zero_where_one_plus_tanh_is(dtype, device):
     assert torch.equal(output.values[1:3], torch.full_like(output.values[1:3], 0x80))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_activations_of_large_values_do_not_overflow(activation, dtype, device):
+    """Powers of two, which e4m3 has: the function is the value itself or 0, its slope 1 or 0."""
+    sizes = torch.tensor([2.0**7, 2.0**43, 2.0**66, 2.0**120], device=device)
+    x = torch.cat((sizes, -sizes)).to(dtype)[:, None].expand(8, 128).contiguous()
+    output, checkpoint = block_activation_forward(x, False, activation)
+    assert torch.equal(block_dequantize(output), x.float().clamp_min(0))
+    grad, *_ = block_activation_backward(torch.ones_like(x), checkpoint, False, activation)
+    assert torch.equal(block_dequantize(grad), (x > 0).float())
+
+
 def test_nothing_to_do(device):
     empty = torch.empty(0, 256, device=device)
     assert block_quantize(empty).shape == (0, 256)
