@@ -75,8 +75,9 @@ __device__ __forceinline__ Real activate(Real x, Real &slope) {
         slope = sigma + out * complement * z_slope;
         return out;
     }
-    const Real positive = kActivation == FM_ACT_IDENTITY || x > 0 ? x : 0;
-    slope = kActivation == FM_ACT_SQUARED_RELU ? 2 * positive : kActivation == FM_ACT_IDENTITY || x > 0 ? 1 : 0;
+    // NaN is no number that either comparison lets go: it stays, in the slope as well.
+    const Real positive = kActivation != FM_ACT_IDENTITY && x <= 0 ? 0 : x;
+    slope = kActivation == FM_ACT_SQUARED_RELU ? 2 * positive : kActivation == FM_ACT_IDENTITY || x > 0 ? 1 : positive;
     return kActivation == FM_ACT_SQUARED_RELU ? positive * positive : positive;
 }
 

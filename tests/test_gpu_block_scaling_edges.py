@@ -1,0 +1,82 @@
+"""Operators on values of 8 bits with a scale per block of 128 at their edges: what is no number, terms that cancel, weights that are quantised where they are needed."""
+
+import pytest
+import torch
+
+from fast_llm_amd.functional.block_scaling import block_activation_backward, block_activation_forward
+from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- infinities and NaN in rows that count ---------------------------------------------------------------
+NAN, INF = float("nan"), float("inf")
+
+
+def _bad_blocks(bad: torch.Tensor) -> torch.Tensor:
+    """[rows, blocks of 128 columns]: those with a bad value."""
+    return torch.nn.functional.pad(bad, (0, -bad.size(1) % 128)).unflatten(1, (-1, 128)).any(-1)
+
+
+def _assert_bad(tensor, bad: torch.Tensor, plain) -> None:
+    """Blocks with a bad value are NaN, with zeros for elements; the others are those of `plain`, which has none."""
+    blocks = _bad_blocks(bad)
+    scales, expected = tensor.scales[:, : tensor.rows].t().cpu(), plain.scales[:, : tensor.rows].t().cpu()
+    assert torch.equal(scales == 255, blocks)
+    assert torch.equal(scales[~blocks], expected[~blocks])
+    elements, expected = (t.values.cpu().unflatten(1, (-1, 128)) for t in (tensor, plain))
+    assert not elements[blocks].any() and torch.equal(elements[~blocks], expected[~blocks])
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_and_nan_in_rows_that_count(dtype, activation, gated, device):
+    generator = torch.Generator().manual_seed(1)
+    rows, ffn = 130, 256
+    x = torch.randn(rows, ffn * (1 + gated), generator=generator).to(dtype)
+    grad = torch.randn(rows, ffn, generator=generator).to(dtype)
+    plain_output, plain_checkpoint = block_activation_forward(x.to(device), gated, activation)
+    plain_grads = block_activation_backward(grad.to(device), plain_checkpoint, gated, activation)
+
+    # Into the gates, row by row; row 7 has one in each block, the last row is in the second block of rows.
+    places = {(3, 5): NAN, (7, 0): NAN, (7, 255): INF, (20, 130): INF, (129, 1): -INF}
+    bad_input, bad_output = torch.zeros(rows, x.size(1), dtype=torch.bool), torch.zeros(rows, ffn, dtype=torch.bool)
+    y = x.clone()
+    for (row, column), value in places.items():
+        y[row, column] = value
+        bad_input[row, column] = True
+        # An infinity is one of the result's; x times a sigmoid has no limit at the lower end in which 0 times it were a number, and ReLUs are 0 there.
+        bad_output[row, column] = not (value == -INF and activation in ("relu", "squared_relu"))
+    if gated:
+        y[40, ffn + 200] = NAN  # an up: its gate is what it was
+        bad_input[40, ffn + 200] = bad_output[40, 200] = True
+    output, checkpoint = block_activation_forward(y.to(device), gated, activation)
+    _assert_bad(checkpoint, bad_input, plain_checkpoint)
+    # (In its row's block -inf becomes 0, which is not what the plain block has: that block is compared by its scale alone.)
+    special = activation in ("relu", "squared_relu")
+    if special:
+        assert output.scales[0, 129] != 255 and output.values[129, 1] & 0x7F == 0
+        output.scales[0, 129], output.values[129, :128] = plain_output.scales[0, 129], plain_output.values[129, :128]
+    _assert_bad(output, bad_output, plain_output)
+
+    # Backward: whatever shares a block with a bad value is NaN.
+    kept = _bad_blocks(bad_input).repeat_interleave(128, 1)
+    gate, up = kept[:, :ffn], kept[:, ffn:] if gated else torch.zeros(rows, ffn, dtype=torch.bool)
+    bad_gate = up if activation == "identity" else gate | up  # (whose slope is 1, whatever it is of)
+    bad_grad = torch.cat((bad_gate, gate), dim=1) if gated else bad_gate
+    grads = block_activation_backward(grad.to(device), checkpoint, gated, activation)
+    _assert_bad(grads[0], bad_grad, plain_grads[0])
+    _assert_bad(grads[1], bad_grad.t(), plain_grads[1])
+    _assert_bad(grads[2], (gate | up).t(), plain_grads[2])
+
+    # Into the gradient, which leaves the activation alone.
+    g = grad.clone()
+    g[9, 3], g[70, 140] = NAN, -INF
+    bad = ~torch.isfinite(g)
+    grads = block_activation_backward(g.to(device), plain_checkpoint, gated, activation)
+    # Zero times an infinity is not a number either.
+    bad = torch.cat((bad, bad), dim=1) if gated else bad
+    _assert_bad(grads[0], bad, plain_grads[0])
+    _assert_bad(grads[1], bad.t(), plain_grads[1])
+    _assert_bad(grads[2], torch.zeros(rows, ffn, dtype=torch.bool).t(), plain_grads[2])
