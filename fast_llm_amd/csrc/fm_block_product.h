@@ -18,7 +18,7 @@ struct ProductArgs {
     int64_t inner;    // padded: a multiple of 128
     int64_t experts;
     int out_dtype, accumulate;
-    int exact;        // sums as for results in fp32 (by rows)
+    int exact;        // sums as for results in fp32, asked for (by rows; by the reduction the result's type says it)
     int out_vectors;  // rows of `out` are aligned to 16 bytes
     int by_inner;     // an expert has a range of the reduction and `rows` rows of the result; otherwise a range of rows
     const void *expert_ends, *expert_pad_begins;
@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t here(uint32_t value) {
 
 // The instruction aligns eight products (of eight neighbours along k) to the largest of them and drops what lies about 14 bits under it: a sum of normal values is 1.5e-5
 // of itself off, whatever its length. A result of 16 bits does not show it, but where that is quantised once more a value in two thousand falls to the other side of
-// a border of e4m3, an eighth of itself away. Results in fp32, and those for which a caller asks, are summed as exactly as fp32: the operands
+// a border of e4m3, an eighth of itself away. Results in fp32, gradients in fp16, and what a caller asks it for, are summed as exactly as fp32: the operands
 // become bf16 on their way to the matrix units, scales included, which loses nothing (but below 2^-126), and the products of those are exact in
 // fp32. Half the rate.
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;

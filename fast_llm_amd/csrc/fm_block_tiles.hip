@@ -598,9 +598,19 @@ static int launch(const ProductArgs &args, hipStream_t stream) {
     return FM_OK;
 }
 
-template <bool kByInner, bool kAccumulate, bool kWide>
-static int launch_half(const ProductArgs &args, hipStream_t stream) {
-    return args.out_dtype == FM_DTYPE_BF16 ? launch<kByInner, kAccumulate, kWide, bf16_t>(args, stream) : launch<kByInner, kAccumulate, kWide, f16_t>(args, stream);
+template <bool kWide>
+static int launch_rows(const ProductArgs &args, hipStream_t stream) {
+    return args.out_dtype == FM_DTYPE_BF16 ? launch<false, false, kWide, bf16_t>(args, stream) : launch<false, false, kWide, f16_t>(args, stream);
+}
+
+// Gradients in fp16 are summed as exactly as those in fp32: micro-batches add up in them, and half a step of fp16 is no more than sixteen times what inexact sums are off.
+template <bool kAccumulate>
+static int launch_gradients(const ProductArgs &args, hipStream_t stream) {
+    switch (args.out_dtype) {
+        case FM_DTYPE_F32: return launch<true, kAccumulate, true, float>(args, stream);
+        case FM_DTYPE_F16: return launch<true, kAccumulate, true, f16_t>(args, stream);
+        default: return launch<true, kAccumulate, false, bf16_t>(args, stream);
+    }
 }
 
 }  // namespace tiles
@@ -614,13 +624,9 @@ bool tile_product_takes(const ProductArgs &args) {
 
 int tile_product(const ProductArgs &args, hipStream_t stream) {
     using namespace tiles;
-    const bool wide = args.out_dtype == FM_DTYPE_F32;
-    if (!args.by_inner) {
-        if (wide) return launch<false, false, true, float>(args, stream);
-        return args.exact ? launch_half<false, false, true>(args, stream) : launch_half<false, false, false>(args, stream);
-    }
-    if (args.accumulate) return wide ? launch<true, true, true, float>(args, stream) : launch_half<true, true, false>(args, stream);
-    return wide ? launch<true, false, true, float>(args, stream) : launch_half<true, false, false>(args, stream);
+    if (args.by_inner) return args.accumulate ? launch_gradients<true>(args, stream) : launch_gradients<false>(args, stream);
+    if (args.out_dtype == FM_DTYPE_F32) return launch<false, false, true, float>(args, stream);
+    return args.exact ? launch_rows<true>(args, stream) : launch_rows<false>(args, stream);
 }
 
 }  // namespace block

@@ -282,7 +282,8 @@ def block_input_row_sparse_matmul(
     The weights' gradients from transposed forms lhs [rows, sparse rows] and rhs [columns, sparse rows] (`block_quantize_both`, `block_activation_backward`),
     which hold zeros where no token is.
     Formula: out[id, j] (+)= sum_ks(lhs[is, ks] * rhs[j, ks]), where ks are the rows of expert id // rows, is = id % rows
-    `out` (of any float type, rows contiguous) or `dtype` gives the result's type.
+    `out` (of any float type, rows contiguous) or `dtype` gives the result's type. Sums are those of `block_sparse_matmul`: in fp32 and fp16 with `exact_sums`, in
+    bf16 without; where large terms cancel in a gradient, its buffer is in fp32.
     """
     refuse_traced()
     Assert.eq(lhs.columns, rhs.columns)
@@ -450,7 +451,7 @@ def block_mlp(
     `grad_buffer`s (of any float type) as everywhere. `weights`: the same weights quantised (`block_quantize_expert_weights`), where there are several calls to one
     optimizer step; otherwise they are quantised here. Rows and gradients between the steps are of 8 bits; the results of both layers, of
     the activation's gradient and of the input's per slot are rounded to the input's type, sums are in fp32 (exact, as `block_sparse_matmul` says, where results are quantised
-    again and in fp16). Differentiable once.
+    again, in fp16, and for gradients in fp16 or fp32). Differentiable once.
     Gated, ffn is a multiple of 128.
     """
     refuse_traced(input_, scores, weight_1, weight_2)

@@ -566,7 +566,8 @@ int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *
                            int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int exact_sums, int out_dtype,
                            int index_dtype, void *stream);
 /* The weights' gradients: out[e rows + i, j] (=, or += with `accumulate`) sum over the rows k of expert e of lhs[i, k] * rhs[j, k], lhs [rows, inner] and rhs
- * [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens have zeros. */
+ * [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens have zeros. Results in fp32
+ * and in fp16 are summed as exactly as fp32, at half the rate; those in bf16, whose steps are coarser, as fm_block_sparse_matmul does without `exact_sums`. */
 int fm_block_input_row_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                                      const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
                                      int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int accumulate, int out_dtype,

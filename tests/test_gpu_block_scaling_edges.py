@@ -3,8 +3,10 @@
 import pytest
 import torch
 
-from fast_llm_amd.functional.block_scaling import block_activation_backward, block_activation_forward
-from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES
+from fast_llm_amd.functional.block_scaling import (
+    block_activation_backward, block_activation_forward, block_input_row_sparse_matmul, block_quantize,
+)  # fmt: skip
+from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES, _map, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +82,64 @@ def test_infinities_and_nan_in_rows_that_count(dtype, activation, gated, device)
     _assert_bad(grads[0], bad, plain_grads[0])
     _assert_bad(grads[1], bad.t(), plain_grads[1])
     _assert_bad(grads[2], torch.zeros(rows, ffn, dtype=torch.bool).t(), plain_grads[2])
+
+
+# ---- sums ------------------------------------------------------------------------------------------------
+def _cancelling(generator, rows: int, columns: int, inner: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Operands whose products have, in each eight neighbours along the reduction, two large ones that cancel, beside small ones."""
+    lhs, rhs = torch.randn(rows, inner, generator=generator), torch.randn(columns, inner, generator=generator)
+    lhs[:, ::8], lhs[:, 1::8], rhs[:, ::8], rhs[:, 1::8] = 400.0, 400.0, 4.0, -4.0
+    return lhs, rhs
+
+
+def _eights(lhs: torch.Tensor, rhs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Of each eight neighbours along the reduction, [eights, rows, columns]: the sum and the largest magnitude of their products."""
+    a, b = (torch.nn.functional.pad(t, (0, -t.size(1) % 8)).unflatten(1, (-1, 8)).transpose(0, 1) for t in (lhs, rhs))
+    products = a[:, :, None] * b[:, None]
+    return products.sum(-1), products.abs().amax(-1)
+
+
+def _rounding(expected: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Half a step of the result (of its smallest normal value, below that)."""
+    return torch.finfo(dtype).eps / 2 * expected.abs().clamp_min(torch.finfo(dtype).smallest_normal)
+
+
+def _exact_tolerance(lhs: torch.Tensor, rhs: torch.Tensor) -> torch.Tensor:
+    """
+    Exact sums: each product is exact. An instruction adds 16 of them, two whole eights, to the sum so far: 16 additions, in any order, of at most (the sum so far and
+    the magnitudes of the 16), each off by a step of fp32 at most. The sum so far is made of whole eights: it is no larger than the magnitudes of their sums.
+    """
+    sums, _ = _eights(lhs, rhs)
+    instructions = -(-lhs.size(1) // 16)
+    return 16 * 2.0**-23 * (lhs.abs() @ rhs.abs().t() + instructions * sums.abs().sum(0))
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("counts", [[30], [300, 0, 257]], ids=str)
+@pytest.mark.parametrize(("rows", "columns"), [(40, 70), (300, 264)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_weight_gradients_keep_small_terms_beside_large_ones(dtype, rows, columns, counts, accumulate, device):
+    """In fp32, and in fp16, of which every bit is one that inexact sums would show."""
+    generator = torch.Generator().manual_seed(rows + columns)
+    sparse_map = _map(counts, device)
+    lhs, rhs = _cancelling(generator, rows, columns, sparse_map.num_rows)
+    before = (torch.randn(len(counts) * rows, columns, generator=generator) * 10).to(dtype)
+    begin = 0
+    for count in counts:  # zeros where no token is
+        lhs[:, begin + count : begin + -(-count // 128) * 128] = 0
+        begin += -(-count // 128) * 128
+    a, b = block_quantize(lhs.to(device)), block_quantize(rhs.to(device))
+    x, y = _values(a), _values(b)
+    out = before.to(device)
+    block_input_row_sparse_matmul(a, b, sparse_map, out=out, accumulate=accumulate)
+    begin = 0
+    for expert, count in enumerate(counts):
+        part = slice(begin, begin + -(-count // 128) * 128)
+        begin = part.stop
+        expected, tolerance = x[:, part] @ y[:, part].t(), _exact_tolerance(x[:, part], y[:, part])
+        if accumulate:
+            earlier = before[expert * rows : (expert + 1) * rows].double()
+            expected += earlier
+            tolerance += 2.0**-24 * (expected.abs() + tolerance)  # one more addition in fp32
+        error = (out[expert * rows : (expert + 1) * rows].cpu().double() - expected).abs()
+        assert (error <= tolerance + _rounding(expected.abs() + tolerance, dtype)).all()
