@@ -13,7 +13,7 @@ import torch
 
 LIBRARY_PATH = pathlib.Path(__file__).resolve().parent / "csrc" / "libfastmoe_hip.so"
 
-FM_VERSION = 14
+FM_VERSION = 15
 
 _c_i64, _c_int, _c_ptr, _c_size = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
 
@@ -110,6 +110,7 @@ SIGNATURES: dict[str, tuple] = {
     "fm_block_dequantize": (_c_int, [_c_ptr] * 3 + [_c_i64] * 4 + [_c_int] + [_c_ptr]),
     "fm_block_copy_dense_to_sparse": (_c_int, [_c_ptr] * 5 + [_c_i64] * 7 + [_c_int] + [_c_ptr]),
     "fm_block_sparse_matmul": (_c_int, [_c_ptr] * 7 + [_c_i64] * 9 + [_c_int] * 3 + [_c_ptr]),
+    "fm_block_sparse_matmul_counted": (_c_int, [_c_ptr] * 7 + [_c_i64] * 10 + [_c_int] * 3 + [_c_ptr]),
     "fm_block_input_row_sparse_matmul": (_c_int, [_c_ptr] * 7 + [_c_i64] * 9 + [_c_int] * 3 + [_c_ptr]),
     "fm_block_activation_forward": (_c_int, [_c_ptr] * 7 + [_c_i64] * 6 + [_c_int] * 4 + [_c_ptr]),
     "fm_block_activation_backward": (_c_int, [_c_ptr] * 11 + [_c_i64] * 9 + [_c_int] * 4 + [_c_ptr]),

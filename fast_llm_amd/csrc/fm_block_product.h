@@ -14,6 +14,7 @@ struct ProductArgs {
     void *out;
     int64_t x_stride, x_scale_stride, weight_stride, weight_scale_stride, out_stride;
     int64_t rows;     // of x (by rows: of the sparse layout)
+    int64_t entries;  // of them those that tokens have, where the caller knows; 0: not known
     int64_t columns;  // of the result
     int64_t inner;    // padded: a multiple of 128
     int64_t experts;
@@ -69,6 +70,13 @@ bool stream_product_takes(const ProductArgs &args);
 int stream_split(const ProductArgs &args);
 // Which of them a product by rows runs on (fm_block_product.hip).
 bool runs_on_tiles(const ProductArgs &args);
+
+// With a map, the rows of a layout that has room for any routing of the tokens: their entries and up to 128 of padding per expert. It is what the choices between kernels
+// go by, so that they are those of the tokens, whatever the layout's own padding is (none, or as much as this very routing needs). Where nothing is
+// known of the entries, the layout is taken to be such a one.
+inline int64_t rows_of_any_routing(const ProductArgs &args) {
+    return args.entries > 0 ? (args.entries + kBlock * args.experts) / kBlock * kBlock : args.rows;
+}
 
 }  // namespace block
 

@@ -172,7 +172,7 @@ int launch(const ProductArgs &args, hipStream_t stream) {
 // As few wavefronts share a reduction as give the device twelve wavefronts per CU.
 int stream_split(const ProductArgs &args) {
     // A map's rows have up to 128 of padding per expert; of its last ones it is not known whether there is anything in them.
-    const int64_t busy = args.expert_ends == nullptr ? 1 : std::min(std::max(args.rows - 128 * args.experts, int64_t(2)), args.experts);
+    const int64_t busy = args.expert_ends == nullptr ? 1 : std::min(std::max(rows_of_any_routing(args) - 128 * args.experts, int64_t(2)), args.experts);
     const int64_t sets = (args.columns + 31) / 32 * busy, chunks = args.inner / kBlock;
     constexpr int kWanted = 12 * 256;
     if (sets >= kWanted || chunks < 4) return 1;

@@ -234,6 +234,12 @@ def block_copy_dense_to_sparse(input_: BlockScaledTensor, sparse_map: SparseMap)
     return out
 
 
+def _has_worst_padding(sparse_map: SparseMap) -> bool:
+    """Whether the layout has room for any routing of its tokens (or nothing says how many rows they have): a product's kernel is then chosen by its rows."""
+    entries = sparse_map.num_rows_unpadded
+    return entries is None or sparse_map.num_rows == (entries + sparse_map.num_experts * BLOCK) // BLOCK * BLOCK
+
+
 def block_sparse_matmul(
     lhs: BlockScaledTensor,
     rhs: BlockScaledTensor,
@@ -262,9 +268,12 @@ def block_sparse_matmul(
     assert out.stride(1) == 1 or columns == 1
     if columns == 0:
         return out
+    name, entries = "fm_block_sparse_matmul", ()
+    if sparse_map is not None and not _has_worst_padding(sparse_map):
+        name, entries = "fm_block_sparse_matmul_counted", (sparse_map.num_rows_unpadded,)
     _lib.call(
-        "fm_block_sparse_matmul", device, *_pointers(lhs), *_pointers(rhs), out.data_ptr(), *pointers, lhs.rows, columns,
-        lhs.columns, experts, *_strides(lhs), *_strides(rhs), out.stride(0) if lhs.rows > 1 else columns, int(exact_sums),
+        name, device, *_pointers(lhs), *_pointers(rhs), out.data_ptr(), *pointers, lhs.rows, columns,
+        lhs.columns, experts, *entries, *_strides(lhs), *_strides(rhs), out.stride(0) if lhs.rows > 1 else columns, int(exact_sums),
         _lib.dtype_tag(out.dtype), index_tag,
     )  # fmt: skip
     return out

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FM_VERSION 14
+#define FM_VERSION 15
 
 /* Element type of activations, weights and outputs. */
 enum fm_dtype { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1, FM_DTYPE_F16 = 2 };
@@ -565,6 +565,13 @@ int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *
                            const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
                            int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int exact_sums, int out_dtype,
                            int index_dtype, void *stream);
+/* The same product of a layout whose padding is not that of the worst case (rows = num_entries + 128 num_experts, rounded down to a multiple of 128, which
+ * fm_block_sparse_matmul takes a map's rows to be): one that holds this routing alone, or without padding. `num_entries`: how many rows tokens have at most (tokens times
+ * experts per token), 0: not known. It only helps to choose a kernel; results are those of the map. */
+int fm_block_sparse_matmul_counted(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
+                                   const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t num_entries,
+                                   int64_t lhs_stride, int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride,
+                                   int exact_sums, int out_dtype, int index_dtype, void *stream);
 /* The weights' gradients: out[e rows + i, j] (=, or += with `accumulate`) sum over the rows k of expert e of lhs[i, k] * rhs[j, k], lhs [rows, inner] and rhs
  * [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens have zeros. Results in fp32
  * and in fp16 are summed as exactly as fp32, at half the rate; those in bf16, whose steps are coarser, as fm_block_sparse_matmul does without `exact_sums`. */

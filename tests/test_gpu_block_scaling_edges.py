@@ -4,8 +4,9 @@ import pytest
 import torch
 
 from fast_llm_amd.functional.block_scaling import (
-    block_activation_backward, block_activation_forward, block_input_row_sparse_matmul, block_quantize,
+    block_activation_backward, block_activation_forward, block_copy_dense_to_sparse, block_input_row_sparse_matmul, block_quantize, block_sparse_matmul,
 )  # fmt: skip
+from fast_llm_amd.functional.sparse_copy import get_sparse_map
 from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES, _map, _values
 
 pytestmark = pytest.mark.gpu
@@ -143,3 +144,20 @@ def test_weight_gradients_keep_small_terms_beside_large_ones(dtype, rows, column
             tolerance += 2.0**-24 * (expected.abs() + tolerance)  # one more addition in fp32
         error = (out[expert * rows : (expert + 1) * rows].cpu().double() - expected).abs()
         assert (error <= tolerance + _rounding(expected.abs() + tolerance, dtype)).all()
+
+
+@pytest.mark.parametrize("per_expert", [1, 20, 100, 300])
+@pytest.mark.parametrize("exact", [False, True])
+def test_the_padding_of_the_layout_changes_nothing(exact, per_expert, device):
+    """Room for any routing, for this one alone, or no padding: the same products run on the same kernel, to the bit."""
+    generator = torch.Generator().manual_seed(per_expert)
+    experts, inner, columns = 8, 512, 1280
+    top_experts = torch.rand(per_expert * experts // 2, experts, generator=generator).topk(2).indices.to(device)
+    rows = block_quantize(torch.randn(top_experts.size(0), inner, generator=generator).to(device))
+    weight = block_quantize(torch.randn(experts * columns, inner, generator=generator).to(device))
+    results = []
+    for options in ({}, {"dynamic_shape": True}, {"dynamic_shape": True, "pad_to_multiple": 1}):
+        sparse_map = get_sparse_map(top_experts, experts, **options)
+        out = block_sparse_matmul(block_copy_dense_to_sparse(rows, sparse_map), weight, sparse_map, exact_sums=exact)
+        results.append(out[sparse_map.sparse_rows.long()])
+    assert all(torch.equal(result, results[0]) for result in results)
