@@ -92,11 +92,11 @@ class BlockScaledTensor:
 
 
 class BlockScaledWeights(typing.NamedTuple):
-    """The expert weights of the sparse MLP in the forms that its products read (`block_quantize_expert_weights`)."""
+    """The expert weights of the sparse MLP in the forms that its products read (`block_quantize_expert_weights`); for inference without those of the backward."""
 
     layer_1: BlockScaledTensor  # [experts * ffn (* 2, gates then ups), hidden]: forward
-    layer_1_transposed: BlockScaledTensor  # [experts * hidden, ffn (* 2)]: input gradient
-    layer_2: BlockScaledTensor  # [experts * ffn, hidden]: input gradient
+    layer_1_transposed: BlockScaledTensor | None  # [experts * hidden, ffn (* 2)]: input gradient
+    layer_2: BlockScaledTensor | None  # [experts * ffn, hidden]: input gradient
     layer_2_transposed: BlockScaledTensor  # [experts * hidden, ffn]: forward
 
 
@@ -210,9 +210,16 @@ def block_dequantize(input_: BlockScaledTensor, dtype: torch.dtype = torch.float
     return out
 
 
-def block_quantize_expert_weights(weight_1: torch.Tensor, weight_2: torch.Tensor, num_experts: int) -> BlockScaledWeights:
-    """The weights of the sparse MLP (layer 1 [experts * ffn (* 2), hidden], layer 2 [experts * ffn, hidden]) in both forms each."""
+def block_quantize_expert_weights(
+    weight_1: torch.Tensor, weight_2: torch.Tensor, num_experts: int, *, training: bool = True
+) -> BlockScaledWeights:
+    """The weights of the sparse MLP (layer 1 [experts * ffn (* 2), hidden], layer 2 [experts * ffn, hidden]) in both forms each, or without
+    `training` in the one that its forward reads."""
     Assert.eq(weight_1.size(1), weight_2.size(1))
+    if not training:
+        return BlockScaledWeights(
+            block_quantize(weight_1), None, None, block_quantize_transposed(weight_2, groups=num_experts)
+        )
     return BlockScaledWeights(
         *block_quantize_both(weight_1, groups=num_experts), *block_quantize_both(weight_2, groups=num_experts)
     )
@@ -398,11 +405,15 @@ class _BlockMLP(torch.autograd.Function):
         del activation
         output = copy_sparse_to_dense(layer_2, scores, sparse_map)
         if training:
-            ctx.save_for_backward(
-                scores, layer_2, rows.values, rows.scales, checkpoint.values, checkpoint.scales, weights.layer_1_transposed.values,
-                weights.layer_1_transposed.scales, weights.layer_2.values, weights.layer_2.scales,
-            )  # fmt: skip
-            ctx.columns = rows.columns, checkpoint.columns, weights.layer_1_transposed.columns, weights.layer_2.columns
+            # The backward's forms of the weights are the caller's, or are made of the weights when it comes to them: kept until then they would take
+            # more than all else. (As these are saved, a weight that changes until then is noticed.)
+            kept, saved = [rows, checkpoint], ()
+            if weights.layer_1_transposed is None:
+                saved = weight_1, weight_2
+            else:
+                kept += weights.layer_1_transposed, weights.layer_2
+            ctx.save_for_backward(scores, layer_2, *(part for tensor in kept for part in (tensor.values, tensor.scales)), *saved)
+            ctx.columns = [tensor.columns for tensor in kept]
             ctx.weights, ctx.options = (weight_1, weight_2), (gated, activation_type, sparse_map)
         return output
 
@@ -410,14 +421,18 @@ class _BlockMLP(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_output: torch.Tensor):
         scores, layer_2, *saved = ctx.saved_tensors
-        rows, checkpoint, layer_1_transposed, layer_2_weight = (
-            BlockScaledTensor(saved[2 * i], saved[2 * i + 1], columns) for i, columns in enumerate(ctx.columns)
-        )
+        kept = [BlockScaledTensor(saved[2 * i], saved[2 * i + 1], columns) for i, columns in enumerate(ctx.columns)]
+        del saved
+        rows, checkpoint, layer_1_transposed, layer_2_weight = kept + [None] * (4 - len(kept))
+        del kept
         (weight_1, weight_2), (gated, activation_type, sparse_map) = ctx.weights, ctx.options
         grad_layer_2, grad_scores = copy_sparse_to_dense_backward(grad_output, (sparse_map, layer_2, scores))
         grad_rows, grad_transposed = block_quantize_both(grad_layer_2, sparse_map=sparse_map)
         del grad_layer_2
+        if layer_2_weight is None:
+            layer_2_weight = block_quantize(weight_2)
         grad_activation = block_sparse_matmul(grad_rows, layer_2_weight, sparse_map, dtype=grad_output.dtype, exact_sums=True)
+        del layer_2_weight
         grad, grad_1_transposed, activation_transposed = block_activation_backward(
             grad_activation, checkpoint, gated, activation_type, sparse_map
         )
@@ -427,9 +442,12 @@ class _BlockMLP(torch.autograd.Function):
         del activation_transposed, grad_transposed
         grad_input = None
         if ctx.needs_input_grad[0]:
+            if layer_1_transposed is None:
+                layer_1_transposed = block_quantize_transposed(weight_1, groups=sparse_map.num_experts)
             grad_sparse = block_sparse_matmul(
                 grad, layer_1_transposed, sparse_map, dtype=grad_output.dtype, exact_sums=_has_fine_results(grad_output)
             )
+            del layer_1_transposed
             grad_input = copy_dense_to_sparse_backward(grad_sparse, (sparse_map, grad_output.shape))
         if weight_1.requires_grad:
             _write_weight_gradient(
@@ -458,7 +476,7 @@ def block_mlp(
     `mlp_autograd` of `input_` [tokens, hidden] with all products in 8 bits: dispatch, layer 1, activation, layer 2 and combine.
     `weight_1` [experts * ffn (* 2), hidden] and `weight_2` [experts * ffn, hidden] are what the gradients are of: they are written to their
     `grad_buffer`s (of any float type) as everywhere. `weights`: the same weights quantised (`block_quantize_expert_weights`), where there are several calls to one
-    optimizer step; otherwise they are quantised here. Rows and gradients between the steps are of 8 bits; the results of both layers, of
+    optimizer step; otherwise they are quantised here, for the backward in the backward, until when they have to stay as they are. Rows and gradients between the steps are of 8 bits; the results of both layers, of
     the activation's gradient and of the input's per slot are rounded to the input's type, sums are in fp32 (exact, as `block_sparse_matmul` says, where results are quantised
     again, in fp16, and for gradients in fp16 or fp32). Differentiable once.
     Gated, ffn is a multiple of 128.
@@ -474,12 +492,15 @@ def block_mlp(
     if gated and ffn % BLOCK != 0:
         raise NotImplementedError(f"a gated activation has whole blocks of {BLOCK} columns, not {ffn}")
     if weights is None:
-        weights = block_quantize_expert_weights(weight_1, weight_2, experts)
+        weights = block_quantize_expert_weights(weight_1, weight_2, experts, training=False)
+    elif training and (weights.layer_1_transposed is None or weights.layer_2 is None):
+        raise ValueError("the weights are quantised for inference: they have nothing for a backward")
     ffn_1 = ffn * (2 if gated else 1)
     Assert.eq(weights.layer_1.shape, (experts * ffn_1, hidden))
-    Assert.eq(weights.layer_1_transposed.shape, (experts * hidden, ffn_1))
-    Assert.eq(weights.layer_2.shape, (experts * ffn, hidden))
     Assert.eq(weights.layer_2_transposed.shape, (experts * hidden, ffn))
+    for form, shape in ((weights.layer_1_transposed, (experts * hidden, ffn_1)), (weights.layer_2, (experts * ffn, hidden))):
+        if form is not None:
+            Assert.eq(form.shape, shape)
     input_, scores = input_.contiguous(), scores.contiguous()
     if not training:
         with torch.no_grad():

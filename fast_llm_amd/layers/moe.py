@@ -321,8 +321,9 @@ class BlockScaledMoEMLP(DroplessMoEMLP):
     """
     `DroplessMoEMLP`, with its options and its parameters by the same names, whose expert products are of 8 bits with a scale for each block of 128 in training and in
     inference (`block_mlp`). Routing, router and scores are the layer's own, on the unquantised input. It keeps 8 bits per value of each slot's input and
-    of the first layer's output for the backward, whatever there is to recompute. `forward` quantises the weights; where they stay the same over several
-    calls (micro-batches of a step, serving) `weights = layer.quantize_weights()` does so once, for `layer(input_, weights=weights)`.
+    of the first layer's output for the backward, whatever there is to recompute, and each slot's output for the scores' gradient. `forward` and its
+    backward quantise the weights, each what it reads; where they stay the same over several calls (micro-batches of a step, serving)
+    `weights = layer.quantize_weights()` does so once, for `layer(input_, weights=weights)`.
     """
 
     def __init__(self, hidden_size: int, intermediate_size: int, experts: int, experts_per_token: int, *, gated: bool = True,
@@ -333,9 +334,9 @@ class BlockScaledMoEMLP(DroplessMoEMLP):
             raise NotImplementedError("what the layer keeps for its backward is settled: there is nothing to recompute")
         super().__init__(hidden_size, intermediate_size, experts, experts_per_token, gated=gated, **options)
 
-    def quantize_weights(self) -> BlockScaledWeights:
-        """The expert weights as they are now."""
-        return block_quantize_expert_weights(self.layer_1, self.layer_2, self.experts)
+    def quantize_weights(self, training: bool = True) -> BlockScaledWeights:
+        """The expert weights as they are now; without `training` for inference alone, in half the memory."""
+        return block_quantize_expert_weights(self.layer_1, self.layer_2, self.experts, training=training)
 
     def forward(
         self,

@@ -1,4 +1,4 @@
-"""Which kernel the products of few and many rows run on: the tokens decide, not how the layout is padded."""
+"""Which kernel the products of few and many rows run on (the tokens decide, not how the layout is padded), and what is quantised when."""
 
 import ctypes
 import subprocess
@@ -102,3 +102,25 @@ def test_counted_products_validate_before_launching(library):
                 dict(lhs_stride=64), dict(dtype=3)):  # fmt: skip
         assert product(**bad) == _lib.FM_ERR_INVALID_ARGUMENT, bad
         assert b"counted" in library.fm_last_error()
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_inference_quantises_what_its_forward_reads(weights, calls):
+    experts, hidden, ffn, tokens = 2, 128, 256, 3
+    weight_1, weight_2 = torch.zeros(experts * 2 * ffn, hidden), torch.zeros(experts * ffn, hidden)
+    quantized = block_scaling.block_quantize_expert_weights(weight_1, weight_2, experts, training=False) if weights else None
+    calls.clear()
+    ends = torch.zeros(experts, dtype=torch.int32)
+    sparse_map = SparseMap(torch.zeros(tokens, 2, dtype=torch.int32), ends, ends, tokens, 256, 6, experts, 2)
+    with torch.no_grad():
+        block_scaling.block_mlp(torch.zeros(tokens, hidden), torch.ones(tokens, 2), weight_1, weight_2, quantized, gated=True, activation_type="silu",
+                                sparse_map=sparse_map, training=False)  # fmt: skip
+    # (rows' values, transposed values) of each quantisation: the input along its rows, and of the weights what the products sum along.
+    made = [(args[1] is not None, args[3] is not None) for name, args in calls if name == "fm_block_quantize"]
+    assert made == ([] if weights else [(True, False), (False, True)]) + [(True, False)]
+    with pytest.raises(ValueError, match="for inference"):
+        block_scaling.block_mlp(
+            torch.zeros(tokens, hidden), torch.ones(tokens, 2), weight_1, weight_2,
+            block_scaling.block_quantize_expert_weights(weight_1, weight_2, experts, training=False),
+            gated=True, activation_type="silu", sparse_map=sparse_map,
+        )  # fmt: skip

@@ -7,6 +7,7 @@ from fast_llm_amd.functional.block_scaling import (
     block_activation_backward, block_activation_forward, block_copy_dense_to_sparse, block_input_row_sparse_matmul, block_quantize, block_sparse_matmul,
 )  # fmt: skip
 from fast_llm_amd.functional.sparse_copy import get_sparse_map
+from fast_llm_amd.layers.moe import BlockScaledMoEMLP
 from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES, _map, _values
 
 pytestmark = pytest.mark.gpu
@@ -161,3 +162,82 @@ def test_the_padding_of_the_layout_changes_nothing(exact, per_expert, device):
         out = block_sparse_matmul(block_copy_dense_to_sparse(rows, sparse_map), weight, sparse_map, exact_sums=exact)
         results.append(out[sparse_map.sparse_rows.long()])
     assert all(torch.equal(result, results[0]) for result in results)
+
+
+# ---- weights that are quantised where they are needed ----------------------------------------------------
+def _layer_step(layer, x, grad, **options):
+    x = x.detach().requires_grad_(True)
+    layer.zero_grad()
+    layer.layer_1.param_grad_is_zero = layer.layer_2.param_grad_is_zero = True
+    output = layer(x, **options)
+    output.backward(grad)
+    return [t.detach().clone() for t in (output, x.grad, layer.router.grad, layer.layer_1.grad_buffer, layer.layer_2.grad_buffer)]
+
+
+@pytest.mark.parametrize("gated", [True, False])
+def test_weights_quantised_in_the_step_are_those_quantised_before_it(gated, device):
+    torch.manual_seed(0)
+    layer = BlockScaledMoEMLP(512, 640, 8, 2, gated=gated, device=device)
+    x, grad = (torch.randn(300, 512, device=device).bfloat16() for _ in range(2))
+    expected = _layer_step(layer, x, grad, weights=layer.quantize_weights())
+    assert all(torch.equal(a, b) for a, b in zip(_layer_step(layer, x, grad), expected))
+    # Twice through the same graph.
+    layer.layer_1.param_grad_is_zero = layer.layer_2.param_grad_is_zero = True
+    y = x.clone().requires_grad_(True)
+    output = layer(y)
+    (first,) = torch.autograd.grad(output, y, grad, retain_graph=True)
+    (second,) = torch.autograd.grad(output, y, grad)
+    assert torch.equal(first, expected[1]) and torch.equal(second, first)
+    # Inference needs half of the forms, and has the same result with either half or all of them.
+    layer.eval()
+    for weights in (None, layer.quantize_weights(), layer.quantize_weights(training=False)):
+        assert torch.equal(layer(x, weights=weights), expected[0])
+    inference = layer.quantize_weights(training=False)
+    assert inference.layer_1_transposed is None and inference.layer_2 is None
+    layer.train()
+    with pytest.raises(ValueError, match="for inference"):
+        layer(x, weights=inference)
+
+
+def test_what_is_kept_between_forward_and_backward(device):
+    """8 bits of each slot's input and of the first layer's output, each slot's output: no form of the weights, which would be the most of it."""
+    torch.manual_seed(0)
+    hidden, ffn, experts, tokens = 512, 640, 8, 64
+    layer = BlockScaledMoEMLP(hidden, ffn, experts, 2, device=device)
+    x = torch.randn(tokens, hidden, device=device).bfloat16().requires_grad_(True)
+    rows = 2 * tokens + 128 * experts
+    most = rows * ((hidden + 2 * ffn) * (1 + 1 / 128) + 2 * hidden) + (1 << 18)  # and what belongs to the routing
+    forms = experts * hidden * 3 * ffn
+    assert most < forms / 1.5
+    layer(x).backward(torch.zeros_like(x))
+    for weights, held in ((None, most), (layer.quantize_weights(), most)):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        output = layer(x, weights=weights)
+        assert torch.cuda.memory_allocated() - before <= held
+        output.backward(torch.zeros_like(x))
+    layer.eval()
+    before = torch.cuda.memory_allocated()
+    weights = layer.quantize_weights(training=False)
+    assert torch.cuda.memory_allocated() - before <= forms * (1 + 1 / 64)
+
+
+def test_weights_that_change_before_the_backward_are_noticed(device):
+    torch.manual_seed(0)
+    layer = BlockScaledMoEMLP(256, 256, 4, 2, device=device)
+    x, grad = (torch.randn(50, 256, device=device).bfloat16() for _ in range(2))
+    for name in ("layer_1", "layer_2"):
+        output = layer(x)
+        with torch.no_grad():
+            getattr(layer, name).mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            output.backward(grad)
+    # Those that the caller has quantised are what the backward goes by.
+    weights = layer.quantize_weights()
+    expected = _layer_step(layer, x, grad, weights=weights)
+    y = x.clone().requires_grad_(True)
+    output = layer(y, weights=weights)
+    with torch.no_grad():
+        layer.layer_1.mul_(2)
+    (ours,) = torch.autograd.grad(output, y, grad)
+    assert torch.equal(ours, expected[1])
