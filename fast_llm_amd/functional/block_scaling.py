@@ -261,8 +261,9 @@ def block_sparse_matmul(
       sparse_index[i] = sum(expert_ends <= i)
     `out` (of any float type, rows contiguous) or `dtype` gives the result's type. Only the rows that tokens have are written: padding and
     the rows behind the last expert stay as they are in `out`, uninitialised without one. Experts may begin anywhere.
-    Sums in fp32, rounded once; those for results of 16 bits are 1.5e-5 of themselves off (the matrix instruction drops what lies 14 bits under the largest of eight
-    products), with `exact_sums` as exact as those for results in float32, at half the rate: for results that are quantised again.
+    Sums in fp32, rounded once. For results of 16 bits each product loses up to 2^-13 of the largest among the eight neighbours along k that it is one of: sums of
+    normally distributed operands are 1.5e-5 of their root mean square off, and those whose large terms cancel may be off altogether. With `exact_sums` they are as
+    exact as those for results in float32, at half the rate: for results that are quantised again, and for sums that cancel.
     """
     refuse_traced()
     Assert.eq(lhs.columns, rhs.columns)

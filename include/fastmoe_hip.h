@@ -557,9 +557,10 @@ int fm_block_copy_dense_to_sparse(const void *values, const void *scales, const 
                                   int64_t scale_stride, int64_t out_scale_stride, int index_dtype, void *stream);
 
 /* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs has `columns` rows of `inner` per expert. Both layers of an expert MLP and
- * both input gradients are such products. Sums in fp32, one rounding. For results of 16 bits the matrix instruction aligns eight products to the largest of them and
- * drops what lies 14 bits under it: a sum of normal values is 1.5e-5 of itself off. Results in fp32, and with `exact_sums` those of 16 bits, are summed as exactly
- * as fp32, at half the rate. Only the rows that tokens have are written, those of lhs that none has are not looked at, and experts may begin anywhere. `out_stride`
+ * both input gradients are such products. Sums in fp32, one rounding. For results of 16 bits the matrix instruction cuts every eight products of neighbours along k
+ * off at 2^-13 of the largest of them: each of the others loses less than that, and a sum less than 7 * 2^-13 times the largest products of all its eights, added up (and
+ * what fp32 additions lose). Sums of normally distributed operands are 1.5e-5 of their root mean square off, of any length; of one whose large terms cancel
+ * nothing may be right. Results in fp32, and with `exact_sums` those of 16 bits, are summed as exactly as fp32, at half the rate. Only the rows that tokens have are written, those of lhs that none has are not looked at, and experts may begin anywhere. `out_stride`
  * in elements. Without a map there is one expert. */
 int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                            const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
