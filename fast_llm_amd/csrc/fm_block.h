@@ -1,11 +1,12 @@
-// Values of 8 bits with a scale for each block of 128: 128 neighbours along a row share a power of two, 2^(byte - 127), and are kept in e4m3. What the
-// kernels that write, read and multiply them have in common.
+// Values of 8 bits with a scale for each block of 128: 128 neighbours along a row share a power of two, 2^(byte - 127), and are kept in e4m3. What
+// the kernels that write, read and multiply them have in common.
 //
 // Rows are stored padded with zeros to whole blocks. The scales of all rows' first blocks come first, then those of their second blocks: a tile of
-// the products then has its scales of a slice in one piece. The scale is the smallest power of two (from 2^-127 on) that leaves the block's largest magnitude
-// at 448 or below, so nothing saturates; elements are value / scale rounded to nearest even. A power of two costs no accuracy next to a scale of 24 bits
-// (but below 2^-14 of the largest value, where elements become subnormal), the matrix instructions apply it by themselves, and a block that is cut along the
-// other axis keeps its elements: a change of scale is exact. A block with an infinity or NaN has scale byte 255, which makes all of it NaN, and zeros for elements.
+// the products then has its scales of a slice in one piece. The scale is the smallest power of two (from 2^-127 on) that leaves the block's largest
+// magnitude at 448 or below, so nothing saturates; elements are value / scale rounded to nearest even. A power of two costs no accuracy next to a
+// scale of 24 bits (but below 2^-14 of the largest value, where elements become subnormal), the matrix instructions apply it by themselves, and a
+// block that is cut along the other axis keeps its elements: a change of scale is exact. A block with an infinity or NaN has scale byte 255, which
+// makes all of it NaN, and zeros for elements.
 #pragma once
 
 #include "fm_mx.h"
@@ -61,7 +62,8 @@ int check_tensor(const char *name, const char *what, const void *values, const v
                  int64_t scale_stride);
 int check_map(const char *name, RowMap &map, const void *expert_ends, const void *expert_pad_begins, int64_t num_experts, int index_dtype);
 
-// How many of the rows from `row0` (a multiple of 128) to row0 + 127 count, up to `rows` in all: they are the first ones. All lanes of the wavefront take part.
+// How many of the rows from `row0` (a multiple of 128) to row0 + 127 count, up to `rows` in all: they are the first ones. All lanes of the wavefront
+// take part.
 __device__ __forceinline__ int rows_in_block(const RowMap &map, int64_t row0, int64_t rows) {
     int64_t end = rows;
     if (map.expert_ends != nullptr) {
@@ -92,9 +94,9 @@ __device__ __forceinline__ Raw<T, kCount> load_part(const T *pointer, int left) 
     return raw;
 }
 
-// Rows `first_row` + kRowStep r, r < kRows, of a block of 128 x 128 that begins at `block`: kCount neighbours of each from `column` on. Those from `count` on are
-// zeros, and so is what is behind the `columns` that there are. `exist`: rows that may be read. Where the columns are whole, no load is behind a
-// branch, so that all are on their way at once.
+// Rows `first_row` + kRowStep r, r < kRows, of a block of 128 x 128 that begins at `block`: kCount neighbours of each from `column` on. Those from
+// `count` on are zeros, and so is what is behind the `columns` that there are. `exist`: rows that may be read. Where the columns are whole, no load
+// is behind a branch, so that all are on their way at once.
 template <int kRows, int kRowStep, typename T, int kCount>
 __device__ __forceinline__ void load_block(const T *block, uint32_t stride, int first_row, int column, int exist, int count, int columns, Raw<T, kCount> (&raw)[kRows]) {
     if (columns == kBlock) {

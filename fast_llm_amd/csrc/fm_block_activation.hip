@@ -1,9 +1,11 @@
-// The MLP's activation between products of 8 bits: forward into the second layer's rows and a checkpoint of the input, both of 8 bits; backward from that
-// checkpoint into what the remaining products read: the input's gradient along its rows and its columns, and the forward's result along its columns.
+// The MLP's activation between products of 8 bits: forward into the second layer's rows and a checkpoint of the input, both of 8 bits; backward from
+// that checkpoint into what the remaining products read: the input's gradient along its rows and its columns, and the forward's result along its
+// columns.
 //
-// Both are one pass over their operands and no 16-bit copy leaves them. 98304 rows of 2 x 1408 in bf16: forward 204 us at 4.9 TB/s, backward 360 at 3.6 (two workgroups per CU; with one
-// 540). The forward is bound by memory. Of the backward every element has four conversions and the slope of the activation, so that memory and arithmetic weigh about the same; a lane keeps its three results (gate's and up's gradient, output)
-// in registers between the two directions of quantisation, eight rows x four columns of each.
+// Both are one pass over their operands and no 16-bit copy leaves them. 98304 rows of 2 x 1408 in bf16: forward 204 us at 4.9 TB/s, backward 360 at
+// 3.6 (two workgroups per CU; with one 540). The forward is bound by memory. Of the backward every element has four conversions and the slope of the
+// activation, so that memory and arithmetic weigh about the same; a lane keeps its three results (gate's and up's gradient, output) in registers
+// between the two directions of quantisation, eight rows x four columns of each.
 #include "fm_activation_math.h"
 #include "fm_block_rows.h"
 
@@ -11,17 +13,18 @@ namespace fm {
 
 namespace block {
 
-// What values of a type are activated in. A step in fp32 is 2^-24 of a value, and it is a border of e4m3 that decides: fp32 goes by fp64, and of 1.5 million values none is off, where
-// hardware functions in fp32 leave four and library functions in fp32 forty. Silu of 98304 rows of 2 x 1408: forward 305 us for 290, backward 740 for 385. What was rounded
-// to 16 bits has hardware exponentials and reciprocals of fp32.
+// What values of a type are activated in. A step in fp32 is 2^-24 of a value, and it is a border of e4m3 that decides: fp32 goes by fp64, and of 1.5
+// million values none is off, where hardware functions in fp32 leave four and library functions in fp32 forty. Silu of 98304 rows of 2 x 1408:
+// forward 305 us for 290, backward 740 for 385. What was rounded to 16 bits has hardware exponentials and reciprocals of fp32.
 template <typename T>
 struct ActivatedIn { typedef float Real; };
 template <>
 struct ActivatedIn<float> { typedef double Real; };
 
-// sigma(x) and 1 - sigma(x). Where gelu's argument is, a third power, the complement is e^-x of sigma, of which nothing is lost beside 1, and the exponent's own rounding, up to 2^-24 of
-// as many units as it has, is made good: without that 1200 bf16 rows of 2 x 1408 have 150 gradients on the other side of a border, with it 110 (of fp32 in library functions 180).
-// For silu it makes no difference, and 98304 such rows take 602 us there and back instead of 566.
+// sigma(x) and 1 - sigma(x). Where gelu's argument is, a third power, the complement is e^-x of sigma, of which nothing is lost beside 1, and the
+// exponent's own rounding, up to 2^-24 of as many units as it has, is made good: without that 1200 bf16 rows of 2 x 1408 have 150 gradients on the
+// other side of a border, with it 110 (of fp32 in library functions 180). For silu it makes no difference, and 98304 such rows take 602 us there and
+// back instead of 566.
 template <bool kFine>
 __device__ __forceinline__ float sigmoid(float x, float &complement) {
     if constexpr (!kFine) {
@@ -37,7 +40,8 @@ __device__ __forceinline__ float sigmoid(float x, float &complement) {
     complement = power * sigma;
     return sigma;
 }
-// In fp64, to 2^-36 of itself: e^-x = 2^n e^g with |g| <= ln(2) / 2 by Taylor's series up to g^9, and a step of Newton's from the hardware's reciprocal. (Beyond 2^+-1000 nothing changes in fp32.)
+// In fp64, to 2^-36 of itself: e^-x = 2^n e^g with |g| <= ln(2) / 2 by Taylor's series up to g^9, and a step of Newton's from the hardware's
+// reciprocal. (Beyond 2^+-1000 nothing changes in fp32.)
 template <bool kFine>
 __device__ __forceinline__ double sigmoid(double x, double &complement) {
     double t = x * -1.4426950408889634;
@@ -55,8 +59,8 @@ __device__ __forceinline__ double sigmoid(double x, double &complement) {
     return sigma;
 }
 
-// act(x), and act'(x) for the backward. Gelu (in its tanh form) and silu are x times a sigmoid, which has no cancellation where it is small: x sigma(z), with the slope
-// sigma + x sigma (1 - sigma) z'.
+// act(x), and act'(x) for the backward. Gelu (in its tanh form) and silu are x times a sigmoid, which has no cancellation where it is small: x
+// sigma(z), with the slope sigma + x sigma (1 - sigma) z'.
 template <int kActivation, typename Real>
 __device__ __forceinline__ Real activate(Real x, Real &slope) {
     if constexpr (kActivation == FM_ACT_GELU || kActivation == FM_ACT_SILU) {
@@ -69,7 +73,8 @@ __device__ __forceinline__ Real activate(Real x, Real &slope) {
             z_slope = linear + 3 * cubic * square;
         }
         Real complement, sigma = sigmoid<kActivation == FM_ACT_GELU>(z, complement);
-        // (1 + tanh in fp32, of which the other activation kernels make gelu, is 0 from here on: so is this, which a block with no larger value would show.)
+        // Gelu is that of the other activation kernels, x / 2 times 1 + tanh in fp32: zero from where this sum is, which a block with no larger value
+        // shows. (Above, where the sum has few bits left, a sigmoid has all of them.)
         if constexpr (kActivation == FM_ACT_GELU) sigma = sigma < static_cast<Real>(0x1p-26) ? 0 : sigma;
         const Real out = x * sigma;
         slope = sigma + out * complement * z_slope;
@@ -81,7 +86,8 @@ __device__ __forceinline__ Real activate(Real x, Real &slope) {
     return kActivation == FM_ACT_SQUARED_RELU ? positive * positive : positive;
 }
 
-// As fp32 in front of a rounding to fewer bits: what fp32 does not have leaves its last bit odd, so that no value comes to lie on a border that it is next to.
+// As fp32 in front of a rounding to fewer bits: what fp32 does not have leaves its last bit odd, so that no value comes to lie on a border that it is
+// next to.
 __device__ __forceinline__ float before_rounding(float value) { return value; }
 __device__ __forceinline__ float before_rounding(double value) {
     const float nearest = static_cast<float>(value);

@@ -25,12 +25,12 @@ int check_result(const char *name, const void *out, int64_t columns, int64_t out
 }  // namespace
 
 bool block::runs_on_tiles(const ProductArgs &args) {
-    // The tiles read the weights once, at 4 TB/s where little is multiplied and there is a tile for every CU; with few rows the weights are read once per 32 rows of
-    // an expert, at up to 6. So it depends on how many experts have over 32 rows, and on the tiles. Measured in us, few rows | tiles, with tokens
-    // at random: 8 experts 4096 -> 2 x 14336, 1 token 42 | 60, 8 rows per expert 153 | 234, 24 rows 197 | 238; 14336 -> 4096 22 | 112, 80 | 164, 103 | 165; 64
-    // experts 2048 -> 2 x 1408, 8 rows 65 | 83, 24 rows 84 | 87; 128 experts 2048 -> 2 x 768, 70 | 86 and 100 | 91. One expert, 4096 -> 28672 (112 tiles): 32 rows 31 | 50, 48 rows
-    // 54 | 50; 14336 -> 4096 (16 tiles): 128 rows 98 | 155, 192 rows 145 | 150. Of a map the host knows the rows with up to 128 of padding per expert (`rows_of_any_routing`);
-    // without one it knows them exactly.
+    // The tiles read the weights once, at 4 TB/s where little is multiplied and there is a tile for every CU; with few rows the weights are read once
+    // per 32 rows of an expert, at up to 6. So it depends on how many experts have over 32 rows, and on the tiles. Measured in us, few rows | tiles,
+    // with tokens at random: 8 experts 4096 -> 2 x 14336, 1 token 42 | 60, 8 rows per expert 153 | 234, 24 rows 197 | 238; 14336 -> 4096 22 | 112, 80
+    // | 164, 103 | 165; 64 experts 2048 -> 2 x 1408, 8 rows 65 | 83, 24 rows 84 | 87; 128 experts 2048 -> 2 x 768, 70 | 86 and 100 | 91. One expert,
+    // 4096 -> 28672 (112 tiles): 32 rows 31 | 50, 48 rows 54 | 50; 14336 -> 4096 (16 tiles): 128 rows 98 | 155, 192 rows 145 | 150. Of a map the host
+    // knows the rows with up to 128 of padding per expert (`rows_of_any_routing`); without one it knows them exactly.
     const int64_t tiles = (args.columns + 255) / 256 * args.experts, times = std::min(std::max(80 / tiles, int64_t(1)), int64_t(5));
     const bool many = args.expert_ends != nullptr ? rows_of_any_routing(args) > (128 + 24 * times) * args.experts : args.rows > 32 * times;
     return (many || !stream_product_takes(args)) && tile_product_takes(args);

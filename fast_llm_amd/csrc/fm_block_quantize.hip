@@ -1,10 +1,11 @@
-// Rows to values of 8 bits with a scale per block of 128, along the rows, along the columns (transposed) or both, and back; their dispatch to the sparse layout.
+// Rows to values of 8 bits with a scale per block of 128, along the rows, along the columns (transposed) or both, and back; their dispatch to the
+// sparse layout.
 //
-// All are bound by memory. Rows alone: a lane takes sixteen neighbours, eight lanes a block, so that the block's maximum is three steps across lanes. With the
-// columns: a workgroup takes a square of 128 x 128, in registers from its one read to the last write, eight rows x four columns a lane: of each row the
-// maximum over 32 lanes, of each column over the lane's rows, two lanes and the eight wavefronts (by way of LDS). The transposed elements pass LDS, so
-// that lines leave whole. In both forms 16384 x 4096 of bf16 take 50 us, 8 x 28672 x 4096 712, at 5.3 TB/s of the 6.5 that a copy reaches: the transposed form leaves as 128 lines of
-// as many rows.
+// All are bound by memory. Rows alone: a lane takes sixteen neighbours, eight lanes a block, so that the block's maximum is three steps across lanes.
+// With the columns: a workgroup takes a square of 128 x 128, in registers from its one read to the last write, eight rows x four columns a lane: of
+// each row the maximum over 32 lanes, of each column over the lane's rows, two lanes and the eight wavefronts (by way of LDS). The transposed
+// elements pass LDS, so that lines leave whole. In both forms 16384 x 4096 of bf16 take 50 us, 8 x 28672 x 4096 712, at 5.3 TB/s of the 6.5 that a
+// copy reaches: the transposed form leaves as 128 lines of as many rows.
 #include "fm_block_rows.h"
 
 namespace fm {

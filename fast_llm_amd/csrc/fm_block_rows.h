@@ -50,8 +50,8 @@ struct Square {
     uint8_t row_scales[kBlock];
 };
 
-// Where the eight rows of row group `group` of column 4 cg + c lie, in words: column by column in the order c, cg, units of 8 bytes swapped so that the writes
-// of a wavefront (32 cg, two groups) meet every bank twice and the reads, whole columns, once.
+// Where the eight rows of row group `group` of column 4 cg + c lie, in words: column by column in the order c, cg, units of 8 bytes swapped so that
+// the writes of a wavefront (32 cg, two groups) meet every bank twice and the reads, whole columns, once.
 __device__ __forceinline__ int transposed_at(int cg, int c, int group) { return (c * 32 + cg) * 32 + ((group ^ (cg >> 1 & 7) << 1) << 1); }
 
 // The largest magnitude over 32 lanes of each of eight values: of value 4 (l / 16 % 2) + 2 (l / 8 % 2) + l / 4 % 2 in lane l. Every step but the last
@@ -70,8 +70,8 @@ __device__ __forceinline__ uint32_t maxima_of_rows(const uint32_t (&rows)[kLaneR
     return max(one, from_lanes<kSwapFours>(one));
 }
 
-// The elements of a square's values, along the columns and (kRows) along the rows. `elements` and `scales`: of the square's first row and column in either form,
-// `rows` and `columns` that exist. Ends with reads of LDS that its next call comes after. All threads take part.
+// The elements of a square's values, along the columns and (kRows) along the rows. `elements` and `scales`: of the square's first row and column in
+// either form, `rows` and `columns` that exist. Ends with reads of LDS that its next call comes after. All threads take part.
 template <bool kRows>
 __device__ __forceinline__ void store_square(const float (&values)[kLaneRows][kLaneColumns], Square &shared, uint8_t *elements, uint32_t stride, uint8_t *scales, int rows,
                                              uint8_t *t_elements, int64_t t_stride, uint8_t *t_scales, int columns) {

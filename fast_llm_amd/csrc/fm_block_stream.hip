@@ -1,13 +1,14 @@
-// Products of a few rows per expert with expert weights of 8 bits and a scale per block of 128: the weights come from memory once and that is the bound.
+// Products of a few rows per expert with expert weights of 8 bits and a scale per block of 128: the weights come from memory once and that is the
+// bound.
 //
-// A wavefront has 32 weight rows of one expert and up to 32 rows of the activations at a time. kSplit wavefronts share the reduction, a stretch of it each, and
-// add up in LDS; kAcross of them sit side by side. The reduction is in chunks of 128, a block of the format and a line of memory of each weight row. A
-// load instruction takes eight whole lines, and the fragments, 16 bytes of each of 32 rows, are read from the wavefront's own part of LDS (XOR-swizzled; a wavefront's
-// LDS operations are carried out in order, so no barrier). kDepth chunks are on their way at a time. Activations, which all workgroups of an expert
-// read, come from L2 as fragments, and the scales as bytes, those of 32 neighbouring rows side by side.
+// A wavefront has 32 weight rows of one expert and up to 32 rows of the activations at a time. kSplit wavefronts share the reduction, a stretch of it
+// each, and add up in LDS; kAcross of them sit side by side. The reduction is in chunks of 128, a block of the format and a line of memory of each
+// weight row. A load instruction takes eight whole lines, and the fragments, 16 bytes of each of 32 rows, are read from the wavefront's own part of
+// LDS (XOR-swizzled; a wavefront's LDS operations are carried out in order, so no barrier). kDepth chunks are on their way at a time. Activations,
+// which all workgroups of an expert read, come from L2 as fragments, and the scales as bytes, those of 32 neighbouring rows side by side.
 //
-// One token and two of 8 experts, 4096 -> 2 x 14336: 40 us, 5.8 TB/s of weights; 96 tokens with 8 of 128, 2048 -> 2 x 768: 66 us, 6.1 TB/s. As fragments straight from memory, 16 bytes of
-// each of 32 lines at a time, the first took 60 and 14336 -> 4096 112 for 22.
+// One token and two of 8 experts, 4096 -> 2 x 14336: 40 us, 5.8 TB/s of weights; 96 tokens with 8 of 128, 2048 -> 2 x 768: 66 us, 6.1 TB/s. As
+// fragments straight from memory, 16 bytes of each of 32 lines at a time, the first took 60 and 14336 -> 4096 112 for 22.
 //
 // Any number of rows per expert is right (they are walked and the weights read again); the caller decides up to where this is the faster way.
 #include <algorithm>

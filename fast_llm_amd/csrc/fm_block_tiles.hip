@@ -1,18 +1,20 @@
-// Products of operands of 8 bits with a scale per block of 128, on tiles of 256 x 256: rows times expert weights, and weight gradients (the same product with
-// an expert's part of the reduction in place of its part of the rows). Both operands lie along the reduction.
+// Products of operands of 8 bits with a scale per block of 128, on tiles of 256 x 256: rows times expert weights, and weight gradients (the same
+// product with an expert's part of the reduction in place of its part of the rows). Both operands lie along the reduction.
 //
 // One workgroup per CU walks over its tiles. Its four wavefronts, one per SIMD, multiply 128 rows x 128 weight rows each (4 x 4 blocks of
-// v_mfma_scale_f32_32x32x64_f8f6f4, 256 accumulation registers; D's rows are weight rows, so that a lane has neighbouring columns of one row). The reduction
-// passes in slices of 128, a block of the format, through two LDS slots of 64 KB, on into the next tile. A slice's bytes go straight from memory into LDS. A step multiplies half of a wavefront's rows
-// over the whole slice, and what the next step needs is read beside it; what has been read makes room for the slice after the next one at once, two to three steps before that is
-// read. Every product has one or two reads or loads in its shadow, and is kept in its place among them. The scales of a slice, a byte for each row, are next to each other: a
-// wavefront brings those of its rows with one load, which pass LDS to the lanes that hold the rows. With exact sums (`kWide`) a step is 64 of the slice, and 256 conversions to bf16 go
-// with 128 products of half the length.
+// v_mfma_scale_f32_32x32x64_f8f6f4, 256 accumulation registers; D's rows are weight rows, so that a lane has neighbouring columns of one row). The
+// reduction passes in slices of 128, a block of the format, through two LDS slots of 64 KB, on into the next tile. A slice's bytes go straight from
+// memory into LDS. A step multiplies half of a wavefront's rows over the whole slice, and what the next step needs is read beside it; what has been
+// read makes room for the slice after the next one at once, two to three steps before that is read. Every product has one or two reads or loads in
+// its shadow, and is kept in its place among them. The scales of a slice, a byte for each row, are next to each other: a wavefront brings those of
+// its rows with one load, which pass LDS to the lanes that hold the rows. With exact sums (`kWide`) a step is 64 of the slice, and 256 conversions to
+// bf16 go with 128 products of half the length.
 //
-// 16384 rows of 8 experts, 14336 -> 4096: 749 us, 2.57 PFLOP/s, matrix units busy 68 % at 1.6 to 1.7 GHz (bound by power, and by waits at the barriers of a step); with steps of half a
-// slice, whose loads were asked for one to two steps ahead, and products that the compiler moved behind the loads, 830. With exact sums 1490 at 1.29 PFLOP/s, busy 66 % at 1.87 GHz: a
-// conversion takes 12 cycles, two of them a product's whole shadow. Weight gradient 14336 x 4096 of as many rows: 900, as every 16 slices have an epilogue. Into fp32 that is
-// added to (128 experts, 1536 x 2048, 131072 rows) 1210, half of it memory at 4.9 TB/s.
+// 16384 rows of 8 experts, 14336 -> 4096: 749 to 780 us by card, 2.47 to 2.57 PFLOP/s, matrix units busy 68 % at 1.6 to 1.7 GHz (bound by power, and
+// by waits at the barriers of a step); with steps of half a slice, whose loads were asked for one to two steps ahead, and products that the compiler
+// moved behind the loads, 830. With exact sums 1490 at 1.29 PFLOP/s, busy 66 % at 1.87 GHz: a conversion takes 12 cycles, two of them a product's
+// whole shadow. Weight gradient 14336 x 4096 of as many rows: 900, as every 16 slices have an epilogue. Into fp32 that is added to (128 experts, 1536
+// x 2048, 131072 rows) 1210, half of it memory at 4.9 TB/s.
 //
 // A row's slice is 128 bytes, in LDS XOR-swizzled in units of 16 bytes so that 16 lanes that read the same unit of neighbouring rows hit all 64
 // banks. Of every 32 weight rows, LDS row 8 a + 4 h + b holds row 16 h + 4 a + b: a lane (h: its half of the wavefront) then has 16 neighbouring
@@ -32,14 +34,16 @@ namespace tiles {
 constexpr int kTile = 256, kSlice = kBlock, kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 4;  // of 32, per wavefront and axis
 constexpr int kOperandBytes = kTile * kSlice, kSlotBytes = 2 * kOperandBytes, kSlots = 2;
-// Scales of a slice: a load per wavefront, of the rows of one half of the tile or of its weight rows, from an address of any alignment in pieces of 16.
+// Scales of a slice: a load per wavefront, of the rows of one half of the tile or of its weight rows, from an address of any alignment in pieces of
+// 16.
 constexpr int kScaleBytes = 1024, kScaleSlots = 3, kScaleSlotBytes = kWaves * kScaleBytes, kScalePieces = 128 / 16 + 1;
 constexpr int kPlaceBytes = 3 * 1024 * 4;  // see Places
 constexpr int kLdsBytes = kSlots * kSlotBytes + kScaleSlots * kScaleSlotBytes + kPlaceBytes;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr int kLoads = kOperandBytes / 1024 / kWaves;  // of a wavefront, per operand and slice
 constexpr int kResident = 256;                         // workgroups: one per CU
-// The loads of scales run this many slices ahead; a tile has no fewer, so that they are at most one tile ahead. (What is behind a tile's last slice is zero.)
+// The loads of scales run this many slices ahead; a tile has no fewer, so that they are at most one tile ahead. (What is behind a tile's last slice
+// is zero.)
 constexpr int kMinSlices = kSlots + 1;
 
 template <int kFirst, int kLast, typename F>
@@ -55,9 +59,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base,
                                              __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), kBufferResourceFlags);
 }
 
-// 16 bytes of each lane -> LDS at `target` + kMore + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and nothing else
-// in this file uses it. Where the compiler has spilled the resource, it brings it back by vector instructions, maybe right in front of this: five wait
-// states up to the load that reads it, which are more than M0's.)
+// 16 bytes of each lane -> LDS at `target` + kMore + 16 * lane; zeros for offsets out of range. (M0 is not handed out by the register allocator and
+// nothing else in this file uses it. Where the compiler has spilled the resource, it brings it back by vector instructions, maybe right in front of
+// this: five wait states up to the load that reads it, which are more than M0's.)
 template <int kMore>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uint32_t offset, int target) {
     asm volatile("s_add_i32 m0, %0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -66,11 +70,12 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t resource, uin
                  : "memory", "scc");
 }
 
-// The products before this are done when it is over. (The compiler counts a product's 16 passes up to the instructions that it knows to read its sums,
-// and does not look into assembly.)
+// The products before this are done when it is over. (The compiler counts a product's 16 passes up to the instructions that it knows to read its
+// sums, and does not look into assembly.)
 __device__ __forceinline__ void wait_for_products() { asm volatile("s_nop 15\n\ts_nop 7"); }
 
-// A block of sums, in accumulation registers up to here. (One by one: the compiler would copy a block that is handed over whole.) After `wait_for_products`.
+// A block of sums, in accumulation registers up to here. (One by one: the compiler would copy a block that is handed over whole.) After
+// `wait_for_products`.
 __device__ __forceinline__ f32x16_t settled(const f32x16_t &sums) {
     f32x16_t values;
 #pragma unroll
@@ -196,9 +201,9 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     if (!places.locate(placement, logical, inner_slices, upcoming)) return;
 
     // ---- loading: the slices of the workgroup's tiles one after the other, the last tile's followed by zeros -----------
-    // `upcoming` is the tile that is loaded. Wavefronts 2 m and 2 m + 1 take turns with 8 rows of the tile's half m, so that a lane has the same unit in all its rows. In two
-    // groups: first the blocks of weight rows but the last of each half, and the first 64 rows of each half of the rows; then the others. (A tile of up to 128 rows, which
-    // both halves of the workgroup share, has 32 rows in place of each 64.)
+    // `upcoming` is the tile that is loaded. Wavefronts 2 m and 2 m + 1 take turns with 8 rows of the tile's half m, so that a lane has the same unit
+    // in all its rows. In two groups: first the blocks of weight rows but the last of each half, and the first 64 rows of each half of the rows; then
+    // the others. (A tile of up to 128 rows, which both halves of the workgroup share, has 32 rows in place of each 64.)
     const uint32_t x_stride = static_cast<uint32_t>(args.x_stride), weight_stride = static_cast<uint32_t>(args.weight_stride);
     const int load_row = (wave & 1) * 8 + (lane >> 3), load_unit = (lane & 7) ^ ((load_row >> 1) & 7);
     const uint32_t x_offset = static_cast<uint32_t>(load_row) * x_stride + load_unit * 16;
@@ -232,9 +237,9 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
         for (int group = 0; group < 2; ++group) x_from[group] += kSlice, x_bytes[group] = load_slice < real_slices ? x_bytes[group] : 0;
         load_target = load_target == lds ? lds + kSlotBytes : lds;
     };
-    // Scales, a slice further ahead: they come from as many places of memory as there are slices, and are the last to arrive. (As far ahead as the slice
-    // itself, 14336 -> 4096 with 16384 rows of 8 experts took 937 us for 800; as bytes for each block of 32 rows, straight to the lanes that hold
-    // them, 998.) The first two wavefronts bring those of the halves of the tile's rows, the others those of the halves of its weight rows.
+    // Scales, a slice further ahead: they come from as many places of memory as there are slices, and are the last to arrive. (As far ahead as the
+    // slice itself, 14336 -> 4096 with 16384 rows of 8 experts took 937 us for 800; as bytes for each block of 32 rows, straight to the lanes that
+    // hold them, 998.) The first two wavefronts bring those of the halves of the tile's rows, the others those of the halves of its weight rows.
     const bool of_weights = wave >= 2;
     const int64_t scale_stride = of_weights ? args.weight_scale_stride : args.x_scale_stride;
     const uint32_t scale_offset = lane < kScalePieces ? lane * 16 : 0x80000000u;
@@ -336,8 +341,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
     for_each<0, kScales>(read_scale);
 #pragma unroll
     for (int i = 0; i < kScales; ++i) scales[i] = kWide ? wide_scale(next_scales[i]) : next_scales[i];
-    // kWide: a step of 64 is four of 16, and while one is multiplied the fragments of the next become bf16: by number four words of each, the weight rows'
-    // first.
+    // kWide: a step of 64 is four of 16, and while one is multiplied the fragments of the next become bf16: by number four words of each, the weight
+    // rows' first.
     constexpr int kParts = kWide ? 4 : 1, kConversions = kWide ? 2 * kBlocks * 4 : 0;
     u32x4_t wide_weight[kWide ? 2 : 1][kBlocks], wide_x[kWide ? 2 : 1][kBlocks];
     const auto widen = [&](auto constant, auto step_constant, auto part_constant, const uint32_t(&factors)[2 * kBlocks]) {
@@ -383,7 +388,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
             };
             // Block m of the tile's rows is the wavefront's block `place_of(m)` in LDS.
             const auto place_of = [](int m) { return kRows == kBlocks ? m : 2 * m; };
-            // Wide: steps of 64. Beside the first the reads of the second, beside the second the reads of the next slice and the loads of the one behind it.
+            // Wide: steps of 64. Beside the first the reads of the second, beside the second the reads of the next slice and the loads of the one
+            // behind it.
             constexpr int kSteps = kParts * kProducts;  // products of a step of 64
             // Reads are there before the step's last part, in which they are widened.
             constexpr int kReadsBusy = 2 * kProducts, kLoadsBusy = kSteps - 2;
@@ -432,8 +438,9 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                     __builtin_amdgcn_sched_barrier(0);
                 });
             };
-            // Narrow: the first step multiplies the whole slice of half of the rows, the second one that of the others. A slice's first group of loads has been read before
-            // its first step and the second group before its second one, and what takes their places is asked for at once, two to three steps before it is read.
+            // Narrow: the first step multiplies the whole slice of half of the rows, the second one that of the others. A slice's first group of
+            // loads has been read before its first step and the second group before its second one, and what takes their places is asked for at once,
+            // two to three steps before it is read.
             constexpr int kHalf = kProducts, kPerWeight = kHalf / kBlocks;  // products of a step, and of a block of weight rows in it
             constexpr int kFirstBusy = kHalf - 2, kFirstReads = 12, kAwaited = kItems + 1;
             const auto narrow_product = [&](auto constant, auto group_constant) {
@@ -448,7 +455,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(ProductArgs args, Gem
                 __builtin_amdgcn_sched_barrier(0);
                 narrow_product(kSecond, kFirst);
                 __builtin_amdgcn_sched_barrier(0);
-                // The second group of slice s is there (all that was asked for after it are two groups and scales), and all wavefronts have read the first one.
+                // The second group of slice s is there (all that was asked for after it are two groups and scales), and all wavefronts have read the
+                // first one.
                 wait_for_memory<kAwaited>();
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
@@ -603,7 +611,8 @@ static int launch_rows(const ProductArgs &args, hipStream_t stream) {
     return args.out_dtype == FM_DTYPE_BF16 ? launch<false, false, kWide, bf16_t>(args, stream) : launch<false, false, kWide, f16_t>(args, stream);
 }
 
-// Gradients in fp16 are summed as exactly as those in fp32: micro-batches add up in them, and half a step of fp16 is no more than sixteen times what inexact sums are off.
+// Gradients in fp16 are summed as exactly as those in fp32: micro-batches add up in them, and half a step of fp16 is no more than sixteen times what
+// inexact sums are off.
 template <bool kAccumulate>
 static int launch_gradients(const ProductArgs &args, hipStream_t stream) {
     switch (args.out_dtype) {

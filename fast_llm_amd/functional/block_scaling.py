@@ -1,13 +1,13 @@
 """
 Values of 8 bits with a scale for each block of 128, and the dropless expert MLP on them, in training and in serving.
 
-128 neighbours along a row share a power of two and are kept in e4m3, as include/fastmoe_hip.h states it. Every product sums along the rows of both its
-operands, so that what is summed along another axis is quantised along that axis and kept transposed: the weights in two forms, gradients and activations
-in one for the input gradient and one for the weights'. Between forward and backward the MLP keeps 8 bits per value: of its input's rows, and of the first
-layer's output, from which the backward has the activation and its slope.
+128 neighbours along a row share a power of two and are kept in e4m3, as include/fastmoe_hip.h states it. Every product sums along the rows of both
+its operands, so that what is summed along another axis is quantised along that axis and kept transposed: the weights in two forms, gradients and
+activations in one for the input gradient and one for the weights'. Between forward and backward the MLP keeps 8 bits per value: of its input's
+rows, and of the first layer's output, from which the backward has the activation and its slope.
 
-The reference has no counterpart. `block_mlp` has a backward. The operators by themselves have none (what is computed of values in 8 bits needs no gradient), and refuse
-forward-mode derivatives and `torch.jit`'s tracer.
+The reference has no counterpart. `block_mlp` has a backward. The operators by themselves have none (what is computed of values in 8 bits needs no
+gradient), and refuse forward-mode derivatives and `torch.jit`'s tracer.
 """
 
 import dataclasses
@@ -92,7 +92,10 @@ class BlockScaledTensor:
 
 
 class BlockScaledWeights(typing.NamedTuple):
-    """The expert weights of the sparse MLP in the forms that its products read (`block_quantize_expert_weights`); for inference without those of the backward."""
+    """
+    The expert weights of the sparse MLP in the forms that its products read (`block_quantize_expert_weights`); for inference without those of
+    the backward.
+    """
 
     layer_1: BlockScaledTensor  # [experts * ffn (* 2, gates then ups), hidden]: forward
     layer_1_transposed: BlockScaledTensor | None  # [experts * hidden, ffn (* 2)]: input gradient
@@ -242,7 +245,10 @@ def block_copy_dense_to_sparse(input_: BlockScaledTensor, sparse_map: SparseMap)
 
 
 def _has_worst_padding(sparse_map: SparseMap) -> bool:
-    """Whether the layout has room for any routing of its tokens (or nothing says how many rows they have): a product's kernel is then chosen by its rows."""
+    """
+    Whether the layout has room for any routing of its tokens (or nothing says how many rows they have): a product's kernel is then chosen by its
+    rows.
+    """
     entries = sparse_map.num_rows_unpadded
     return entries is None or sparse_map.num_rows == (entries + sparse_map.num_experts * BLOCK) // BLOCK * BLOCK
 
@@ -261,9 +267,11 @@ def block_sparse_matmul(
       sparse_index[i] = sum(expert_ends <= i)
     `out` (of any float type, rows contiguous) or `dtype` gives the result's type. Only the rows that tokens have are written: padding and
     the rows behind the last expert stay as they are in `out`, uninitialised without one. Experts may begin anywhere.
-    Sums in fp32, rounded once. For results of 16 bits each product loses up to 2^-13 of the largest among the eight neighbours along k that it is one of: sums of
-    normally distributed operands are 1.5e-5 of their root mean square off, and those whose large terms cancel may be off altogether. With `exact_sums` they are as
-    exact as those for results in float32, at half the rate: for results that are quantised again, and for sums that cancel.
+    Sums in fp32, rounded once. For results of 16 bits each product loses up to 2^-13 of the largest among the eight neighbours along k that it is
+    one of: sums of normally distributed operands are 1.5e-5 of their root mean square off, and those whose large terms cancel may be off
+    altogether. With `exact_sums` they are as exact as those for results in float32, at half the rate: for results that are quantised again, and for
+    sums that cancel. (Operands then have the range of bfloat16: magnitudes from 3.3e38 on, quantised to 2^128, are infinities, and those below
+    2^-126 are rounded to multiples of 2^-133.)
     """
     refuse_traced()
     Assert.eq(lhs.columns, rhs.columns)
@@ -296,11 +304,11 @@ def block_input_row_sparse_matmul(
     dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
     """
-    The weights' gradients from transposed forms lhs [rows, sparse rows] and rhs [columns, sparse rows] (`block_quantize_both`, `block_activation_backward`),
-    which hold zeros where no token is.
+    The weights' gradients from transposed forms lhs [rows, sparse rows] and rhs [columns, sparse rows] (`block_quantize_both`,
+    `block_activation_backward`), which hold zeros where no token is.
     Formula: out[id, j] (+)= sum_ks(lhs[is, ks] * rhs[j, ks]), where ks are the rows of expert id // rows, is = id % rows
-    `out` (of any float type, rows contiguous) or `dtype` gives the result's type. Sums are those of `block_sparse_matmul`: in fp32 and fp16 with `exact_sums`, in
-    bf16 without; where large terms cancel in a gradient, its buffer is in fp32.
+    `out` (of any float type, rows contiguous) or `dtype` gives the result's type. Sums are those of `block_sparse_matmul`: in fp32 and fp16 with
+    `exact_sums`, in bf16 without; where large terms cancel in a gradient, its buffer is in fp32.
     """
     refuse_traced()
     Assert.eq(lhs.columns, rhs.columns)
@@ -330,8 +338,8 @@ def block_activation_forward(
     input_: torch.Tensor, gated: bool, activation_type: ActivationType | str, sparse_map: SparseMap | None = None
 ) -> tuple[BlockScaledTensor, BlockScaledTensor]:
     """
-    (`mlp_activation_forward` of `input_` [rows, columns] in 8 bits, of the fp32 result; `input_` itself in 8 bits, for the backward.) With a map the rows that
-    no token has are zeros. Gated, gates and ups have whole blocks of 128 columns.
+    (`mlp_activation_forward` of `input_` [rows, columns] in 8 bits, of the fp32 result; `input_` itself in 8 bits, for the backward.) With a map
+    the rows that no token has are zeros. Gated, gates and ups have whole blocks of 128 columns.
     """
     refuse_traced(input_)
     Assert.eq(input_.dim(), 2)
@@ -357,8 +365,9 @@ def block_activation_backward(
     sparse_map: SparseMap | None = None,
 ) -> tuple[BlockScaledTensor, BlockScaledTensor, BlockScaledTensor]:
     """
-    The backward of `block_activation_forward` at what its checkpoint holds: the input's gradient along its rows (for the input gradient's product) and
-    transposed (for the weights'), and the activation's result transposed, all in 8 bits of fp32 values. With a map the rows that no token has are zeros.
+    The backward of `block_activation_forward` at what its checkpoint holds: the input's gradient along its rows (for the input gradient's product)
+    and transposed (for the weights'), and the activation's result transposed, all in 8 bits of fp32 values. With a map the rows that no token has
+    are zeros.
     """
     refuse_traced(grad_output)
     Assert.eq(grad_output.dim(), 2)
@@ -388,8 +397,10 @@ def _write_weight_gradient(weight: torch.Tensor, lhs: BlockScaledTensor, rhs: Bl
 
 
 def _has_fine_results(tensor: torch.Tensor) -> bool:
-    """Whether results of the tensor's type show the error of sums that are not exact: it is a sixteenth of half a step of fp16, which moves results that are rounded and added up by up
-    to half again as much as the roundings do, and a 128th of half a step of bf16."""
+    """
+    Whether results of the tensor's type show the error of sums that are not exact: it is a sixteenth of half a step of fp16, which moves results
+    that are rounded and added up by up to half again as much as the roundings do, and a 128th of half a step of bf16.
+    """
     return tensor.dtype == torch.float16
 
 
@@ -476,10 +487,11 @@ def block_mlp(
     """
     `mlp_autograd` of `input_` [tokens, hidden] with all products in 8 bits: dispatch, layer 1, activation, layer 2 and combine.
     `weight_1` [experts * ffn (* 2), hidden] and `weight_2` [experts * ffn, hidden] are what the gradients are of: they are written to their
-    `grad_buffer`s (of any float type) as everywhere. `weights`: the same weights quantised (`block_quantize_expert_weights`), where there are several calls to one
-    optimizer step; otherwise they are quantised here, for the backward in the backward, until when they have to stay as they are. Rows and gradients between the steps are of 8 bits; the results of both layers, of
-    the activation's gradient and of the input's per slot are rounded to the input's type, sums are in fp32 (exact, as `block_sparse_matmul` says, where results are quantised
-    again, in fp16, and for gradients in fp16 or fp32). Differentiable once.
+    `grad_buffer`s (of any float type) as everywhere. `weights`: the same weights quantised (`block_quantize_expert_weights`), where there are
+    several calls to one optimizer step; otherwise they are quantised here, for the backward in the backward, until when they have to stay as they
+    are. Rows and gradients between the steps are of 8 bits; the results of both layers, of the activation's gradient and of the input's per slot
+    are rounded to the input's type, sums are in fp32 (exact, as `block_sparse_matmul` says, where results are quantised again, in fp16, and for
+    gradients in fp16 or fp32). Differentiable once.
     Gated, ffn is a multiple of 128.
     """
     refuse_traced(input_, scores, weight_1, weight_2)

@@ -529,18 +529,19 @@ int fm_rms_norm_backward(const void *grad_normalized, const void *grad_stream, c
 
 /* ---------------------------------------------------------------------------------------------------------
  * Values of 8 bits with a scale for each block of 128: 128 neighbours along a row share the scale 2^(byte - 127) and are kept in e4m3. A tensor of
- * [rows, columns] is two arrays of bytes: values, row-major, `columns` bytes a row where `columns` is rounded up to a multiple of 128 (zeros behind the last
- * column); and scales, the blocks of 128 columns one after the other, of each a byte per row: `scale_stride` bytes from one block's to the next one's, at least
- * the rows rounded up to a multiple of 16. Strides are in bytes and multiples of 16, values and scales are 16-byte aligned. Results are contiguous.
+ * [rows, columns] is two arrays of bytes: values, row-major, `columns` bytes a row where `columns` is rounded up to a multiple of 128 (zeros behind
+ * the last column); and scales, the blocks of 128 columns one after the other, of each a byte per row: `scale_stride` bytes from one block's to the
+ * next one's, at least the rows rounded up to a multiple of 16. Strides are in bytes and multiples of 16, values and scales are 16-byte aligned.
+ * Results are contiguous.
  *   scale = the smallest power of two, from 2^-127 on, with (largest magnitude) <= 448 * scale;   element = value / scale, rounded to nearest even.
  *   A block with an infinity or NaN: scale byte 255 (all of it is NaN), elements 0.
  * `expert_ends` and `expert_pad_begins` [num_experts] (of `index_dtype`, as in fm_sparse_map; null, both: all rows count) say which rows tokens have;
  * the experts' rows begin at multiples of 128 here (whatever they hold, nothing out of range is read or written). The rows that no token has are not
  * looked at and count as zeros: the padding of an expert and what is behind the last one. At most 1024 experts.
  * --------------------------------------------------------------------------------------------------------- */
-/* `groups` matrices of `rows` x `columns` one after the other, rows `input_row_stride` elements apart, quantised along the rows ([groups * rows, columns]),
- * along the columns with the result transposed ([groups * columns, rows], padded to a multiple of 128 with zeros), or both: what is null is not computed. With
- * a map there is one group, and the transposed form. */
+/* `groups` matrices of `rows` x `columns` one after the other, rows `input_row_stride` elements apart, quantised along the rows ([groups * rows,
+ * columns]), along the columns with the result transposed ([groups * columns, rows], padded to a multiple of 128 with zeros), or both: what is null
+ * is not computed. With a map there is one group, and the transposed form. */
 int fm_block_quantize(const void *input, void *values, void *scales, void *transposed_values, void *transposed_scales, const void *expert_ends,
                       const void *expert_pad_begins, int64_t groups, int64_t rows, int64_t columns, int64_t num_experts, int64_t input_row_stride,
                       int64_t scale_stride, int64_t transposed_scale_stride, int dtype, int index_dtype, void *stream);
@@ -556,39 +557,43 @@ int fm_block_copy_dense_to_sparse(const void *values, const void *scales, const 
                                   int64_t num_rows_dense, int64_t columns, int64_t num_experts_per_token, int64_t num_rows_sparse, int64_t value_stride,
                                   int64_t scale_stride, int64_t out_scale_stride, int index_dtype, void *stream);
 
-/* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs has `columns` rows of `inner` per expert. Both layers of an expert MLP and
- * both input gradients are such products. Sums in fp32, one rounding. For results of 16 bits the matrix instruction cuts every eight products of neighbours along k
- * off at 2^-13 of the largest of them: each of the others loses less than that, and a sum less than 7 * 2^-13 times the largest products of all its eights, added up (and
- * what fp32 additions lose). Sums of normally distributed operands are 1.5e-5 of their root mean square off, of any length; of one whose large terms cancel
- * nothing may be right. Results in fp32, and with `exact_sums` those of 16 bits, are summed as exactly as fp32, at half the rate. Only the rows that tokens have are written, those of lhs that none has are not looked at, and experts may begin anywhere. `out_stride`
- * in elements. Without a map there is one expert. */
+/* out[i, j] = sum_k lhs[i, k] * rhs[e columns + j, k], e the expert of row i: rhs has `columns` rows of `inner` per expert. Both layers of an expert
+ * MLP and both input gradients are such products. Sums in fp32, one rounding. For results of 16 bits the matrix instruction cuts every eight products
+ * of neighbours along k off at 2^-13 of the largest of them: each of the others loses less than that, and a sum less than 7 * 2^-13 times the largest
+ * products of all its eights, added up (and what fp32 additions lose). Sums of normally distributed operands are 1.5e-5 of their root mean square
+ * off, of any length; of one whose large terms cancel nothing may be right. Results in fp32, and with `exact_sums` those of 16 bits, are summed as
+ * exactly as fp32, at half the rate; there operands have the range of bf16: 2^128, to which magnitudes over 248 * 2^120 are quantised, is an
+ * infinity, and what is below 2^-126 is rounded to multiples of 2^-133. Only the rows that tokens have are written, those of lhs that none has are
+ * not looked at, and experts may begin anywhere. `out_stride` in elements. Without a map there is one expert. */
 int fm_block_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                            const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
                            int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int exact_sums, int out_dtype,
                            int index_dtype, void *stream);
-/* The same product of a layout whose padding is not that of the worst case (rows = num_entries + 128 num_experts, rounded down to a multiple of 128, which
- * fm_block_sparse_matmul takes a map's rows to be): one that holds this routing alone, or without padding. `num_entries`: how many rows tokens have at most (tokens times
- * experts per token), 0: not known. It only helps to choose a kernel; results are those of the map. */
+/* The same product of a layout whose padding is not that of the worst case (rows = num_entries + 128 num_experts, rounded down to a multiple of 128,
+ * which fm_block_sparse_matmul takes a map's rows to be): one that holds this routing alone, or without padding. `num_entries`: how many rows tokens
+ * have at most (tokens times experts per token), 0: not known. It only helps to choose a kernel; results are those of the map. */
 int fm_block_sparse_matmul_counted(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                                    const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t num_entries,
                                    int64_t lhs_stride, int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride,
                                    int exact_sums, int out_dtype, int index_dtype, void *stream);
-/* The weights' gradients: out[e rows + i, j] (=, or += with `accumulate`) sum over the rows k of expert e of lhs[i, k] * rhs[j, k], lhs [rows, inner] and rhs
- * [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens have zeros. Results in fp32
- * and in fp16 are summed as exactly as fp32, at half the rate; those in bf16, whose steps are coarser, as fm_block_sparse_matmul does without `exact_sums`. */
+/* The weights' gradients: out[e rows + i, j] (=, or += with `accumulate`) sum over the rows k of expert e of lhs[i, k] * rhs[j, k], lhs [rows, inner]
+ * and rhs [columns, inner] being transposed forms that hold zeros where no token is; `inner`: the rows of the sparse layout. Experts without tokens
+ * have zeros. Results in fp32 and in fp16 are summed as exactly as fp32, at half the rate; those in bf16, whose steps are coarser, as
+ * fm_block_sparse_matmul does without `exact_sums`. */
 int fm_block_input_row_sparse_matmul(const void *lhs, const void *lhs_scales, const void *rhs, const void *rhs_scales, void *out, const void *expert_ends,
                                      const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t inner, int64_t num_experts, int64_t lhs_stride,
                                      int64_t lhs_scale_stride, int64_t rhs_stride, int64_t rhs_scale_stride, int64_t out_stride, int accumulate, int out_dtype,
                                      int index_dtype, void *stream);
 
 /* The MLP's activation of `input` [rows, columns] (gated: [rows, 2 columns], gates and then ups, `columns` a multiple of 128; FM_ERR_UNSUPPORTED
- * otherwise): `output` [rows, columns] in 8 bits, of the fp32 result, and `checkpoint`, the input in 8 bits. */
+ * otherwise): `output` [rows, columns] in 8 bits, of the fp32 result, and `checkpoint`, the input in 8 bits. FM_ACT_GELU, x / 2 (1 + tanh z), is 0
+ * where 1 + tanh z is in fp32 (below 2^-25), and its slope is 0 there too. NaN stays NaN in all of them. */
 int fm_block_activation_forward(const void *input, void *output, void *output_scales, void *checkpoint, void *checkpoint_scales, const void *expert_ends,
                                 const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t num_experts, int64_t input_stride,
                                 int64_t output_scale_stride, int64_t checkpoint_scale_stride, int gated, int activation, int dtype, int index_dtype,
                                 void *stream);
-/* Its backward from the checkpoint: the input's gradient for `grad_output` [rows, columns] of `dtype` (rows `grad_output_stride` elements apart) along its rows and
- * transposed, and the transposed form of the activation of what the checkpoint holds. */
+/* Its backward from the checkpoint: the input's gradient for `grad_output` [rows, columns] of `dtype` (rows `grad_output_stride` elements apart)
+ * along its rows and transposed, and the transposed form of the activation of what the checkpoint holds. */
 int fm_block_activation_backward(const void *grad_output, const void *checkpoint, const void *checkpoint_scales, void *grad, void *grad_scales,
                                  void *grad_transposed, void *grad_transposed_scales, void *output_transposed, void *output_transposed_scales,
                                  const void *expert_ends, const void *expert_pad_begins, int64_t rows, int64_t columns, int64_t num_experts,

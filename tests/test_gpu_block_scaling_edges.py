@@ -243,6 +243,27 @@ def test_a_layer_in_fp16_has_exact_sums_throughout(device):
             assert torch.equal(weight.grad_buffer, block_input_row_sparse_matmul(lhs, rhs, sparse_map, dtype=torch.float32).half())
 
 
+@pytest.mark.parametrize("rows", [1, 300])  # few rows, and tiles
+def test_the_range_of_operands(rows, device):
+    """Everything that 8 bits and a scale stand for; with exact sums what bf16 does: no 2^128, and multiples of 2^-133."""
+    top, small = torch.finfo(torch.bfloat16).max, 2.0**-133
+
+    def product(value: float, factor: float, exact: bool) -> float:
+        lhs, rhs = (block_quantize(torch.full((n, 128), v, device=device)) for n, v in ((rows, value), (1, factor)))
+        out = block_sparse_matmul(lhs, rhs, dtype=torch.bfloat16, exact_sums=exact)
+        assert torch.equal(out.isnan(), out[:1].isnan().expand_as(out)) and torch.equal(out.nan_to_num(), out[:1].expand_as(out).nan_to_num())
+        return out[0, 0].item()
+
+    # (128 products of powers of two, or of numbers of four bits: exact in bf16.)
+    for exact in (False, True):
+        for value in (240 * 2.0**120, -(2.0**127), 2.0**-126, 2.0**-127, small, -3 * small):
+            factor = 2.0**-40 if abs(value) > 1 else 2.0**120
+            assert product(value, factor, exact) == 128 * value * factor
+    assert product(top, 2.0**-40, False) == 128 * 2.0**88 and product(-top, 0.0, False) == 0
+    assert product(top, 2.0**-40, True) == INF and torch.tensor(product(-top, 0.0, True)).isnan()
+    assert product(small / 4, 2.0**120, False) == 128 * 2.0**-15 and product(small / 4, 2.0**120, True) == 0
+
+
 @pytest.mark.parametrize("per_expert", [1, 20, 100, 300])
 @pytest.mark.parametrize("exact", [False, True])
 def test_the_padding_of_the_layout_changes_nothing(exact, per_expert, device):
