@@ -515,6 +515,9 @@ def block_mlp(
         if form is not None:
             Assert.eq(form.shape, shape)
     input_, scores = input_.contiguous(), scores.contiguous()
+    if sparse_map.num_rows == 0:
+        # No token has an expert, in a layout for this routing alone: a block of rows that no expert has stands in for none at all.
+        sparse_map = dataclasses.replace(sparse_map, num_rows=BLOCK)
     if not training:
         with torch.no_grad():
             output = _BlockMLP.apply(input_, scores, weight_1, weight_2, weights, gated, activation_type, sparse_map, False, None)

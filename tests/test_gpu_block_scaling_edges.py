@@ -4,12 +4,13 @@ import pytest
 import torch
 
 from fast_llm_amd.functional.block_scaling import (
-    block_activation_backward, block_activation_forward, block_copy_dense_to_sparse, block_input_row_sparse_matmul, block_quantize, block_quantize_both,
-    block_quantize_transposed, block_sparse_matmul,
+    block_activation_backward, block_activation_forward, block_copy_dense_to_sparse, block_input_row_sparse_matmul, block_mlp, block_quantize,
+    block_quantize_both, block_quantize_transposed, block_sparse_matmul,
 )  # fmt: skip
 from fast_llm_amd.functional.sparse_copy import copy_dense_to_sparse_backward, copy_sparse_to_dense, copy_sparse_to_dense_backward, get_sparse_map
-from fast_llm_amd.layers.moe import BlockScaledMoEMLP
-from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES, _map, _values
+from fast_llm_amd.layers.moe import BlockScaledMoEMLP, attach_grad_buffer
+from oracle import block_oracle
+from tests.test_gpu_block_scaling import ACTIVATIONS, DTYPES, MLP_TOLERANCE, _difference, _map, _mlp_inputs, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -363,3 +364,48 @@ def test_weights_that_change_before_the_backward_are_noticed(device):
         layer.layer_1.mul_(2)
     (ours,) = torch.autograd.grad(output, y, grad)
     assert torch.equal(ours, expected[1])
+
+
+# ---- routings and sizes that the layer allows and seldom meets -------------------------------------------
+@pytest.mark.parametrize("dynamic", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize(("hidden", "ffn", "gated"), [(129, 100, False), (8, 1, False), (320, 128, True)])
+def test_mlp_step_of_tokens_without_experts_and_with_one_twice(hidden, ffn, gated, dtype, dynamic, device):
+    tokens, experts, slots = 90, 5, 3
+    input_, scores, top_experts, weight_1, weight_2, grad = _mlp_inputs(tokens, hidden, ffn, experts, slots, gated, dtype, device, seed=hidden)
+    top_experts[::7] = -1  # the padding of a batch
+    top_experts[1::7, 1] = -1
+    top_experts[2::7] = top_experts[2::7, :1]  # the same expert in all slots
+    expected = block_oracle.mlp_step(input_, scores, top_experts, weight_1, weight_2, experts, gated, "silu", grad, dtype)
+    x, s = input_.to(device).requires_grad_(True), scores.to(device).requires_grad_(True)
+    weights = [attach_grad_buffer(w.to(device).requires_grad_(True)) for w in (weight_1, weight_2)]
+    sparse_map = get_sparse_map(top_experts.to(device), experts, dynamic_shape=dynamic)
+    output = block_mlp(x, s, *weights, gated=gated, activation_type="silu", sparse_map=sparse_map)
+    output.backward(grad.to(device))
+    ours = {"output": output, "grad_input": x.grad, "grad_scores": s.grad, "grad_weight_1": weights[0].grad_buffer, "grad_weight_2": weights[1].grad_buffer}
+    for name, theirs in expected.items():
+        assert _difference(ours[name], theirs) <= MLP_TOLERANCE, name
+    assert not output[::7].any() and not x.grad[::7].any() and not s.grad[::7].any()
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+@pytest.mark.parametrize("without", [slice(None), slice(None, None, 5)], ids=["all", "some"])
+def test_tokens_without_experts_may_hold_anything(without, dynamic, device):
+    input_, scores, top_experts, weight_1, weight_2, grad = (t.to(device) for t in _mlp_inputs(60, 256, 128, 4, 2, True, torch.bfloat16, device))
+    top_experts[without] = -1
+    weights = [attach_grad_buffer(w.requires_grad_(True)) for w in (weight_1, weight_2)]
+    sparse_map = get_sparse_map(top_experts, 4, dynamic_shape=dynamic)
+    results = []
+    for value in (0.0, NAN):
+        x, s, g = input_.clone(), scores.clone(), grad.clone()
+        x[without], s[without], g[without] = value, value, value
+        x.requires_grad_(True), s.requires_grad_(True)
+        for weight in weights:
+            weight.param_grad_is_zero = True
+        output = block_mlp(x, s, *weights, gated=True, activation_type="silu", sparse_map=sparse_map)
+        output.backward(g)
+        results.append([t.detach().clone() for t in (output, x.grad, s.grad, *(w.grad_buffer for w in weights))])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert not any(t[without].any() for t in results[1][:3])
+    if without == slice(None):
+        assert not any(t.any() for t in results[1])
